@@ -414,6 +414,36 @@ THC_API int THGPUNN_SpatialAveragePooling_updateOutput(THGPUTensor *input, THGPU
     int kW, int kH, int dW, int dH);
 THC_API int THGPUNN_SpatialAveragePooling_updateGradInput(THGPUTensor *input, THGPUTensor *gradOutput,
     THGPUTensor *gradInput, int kW, int kH, int dW, int dH);
+/* LayerNorm (no counterpart in the reference): rows of `size` values, the trailing dimensions of the input that come to it, of mean zero
+ * and variance one, times a weight plus a bias:
+ *   output = (x - mean) * invStd * weight + bias,  invStd = 1 / sqrt(variance + eps), the variance over `size` values.
+ * weight and bias are both given or both NULL; so are mean and invStd, which receive one value a row for the backward pass.
+ * backward: gradInput (skipped when NULL), and gradWeight += scale * ..., gradBias += scale * ... (both or neither).  Sums are in FP32, in
+ * an order that the sizes alone decide.  Results may not share memory with operands. */
+THC_API int THGPUNN_LayerNorm_updateOutput(THGPUTensor *input, THGPUTensor *output, THGPUTensor *weight, THGPUTensor *bias,
+    THGPUTensor *mean, THGPUTensor *invStd, long size, double eps);
+THC_API int THGPUNN_LayerNorm_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *weight,
+    THGPUTensor *gradWeight, THGPUTensor *gradBias, THGPUTensor *mean, THGPUTensor *invStd, long size, float scale);
+/* FusedLinear (no counterpart in the reference): output = activation(input * weight^T + bias) + residual in one product whose
+ * epilogue does the rest.  input [R, I], weight [O, I], bias [O] or NULL, residual [R, O] or NULL.  activation: 0 none, 1 relu, 2 gelu
+ * (z times the standard normal distribution's integral up to z), 3 silu (z / (1 + exp(-z))).  preactivation, unless NULL, receives
+ * input * weight^T + bias, which backward reads where there is an activation.
+ * backward: gradPre receives gradOutput times the activation's slope (untouched without an activation, may then be NULL);
+ * gradInput = gradPre * weight, gradWeight += scale * gradPre^T * input, gradBias += scale * column sums; each is skipped when NULL.
+ * The residual's gradient is gradOutput itself.  Products follow the math mode.  Results may not share memory with operands. */
+THC_API int THGPUNN_FusedLinear_updateOutput(THGPUTensor *input, THGPUTensor *residual, THGPUTensor *output,
+    THGPUTensor *preactivation, THGPUTensor *weight, THGPUTensor *bias, int activation);
+THC_API int THGPUNN_FusedLinear_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput,
+    THGPUTensor *preactivation, THGPUTensor *gradPre, THGPUTensor *weight, THGPUTensor *gradWeight, THGPUTensor *gradBias,
+    int activation, float scale);
+/* GroupedLinear (no counterpart in the reference): FusedLinear without a residual where the rows of each group have a weight of their
+ * own.  input [R, I] sorted by group; counts: HOST array of the rows of each of `groups` groups, zeros among them, R in all;
+ * weight [groups, O, I], bias [groups, O] or NULL.  Gradients of groups without rows stay as they are. */
+THC_API int THGPUNN_GroupedLinear_updateOutput(THGPUTensor *input, const long *counts, int groups, THGPUTensor *output,
+    THGPUTensor *preactivation, THGPUTensor *weight, THGPUTensor *bias, int activation);
+THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *counts, int groups, THGPUTensor *gradOutput,
+    THGPUTensor *gradInput, THGPUTensor *preactivation, THGPUTensor *gradPre, THGPUTensor *weight, THGPUTensor *gradWeight,
+    THGPUTensor *gradBias, int activation, float scale);
 /* Parameter update over flat buffers.  momentum == 0: w -= lr*g, i.e. Module:updateParameters
  * (mcw_nn/Module.lua:75-82).  momentum != 0: v = momentum*v + g; w -= lr*v (not in the reference). */
 THC_API int THGPUNN_SGD_update(THGPUTensor *weight, THGPUTensor *grad, THGPUTensor *velocity,

@@ -5,6 +5,8 @@ if it is missing, or no CUDA device is present, calls fail loudly."""
 import ctypes as C
 import os
 
+import numpy as np
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libTHC.so")
 
@@ -103,6 +105,7 @@ FTP = C.POINTER(THFloatTensor)
 FSP = C.POINTER(THFloatStorage)
 f, l, i, d, vp, ch = C.c_float, C.c_long, C.c_int, C.c_double, C.c_void_p, C.c_char
 fp = C.POINTER(C.c_float)
+COUNTS = np.ctypeslib.ndpointer(np.int64, ndim=1, flags="C_CONTIGUOUS")   # a host array of whole numbers
 
 # name -> (restype, argtypes); every symbol include/THC.h declares
 SIGNATURES = {
@@ -191,6 +194,12 @@ SIGNATURES = {
     "THGPUNN_ClassNLLCriterion_updateOutput": (i, [TP, TP, TP, i]),
     "THGPUNN_ClassNLLCriterion_updateGradInput": (i, [TP, TP, TP, i]),
     "THGPUNN_SGD_update": (i, [TP, TP, TP, f, f]),
+    "THGPUNN_LayerNorm_updateOutput": (i, [TP, TP, TP, TP, TP, TP, l, d]),
+    "THGPUNN_LayerNorm_backward": (i, [TP, TP, TP, TP, TP, TP, TP, TP, l, f]),
+    "THGPUNN_FusedLinear_updateOutput": (i, [TP, TP, TP, TP, TP, TP, i]),
+    "THGPUNN_FusedLinear_backward": (i, [TP, TP, TP, TP, TP, TP, TP, TP, i, f]),
+    "THGPUNN_GroupedLinear_updateOutput": (i, [TP, COUNTS, i, TP, TP, TP, TP, i]),
+    "THGPUNN_GroupedLinear_backward": (i, [TP, COUNTS, i, TP, TP, TP, TP, TP, TP, TP, i, f]),
 }
 
 for _n, (_np, _st, _tn) in HOST_TYPES.items():

@@ -56,6 +56,13 @@ template <class T> bool take(PyObject *o, T &out) {
     if (v == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
     out = (T)v;
     return true;
+  } else if constexpr (std::is_same<T, const long *>::value) {   // a dense host array of int64, whose length is another argument
+    Py_buffer b;
+    if (PyObject_GetBuffer(o, &b, PyBUF_C_CONTIGUOUS | PyBUF_FORMAT) != 0) { PyErr_Clear(); return false; }
+    const bool ok = b.ndim == 1 && b.itemsize == 8 && b.format && std::strcmp(b.format, "l") == 0;
+    out = (const long *)b.buf;   // (the caller's argument keeps it alive)
+    PyBuffer_Release(&b);
+    return ok;
   } else {
     return false;
   }
@@ -129,7 +136,9 @@ const Entry kEntries[] = {
   E(THGPUNN_SpatialMaxPooling_updateGradInput) E(THGPUNN_Threshold_updateOutput) E(THGPUNN_Threshold_updateGradInput)
   E(THGPUNN_Threshold_SpatialMaxPooling_updateOutput) E(THGPUNN_Threshold_SpatialMaxPooling_updateGradInput)
   E(THGPUNN_Linear_updateOutput) E(THGPUNN_LogSoftMax_updateOutput) E(THGPUNN_LogSoftMax_updateGradInput) E(THGPUNN_ClassNLLCriterion_updateOutput)
-  E(THGPUNN_ClassNLLCriterion_updateGradInput) E(THGPUNN_SGD_update)
+  E(THGPUNN_ClassNLLCriterion_updateGradInput) E(THGPUNN_SGD_update) E(THGPUNN_LayerNorm_updateOutput) E(THGPUNN_LayerNorm_backward)
+  E(THGPUNN_FusedLinear_updateOutput) E(THGPUNN_FusedLinear_backward) E(THGPUNN_GroupedLinear_updateOutput)
+  E(THGPUNN_GroupedLinear_backward)
   UNARY(EU) COMPARE(EC)
 };
 

@@ -87,6 +87,18 @@ class Module:
                 setattr(self, k, gpu(v))
         return self
 
+    def training(self):
+        """mcw_nn/Dropout.lua's `train` field for every module: forward passes keep what a backward pass reads."""
+        return self._set_train(True)
+
+    def evaluate(self):
+        return self._set_train(False)
+
+    def _set_train(self, on):
+        for m in self.modules_list():
+            m.train = on
+        return self
+
     def modules_list(self):
         return [self]
 
@@ -368,8 +380,8 @@ class Linear(Module):
         super().__init__()
         self.weight = np.empty((outputSize, inputSize), np.float32)
         self.bias = np.empty((outputSize,), np.float32)
-        self.gradWeight = np.zeros_like(self.weight)
-        self.gradBias = np.zeros_like(self.bias)
+        self.gradWeight = np.zeros((outputSize, inputSize), np.float32)
+        self.gradBias = np.zeros((outputSize,), np.float32)
         self._ones = None
         self.reset(rng=rng)
 
@@ -405,6 +417,195 @@ class Linear(Module):
     def accGradParameters(self, input, gradOutput, scale=1.0):
         self.gradWeight.addmm(scale, gradOutput.t(), input)
         self.gradBias.addmv(scale, gradOutput.t(), self._ones_vec(input.size(1)))
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("activation %r: one of %s expected" % (name, ", ".join(ACTIVATIONS)))
+    return ACTIVATIONS[name]
+
+
+class LayerNorm(Module):
+    """Rows normalised to mean zero and variance one over the trailing `sizes`, times `weight` plus `bias` (one of each for every place
+    in a row); with affine=False the normalised rows themselves.  `mean` and `invStd` keep each row's statistics for the backward
+    pass; after evaluate() they are left alone."""
+
+    def __init__(self, *sizes, eps=1e-5, affine=True):
+        super().__init__()
+        self.size, self.eps, self.train = math.prod(sizes), eps, True
+        if not sizes or min(sizes) < 1:
+            raise ValueError("LayerNorm: positive sizes expected")
+        self.mean, self.invStd = GPUTensor(), GPUTensor()
+        self.weight = self.bias = self.gradWeight = self.gradBias = None
+        if affine:
+            self.weight, self.bias = np.ones(self.size, np.float32), np.zeros(self.size, np.float32)
+            self.gradWeight, self.gradBias = np.zeros(self.size, np.float32), np.zeros(self.size, np.float32)
+
+    def _affine(self):
+        if self.weight is None:
+            return None, None
+        return _need_gpu(self.weight, "LayerNorm.weight")._p, self.bias._p
+
+    def updateOutput(self, input):
+        _need_gpu(input, "LayerNorm")
+        w, b = self._affine()
+        keep = (self.mean._p, self.invStd._p) if self.train else (None, None)
+        lib().THGPUNN_LayerNorm_updateOutput(input._p, self.output._p, w, b, keep[0], keep[1], self.size, self.eps)
+        return self.output
+
+    def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
+        lib().THGPUNN_LayerNorm_backward(input._p, gradOutput._p, gradInput, self._affine()[0], gradWeight, gradBias, self.mean._p, self.invStd._p,
+                                         self.size, scale)
+
+    def updateGradInput(self, input, gradOutput):
+        if self.gradInput is None:
+            return None
+        self._back(input, gradOutput, self.gradInput._p, None, None, 1.0)
+        return self.gradInput
+
+    def accGradParameters(self, input, gradOutput, scale=1.0):
+        if self.weight is not None:
+            self._back(input, gradOutput, None, self.gradWeight._p, self.gradBias._p, scale)
+
+    def backward(self, input, gradOutput, scale=1.0):
+        """updateGradInput + accGradParameters in one library call."""
+        gi = self.gradInput._p if self.gradInput is not None else None
+        gw, gb = (self.gradWeight._p, self.gradBias._p) if self.weight is not None else (None, None)
+        self._back(input, gradOutput, gi, gw, gb, scale)
+        return self.gradInput
+
+
+class FusedLinear(Linear):
+    """activation(input * weight^T + bias), or that plus a residual for the input [rows, residual], in one product whose epilogue does the
+    rest.  activation: "none", "relu", "gelu" (of the normal distribution's integral) or "silu".  `preactivation` keeps the sum that the
+    activation is taken of for the backward pass; after evaluate() forward passes leave it alone.
+    With a residual gradInput is [the rows' gradient, gradOutput]: the second is the given tensor itself."""
+
+    def __init__(self, inputSize, outputSize, activation="none", rng=None):
+        super().__init__(inputSize, outputSize, rng=rng)
+        self.activation, self.train = activation, True
+        self._code = _activation(activation)
+        self.preactivation, self.gradPreactivation = GPUTensor(), GPUTensor()
+
+    def _split(self, input):
+        if isinstance(input, (list, tuple)):
+            rows, residual = input
+            return _need_gpu(rows, type(self).__name__), _need_gpu(residual, type(self).__name__ + " residual")
+        return _need_gpu(input, type(self).__name__), None
+
+    def updateOutput(self, input):
+        x, residual = self._split(input)
+        _need_gpu(self.weight, "FusedLinear.weight")
+        keep = self.preactivation._p if self.train and self._code else None
+        lib().THGPUNN_FusedLinear_updateOutput(x._p, residual._p if residual is not None else None, self.output._p, keep, self.weight._p, self.bias._p,
+                                               self._code)
+        return self.output
+
+    def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
+        x, residual = self._split(input)
+        lib().THGPUNN_FusedLinear_backward(x._p, gradOutput._p, gradInput, self.preactivation._p, self.gradPreactivation._p, self.weight._p, gradWeight,
+                                           gradBias, self._code, scale)
+        return residual
+
+    def _grad_rows(self):
+        """The rows' gradient in `gradInput`, which is a pair after a call with a residual."""
+        return self.gradInput[0] if isinstance(self.gradInput, list) else self.gradInput
+
+    def updateGradInput(self, input, gradOutput):
+        gi = self._grad_rows()
+        if gi is None:
+            return None
+        residual = self._back(input, gradOutput, gi._p, None, None, 1.0)
+        self.gradInput = gi if residual is None else [gi, gradOutput]
+        return self.gradInput
+
+    def accGradParameters(self, input, gradOutput, scale=1.0):
+        self._back(input, gradOutput, None, self.gradWeight._p, self.gradBias._p, scale)
+
+    def backward(self, input, gradOutput, scale=1.0):
+        """updateGradInput + accGradParameters in one library call, which takes the activation's slope once."""
+        gi = self._grad_rows()
+        residual = self._back(input, gradOutput, gi._p if gi is not None else None, self.gradWeight._p, self.gradBias._p, scale)
+        if gi is not None:
+            self.gradInput = gi if residual is None else [gi, gradOutput]
+        return self.gradInput
+
+
+class GroupedLinear(Module):
+    """activation(input * weight[e]^T + bias[e]) for the rows of group e: a layer of experts.  The input is [rows, counts], the rows sorted by
+    group and `counts` a host sequence with the number of rows of each group (zeros among them).  GPUTensor.index with the sorted rows'
+    positions brings rows into that order and indexCopy brings results back.  weight is [groups, outputSize, inputSize], bias
+    [groups, outputSize]; gradients of groups without rows stay as they are.  gradInput is [the rows' gradient, None].
+    `activation`, `preactivation` and evaluate() as for FusedLinear.  In the "bf16" math mode the products stay FP32-accurate."""
+
+    def __init__(self, groups, inputSize, outputSize, activation="none", rng=None):
+        super().__init__()
+        self.groups, self.activation, self.train = groups, activation, True
+        self._code = _activation(activation)
+        self.weight = np.empty((groups, outputSize, inputSize), np.float32)
+        self.bias = np.empty((groups, outputSize), np.float32)
+        self.gradWeight = np.zeros((groups, outputSize, inputSize), np.float32)
+        self.gradBias = np.zeros((groups, outputSize), np.float32)
+        self.preactivation, self.gradPreactivation = GPUTensor(), GPUTensor()
+        self.reset(rng=rng)
+
+    def reset(self, stdv=None, rng=None):
+        """Each group as Linear.reset draws a layer's."""
+        rng = rng or _default_rng
+        host = isinstance(self.weight, np.ndarray)
+        shape = tuple(self.weight.shape) if host else self.weight.size()
+        stdv = stdv * math.sqrt(3) if stdv else 1.0 / math.sqrt(shape[2])
+        w, b = rng.uniform(shape, -stdv, stdv), rng.uniform(shape[:2], -stdv, stdv)
+        if host:
+            self.weight, self.bias = w, b
+        else:
+            self.weight.copy(w); self.bias.copy(b)
+
+    def _split(self, input):
+        x, counts = input
+        if isinstance(counts, GPUTensor):
+            raise TypeError("GroupedLinear: counts are a host sequence")
+        counts = np.asarray(counts)
+        if counts.shape != (self.groups,) or counts.dtype.kind not in "iu":
+            raise ValueError("GroupedLinear: one whole number of rows for each of %d groups expected" % self.groups)
+        return _need_gpu(x, "GroupedLinear"), np.ascontiguousarray(counts, np.int64)
+
+    def updateOutput(self, input):
+        x, counts = self._split(input)
+        _need_gpu(self.weight, "GroupedLinear.weight")
+        keep = self.preactivation._p if self.train and self._code else None
+        lib().THGPUNN_GroupedLinear_updateOutput(x._p, counts, self.groups, self.output._p, keep, self.weight._p, self.bias._p, self._code)
+        return self.output
+
+    def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
+        x, counts = self._split(input)
+        lib().THGPUNN_GroupedLinear_backward(x._p, counts, self.groups, gradOutput._p, gradInput, self.preactivation._p, self.gradPreactivation._p,
+                                             self.weight._p, gradWeight, gradBias, self._code, scale)
+
+    def _grad_rows(self):
+        return self.gradInput[0] if isinstance(self.gradInput, list) else self.gradInput
+
+    def updateGradInput(self, input, gradOutput):
+        gi = self._grad_rows()
+        if gi is None:
+            return None
+        self._back(input, gradOutput, gi._p, None, None, 1.0)
+        self.gradInput = [gi, None]
+        return self.gradInput
+
+    def accGradParameters(self, input, gradOutput, scale=1.0):
+        self._back(input, gradOutput, None, self.gradWeight._p, self.gradBias._p, scale)
+
+    def backward(self, input, gradOutput, scale=1.0):
+        """updateGradInput + accGradParameters in one library call."""
+        gi = self._grad_rows()
+        self._back(input, gradOutput, gi._p if gi is not None else None, self.gradWeight._p, self.gradBias._p, scale)
+        if gi is not None:
+            self.gradInput = [gi, None]
+        return self.gradInput
 
 
 class LogSoftMax(Module):
