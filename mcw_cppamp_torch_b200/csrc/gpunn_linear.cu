@@ -3,116 +3,140 @@
 //   FusedLinear    z = x w^T + b,  y = act(z) + residual          x [R][I], w [O][I], b [O], residual [R][O]
 //   GroupedLinear  the same for the rows of group e with w[e], b[e], no residual: rows sorted by group, counts[e] of them each
 //   backward       gz = g act'(z);  dx = gz w,  dw += scale gz^T x,  db += scale sum_rows gz  (the residual's gradient is g)
-#include <type_traits>
-
 #include "nn_activation.cuh"
 #include "nn_args.h"
+#include "nn_linear.h"
 
 namespace thc {
 
-// y = act(z) + residual over rows of `cols` values; y may be z.
-template <int ACT>
-static __global__ void __launch_bounds__(256) act_rows_kernel(const float *z, float *y, const float *__restrict__ residual, long rows, long cols, long ldr) {
-  pdl_begin();
-  const long n = rows * cols;
-  for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += gridDim.x * 256l) {
-    float v = activation<ACT>(z[i]);
-    if (residual) {
-      const long r = i / cols;
-      v += residual[r * ldr + (i - r * cols)];
-    }
-    y[i] = v;
+// gz = g act'(z) over [first, end) of the rows, a piece of a group (blockIdx.y), with the sums of 128 columns over them: part[blockIdx.y][cols].  gz or
+// part may be null.  12 bytes a value: bound by HBM, or by latency where there are few rows.  A thread has four neighbouring columns (VEC), or one
+// of each 32, and every eighth row, four rows on the way.
+struct RowPiece { int group, first, end; };
+constexpr int kRowPieces = 256;
+struct RowPieces {
+  int count;
+  long per;          // rows of a piece, where there is one group
+  int groups;        // 1: pieces of `per` rows; else `at`
+  long rows;
+  RowPiece at[kRowPieces];
+  __device__ __forceinline__ RowPiece piece(int i) const {
+    if (groups > 1) return at[i];
+    return RowPiece{0, (int)(i * per), (int)min(rows, (i + 1) * per)};
   }
-}
-
-// gz = g act'(z) for a part of the rows (blockIdx.y), with the sums of 32 columns over them: part[blockIdx.y][cols].  gz or part may be null.
-template <int ACT>
-static __global__ void __launch_bounds__(256) act_grad_kernel(const float *__restrict__ g, long ldg, const float *__restrict__ z, float *gz, long rows, long cols,
-                                                              long per, float *part) {
+};
+template <int ACT, bool VEC>
+static __global__ void __launch_bounds__(256) act_grad_kernel(const float *__restrict__ g, long ldg, const float *__restrict__ z, float *gz, long cols, float *part,
+                                                              const __grid_constant__ RowPieces pieces) {
   pdl_begin();
-  __shared__ float sm[8][32];
+  __shared__ float sm[8][128];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long end = min(rows, (blockIdx.y + 1) * per);
-  for (long c0 = blockIdx.x * 32l; c0 < cols; c0 += gridDim.x * 32l) {
-    const long c = c0 + tx;
-    float s = 0.f;
-    if (c < cols)
-      for (long r = blockIdx.y * per + ty; r < end; r += 8) {
-        float v = g[r * ldg + c];
-        if constexpr (ACT != kActNone) {
-          v *= activation_slope<ACT>(z[r * cols + c]);
-          if (gz) gz[r * cols + c] = v;
+  const RowPiece p = pieces.piece(blockIdx.y);
+  const long c0 = blockIdx.x * 128l;
+  auto column = [&](int j) { return c0 + (VEC ? 4 * tx + j : tx + 32 * j); };
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
+  for (long r0 = p.first + ty; r0 < p.end; r0 += 8 * U) {
+    float gv[U][4], zv[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const long r = r0 + 8 * u;
+      auto read = [&](const float *m, long ld, float (&v)[4]) {
+        if constexpr (VEC) {
+          float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < p.end && column(0) < cols) q = __ldg(reinterpret_cast<const float4 *>(m + r * ld + column(0)));
+          v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[j] = r < p.end && column(j) < cols ? __ldg(m + r * ld + column(j)) : 0.f;
         }
-        s += v;
-      }
-    sm[ty][tx] = s;
-    __syncthreads();
-    if (part && ty == 0 && c < cols) {
-      for (int i = 1; i < 8; i++) s += sm[i][tx];
-      part[blockIdx.y * cols + c] = s;
+      };
+      read(g, ldg, gv[u]);
+      if constexpr (ACT != kActNone) read(z, cols, zv[u]);
     }
-    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const long r = r0 + 8 * u;
+      if constexpr (ACT != kActNone) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) gv[u][j] *= activation_slope<ACT>(zv[u][j]);
+        if (r < p.end && gz) {
+          if constexpr (VEC) {
+            if (column(0) < cols) *reinterpret_cast<float4 *>(gz + r * cols + column(0)) = make_float4(gv[u][0], gv[u][1], gv[u][2], gv[u][3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              if (column(j) < cols) gz[r * cols + column(j)] = gv[u][j];
+          }
+        }
+      }
+      if (r < p.end)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] += gv[u][j];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int j = 0; j < 4; j++) sm[ty][column(j) - c0] = s[j];
+  __syncthreads();
+  if (threadIdx.x < 128 && c0 + threadIdx.x < cols) {
+    float t = sm[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 8; i++) t += sm[i][threadIdx.x];
+    part[blockIdx.y * cols + c0 + threadIdx.x] = t;
   }
 }
-// out += scale * sum of the parts, in their order
-static __global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ part, int parts, long cols, float *out, float scale) {
+// out[group] += scale * sum of the group's parts, in their order.  Block (a, b) has 256 columns of the group that starts with piece b.
+static __global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ part, long cols, float *out, float scale,
+                                                                  const __grid_constant__ RowPieces pieces) {
   pdl_begin();
   const long c = blockIdx.x * 256l + threadIdx.x;
-  if (c >= cols) return;
+  int i = blockIdx.y;
+  const int group = pieces.piece(i).group;
+  if (c >= cols || (i > 0 && pieces.piece(i - 1).group == group)) return;
   float s = 0.f;
-  for (int p = 0; p < parts; p++) s += part[p * cols + c];
-  out[c] = fmaf(scale, s, out[c]);
-}
-
-// One product's operands and results.
-struct LinearForward {
-  const float *x; long ldx, rows, in, out;
-  const float *w, *b;             // b may be null
-  const float *residual; long ldr;   // may be null
-  float *z, *y;                   // z may be null
-  int act;
-};
-static void linear_forward(const LinearForward &l) {
-  if (l.rows <= 0) return;
-  float *z = l.z ? l.z : l.y;
-  gemm('t', 'n', l.out, l.rows, l.in, 1.f, l.w, l.in, l.x, l.ldx, 0.f, z, l.out, l.b);
-  if (l.act == kActNone && !l.residual && z == l.y) return;
-  const long n = l.rows * l.out;
-  with_activation(l.act, [&](auto a) {
-    pdl_launch(act_rows_kernel<decltype(a)::value>, (unsigned)std::min<long>((n + 255) / 256, ctx().sm_count * 16l), 256, 0, z, l.y, l.residual, l.rows, l.out,
-               l.ldr);
-  });
-  check_launch("linear activation");
-}
-struct LinearBackward {
-  const float *x; long ldx, rows, in, out;
-  const float *g; long ldg;
-  const float *z;                 // null for no activation
-  float *gz;                      // room for g act'(z); unused without an activation
-  const float *w;
-  float *gx, *gw, *gb;            // each may be null
-  int act;
-  float scale;
-};
-static void linear_backward(const LinearBackward &l) {
-  if (l.rows <= 0) return;
-  if (l.act != kActNone || l.gb) {
-    const long columns = std::min<long>((l.out + 31) / 32, 1l << 20);
-    const long parts = std::max(1l, std::min(std::min((l.rows + 31) / 32, (ctx().sm_count * 8l + columns - 1) / columns), 65535l)), per = (l.rows + parts - 1) / parts;
-    float *part = l.gb ? (float *)ws_alloc(sizeof(float) * parts * l.out) : nullptr;
-    with_activation(l.act, [&](auto a) {
-      pdl_launch(act_grad_kernel<decltype(a)::value>, dim3((unsigned)columns, (unsigned)parts), 256, 0, l.g, l.ldg, l.z, l.gz, l.rows, l.out, per, part);
-    });
-    check_launch("linear activation gradient");
-    if (l.gb) {
-      pdl_launch(fold_columns_kernel, ceil_div(l.out, 256), 256, 0, part, (int)parts, l.out, l.gb, l.scale);
-      check_launch("linear bias gradient");
-    }
+  if (pieces.groups == 1) {
+#pragma unroll 8
+    for (; i < pieces.count; i++) s += part[i * cols + c];
+  } else {
+    for (; i < pieces.count && pieces.piece(i).group == group; i++) s += part[i * cols + c];
   }
-  const float *gz = l.act == kActNone ? l.g : l.gz;
-  const long ldgz = l.act == kActNone ? l.ldg : l.out;
-  if (l.gx) gemm('n', 'n', l.in, l.rows, l.out, 1.f, l.w, l.in, gz, ldgz, 0.f, l.gx, l.in);
-  if (l.gw) gemm('n', 't', l.in, l.out, l.rows, l.scale, l.x, l.ldx, gz, ldgz, 1.f, l.gw, l.in);
+  float *o = out + group * cols + c;
+  *o = fmaf(scale, s, *o);
+}
+static void act_grad(const Groups &groups, const float *g, long ldg, const float *z, float *gz, long cols, int act, float *gb, float scale) {
+  const bool vec = cols % 4 == 0 && ldg % 4 == 0 && (((uintptr_t)g | (uintptr_t)z | (uintptr_t)gz) & 15) == 0;
+  const long tiles = (cols + 127) / 128;
+  // pieces of 32 rows and more, as many as leave eight blocks an SM
+  const long wanted = std::max(1l, ctx().sm_count * 8l / tiles), per = std::max(32l, (groups.rows + wanted - 1) / wanted);
+  auto run = [&](const RowPieces &p) {
+    if (!p.count) return;
+    float *part = gb ? (float *)ws_alloc(sizeof(float) * p.count * cols) : nullptr;
+    const dim3 grid((unsigned)tiles, (unsigned)p.count);
+    with_activation(act, [&](auto a) {
+      if (vec) pdl_launch(act_grad_kernel<decltype(a)::value, true>, grid, 256, 0, g, ldg, z, gz, cols, part, p);
+      else pdl_launch(act_grad_kernel<decltype(a)::value, false>, grid, 256, 0, g, ldg, z, gz, cols, part, p);
+    });
+    check_launch("activation gradient");
+    if (!gb) return;
+    pdl_launch(fold_columns_kernel, dim3((unsigned)ceil_div(cols, 256), p.groups == 1 ? 1u : (unsigned)p.count), 256, 0, part, cols, gb, scale, p);
+    check_launch("bias gradient");
+  };
+  RowPieces p;
+  p.groups = groups.n; p.rows = groups.rows; p.per = per; p.count = 0;
+  if (groups.n == 1) {
+    p.count = (int)((groups.rows + per - 1) / per);
+    run(p);
+    return;
+  }
+  // a group's pieces stay together: one whose pieces no longer fit starts the next launch, in larger pieces if it has to
+  long r = 0;
+  for (int e = 0; e < groups.n; r += groups.counts[e++]) {
+    const long n = groups.counts[e], step = std::max(per, (n + kRowPieces - 1) / kRowPieces);
+    if (p.count + (n + step - 1) / step > kRowPieces) { run(p); p.count = 0; }
+    for (long i = 0; i < n; i += step) p.at[p.count++] = RowPiece{e, (int)(r + i), (int)(r + std::min(n, i + step))};
+  }
+  run(p);
 }
 
 static bool same_shape(const THGPUTensor *t, int nd, const long *size) {
@@ -123,6 +147,11 @@ static bool same_shape(const THGPUTensor *t, int nd, const long *size) {
 }
 static void check_act(int act, int argn) { THC_ARG(act >= 0 && act < kActs, argn, "activation must be 0 (none), 1 (relu), 2 (gelu) or 3 (silu)"); }
 
+// Rows, inputs and outputs are counted in 32 bits.
+static void check_sizes(const THGPUTensor *input, long in, long out) {
+  constexpr long kMost = 1l << 30;
+  THC_ARG((nelem(input) == 0 || input->size[0] <= kMost) && in <= kMost && out <= kMost, 1, "more than 2^30 rows, inputs or outputs");
+}
 // What both operators check of a forward call.  `groups`: 0 for a plain layer, whose weight is a matrix.
 static void check_forward(THGPUTensor *input, THGPUTensor *weight, THGPUTensor *bias, long groups, int argw) {
   const int nd = groups ? 3 : 2;
@@ -131,6 +160,7 @@ static void check_forward(THGPUTensor *input, THGPUTensor *weight, THGPUTensor *
   const long out = weight->size[nd - 2], in = weight->size[nd - 1], bs[2] = {groups, out};
   if (bias) THC_ARG(same_shape(bias, nd - 1, bs + 3 - nd) && is_contiguous(bias), argw + 1, "contiguous bias of one value a result expected");
   if (nelem(input)) THC_ARG(input->nDimension == 2 && input->size[1] == in, 1, "batch of rows of the weight's input size expected");
+  check_sizes(input, in, out);
 }
 // Sizes the results of a forward call and holds them apart from its operands.
 static void size_forward(THGPUTensor *input, THGPUTensor *residual, THGPUTensor *output, THGPUTensor *preactivation, THGPUTensor *weight, THGPUTensor *bias, long rows,
@@ -148,6 +178,7 @@ static void check_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTen
           groups ? "contiguous weight of one matrix a group expected" : "contiguous matrix expected");
   const long out = weight->size[nd - 2], in = weight->size[nd - 1], rows = nelem(input) ? input->size[0] : 0, bs[2] = {groups, out}, s[2] = {rows, out};
   if (rows) THC_ARG(input->nDimension == 2 && input->size[1] == in, 1, "batch of rows of the weight's input size expected");
+  check_sizes(input, in, out);
   THC_ARG(rows ? same_shape(gradOutput, 2, s) : nelem(gradOutput) == 0, first + 1, "gradOutput has the wrong size");
   if (gradWeight) THC_ARG(same_shape(gradWeight, nd, weight->size) && is_contiguous(gradWeight), first + 6, "contiguous gradWeight of the weight's size expected");
   if (gradBias) THC_ARG(same_shape(gradBias, nd - 1, bs + 3 - nd) && is_contiguous(gradBias), first + 7, "contiguous gradBias of one value a result expected");
@@ -190,14 +221,15 @@ THC_API int THGPUNN_FusedLinear_updateOutput(THGPUTensor *input, THGPUTensor *re
   if (rows == 0) return 0;
   WsScope scope;
   DenseRows x(input);
-  LinearForward l = {x.p, x.ld, rows, in, out, data_ptr(weight), bias ? data_ptr(bias) : nullptr, nullptr, 0, preactivation ? data_ptr(preactivation) : nullptr,
-                     data_ptr(output), activation};
+  LinearTail tail;
+  tail.act = activation;
+  tail.z = preactivation ? data_ptr(preactivation) : nullptr;
   if (residual) {
     DenseRows r(residual);
-    l.residual = r.p; l.ldr = r.ld;
-    linear_forward(l);
+    tail.residual = r.p; tail.ldr = r.ld;
+    linear_product(x.p, x.ld, rows, in, out, data_ptr(weight), bias ? data_ptr(bias) : nullptr, data_ptr(output), tail);
   } else {
-    linear_forward(l);
+    linear_product(x.p, x.ld, rows, in, out, data_ptr(weight), bias ? data_ptr(bias) : nullptr, data_ptr(output), tail);
   }
   return 0;
   THC_END(1)
@@ -214,9 +246,14 @@ THC_API int THGPUNN_FusedLinear_backward(THGPUTensor *input, THGPUTensor *gradOu
   WsScope scope;
   DenseRows x(input), g(gradOutput);
   const bool act = activation != kActNone;
-  linear_backward({x.p, x.ld, rows, weight->size[1], weight->size[0], g.p, g.ld, act ? data_ptr(preactivation) : nullptr, act ? data_ptr(gradPre) : nullptr,
-                   data_ptr(weight), gradInput ? data_ptr(gradInput) : nullptr, gradWeight ? data_ptr(gradWeight) : nullptr,
-                   gradBias ? data_ptr(gradBias) : nullptr, activation, scale});
+  const long out = weight->size[0], in = weight->size[1];
+  const float *gz = act ? data_ptr(gradPre) : g.p;
+  const long ldgz = act ? out : g.ld;
+  if (act || gradBias)
+    act_grad(Groups{&rows, 1, rows}, g.p, g.ld, act ? data_ptr(preactivation) : nullptr, act ? data_ptr(gradPre) : nullptr, out, activation,
+             gradBias ? data_ptr(gradBias) : nullptr, scale);
+  if (gradInput) gemm('n', 'n', in, rows, out, 1.f, data_ptr(weight), in, gz, ldgz, 0.f, data_ptr(gradInput), in);
+  if (gradWeight) gemm('n', 't', in, out, rows, scale, x.p, x.ld, gz, ldgz, 1.f, data_ptr(gradWeight), in);
   return 0;
   THC_END(1)
 }
@@ -234,10 +271,8 @@ THC_API int THGPUNN_GroupedLinear_updateOutput(THGPUTensor *input, const long *c
   if (rows == 0) return 0;
   WsScope scope;
   DenseRows x(input);
-  long r0 = 0;
-  for (int e = 0; e < groups; r0 += counts[e++])
-    linear_forward({x.p + r0 * x.ld, x.ld, counts[e], in, out, data_ptr(weight) + e * out * in, bias ? data_ptr(bias) + e * out : nullptr, nullptr, 0,
-                    preactivation ? data_ptr(preactivation) + r0 * out : nullptr, data_ptr(output) + r0 * out, activation});
+  group_forward(Groups{counts, groups, rows}, x.p, x.ld, in, out, data_ptr(weight), bias ? data_ptr(bias) : nullptr, data_ptr(output), activation,
+                preactivation ? data_ptr(preactivation) : nullptr);
   return 0;
   THC_END(1)
 }
@@ -256,11 +291,13 @@ THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *count
   DenseRows x(input), g(gradOutput);
   const bool act = activation != kActNone;
   const long out = weight->size[1], in = weight->size[2];
-  long r0 = 0;
-  for (int e = 0; e < groups; r0 += counts[e++])
-    linear_backward({x.p + r0 * x.ld, x.ld, counts[e], in, out, g.p + r0 * g.ld, g.ld, act ? data_ptr(preactivation) + r0 * out : nullptr,
-                     act ? data_ptr(gradPre) + r0 * out : nullptr, data_ptr(weight) + e * out * in, gradInput ? data_ptr(gradInput) + r0 * in : nullptr,
-                     gradWeight ? data_ptr(gradWeight) + e * out * in : nullptr, gradBias ? data_ptr(gradBias) + e * out : nullptr, activation, scale});
+  const Groups gr{counts, groups, rows};
+  const float *gz = act ? data_ptr(gradPre) : g.p;
+  const long ldgz = act ? out : g.ld;
+  if (act || gradBias)
+    act_grad(gr, g.p, g.ld, act ? data_ptr(preactivation) : nullptr, act ? data_ptr(gradPre) : nullptr, out, activation, gradBias ? data_ptr(gradBias) : nullptr, scale);
+  if (gradInput) group_grad_input(gr, gz, ldgz, in, out, data_ptr(weight), data_ptr(gradInput));
+  if (gradWeight) group_grad_weight(gr, x.p, x.ld, gz, ldgz, in, out, data_ptr(gradWeight), scale);
   return 0;
   THC_END(1)
 }

@@ -178,7 +178,7 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_forward_kernel(
 // worked on, and with the sums of its columns for the weight's and the bias's gradient in registers, which part[block or cluster][2][D] gets.
 // gx or part may be null.
 template <int T, int V, bool VEC, bool CLUSTER>
-static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_backward_kernel(const float *__restrict__ x, const float *__restrict__ g, float *__restrict__ gx,
+static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) norm_backward_kernel(const float *__restrict__ x, const float *__restrict__ g, float *__restrict__ gx,
                                                                                const float *__restrict__ w, const float *__restrict__ mean,
                                                                                const float *__restrict__ inv, long rows, int D, int slice, float *part) {
   pdl_begin();
@@ -356,28 +356,30 @@ static __global__ void __launch_bounds__(256) norm_columns_kernel(const float *_
     __syncthreads();
   }
 }
-// gw += scale * sum of part[.][0], gb += scale * sum of part[.][1]: 32 columns a block, 32 threads each, which take every 32nd part and meet in the
-// order of their places.  (A thread for each column takes 20 us for the 296 parts of 4096 columns.)
-static __global__ void __launch_bounds__(1024) norm_fold_kernel(const float *__restrict__ part, int parts, long D, float *gw, float *gb, float scale) {
+// gw += scale * sum of part[.][0], gb += scale * sum of part[.][1]: LANES threads a column, which take every LANES-th part and meet in the order of
+// their places.
+template <int LANES>
+static __global__ void __launch_bounds__(256) norm_fold_kernel(const float *__restrict__ part, int parts, long D, float *gw, float *gb, float scale) {
   pdl_begin();
-  __shared__ float sm[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long c = blockIdx.x * 32l + tx;
+  constexpr int COLS = 256 / LANES;
+  __shared__ float sm[LANES][COLS];
+  const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+  const long c = blockIdx.x * (long)COLS + tx;
   float s = 0.f;
   if (c < 2 * D) {
-#pragma unroll 4
-    for (int p = ty; p < parts; p += 32) s += part[p * 2l * D + c];
+#pragma unroll 8
+    for (int p = ty; p < parts; p += LANES) s += part[p * 2l * D + c];
   }
-  sm[ty][tx] = s;
-  __syncthreads();
-  s = sm[tx][ty];
+  if constexpr (LANES > 1) {
+    sm[ty][tx] = s;
+    __syncthreads();
+    if (ty) return;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const long d = blockIdx.x * 32l + ty;
-  if (tx == 0 && d < 2 * D) {
-    float *o = d < D ? gw + d : gb + (d - D);
-    *o = fmaf(scale, s, *o);
+    for (int i = 1; i < LANES; i++) s += sm[i][tx];
   }
+  if (c >= 2 * D) return;
+  float *o = c < D ? gw + c : gb + (c - D);
+  *o = fmaf(scale, s, *o);
 }
 
 // How rows of D values are shared out.
@@ -400,6 +402,7 @@ template <class F> static void with_norm_config(long D, const NormShape &s, F f)
   if (s.blocks > 1) f(NormConfig<512, 4, true>());
   else if (D <= 128) f(NormConfig<32, 1, false>());
   else if (D <= 256) f(NormConfig<32, 2, false>());
+  else if (D <= 384) f(NormConfig<32, 3, false>());
   else if (D <= 512) f(NormConfig<32, 4, false>());
   else if (D <= 1024) f(NormConfig<128, 2, false>());
   else if (D <= 2048) f(NormConfig<256, 2, false>());
@@ -502,7 +505,11 @@ static void norm_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTens
     }
   }
   if (gradWeight) {
-    pdl_launch(norm_fold_kernel, ceil_div(2 * size, 32), 1024, 0, part, (int)parts, size, data_ptr(gradWeight), data_ptr(gradBias), scale);
+    // a thread a column where that fills the device or there is little to add up
+    if (parts <= 8 || size >= 32768)
+      pdl_launch(norm_fold_kernel<1>, ceil_div(2 * size, 256), 256, 0, part, (int)parts, size, data_ptr(gradWeight), data_ptr(gradBias), scale);
+    else
+      pdl_launch(norm_fold_kernel<16>, ceil_div(2 * size, 16), 256, 0, part, (int)parts, size, data_ptr(gradWeight), data_ptr(gradBias), scale);
     check_launch("LayerNorm_backward");
   }
 }

@@ -301,24 +301,36 @@ static void launch_raw(P p, Attach attach) {
 }
 
 // ---- small and narrow products (mm_small.cuh) ----------------------------------------------------------------------
-template <int BN, int WM, int WN, bool A_K, bool B_K>
-static void launch_small_kernel(const SmallProblem &p) {
+template <int BN, int WM, int WN, bool A_K, bool B_K, class P>
+static void launch_small_kernel(const P &p) {
   constexpr int BM = 64, SMEM = SM_STAGES * (SmallTile<BM, A_K>::FLOATS + SmallTile<BN, B_K>::FLOATS) * 4;
   static thread_local int configured_for = -1;
   if (SMEM > 47 * 1024 && configured_for != ctx().device) {
-    THC_CUDA(cudaFuncSetAttribute(small_kernel<BM, BN, WM, WN, A_K, B_K>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    THC_CUDA(cudaFuncSetAttribute(small_kernel<BM, BN, WM, WN, A_K, B_K, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     configured_for = ctx().device;
   }
-  const dim3 grid((unsigned)ceil_div(p.M, BM), (unsigned)ceil_div(p.N, BN), (unsigned)p.slices);
-  pdl_launch(small_kernel<BM, BN, WM, WN, A_K, B_K>, grid, SM_THREADS, SMEM, p);
+  dim3 grid((unsigned)ceil_div(p.M, BM), (unsigned)ceil_div(p.N, BN), (unsigned)p.slices);
+  if constexpr (P::GROUPS) grid.y = (unsigned)(p.list.count * p.column_tiles);
+  pdl_launch(small_kernel<BM, BN, WM, WN, A_K, B_K, P>, grid, SM_THREADS, SMEM, p);
   check_launch("small_kernel");
 }
-template <int BN, int WM, int WN>
-static void launch_small_layout(const SmallProblem &p, bool a_k, bool b_k) {
-  if (a_k && b_k) launch_small_kernel<BN, WM, WN, true, true>(p);
-  else if (a_k) launch_small_kernel<BN, WM, WN, true, false>(p);
-  else if (b_k) launch_small_kernel<BN, WM, WN, false, true>(p);
-  else launch_small_kernel<BN, WM, WN, false, false>(p);
+// Layouts there are: all four of a plain product; K-major operands (a linear layer's) with an epilogue; those of a grouped layer's three passes.
+template <int BN, int WM, int WN, class P>
+static void launch_small_layout(const P &p, bool a_k, bool b_k) {
+  if (a_k && b_k) { launch_small_kernel<BN, WM, WN, true, true>(p); return; }
+  if constexpr (!P::FUSED || P::GROUPS) {
+    if (!a_k && b_k) { launch_small_kernel<BN, WM, WN, false, true>(p); return; }
+    if (!a_k && !b_k) { launch_small_kernel<BN, WM, WN, false, false>(p); return; }
+  }
+  if constexpr (!P::FUSED) launch_small_kernel<BN, WM, WN, true, false>(p);
+  else fail("internal: operand layout that this product does not have");
+}
+template <class P>
+static void launch_small_width(const P &p, int bn, bool a_k, bool b_k) {
+  if (bn == 8) launch_small_layout<8, 4, 1>(p, a_k, b_k);
+  else if (bn == 16) launch_small_layout<16, 4, 1>(p, a_k, b_k);
+  else if (bn == 32) launch_small_layout<32, 4, 1>(p, a_k, b_k);
+  else launch_small_layout<64, 2, 2>(p, a_k, b_k);
 }
 inline SmallOperand small_operand(const float *base, long ld) {
   return SmallOperand{base, ld, ((uintptr_t)base & 15) == 0 && ld % 4 == 0 ? 1 : 0};
@@ -345,23 +357,26 @@ inline double small_product_us(long m, long n, long k, bool aligned) {
 // few_rows_kernel, for both operands along k in whole 16-byte pieces: up to 4 rows on the short side, and up to 8 while the
 // matrix stays in L2 many times over (a 4096 x 1000 one: 12.8 -> 9 us); beyond, the reads of the rows outweigh those
 // of the matrix and the MMA tiles win (8 rows against 4096 x 9216: 43 us, here 53).
-static bool launch_few_rows(const SmallProblem &p, bool a_k, bool b_k) {
+template <class P>
+static bool launch_few_rows(const P &p, bool a_k, bool b_k) {
   if (!(a_k && b_k && p.a.vec4 && p.b.vec4 && p.K % 4 == 0 && p.K <= 1 << 30 && p.N <= 8 && (p.N <= 4 || (long)p.M * p.K <= 1l << 23))) return false;
   const int ra = p.N == 1 || (p.N > 2 && p.N <= 4) ? 4 : 8;
   int groups = 8;   // sets of rows per block: as many as leave two blocks per SM, since they share the few rows
   while (groups > 1 && ceil_div(p.M, ra * groups) < 2 * ctx().sm_count) groups /= 2;
   const unsigned blocks = (unsigned)ceil_div(p.M, ra * groups);
-  if (p.N == 1) pdl_launch(few_rows_kernel<1, 4, 2>, blocks, 256, 0, p, groups);
-  else if (p.N == 2) pdl_launch(few_rows_kernel<2, 8, 2>, blocks, 256, 0, p, groups);
-  else if (p.N <= 4) pdl_launch(few_rows_kernel<4, 4, 3>, blocks, 256, 0, p, groups);
-  else pdl_launch(few_rows_kernel<8, 8, 1>, blocks, 256, 0, p, groups);
+  if (p.N == 1) pdl_launch(few_rows_kernel<1, 4, 2, P>, blocks, 256, 0, p, groups);
+  else if (p.N == 2) pdl_launch(few_rows_kernel<2, 8, 2, P>, blocks, 256, 0, p, groups);
+  else if (p.N <= 4) pdl_launch(few_rows_kernel<4, 4, 3, P>, blocks, 256, 0, p, groups);
+  else pdl_launch(few_rows_kernel<8, 8, 1, P>, blocks, 256, 0, p, groups);
   check_launch("few_rows");
   return true;
 }
 // D = alpha * A * B^T + beta * D (+ bias) for A [M][K] and B [N][K]; a_k / b_k: the operand's memory runs along k.
-static void launch_small(SmallProblem p, bool a_k, bool b_k) {
+template <class P>
+static void launch_small(P p, bool a_k, bool b_k) {
   if (p.N > p.M) {   // the longer side takes the 64-row tiles
     std::swap(p.a, p.b); std::swap(a_k, b_k); std::swap(p.M, p.N); std::swap(p.sm, p.sn); std::swap(p.bias_m, p.bias_n);
+    if constexpr (P::FUSED) std::swap(p.rm, p.rn);
   }
   p.stalled = stall_ctl().dev_flag;
   if (launch_few_rows(p, a_k, b_k)) return;
@@ -373,10 +388,7 @@ static void launch_small(SmallProblem p, bool a_k, bool b_k) {
     p.ws = (float *)ws_alloc(sizeof(float) * tiles * p.slices * 64 * bn);
     p.tickets = zero_words();
   }
-  if (bn == 8) launch_small_layout<8, 4, 1>(p, a_k, b_k);
-  else if (bn == 16) launch_small_layout<16, 4, 1>(p, a_k, b_k);
-  else if (bn == 32) launch_small_layout<32, 4, 1>(p, a_k, b_k);
-  else launch_small_layout<64, 2, 2>(p, a_k, b_k);
+  launch_small_width(p, bn, a_k, b_k);
 }
 
 template <class Main, class First = NoPass, class Second = NoPass>

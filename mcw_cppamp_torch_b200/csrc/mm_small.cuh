@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "mm_tc.cuh"
+#include "nn_activation.cuh"
 
 namespace thc {
 namespace mm {
@@ -42,6 +43,61 @@ struct SmallProblem {
   float *ws;                 // [tile][slice][value][thread] partial sums
   unsigned *tickets;         // one zero word per tile
   const int *stalled;        // the stream's stall flag (StallCtl::dev_flag): behind a stalled kernel nothing is written
+  static constexpr bool FUSED = false, GROUPS = false;
+  __device__ __forceinline__ const SmallProblem &at_block(int &, int &) const { return *this; }
+};
+// The same with D = act(A B^T + bias) + residual; z, unless null, gets the sum that the activation is taken of, laid out as D.  beta == 0.
+struct SmallFused : SmallProblem {
+  int act = kActNone;
+  const float *residual = nullptr;   // at residual[m * rm + n * rn]; may be null
+  long rm = 0, rn = 0;
+  float *z = nullptr;
+  static constexpr bool FUSED = true;
+  __device__ __forceinline__ const SmallFused &at_block(int &, int &) const { return *this; }
+};
+
+// ---- groups ----------------------------------------------------------------------------------------------------------
+// Products where the rows of each group meet a matrix of their own, in one launch.  An entry is a piece of a group's rows: a tile of columns of
+// the result (rows [first, end), the tile's width or less), or (kGroupSums) all rows of the group, which are summed over.
+enum : int { kGroupRows = 0, kGroupSums = 1 };
+struct GroupEntry { int group, first, end; };
+constexpr int kGroupEntries = 160;   // that travel with a launch; more of them lie in device memory
+struct GroupList {
+  int count;
+  const GroupEntry *more;            // all of them, or null
+  GroupEntry few[kGroupEntries];
+  __device__ __forceinline__ GroupEntry at(int i) const { return more ? more[i] : few[i]; }
+};
+// Offsets of a group's, and of a row's, part of the operands and results.
+struct GroupPlaces {
+  long a_group, a_row, b_row, c_group, c_row, bias_group;
+};
+struct SmallGroups : SmallFused {
+  int kind;                  // kGroupRows: A belongs to the group, B's rows and D's columns to the entry; kGroupSums: k belongs to the entry, D to the group
+  int column_tiles;          // of an entry
+  GroupPlaces at;
+  GroupList list;
+  static constexpr bool GROUPS = true;
+  // This block's product, with its first column.
+  __device__ __forceinline__ SmallFused at_block(int &column, int &k_tiles) const {
+    SmallFused p = *this;
+    const int e = (int)blockIdx.y / column_tiles;
+    const GroupEntry g = list.at(e);
+    p.a.base += g.group * at.a_group + g.first * at.a_row;
+    p.b.base += g.first * at.b_row;
+    const long c = g.group * at.c_group + g.first * at.c_row;
+    p.c += c;
+    if (p.z) p.z += c;
+    if (p.bias) p.bias += g.group * at.bias_group;
+    column = (int)blockIdx.y - e * column_tiles;
+    if (kind == kGroupRows) {
+      p.N = g.end - g.first;
+    } else {
+      p.K = g.end - g.first;
+      k_tiles = (p.K + TC_BK - 1) / TC_BK;
+    }
+    return p;
+  }
 };
 
 constexpr int SM_THREADS = 128;
@@ -151,9 +207,11 @@ __device__ __forceinline__ float fp32_sum(const SmallProblem &p, long m, long n,
 }
 
 // WM x WN warps, each (BM / WM) x (BN / WN)
-template <int BM, int BN, int WM, int WN, bool A_K, bool B_K>
-__global__ void __launch_bounds__(SM_THREADS) small_kernel(const SmallProblem p) {
+template <int BM, int BN, int WM, int WN, bool A_K, bool B_K, class P = SmallProblem>
+__global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant__ P whole) {
   pdl_begin();
+  int column = blockIdx.y, tiles_per_slice = whole.tiles_per_slice;
+  const auto &p = whole.at_block(column, tiles_per_slice);
   static_assert(WM * WN * 32 == SM_THREADS && BM % (16 * WM) == 0 && BN % (8 * WN) == 0, "warp layout");
   constexpr int MT = BM / WM / 16, NT = BN / WN / 8;
   constexpr int A_FLOATS = SmallTile<BM, A_K>::FLOATS, B_FLOATS = SmallTile<BN, B_K>::FLOATS, STAGE = A_FLOATS + B_FLOATS;
@@ -161,10 +219,10 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const SmallProblem p)
   __shared__ bool is_last;
   const int stalled = *reinterpret_cast<const volatile int *>(p.stalled);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN;
+  const int m0 = blockIdx.x * BM, n0 = column * BN;
   const int wm = (warp % WM) * (BM / WM), wn = (warp / WM) * (BN / WN);
-  const int kt0 = blockIdx.z * p.tiles_per_slice;
-  const int nk = min(p.tiles_per_slice, (p.K + TC_BK - 1) / TC_BK - kt0);
+  const int kt0 = blockIdx.z * tiles_per_slice;
+  const int nk = min(tiles_per_slice, (p.K + TC_BK - 1) / TC_BK - kt0);
   // the rows a thread's fragment registers stand for: fragment row r = 16 i + g + 8 e (A) or 8 j + g (B) of a warp's share
   // is this row of it
   auto a_row = [&](int i, int gr, int e) { return wm + (A_K ? 16 * i + gr + 8 * e : gr * 2 * MT + 2 * i + e); };
@@ -314,6 +372,34 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const SmallProblem p)
           for (int e = 0; e < 4; e++) acc[i][j][e] += __ldcg(all + ((long)z * NV + (i * NT + j) * 4 + e) * SM_THREADS);
   }
   if (stalled) return;
+  if constexpr (P::FUSED) {
+    if (p.beta == 0.f) {
+      with_activation(p.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; e2++) {
+            const int m = m0 + a_row(i, g, e2);
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+              for (int e1 = 0; e1 < 2; e1++) {
+                const int n = n0 + b_row(j, 2 * t + e1);
+                if (n >= p.N) continue;
+                const long o = (long)m * p.sm + (long)n * p.sn;
+                float v = p.alpha * acc[i][j][2 * e2 + e1];
+                if (p.bias) v += p.bias[m * p.bias_m + n * p.bias_n];
+                if (p.z) p.z[o] = v;
+                v = activation<decltype(act)::value>(v);
+                if (p.residual) v += p.residual[m * p.rm + n * p.rn];
+                p.c[o] = v;
+              }
+          }
+      });
+      return;
+    }
+  }
   auto store = [&](auto accumulate) {
     constexpr bool OLD = decltype(accumulate)::value;
     // Old values are asked for together, before the first store: otherwise each waits for its own round trip, up to 32 of them one
@@ -362,8 +448,8 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const SmallProblem p)
 // matrix, against the tiles above: 9216 -> 4096 outputs (151 MB) 42.5 -> 26 us for one and two rows (5.8 TB/s), 33 for four;
 // 4096 -> 1000 (16 MB, which then stays in L2) 12.5 -> 6.5; 512 -> 512 5.0 -> 3.3.  With the matrix in DRAM: 32, 18 (4096 -> 4096) and
 // 11 us, i.e. 4.7, 3.7 and 1.5 TB/s: the shorter the launch, the more of it is its start.
-template <int R, int RA, int UNROLL>
-__global__ void __launch_bounds__(256) few_rows_kernel(const SmallProblem p, int groups) {
+template <int R, int RA, int UNROLL, class P = SmallProblem>
+__global__ void __launch_bounds__(256) few_rows_kernel(const P p, int groups) {
   pdl_begin();
   __shared__ float part[8][RA * R];
   const int stalled = *reinterpret_cast<const volatile int *>(p.stalled);
@@ -421,7 +507,13 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const SmallProblem p, int
     float *o = p.c + (long)m * p.sm + (long)n * p.sn;
     float v = p.alpha * sum;
     if (p.bias) v += p.bias[m * p.bias_m + n * p.bias_n];
-    if (p.beta != 0.f) v += p.beta * *o;
+    if constexpr (P::FUSED) {
+      if (p.z) p.z[(long)m * p.sm + (long)n * p.sn] = v;
+      with_activation(p.act, [&](auto act) { v = activation<decltype(act)::value>(v); });
+      if (p.residual) v += p.residual[m * p.rm + n * p.rn];
+    } else if (p.beta != 0.f) {
+      v += p.beta * *o;
+    }
     *o = v;
   }
 }

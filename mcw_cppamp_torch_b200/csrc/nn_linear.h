@@ -1,0 +1,36 @@
+// Products of nn.FusedLinear and nn.GroupedLinear: declared here, made by thc_blas.cu (plain layers) and thc_groups.cu (groups).
+#ifndef THC_NN_LINEAR_H
+#define THC_NN_LINEAR_H
+
+#include <vector>
+
+#include "thc_internal.h"
+
+namespace thc {
+
+// What follows a linear layer's product, for results laid out [rows][out].
+struct LinearTail {
+  int act = 0;                       // kActNone ...
+  const float *residual = nullptr;   // row r at residual + r * ldr; may be null
+  long ldr = 0;
+  float *z = nullptr;                // receives the sum that the activation is taken of; may be null
+};
+// y = act(z) + residual with z = x w^T + b: x [rows][in] at pitch ldx, w [out][in], b may be null
+void linear_product(const float *x, long ldx, long rows, long in, long out, const float *w, const float *b, float *y, const LinearTail &tail);
+
+// Rows of group e: the counts[e] from the sum of the counts before it on.
+struct Groups {
+  const long *counts;
+  int n;
+  long rows;
+};
+// For the rows of each group e: y = act(z), z = x w[e]^T + b[e]
+void group_forward(const Groups &g, const float *x, long ldx, long in, long out, const float *w, const float *b, float *y, int act, float *z);
+// gx = gz w[e]
+void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx);
+// gw[e] += scale * gz^T x over the group's rows
+void group_grad_weight(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale);
+
+}  // namespace thc
+
+#endif

@@ -4,6 +4,7 @@
 // :470-483, ger :486-502.  Here gemm maps onto the shared matrix-multiply engines (tcgen05 3xTF32
 // by default: the two-SM one, or a warp-level one for small and narrow products), all leading dimensions are honoured and C is not read when beta == 0.
 #include "mm_launch.cuh"
+#include "nn_linear.h"
 
 namespace thc {
 
@@ -243,6 +244,64 @@ void gemm(char transa, char transb, long m, long n, long k, float alpha, const f
   else if (small_is_faster(m, n, k, aligned)) gemm_small(x, y, k, alpha, beta, c, ldc, row_bias);
   else if (!(mode == 0 && pairs_are_faster(m, n, k) && gemm_pairs(x, y, k, alpha, beta, c, ldc, row_bias)))
     gemm_raw(x, y, k, alpha, beta, c, ldc, row_bias);
+}
+
+// y = act(z) + residual over rows of `cols` values; y may be z.
+template <int ACT>
+static __global__ void __launch_bounds__(256) linear_tail_kernel(const float *z, float *y, const float *__restrict__ residual, long rows, long cols, long ldr, bool vec) {
+  pdl_begin();
+  const long stride = gridDim.x * 256l, start = blockIdx.x * 256l + threadIdx.x;
+  if (vec) {
+    const long per = cols / 4, n = rows * per;
+    for (long i = start; i < n; i += stride) {
+      float4 v = reinterpret_cast<const float4 *>(z)[i];
+      v = make_float4(activation<ACT>(v.x), activation<ACT>(v.y), activation<ACT>(v.z), activation<ACT>(v.w));
+      if (residual) {
+        const long r = i / per;
+        const float4 q = __ldg(reinterpret_cast<const float4 *>(residual + r * ldr) + (i - r * per));
+        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+      }
+      reinterpret_cast<float4 *>(y)[i] = v;
+    }
+    return;
+  }
+  const long n = rows * cols;
+  for (long i = start; i < n; i += stride) {
+    float v = activation<ACT>(z[i]);
+    if (residual) {
+      const long r = i / cols;
+      v += residual[r * ldr + (i - r * cols)];
+    }
+    y[i] = v;
+  }
+}
+void linear_product(const float *x, long ldx, long rows, long in, long out, const float *w, const float *b, float *y, const LinearTail &tail) {
+  if (rows <= 0) return;
+  const int mode = ctx().math_mode;
+  const bool aligned = mm::raw_matrix_ok(w, in) && mm::raw_matrix_ok(x, ldx);
+  constexpr long kPart = 1l << 30;   // what the engines count in 32 bits
+  if (mode != 1 && !(mode == 2 && out > 128 && rows > 32) && std::max(std::max(rows, in), out) <= kPart && small_is_faster(out, rows, in, aligned)) {
+    WsScope scope;
+    mm::SmallFused p = {};
+    p.a = mm::small_operand(w, in); p.b = mm::small_operand(x, ldx);
+    p.M = (int)out; p.N = (int)rows; p.K = (int)in;
+    p.c = y; p.sm = 1; p.sn = out;
+    p.alpha = 1.f;
+    p.bias = b; p.bias_m = 1;
+    p.act = tail.act; p.residual = tail.residual; p.rm = 1; p.rn = tail.ldr; p.z = tail.z;
+    mm::launch_small(p, true, true);
+    return;
+  }
+  float *z = tail.z ? tail.z : y;
+  gemm('t', 'n', out, rows, in, 1.f, w, in, x, ldx, 0.f, z, out, b);
+  if (tail.act == kActNone && !tail.residual && z == y) return;
+  const bool vec = out % 4 == 0 && tail.ldr % 4 == 0 && (((uintptr_t)z | (uintptr_t)y | (uintptr_t)tail.residual) & 15) == 0;
+  const long n = rows * out / (vec ? 4 : 1);
+  with_activation(tail.act, [&](auto a) {
+    pdl_launch(linear_tail_kernel<decltype(a)::value>, (unsigned)std::min<long>((n + 255) / 256, ctx().sm_count * 16l), 256, 0, z, y, tail.residual, rows, out, tail.ldr,
+               vec);
+  });
+  check_launch("linear_tail");
 }
 
 // y = beta*y + alpha*op(A)*x.  'n': A is m x n column-major, y has m entries: threads own rows
