@@ -107,6 +107,33 @@ static int choose_tail_splits(long tail, long ktiles, int slots, double tile_us)
 static bool raw_matrix_ok(const float *base, long ld) {
   return encode_tiled_fn() && ((uintptr_t)base & 15) == 0 && ld % 4 == 0 && ld > 0;
 }
+// Up to two matrices copied to pitches that TMA can address (blockIdx.y: which): lines of `run` floats.
+struct PackJob { const float *src; float *dst; long lines, run, src_ld, dst_ld; };
+static __global__ void __launch_bounds__(256) pack_matrix_kernel(const PackJob a, const PackJob b) {
+  pdl_begin();
+  // a warp copies up to 1024 floats of a line, all its loads in flight before the first store
+  const PackJob &j = blockIdx.y ? b : a;
+  const int lane = threadIdx.x & 31;
+  const long warps = (long)gridDim.x * (blockDim.x >> 5), parts = (j.run + 1023) / 1024;
+  for (long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < j.lines * parts; w += warps) {
+    const long l = w / parts, i0 = (w - l * parts) * 1024 + lane;
+    const float *s = j.src + l * j.src_ld;
+    float *d = j.dst + l * j.dst_ld;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = i0 + 32 * i < j.run ? s[i0 + 32 * i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+      if (i0 + 32 * i < j.run) d[i0 + 32 * i] = v[i];
+  }
+}
+
+static void launch_pack(const PackJob &a, const PackJob &b) {
+  const long pieces = std::max(a.lines * ((a.run + 1023) / 1024), b.lines * ((b.run + 1023) / 1024));
+  pdl_launch(pack_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), 2), 256, 0, a, b);
+  check_launch("pack_matrix");
+}
+
 // Element (r, k) of the matrix at base[r * ld + k], or base[k * ld + r] for MN; tile_rows: K-major rows per load.
 static void encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int size, const void *base, bool mn, long rows, long K, long ld, int tile_rows) {
   const cuuint32_t kv = 128 / (cuuint32_t)size;
@@ -119,6 +146,20 @@ static void encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int size, 
   const CUresult r = enc(map, type, 2, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          mn && size == 4 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  THC_CHECK(r == CUDA_SUCCESS, "internal: cuTensorMapEncodeTiled failed");
+}
+// One matrix a group, one behind the other, their lines `ld` apart: `rows` x K as above.
+static void encode_groups(CUtensorMap *map, const float *base, bool mn, long groups, long rows, long K, long ld, int tile_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  const long inner = mn ? rows : K, mid = mn ? K : rows;
+  THC_CHECK(enc && ((uintptr_t)base & 15) == 0 && ld % 4 == 0, "internal: matrices not addressable by TMA");
+  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)mid, (cuuint64_t)groups};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 4, (cuuint64_t)ld * mid * 4};
+  const cuuint32_t box[3] = {32, mn ? 32 : (cuuint32_t)tile_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         mn ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   THC_CHECK(r == CUDA_SUCCESS, "internal: cuTensorMapEncodeTiled failed");
 }
 // kPairs: `ld` is the padded length of a line's halves, whose FP32 form has that pitch.
@@ -292,6 +333,12 @@ static void launch_raw(P p, Attach attach) {
   ctx().products[P::PREC]++;
   if (p.ws) {
     // a few thousand blocks whatever the number of tail tiles: a lone tile cut into many slices gets a block per column
+    if constexpr (P::FUSED) {
+      const long by = std::min<long>(bn2, std::max<long>(32, ceil_div(8l * ctx().sm_count, tail)));
+      pdl_launch(tail_finish_linear_kernel, dim3((unsigned)tail, (unsigned)by), 256, 0, p.ws, p.tail_splits, bn2, p.tail_first, gm, p.M, p.N, p.epi, p.tail);
+      check_launch("tail_finish");
+      return;
+    }
     const bool four = tail * (bn2 / 4) >= 2l * ctx().sm_count;
     const long blocks = ceil_div(8l * ctx().sm_count, tail), by = four ? std::min<long>(bn2 / 4, std::max<long>(16, blocks)) : std::min<long>(bn2, std::max<long>(32, blocks));
     pdl_launch(four ? tail_finish_kernel<4> : tail_finish_kernel<1>, dim3((unsigned)tail, (unsigned)by), 256, 0, p.ws, p.tail_splits, bn2, p.tail_first, gm, p.M, p.N,

@@ -1045,6 +1045,37 @@ static __global__ void __launch_bounds__(256) tail_finish_kernel(const float *__
   }
 }
 
+// The same for a linear layer's epilogue: one column at a time.
+static __global__ void __launch_bounds__(256) tail_finish_linear_kernel(const float *__restrict__ ws, int splits, int bn2, long tail_first, long gm, long M, long N,
+                                                                        Epilogue epi, LinearEpilogue tail) {
+  pdl_begin();
+  const long tile = tail_first + blockIdx.x;
+  const long nt = Epilogue::quotient(tile, gm), mt = tile - nt * gm;
+  const long m = mt * 256 + threadIdx.x;
+  if (m >= M) return;
+  const long mo = epi.moff<false>(m);
+  const float row_b = epi.rb(m);
+  const bool deferred = tail.deferred();
+  const float *base = ws + (long)blockIdx.x * splits * bn2 * 256 + threadIdx.x;
+  for (int c = blockIdx.y; c < bn2; c += gridDim.y) {
+    const long n = nt * bn2 + c;
+    if (n >= N) break;
+    float acc = 0.f;
+#pragma unroll 8
+    for (int z = 0; z < splits; z++) acc += base[((long)z * bn2 + c) * 256];
+    const long o = mo + n * epi.nstride;
+    float v = epi.value(n, acc, row_b, 0.f);
+    if (deferred) {
+      (tail.z ? tail.z : epi.out)[o] = v;
+      continue;
+    }
+    if (tail.z) tail.z[o] = v;
+    with_activation(tail.act, [&](auto act) { v = activation<decltype(act)::value>(v); });
+    if (tail.residual) v += tail.residual[m * tail.rm + n * tail.rn];
+    epi.out[o] = v;
+  }
+}
+
 }  // namespace mm
 }  // namespace thc
 

@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "nn_activation.cuh"
 #include "thc_internal.h"
 
 namespace thc {
@@ -210,6 +211,13 @@ struct RawOperand : TensorMaps<PREC> {
   static constexpr bool MN_MAJOR = MN_, GATHERED = false;
 };
 
+// One matrix of each group, element (r, k) of group e at base[(e * rows + r) * K + k], or base[(e * K + k) * rows + r] for MN: tmap has the groups as
+// its third dimension, so that what lies beyond a group's rows or K reads as zeros and not as the next group's values.
+template <bool MN_, int PREC = kTf32>
+struct GroupOperand : TensorMaps<PREC> {
+  static constexpr bool MN_MAJOR = MN_, GATHERED = false;
+};
+
 // Convolution windows over a channels-last plane [n_img][H][W][C] (C a multiple of KV), as rows (K-major): row = window (img,
 // y, x) of the product's grid, k = (i, j, c).  tmap: im2col map {C, W, H, n_img}, KV channels of 128 consecutive windows at
 // one filter tap per load, padding read as zeros.
@@ -353,6 +361,8 @@ struct Problem {
   typedef OpA_ OpA;
   typedef OpB_ OpB;
   static constexpr bool PAIR = PAIR_;   // pixel-pair epilogue (see Epilogue)
+  static constexpr bool FUSED = false;  // a linear layer's epilogue (LinearEpilogue)
+  static constexpr int GROUPS = 0;      // kGroupRows or kGroupSums (GroupProblem)
   static constexpr int PREC = PREC_;    // operands of the two-SM engine
   static constexpr int KV = PREC_ != kTf32 ? 64 : 32;   // k per tile of the two-SM engine
   // kPairs: the operands' records, and all that decide on the form
@@ -373,6 +383,131 @@ struct Problem {
   long tail_first = 0;
   int tail_splits = 1;
 };
+
+// ---- a linear layer's epilogue -----------------------------------------------------------------------------------------
+// out = act(z) + residual with z the product and its bias, which `z` receives unless null, laid out as the result.  beta == 0.
+// Pairs leave out their operands' strays, which are added to the stored sums afterwards (mm_strays.cuh): where there are any, the product
+// stores z itself, in `z` or else in the result, and linear_tail_kernel finishes it.
+struct LinearEpilogue {
+  int act = kActNone;
+  const float *residual = nullptr;   // at residual[m * rm + n * rn]; may be null
+  long rm = 0, rn = 0;
+  float *z = nullptr;
+  const RangeRec *a = nullptr, *b = nullptr;   // of a product over pairs, with what else decides on the form
+  Ranges ranges;
+  __device__ __forceinline__ bool deferred() const { return a && !ranges.wide() && (a->strays | b->strays); }
+};
+template <class OpA_, class OpB_, int PREC_>
+struct FusedProblem : Problem<OpA_, OpB_, false, PREC_> {
+  static constexpr bool FUSED = true;
+  LinearEpilogue tail;
+};
+
+// ---- groups --------------------------------------------------------------------------------------------------------------
+// Products where the rows of each group meet a matrix of their own, in one launch.  An entry is a piece of a group's rows: a tile of columns of
+// the result (rows [first, end), the tile's width or less), or (kGroupSums) all rows of the group, which are summed over.
+enum : int { kGroupRows = 1, kGroupSums = 2 };
+struct GroupEntry { int group, first, end; };
+constexpr int kGroupEntries = 160;   // that travel with a launch; more of them lie in device memory
+struct GroupList {
+  int count;
+  const GroupEntry *more;            // all of them, or null
+  GroupEntry few[kGroupEntries];
+  __device__ __forceinline__ GroupEntry at(int i) const { return more ? more[i] : few[i]; }
+};
+// For the two-SM engine.  kGroupRows: A is the groups' (GroupOperand), column n of the result is row n of B; the list's pieces are tiles wide.
+// kGroupSums: k is the rows, each entry has a result of its own.  Tiles of an entry: m fastest.
+template <class OpA_, class OpB_, int GROUPS_, bool FUSED_>
+struct GroupProblem : Problem<OpA_, OpB_> {
+  static constexpr int GROUPS = GROUPS_;
+  static constexpr bool FUSED = FUSED_;
+  LinearEpilogue tail;      // (FUSED)
+  long bias_group = 0, out_group = 0;
+  long items;
+  GroupList list;
+};
+// What a drain thread stores by, where a problem is not one product.
+struct ResultView {
+  static constexpr bool PAIR = false;
+  Epilogue epi;
+  long M, N;
+};
+
+// Epilogue of one drain thread with a linear layer's tail.  The tensor pipe waits for it once all accumulators are full.  The activations run in a loop
+// over the columns, kLinearStep at a time in the first registers and all columns moved on by as many: straight-line code for 128 values at some
+// 25 instructions each, 50 KB of it, runs at the pace that instructions arrive from L2 (50 us a 256 x 256 tile).  What is stored is
+// stored in straight lines with one pointer and a constant stride, as in tc2_store_rows.
+constexpr int kLinearStep = 16;
+template <int ACT, int NCOL> __device__ __forceinline__ void tc2_activate(float (&acc)[NCOL]) {
+  if constexpr (ACT == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < NCOL; j++) acc[j] = activation<ACT>(acc[j]);
+  } else if constexpr (ACT != kActNone) {
+#pragma unroll 1
+    for (int i = 0; i < NCOL; i += kLinearStep) {
+      float v[kLinearStep];
+#pragma unroll
+      for (int j = 0; j < kLinearStep; j++) v[j] = activation<ACT>(acc[j]);
+#pragma unroll
+      for (int j = 0; j + kLinearStep < NCOL; j++) acc[j] = acc[j + kLinearStep];
+#pragma unroll
+      for (int j = 0; j < kLinearStep; j++) acc[NCOL - kLinearStep + j] = v[j];
+    }
+  }
+}
+// Columns [0, left) of the row at o, `st` apart.
+template <int NCOL> __device__ __forceinline__ void tc2_put(float *o, long st, int left, const float (&acc)[NCOL]) {
+  if (st == 1 && left >= NCOL && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < NCOL; j += 4) *reinterpret_cast<float4 *>(o + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+  } else if (left >= NCOL) {
+#pragma unroll
+    for (int j = 0; j < NCOL; j++) o[j * st] = acc[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < NCOL; j++)
+      if (j < left) o[j * st] = acc[j];
+  }
+}
+template <class V, int NCOL>
+__device__ __forceinline__ void tc2_store_linear(const V &p, const LinearEpilogue &l, bool deferred, float (&acc)[NCOL], long m, long nb) {
+  const int left = m < p.M ? (int)max(0l, min((long)NCOL, p.N - nb)) : 0;
+  if (left == 0) return;
+  const long st = p.epi.nstride, o = p.epi.template moff<false>(m) + nb * st;
+  if (p.epi.bias) {
+    const float *bias = p.epi.bias + nb;
+#pragma unroll
+    for (int j0 = 0; j0 < NCOL; j0 += 16) {
+      float b[16];
+#pragma unroll
+      for (int j = 0; j < 16; j++) b[j] = j0 + j < left ? __ldg(bias + j0 + j) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
+    }
+  } else {
+    const float row_b = p.epi.rb(m);
+#pragma unroll
+    for (int j = 0; j < NCOL; j++) acc[j] += row_b;
+  }
+  if (deferred || l.z) tc2_put(deferred && !l.z ? p.epi.out + o : l.z + o, st, left, acc);
+  if (deferred) return;
+  if (l.act == kActRelu) tc2_activate<kActRelu>(acc);
+  else if (l.act == kActGelu) tc2_activate<kActGelu>(acc);
+  else if (l.act == kActSilu) tc2_activate<kActSilu>(acc);
+  if (l.residual) {
+    const float *r = l.residual + m * l.rm + nb * l.rn;
+    const long rn = l.rn;
+#pragma unroll
+    for (int j0 = 0; j0 < NCOL; j0 += 16) {
+      float b[16];
+#pragma unroll
+      for (int j = 0; j < 16; j++) b[j] = j0 + j < left ? __ldg(r + (j0 + j) * rn) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
+    }
+  }
+  tc2_put(p.epi.out + o, st, left, acc);
+}
 
 // Epilogue of one drain thread: its row m of the tile, NCOL columns from nb on.
 template <class P, int NCOL>

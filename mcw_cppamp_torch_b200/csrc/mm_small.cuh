@@ -20,7 +20,6 @@
 #include <type_traits>
 
 #include "mm_tc.cuh"
-#include "nn_activation.cuh"
 
 namespace thc {
 namespace mm {
@@ -57,17 +56,6 @@ struct SmallFused : SmallProblem {
 };
 
 // ---- groups ----------------------------------------------------------------------------------------------------------
-// Products where the rows of each group meet a matrix of their own, in one launch.  An entry is a piece of a group's rows: a tile of columns of
-// the result (rows [first, end), the tile's width or less), or (kGroupSums) all rows of the group, which are summed over.
-enum : int { kGroupRows = 0, kGroupSums = 1 };
-struct GroupEntry { int group, first, end; };
-constexpr int kGroupEntries = 160;   // that travel with a launch; more of them lie in device memory
-struct GroupList {
-  int count;
-  const GroupEntry *more;            // all of them, or null
-  GroupEntry few[kGroupEntries];
-  __device__ __forceinline__ GroupEntry at(int i) const { return more ? more[i] : few[i]; }
-};
 // Offsets of a group's, and of a row's, part of the operands and results.
 struct GroupPlaces {
   long a_group, a_row, b_row, c_group, c_row, bias_group;

@@ -71,7 +71,8 @@ constexpr int kGatherAhead = 4;     // tiles on the way to a warp that gathers A
 constexpr int T2R_TMA_WARP = 5;
 constexpr int T2R_MMA_WARP2 = 6;
 
-template <int BN2, int PREC> struct Tc2rCfg {
+// DEEP: four accumulators also for FP32 values where tensor memory has room (see tc2r_deep).
+template <int BN2, int PREC, bool DEEP = false> struct Tc2rCfg {
   static constexpr bool HALF = PREC != kTf32;
   static constexpr int BH = BN2 / 2;
   static constexpr int A_BYTES = TC_BM * 128;
@@ -80,13 +81,16 @@ template <int BN2, int PREC> struct Tc2rCfg {
   static constexpr int LO_SLOTS = HALF ? 0 : 3;
   static constexpr int HI_MAX = (227 * 1024 - 1024 - 512) / SLOT_BYTES - LO_SLOTS;
   static constexpr int HI_SLOTS = HI_MAX > (HALF ? 8 : 6) ? (HALF ? 8 : 6) : HI_MAX;
-  static constexpr int ACCS = HALF && BN2 <= 128 ? 4 : 2;       // accumulator buffers
+  static constexpr int ACCS = (HALF || DEEP) && BN2 <= 128 ? 4 : 2;       // accumulator buffers
   static constexpr int TMEM_COLS = ACCS * BN2 > 256 ? 512 : 256;
   static constexpr int SMEM_BYTES = (HI_SLOTS + LO_SLOTS) * SLOT_BYTES + 512 + 1024;
   static_assert(HI_SLOTS >= LO_SLOTS, "ring sizes");
   static_assert(HALF || HI_SLOTS % 2 == 0 || HI_SLOTS <= LO_SLOTS + 2, "an odd hi ring must not be longer than the lo ring + 2 (parity waits of the two MMA warps)");
 };
 
+// A linear layer's epilogue takes some 2 us for 128 columns (tc2_store_linear), in which the MMAs of the next item run on through as many
+// accumulators as there are.
+template <class P> __host__ __device__ constexpr bool tc2r_deep() { return P::FUSED; }
 // What a launch asks for: one over pairs may have to run as kTf32.
 template <int BN2, int PREC> __host__ __device__ constexpr int tc2r_smem_bytes() {
   constexpr int own = Tc2rCfg<BN2, PREC>::SMEM_BYTES, wide = Tc2rCfg<BN2, kTf32>::SMEM_BYTES;
@@ -142,6 +146,31 @@ struct TileLoader<ROWS, PREC, WIDE, RawOperand<MN, OWN>> {
   }
   __device__ __forceinline__ void next(const RawOperand<MN, OWN> &) { k += KV; }
 };
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, int x, int y, int z, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"((unsigned long long)tmap), "r"(mbar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// The same of a group's matrix.
+template <int ROWS, int PREC, bool WIDE, bool MN, int OWN>
+struct TileLoader<ROWS, PREC, WIDE, GroupOperand<MN, OWN>> {
+  static constexpr int KV = PREC == kTf32 ? 32 : 64;
+  int row, k, group;
+  __device__ __forceinline__ TileLoader(const GroupOperand<MN, OWN> &, long row0, long k0, int g) : row((int)row0), k((int)k0), group(g) {}
+  __device__ __forceinline__ void issue(const GroupOperand<MN, OWN> &op, uint32_t dst, bool lo, uint32_t mbar) const {
+    if constexpr (MN) {
+      static_assert(ROWS % KV == 0, "whole row blocks");
+#pragma unroll
+      for (int a = 0; a < ROWS / KV; a++) tma_load_3d(dst + a * KV * 128, op.map(WIDE), row + KV * a + op.half(lo), k, group, mbar);
+    } else {
+      tma_load_3d(dst, op.map(WIDE), k + op.half(lo), row, group, mbar);
+    }
+  }
+  __device__ __forceinline__ void next(const GroupOperand<MN, OWN> &) { k += KV; }
+};
+template <class L, class Op> __device__ __forceinline__ L make_loader(const Op &op, long row0, long k0, int) { return L(op, row0, k0); }
+template <class L, bool MN, int OWN> __device__ __forceinline__ L make_loader(const GroupOperand<MN, OWN> &op, long row0, long k0, int group) { return L(op, row0, k0, group); }
 // Convolution windows as rows (K-major): one im2col load of KV channels of ROWS = 128 consecutive windows.
 template <int ROWS, int PREC, bool WIDE, int OWN>
 struct TileLoader<ROWS, PREC, WIDE, PlanesWindowOperand<OWN>> {
@@ -247,6 +276,8 @@ struct Tc2rItem {
   long z;      // k slice of a tail tile, -1 for a whole-reduction tile
   long slot;   // partial-sum block of the workspace (tail items only)
   int num_k_tiles;
+  int group, k_left;   // of a grouped product: the group, and the k of this item
+  long n_end;          // the end of this item's columns
 };
 
 // Persistent: the launch has as many clusters as the device runs at once; cluster c starts with item c and takes
@@ -263,7 +294,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
   constexpr int PARTS = PAIRS ? 2 : 1;     // ring slots of a k tile: lo, then hi, which is needed longest
   constexpr int KV = HALF ? 64 : 32;
   constexpr int CHAIN = PAIRS ? 1 : T2R_HALF_CHAIN;
-  typedef Tc2rCfg<BN2, PREC> Cfg;
+  typedef Tc2rCfg<BN2, PREC, tc2r_deep<P>()> Cfg;
   constexpr int R = Cfg::HI_SLOTS, L = Cfg::LO_SLOTS, LM = L > 0 ? L : 1, ACCS = Cfg::ACCS;
   constexpr int BH = Cfg::BH;
   extern __shared__ uint8_t smem_raw[];
@@ -283,11 +314,27 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
   const uint32_t gm = (uint32_t)((p.M + 255) / 256), gn = (uint32_t)((p.N + BN2 - 1) / BN2);
   const uint32_t tiles = gm * gn, tail_first = p.ws ? (uint32_t)p.tail_first : tiles;
   const uint32_t tail_tiles = tiles - tail_first;
-  const uint32_t items = tail_first + tail_tiles * (uint32_t)p.tail_splits, cluster_id = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  uint32_t items = tail_first + tail_tiles * (uint32_t)p.tail_splits;
+  if constexpr (P::GROUPS != 0) items = (uint32_t)p.items;
+  const uint32_t cluster_id = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   // Items 0 .. tail_first - 1 are whole tiles; the rest are the k slices of the tail tiles, slice-major (clusters
   // running side by side then work on neighbouring tiles of one k range and share its B rows in L2).
   auto item_at = [&](uint32_t w) {
     Tc2rItem t;
+    if constexpr (P::GROUPS != 0) {
+      const uint32_t per = P::GROUPS == kGroupRows ? gm : gm * gn, e = w / per, r = w - e * per, nt = r / gm;
+      const GroupEntry g = p.list.at((int)e);
+      t.z = -1;
+      t.group = g.group;
+      t.m_tile0 = (long)(r - nt * gm) * 256;
+      if constexpr (P::GROUPS == kGroupRows) {
+        t.n_tile0 = g.first; t.n_end = g.end; t.k_begin = 0; t.k_left = (int)p.K;
+      } else {
+        t.n_tile0 = (long)nt * BN2; t.n_end = p.N; t.k_begin = g.first; t.k_left = g.end - g.first;
+      }
+      t.num_k_tiles = (t.k_left + KV - 1) / KV;
+      return t;
+    }
     uint32_t tile = w;
     t.z = -1;
     t.k_begin = 0;
@@ -415,7 +462,8 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
       if (!ok) break;
       if (lane == 0) sched.done(n);
       if (w == T2R_NO_ITEM) break;
-      const int nk = item_at(w).num_k_tiles;
+      const Tc2rItem item = item_at(w);
+      const int nk = item.num_k_tiles;
       for (int it = (g0 + grp) & 1; it < nk; it += 2) {
         const int g = g0 + it;
         const int s = g % R, ls = g % LM;
@@ -433,11 +481,25 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         // a quarter of the group's 16-byte chunks per batch: all loads of a batch are in flight before its first store
         constexpr int GT = T2_PRODUCERS / 2, PASSES = Cfg::SLOT_BYTES / (GT * 16), BATCH = PASSES <= 24 ? PASSES / 2 : PASSES / 4;
         static_assert(Cfg::SLOT_BYTES % (GT * 16 * 4) == 0, "slot size");
+        // The rows of the group that end inside this k tile are followed by the next group's: zeros in their place, in both slots.  Both
+        // operands' lines of 128 bytes are k, 32 of them a block.
+        const int k_left = P::GROUPS == kGroupSums ? item.k_left - 32 * it : 32;
 #pragma unroll
         for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
           uint4 v[BATCH];
 #pragma unroll
           for (int i = 0; i < BATCH; i++) v[i] = lds128(src + (uint32_t)((i0 + i) * GT * 16));
+          if constexpr (P::GROUPS == kGroupSums) {
+            static_assert(P::OpA::MN_MAJOR && P::OpB::MN_MAJOR, "lines are k");
+            if (k_left < 32) {
+#pragma unroll
+              for (int i = 0; i < BATCH; i++)
+                if ((((gtid >> 3) + (i0 + i) * (GT / 8)) & 31) >= k_left) {
+                  v[i] = make_uint4(0, 0, 0, 0);
+                  sts128(src + (uint32_t)((i0 + i) * GT * 16), v[i]);
+                }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < BATCH; i++) sts128(dst + (uint32_t)((i0 + i) * GT * 16), tf32_lo4(v[i]));
         }
@@ -523,7 +585,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
       // guarantee and stalls.
       constexpr bool A_MN = P::OpA::MN_MAJOR, B_MN = P::OpB::MN_MAJOR;
       constexpr uint32_t idesc = umma2_idesc_tf32(BN2, A_MN, B_MN);
-      const int buf = warp == T2_MMA_WARP ? 0 : 1;
+      const int mine = warp == T2_MMA_WARP ? 0 : 1;
       int g0 = 0;
       for (uint32_t n = 0; ok; n++) {
         uint32_t w = T2R_NO_ITEM;
@@ -533,10 +595,10 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         if (lane == 0) sched.done(n);
         if (w == T2R_NO_ITEM) break;
         const int nk = item_at(w).num_k_tiles;
-        for (int it = (g0 + buf) & 1; it < nk; it += 2) {
+        for (int it = (g0 + mine) & 1; it < nk; it += 2) {
           const int g = g0 + it;
-          const int s = g % R, ls = g % LM;
-          const uint32_t phase = (uint32_t)(g / R) & 1u, acc_phase = (uint32_t)(g >> 1) & 1u;
+          const int s = g % R, ls = g % LM, buf = ACCS == 2 ? mine : g % ACCS;
+          const uint32_t phase = (uint32_t)(g / R) & 1u, acc_phase = (uint32_t)(g / ACCS) & 1u;
           ok = mbar_wait_spin(bar_acc_empty + 8 * buf, acc_phase ^ 1u, abort_flag, kWaitAccEmpty);
           ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(bar_full + 8 * s, phase, abort_flag, kWaitTileFull));
           if (!ok) break;
@@ -583,7 +645,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         if (w == T2R_NO_ITEM) break;
         if (rank == 0 && lane == 0) mbar_arrive_local(bar_sched_go);   // item n is under way: time to fetch the number of item n + 1
         const Tc2rItem item = item_at(w);
-        TileLoader<TC_BM, PREC, WIDE, typename P::OpA> load_a(p.a, item.m_tile0 + (long)rank * TC_BM, item.k_begin);   // (gathered: nothing)
+        auto load_a = make_loader<TileLoader<TC_BM, PREC, WIDE, typename P::OpA>>(p.a, item.m_tile0 + (long)rank * TC_BM, item.k_begin, item.group);   // (gathered: nothing)
         TileLoader<BH, PREC, WIDE, typename P::OpB> load_b(p.b, item.n_tile0 + (long)rank * BH, item.k_begin);
         for (int t = 0; ok && t < item.num_k_tiles; t++) {
 #pragma unroll
@@ -684,6 +746,17 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
           float *o = p.ws + (item.slot * BN2 + h * NCOL) * 256 + (rank * TC_BM + q * 32 + lane);
 #pragma unroll
           for (int j = 0; j < NCOL; j++) o[j * 256] = acc[j];
+        } else if constexpr (P::GROUPS != 0) {
+          ResultView view{p.epi, p.M, item.n_end};
+          if constexpr (P::GROUPS == kGroupRows) {
+            if (view.epi.row_bias) view.epi.row_bias += item.group * p.bias_group;
+          } else {
+            view.epi.out += item.group * p.out_group;
+          }
+          if constexpr (P::FUSED) tc2_store_linear(view, p.tail, false, acc, m, item.n_tile0 + h * NCOL);
+          else tc2_store_rows<ResultView, NCOL>(view, acc, m, item.n_tile0 + h * NCOL);
+        } else if constexpr (P::FUSED) {
+          tc2_store_linear(p, p.tail, PAIRS && p.tail.deferred(), acc, m, item.n_tile0 + h * NCOL);
         } else if constexpr (P::PAIR && BN2 == 128) {
           if (pair_lines) tc2_store_pair_rows<P>(p, acc, m, h * 32);
           else tc2_store_rows<P, NCOL>(p, acc, m, item.n_tile0 + h * NCOL);

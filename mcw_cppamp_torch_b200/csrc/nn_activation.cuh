@@ -14,29 +14,52 @@ namespace thc {
 enum : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActs = 4 };
 
 #ifdef __CUDACC__
-// P(z) = erfc(-z / sqrt 2) / 2.  For z < 0 the Chebyshev fit of Numerical Recipes (section 6.2, `erfcc`), erfc(a) = t exp(-a^2 + q(t)) with
-// t = 1 / (1 + a / 2), whose relative error is below 1.2e-7 however small erfc is; for z > 0 one minus that of -z.  -a^2 is -z^2 / 2, rounded
-// once with q(t).  No branch and some 20 instructions, which the epilogues below pay for every value (erfcf takes about three
-// times that).
+// P(-a) = erfc(a / sqrt 2) / 2 for a >= 0 by the Chebyshev fit of Numerical Recipes (section 6.2, `erfcc`): erfc(x) = t exp(-x^2 + q(t)) with
+// t = 1 / (1 + x / 2), whose relative error is below 1.2e-7 however small erfc is.  Here in powers of two, with the half in q: its
+// coefficients divided by ln 2, and one less.  The epilogues of the products pay for every instruction 128 times a thread: 15 of them, no branch (erfcf
+// takes some three times that).
+__device__ __forceinline__ float normal_tail(float a) {
+  float t, e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(a, 0.35355339059327376f, 1.f)));
+  float q = 0.246517298f;
+  q = fmaf(t, q, -1.186114945f);
+  q = fmaf(t, q, 2.147474464f);
+  q = fmaf(t, q, -1.637753152f);
+  q = fmaf(t, q, 0.402321582f);
+  q = fmaf(t, q, -0.268756860f);
+  q = fmaf(t, q, 0.139630057f);
+  q = fmaf(t, q, 0.539700616f);
+  q = fmaf(t, q, 1.442729204f);
+  q = fmaf(t, q, -2.825748218f);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(-0.72134752044448170f * a, a, q)));
+  return t * e;
+}
 __device__ __forceinline__ float normal_below(float z) {
-  const float t = __fdividef(1.f, fmaf(fabsf(z), 0.35355339059327376f, 1.f));
-  float q = 0.17087277f;
-  q = fmaf(t, q, -0.82215223f);
-  q = fmaf(t, q, 1.48851587f);
-  q = fmaf(t, q, -1.13520398f);
-  q = fmaf(t, q, 0.27886807f);
-  q = fmaf(t, q, -0.18628806f);
-  q = fmaf(t, q, 0.09678418f);
-  q = fmaf(t, q, 0.37409196f);
-  q = fmaf(t, q, 1.00002368f);
-  q = fmaf(t, q, -1.26551223f);
-  const float p = 0.5f * t * __expf(fmaf(-0.5f * z, z, q));
+  const float p = normal_tail(fabsf(z));
   return z > 0.f ? 1.f - p : p;
+}
+// z P(z) = max(z, 0) - |z| P(-|z|); beyond 30 the second term is zero, and an infinite z would make it none.
+__device__ __forceinline__ float gelu(float z) {
+  const float a = fminf(fabsf(z), 30.f);
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(z), "f"(0.f));
+  return fmaf(-a, normal_tail(a), m);
+}
+// z / (1 + exp(-z)) through e = exp(-|z|), which does not overflow: z / (1 + e), and e times that for z < 0.  The exponent's product with log2 e
+// is taken in two parts, so that e is as exact for large |z| as for small.
+__device__ __forceinline__ float silu(float z) {
+  const float a = fminf(fabsf(z), 128.f), s = a * -1.44269504f;
+  const float rest = fmaf(a, -1.92596303e-8f, fmaf(a, -1.44269504f, -s));
+  float e, t;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(s));
+  e = fmaf(e, rest * 0.69314718f, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(1.f + e));
+  return z * (z < 0.f ? e * t : t);
 }
 template <int ACT> __device__ __forceinline__ float activation(float z) {
   if constexpr (ACT == kActRelu) return z > 0.f ? z : 0.f;
-  else if constexpr (ACT == kActGelu) return z * normal_below(z);
-  else if constexpr (ACT == kActSilu) return z / (1.f + expf(-z));
+  else if constexpr (ACT == kActGelu) return gelu(z);
+  else if constexpr (ACT == kActSilu) return silu(z);
   else return z;
 }
 template <int ACT> __device__ __forceinline__ float activation_slope(float z) {

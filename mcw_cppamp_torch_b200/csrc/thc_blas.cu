@@ -26,34 +26,24 @@ static __global__ void broadcast_rows_kernel(float *c, long m, long n, long ldc,
   const long j = t / m, i = t - j * m;
   c[i + j * ldc] = bias[i];
 }
-// Up to two matrices copied to pitches that TMA can address (blockIdx.y: which): lines of `run` floats.
-struct PackJob { const float *src; float *dst; long lines, run, src_ld, dst_ld; };
-static __global__ void __launch_bounds__(256) pack_matrix_kernel(const PackJob a, const PackJob b) {
-  pdl_begin();
-  // a warp copies up to 1024 floats of a line, all its loads in flight before the first store
-  const PackJob &j = blockIdx.y ? b : a;
-  const int lane = threadIdx.x & 31;
-  const long warps = (long)gridDim.x * (blockDim.x >> 5), parts = (j.run + 1023) / 1024;
-  for (long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < j.lines * parts; w += warps) {
-    const long l = w / parts, i0 = (w - l * parts) * 1024 + lane;
-    const float *s = j.src + l * j.src_ld;
-    float *d = j.dst + l * j.dst_ld;
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = i0 + 32 * i < j.run ? s[i0 + 32 * i] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-      if (i0 + 32 * i < j.run) d[i0 + 32 * i] = v[i];
-  }
-}
-
 // Tensor-core path over the matrices as they lie in memory (raw-operand engine): TMA reads either layout of
 // either operand, so no pass over the operands precedes the product.
-template <bool A_MN, bool B_MN>
-static void gemm_raw_t(const float *a, long lda, const float *b, long ldb, long m, long n, long k, const mm::Epilogue &epi) {
+// The problem of a plain product, or with a linear layer's epilogue, whose operands are K-major.
+template <bool A_MN, bool B_MN, int PREC, bool FUSED> struct MatrixProblem {
+  typedef mm::Problem<mm::RawOperand<A_MN, PREC>, mm::RawOperand<B_MN, PREC>, false, PREC> type;
+};
+template <int PREC> struct MatrixProblem<false, false, PREC, true> {
+  typedef mm::FusedProblem<mm::RawOperand<false, PREC>, mm::RawOperand<false, PREC>, PREC> type;
+};
+template <class P> static void set_tail(P &p, const mm::LinearEpilogue *tail) {
+  if constexpr (P::FUSED) p.tail = *tail;
+}
+template <bool A_MN, bool B_MN, bool FUSED = false>
+static void gemm_raw_t(const float *a, long lda, const float *b, long ldb, long m, long n, long k, const mm::Epilogue &epi, const mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
-  Problem<RawOperand<A_MN>, RawOperand<B_MN>> p;
+  typename MatrixProblem<A_MN, B_MN, kTf32, FUSED>::type p;
   p.epi = epi;
+  set_tail(p, tail);
   p.M = m; p.N = n; p.K = k;
   launch_raw(p, [&](auto &q, int bn2) {
     attach_raw_map<kTf32>(q.a, a, m, k, lda, TC_BM);
@@ -64,9 +54,10 @@ static void gemm_raw_t(const float *a, long lda, const float *b, long ldb, long 
 struct GemmSide { const float *p; long ld; bool along_k; long rows; };
 // Orientation of the 256-row tiles and the epilogue for D(i, j) at c[i + j * ldc]: the first side takes the rows unless it has
 // no more than half a tile of them and the other has more.
-static mm::Epilogue gemm_sides(GemmSide &x, GemmSide &y, float alpha, float beta, float *c, long ldc, const float *row_bias) {
+static mm::Epilogue gemm_sides(GemmSide &x, GemmSide &y, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   if (x.rows <= 128 && y.rows > x.rows) {
     std::swap(x, y);
+    if (tail) std::swap(tail->rm, tail->rn);
     mm::Epilogue e{c, row_bias, alpha, beta, 1, ldc, 1};   // rows of the product are columns of c: out[m * ldc + n]
     return e;
   }
@@ -76,10 +67,12 @@ static mm::Epilogue gemm_sides(GemmSide &x, GemmSide &y, float alpha, float beta
 }
 // BF16 math mode: one K-major BF16 plane per operand, BF16 products.  For results of more than half a tile's rows and more
 // than 32 columns; smaller ones stay FP32-accurate.
-static void gemm_half(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias) {
+template <bool FUSED = false>
+static void gemm_half(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
-  Problem<RawOperand<false, kBf16>, RawOperand<false, kBf16>, false, kBf16> p;
-  p.epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias);
+  typename MatrixProblem<false, false, kBf16, FUSED>::type p;
+  p.epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
+  set_tail(p, tail);
   const HalfMatrix hx = make_half_matrix(x.p, x.along_k ? x.ld : 1, x.along_k ? 1 : x.ld, x.rows, k);
   const HalfMatrix hy = make_half_matrix(y.p, y.along_k ? y.ld : 1, y.along_k ? 1 : y.ld, y.rows, k);
   p.M = x.rows; p.N = y.rows; p.K = hx.ld;
@@ -88,37 +81,38 @@ static void gemm_half(GemmSide x, GemmSide y, long k, float alpha, float beta, f
     attach_raw_map<kBf16>(q.b, hy.p, y.rows, hy.ld, hy.ld, bn2 / 2);
   });
 }
-static void gemm_raw(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias) {
-  const mm::Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias);
+template <bool FUSED = false>
+static void gemm_raw(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
+  const mm::Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
   if (!mm::raw_matrix_ok(x.p, x.ld) || !mm::raw_matrix_ok(y.p, y.ld)) {
     // a pitch or address that TMA cannot take: copy that matrix (a hundredth of the product's time at the sizes that come
     // here) instead of feeding the product through per-thread copies
-    PackJob jobs[2] = {};
+    mm::PackJob jobs[2] = {};
     GemmSide *sides[2] = {&x, &y};
     for (int i = 0; i < 2; i++) {
       GemmSide &s = *sides[i];
       if (mm::raw_matrix_ok(s.p, s.ld)) continue;
-      PackJob &j = jobs[i];
-      j = PackJob{s.p, nullptr, s.along_k ? s.rows : k, s.along_k ? k : s.rows, s.ld, ((s.along_k ? k : s.rows) + 3) / 4 * 4};
+      mm::PackJob &j = jobs[i];
+      j = mm::PackJob{s.p, nullptr, s.along_k ? s.rows : k, s.along_k ? k : s.rows, s.ld, ((s.along_k ? k : s.rows) + 3) / 4 * 4};
       j.dst = (float *)ws_alloc(sizeof(float) * j.lines * j.dst_ld);
       s.p = j.dst; s.ld = j.dst_ld;
     }
-    const long pieces = std::max(jobs[0].lines * ((jobs[0].run + 1023) / 1024), jobs[1].lines * ((jobs[1].run + 1023) / 1024));
-    pdl_launch(pack_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), 2), 256, 0, jobs[0], jobs[1]);
-    check_launch("pack_matrix");
+    mm::launch_pack(jobs[0], jobs[1]);
   }
+  if constexpr (FUSED) { gemm_raw_t<false, false, true>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi, tail); return; }
   if (!x.along_k && y.along_k) gemm_raw_t<true, false>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
   else if (x.along_k && y.along_k) gemm_raw_t<false, false>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
   else if (!x.along_k) gemm_raw_t<true, true>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
   else gemm_raw_t<false, true>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
 }
 // The same over FP16 pairs: a pass measures both operands and one splits them, each as it lies in memory.
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool FUSED = false>
 static void gemm_pairs_t(const void *a, long lda, const void *b, long ldb, long m, long n, long k, const mm::Epilogue &epi,
-                         const mm::Ranges &ranges) {
+                         const mm::Ranges &ranges, const mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
-  Problem<RawOperand<A_MN, kPairs>, RawOperand<B_MN, kPairs>, false, kPairs> p;
+  typename MatrixProblem<A_MN, B_MN, kPairs, FUSED>::type p;
   p.epi = epi;
+  set_tail(p, tail);
   p.M = m; p.N = n; p.K = k;
   p.range_a = ranges.rec[0]; p.range_b = ranges.rec[1]; p.ranges = ranges;
   launch_raw(p, [&](auto &q, int bn2) {
@@ -127,14 +121,15 @@ static void gemm_pairs_t(const void *a, long lda, const void *b, long ldb, long 
   });
 }
 // False: there is no room for the pairs, and nothing has been done.
-static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias) {
+template <bool FUSED = false>
+static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
   // the copies, with a little for the measures (under a hundredth of them) and the partial sums (blocks of 256 KB, up to
   // five rounds of clusters)
   double need = 96e6;
   for (const GemmSide &s : {x, y}) need += 4.1 * (double)(s.along_k ? s.rows : k) * (double)((s.along_k ? k : s.rows) + 64);
   if (!ws_reserve((size_t)need)) return false;
-  const Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias);
+  const Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
   const Measured m[2] = {new_measured(), new_measured()};
   RangeJob ranges[2];
   PairJob jobs[2];
@@ -154,6 +149,15 @@ static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, 
   pdl_launch(split_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), 2), 256, 0, jobs[0], jobs[1]);
   check_launch("split_matrix");
   const Ranges &r = jobs[0].ranges;
+  if constexpr (FUSED) {
+    tail->a = m[0].rec; tail->b = m[1].rec; tail->ranges = r;
+    gemm_pairs_t<false, false, true>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r, tail);
+    Epilogue sums = epi;   // where there are strays the product has left the sums there
+    if (tail->z) sums.out = tail->z;
+    pdl_launch(matrix_strays_kernel, dim3((unsigned)std::min(ceil_div(y.rows, 256), ctx().sm_count), 4), 256, 0, strays[0], strays[1], x.rows, y.rows, sums, r);
+    check_launch("matrix_strays");
+    return true;
+  }
   if (!x.along_k && y.along_k) gemm_pairs_t<true, false>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
   else if (x.along_k && y.along_k) gemm_pairs_t<false, false>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
   else if (!x.along_k) gemm_pairs_t<true, true>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
@@ -246,10 +250,12 @@ void gemm(char transa, char transb, long m, long n, long k, float alpha, const f
     gemm_raw(x, y, k, alpha, beta, c, ldc, row_bias);
 }
 
-// y = act(z) + residual over rows of `cols` values; y may be z.
+// y = act(z) + residual over rows of `cols` values; y may be z.  With records of a product over pairs: only where that has left its sums.
 template <int ACT>
-static __global__ void __launch_bounds__(256) linear_tail_kernel(const float *z, float *y, const float *__restrict__ residual, long rows, long cols, long ldr, bool vec) {
+static __global__ void __launch_bounds__(256) linear_tail_kernel(const float *z, float *y, const float *__restrict__ residual, long rows, long cols, long ldr, bool vec,
+                                                                 const mm::LinearEpilogue product) {
   pdl_begin();
+  if (product.a && !product.deferred()) return;
   const long stride = gridDim.x * 256l, start = blockIdx.x * 256l + threadIdx.x;
   if (vec) {
     const long per = cols / 4, n = rows * per;
@@ -275,33 +281,45 @@ static __global__ void __launch_bounds__(256) linear_tail_kernel(const float *z,
     y[i] = v;
   }
 }
+static void linear_tail(const float *z, float *y, long rows, long out, const LinearTail &tail, const mm::LinearEpilogue &product) {
+  const bool vec = out % 4 == 0 && tail.ldr % 4 == 0 && (((uintptr_t)z | (uintptr_t)y | (uintptr_t)tail.residual) & 15) == 0;
+  const long n = rows * out / (vec ? 4 : 1);
+  with_activation(tail.act, [&](auto a) {
+    pdl_launch(linear_tail_kernel<decltype(a)::value>, (unsigned)std::min<long>((n + 255) / 256, ctx().sm_count * 16l), 256, 0, z, y, tail.residual, rows, out, tail.ldr,
+               vec, product);
+  });
+  check_launch("linear_tail");
+}
 void linear_product(const float *x, long ldx, long rows, long in, long out, const float *w, const float *b, float *y, const LinearTail &tail) {
   if (rows <= 0) return;
+  WsScope scope;
   const int mode = ctx().math_mode;
+  if (mode == 1) {   // the FP32 engine: its result in a pass of its own
+    float *z = tail.z ? tail.z : y;
+    gemm('t', 'n', out, rows, in, 1.f, w, in, x, ldx, 0.f, z, out, b);
+    if (tail.act != kActNone || tail.residual || z != y) linear_tail(z, y, rows, out, tail, {});
+    return;
+  }
   const bool aligned = mm::raw_matrix_ok(w, in) && mm::raw_matrix_ok(x, ldx);
-  constexpr long kPart = 1l << 30;   // what the engines count in 32 bits
-  if (mode != 1 && !(mode == 2 && out > 128 && rows > 32) && std::max(std::max(rows, in), out) <= kPart && small_is_faster(out, rows, in, aligned)) {
-    WsScope scope;
+  const GemmSide ws{w, in, true, out}, xs{x, ldx, true, rows};
+  mm::LinearEpilogue e;
+  e.act = tail.act; e.residual = tail.residual; e.rm = 1; e.rn = tail.ldr; e.z = tail.z;
+  if (mode == 2 && out > 128 && rows > 32) {
+    gemm_half<true>(ws, xs, in, 1.f, 0.f, y, out, b, &e);
+  } else if (small_is_faster(out, rows, in, aligned)) {
     mm::SmallFused p = {};
     p.a = mm::small_operand(w, in); p.b = mm::small_operand(x, ldx);
     p.M = (int)out; p.N = (int)rows; p.K = (int)in;
     p.c = y; p.sm = 1; p.sn = out;
     p.alpha = 1.f;
     p.bias = b; p.bias_m = 1;
-    p.act = tail.act; p.residual = tail.residual; p.rm = 1; p.rn = tail.ldr; p.z = tail.z;
+    p.act = e.act; p.residual = e.residual; p.rm = e.rm; p.rn = e.rn; p.z = e.z;
     mm::launch_small(p, true, true);
-    return;
+  } else if (mode == 0 && pairs_are_faster(out, rows, in) && gemm_pairs<true>(ws, xs, in, 1.f, 0.f, y, out, b, &e)) {
+    linear_tail(e.z ? e.z : y, y, rows, out, tail, e);
+  } else {
+    gemm_raw<true>(ws, xs, in, 1.f, 0.f, y, out, b, &e);
   }
-  float *z = tail.z ? tail.z : y;
-  gemm('t', 'n', out, rows, in, 1.f, w, in, x, ldx, 0.f, z, out, b);
-  if (tail.act == kActNone && !tail.residual && z == y) return;
-  const bool vec = out % 4 == 0 && tail.ldr % 4 == 0 && (((uintptr_t)z | (uintptr_t)y | (uintptr_t)tail.residual) & 15) == 0;
-  const long n = rows * out / (vec ? 4 : 1);
-  with_activation(tail.act, [&](auto a) {
-    pdl_launch(linear_tail_kernel<decltype(a)::value>, (unsigned)std::min<long>((n + 255) / 256, ctx().sm_count * 16l), 256, 0, z, y, tail.residual, rows, out, tail.ldr,
-               vec);
-  });
-  check_launch("linear_tail");
 }
 
 // y = beta*y + alpha*op(A)*x.  'n': A is m x n column-major, y has m entries: threads own rows

@@ -54,17 +54,36 @@ static std::vector<GroupEntry> whole_groups(const Groups &g) {
     if (g.counts[e]) v.push_back(GroupEntry{e, (int)r, (int)(r + g.counts[e])});
   return v;
 }
-// The width of the warp-level engine's tiles that takes the groups' rows in the least time: a tile's cost by width, from the times that
-// small_product_us() goes by.
-static int small_group_width(const Groups &g) {
-  const int widths[4] = {64, 32, 16, 8};
-  const double cost[4] = {2.9, 1.9, 1.2, 1.0};
-  int best = 64;
+// The warp-level engine's time, by small_product_us()'s figures: `features` tiles of 64, times `tiles` along the groups' rows (or the other features), which
+// take `steps` k tiles in all.  A tile's start and end cost as much as three k tiles.
+static double small_groups_us(double features, double tiles, double steps, int bn, bool aligned) {
+  const double blocks = features * tiles / ctx().sm_count, depth = bn == 64 ? 3 : bn == 8 ? 5 : 4, resident = std::min(std::max(blocks, 1.0), depth);
+  const double step = bn == 64 ? 1.35 + 0.4 * resident : bn == 32 ? 1.3 + 0.15 * resident : bn == 16 ? 0.6 + 0.15 * resident : 0.45 + 0.15 * resident;
+  return 5 + (aligned ? 1.0 : 1.3) * step * features * (steps + 3 * tiles) / ctx().sm_count / resident;
+}
+// The two-SM engine's k tile over FP32 values: 16 groups of 512 rows, 1024 -> 4096, 298 / 342 / 336 / 495 us with tiles of 256 / 192 / 128 / 64 columns.
+static double group_tile_us(int width) { return width == 256 ? 1.25 : width == 192 ? 0.91 : width == 128 ? 0.71 : 0.52; }
+static long tiles_of(const Groups &g, long width) {
+  long t = 0;
+  for (int e = 0; e < g.n; e++) t += (g.counts[e] + width - 1) / width;
+  return t;
+}
+struct Choice { bool engine; int width; };
+// For kGroupRows: the engine and the width of its tiles along the rows that finish first.  The two-SM engine takes all tiles round by round, with two k
+// tiles for a tile's epilogue and, where its operands have to be copied, `pack` bytes at 2 TB/s.
+static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, bool tma) {
+  Choice best{false, 64};
   double least = 0;
-  for (int i = 0; i < 4; i++) {
-    double t = 0;
-    for (int e = 0; e < g.n; e++) t += cost[i] * (double)((g.counts[e] + widths[i] - 1) / widths[i]);
-    if (!i || t < least) { best = widths[i]; least = t; }
+  const long ktiles = (K + 31) / 32;
+  for (int w : {64, 32, 16, 8}) {
+    const double n = (double)tiles_of(g, w), us = small_groups_us((double)((features + 63) / 64), n, n * (double)ktiles, w, small_aligned);
+    if (!least || us < least) { best = Choice{false, w}; least = us; }
+  }
+  if (!tma) return best;
+  for (int w : {256, 192, 128, 64}) {
+    const double tiles = (double)((features + 255) / 256) * (double)tiles_of(g, w);
+    const double us = 10 + std::ceil(tiles / (ctx().sm_count / 2)) * (double)(ktiles + 2) * group_tile_us(w) + (pack ? 5 + pack / 2e6 : 0);
+    if (us < least) { best = Choice{true, w}; least = us; }
   }
   return best;
 }
@@ -103,6 +122,61 @@ template <class F> static bool each_group(const Groups &g, F f) {
   return true;
 }
 
+// ---- the two-SM engine ----------------------------------------------------------------------------------------------
+// An operand's lines at a pitch that TMA takes: as they are, or copied.
+struct Lines {
+  const float *p;
+  long lines, run, ld;
+  bool ok() const { return raw_matrix_ok(p, ld); }
+};
+static double pack_bytes(const Lines &a, const Lines &b) {
+  return (a.ok() ? 0 : 8. * (double)a.lines * (double)a.run) + (b.ok() ? 0 : 8. * (double)b.lines * (double)b.run);
+}
+static void pack(Lines &a, Lines &b) {
+  PackJob jobs[2] = {};
+  Lines *l[2] = {&a, &b};
+  bool any = false;
+  for (int i = 0; i < 2; i++) {
+    if (l[i]->ok()) continue;
+    any = true;
+    const long ld = (l[i]->run + 3) / 4 * 4;
+    float *to = (float *)ws_alloc(sizeof(float) * l[i]->lines * ld);
+    jobs[i] = PackJob{l[i]->p, to, l[i]->lines, l[i]->run, l[i]->ld, ld};
+    l[i]->p = to; l[i]->ld = ld;
+  }
+  if (any) launch_pack(jobs[0], jobs[1]);
+}
+template <class P, class Attach>
+static void launch_groups(P p, int bn2, const std::vector<GroupEntry> &entries, long tiles_of_entry, Attach attach) {
+  p.list = make_list(entries.data(), (int)entries.size());
+  p.ws = nullptr; p.k_per_split = 0;
+  p.items = (long)entries.size() * tiles_of_entry;
+  THC_CHECK(p.items < (1l << 31) - 4096, "grouped product with too many tiles for one launch");
+  attach(p, bn2);
+  auto go = [&](auto w) { launch_tc2r_kernel<P, decltype(w)::value>(p, p.items, false); };
+  if (bn2 == 256) go(std::integral_constant<int, 256>());
+  else if (bn2 == 192) go(std::integral_constant<int, 192>());
+  else if (bn2 == 128) go(std::integral_constant<int, 128>());
+  else go(std::integral_constant<int, 64>());
+  ctx().products[kTf32]++;
+}
+
+// D(f, r) = sum_k A[e](f, k) B(r, k): the forward pass (the features are w's rows) and gradInput (its columns, MN).
+template <bool MN, bool FUSED>
+static void engine_rows(const Groups &g, Lines a, Lines b, long features, long K, int width, const Epilogue &epi, long bias_group, const LinearEpilogue &tail) {
+  pack(a, b);
+  GroupProblem<GroupOperand<MN>, RawOperand<false>, kGroupRows, FUSED> p;
+  p.epi = epi;
+  p.M = features; p.N = g.rows; p.K = K;
+  p.bias_group = bias_group;
+  p.tail = tail;
+  launch_groups(p, width, row_tiles(g, width), (features + 255) / 256, [&](auto &q, int bn2) {
+    encode_groups(&q.a.tmap, a.p, MN, g.n, features, K, a.ld, TC_BM);
+    attach_raw_map<kTf32>(q.b, b.p, g.rows, K, b.ld, bn2 / 2);
+  });
+}
+
+// ---- the passes -------------------------------------------------------------------------------------------------------
 void group_forward(const Groups &g, const float *x, long ldx, long in, long out, const float *w, const float *b, float *y, int act, float *z) {
   if (each_group(g, [&](int e, long r, long n) {
         LinearTail tail;
@@ -111,6 +185,17 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
         linear_product(x + r * ldx, ldx, n, in, out, w + e * out * in, b ? b + e * out : nullptr, y + r * out, tail);
       }))
     return;
+  WsScope scope;
+  const Lines ws{w, (long)g.n * out, in, in}, xs{x, g.rows, in, ldx};
+  const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), encode_tiled_fn() != nullptr);
+  if (c.engine) {
+    Epilogue epi{y, nullptr, 1.f, 0.f, LONG_MAX, 0, out};
+    epi.row_bias = b;
+    LinearEpilogue tail;
+    tail.act = act; tail.z = z;
+    engine_rows<false, true>(g, ws, xs, out, in, c.width, epi, out, tail);
+    return;
+  }
   SmallGroups p = {};
   p.a = small_operand(w, in); p.b = small_operand(x, ldx);
   p.M = (int)out; p.N = 0; p.K = (int)in;
@@ -120,11 +205,17 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
   p.act = act; p.z = z;
   p.kind = kGroupRows; p.column_tiles = 1;
   p.at = GroupPlaces{out * in, 0, ldx, 0, out, out};
-  const int bn = small_group_width(g);
-  small_groups(p, row_tiles(g, bn), bn, true, true);
+  small_groups(p, row_tiles(g, c.width), c.width, true, true);
 }
 void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
   if (each_group(g, [&](int e, long r, long n) { gemm('n', 'n', in, n, out, 1.f, w + e * out * in, in, gz + r * ldg, ldg, 0.f, gx + r * in, in); })) return;
+  WsScope scope;
+  const Lines ws{w, (long)g.n * out, in, in}, gs{gz, g.rows, out, ldg};
+  const Choice c = choose_rows(g, in, out, ws.ok() && gs.ok(), pack_bytes(ws, gs), encode_tiled_fn() != nullptr);
+  if (c.engine) {
+    engine_rows<true, false>(g, ws, gs, in, out, c.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, 0, {});
+    return;
+  }
   SmallGroups p = {};
   p.a = small_operand(w, in); p.b = small_operand(gz, ldg);
   p.M = (int)in; p.N = 0; p.K = (int)out;
@@ -132,21 +223,47 @@ void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long 
   p.alpha = 1.f;
   p.kind = kGroupRows; p.column_tiles = 1;
   p.at = GroupPlaces{out * in, 0, ldg, 0, in, 0};
-  const int bn = small_group_width(g);
-  small_groups(p, row_tiles(g, bn), bn, false, true);
+  small_groups(p, row_tiles(g, c.width), c.width, false, true);
 }
 void group_grad_weight(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale) {
   if (each_group(g, [&](int e, long r, long n) { gemm('n', 't', in, out, n, scale, x + r * ldx, ldx, gz + r * ldg, ldg, 1.f, gw + e * out * in, in); })) return;
+  WsScope scope;
+  Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
+  const int bn2 = tc2_tile_width(out), bn = small_tile_width(out);
+  long ktiles = 0, most = 0;
+  std::vector<GroupEntry> entries = whole_groups(g);
+  for (const GroupEntry &e : entries) {
+    const long t = (e.end - e.first + 31) / 32;
+    ktiles += t;
+    most = std::max(most, t);
+  }
+  const double bytes = pack_bytes(xs, gs), tiles = (double)((in + 255) / 256) * (double)((out + bn2 - 1) / bn2);
+  const double engine = 10 + std::max(tiles * (double)(ktiles + 2 * (long)entries.size()) / (ctx().sm_count / 2), (double)(most + 2)) * group_tile_us(bn2) +
+                        (bytes ? 5 + bytes / 2e6 : 0);
+  const double columns = (double)((out + bn - 1) / bn);
+  if (encode_tiled_fn() && engine < small_groups_us((double)((in + 63) / 64), columns * (double)entries.size(), columns * (double)ktiles, bn, xs.ok() && gs.ok())) {
+    pack(xs, gs);
+    // the largest first: the clusters take items as they finish, and short ones level the end
+    std::stable_sort(entries.begin(), entries.end(), [](const GroupEntry &a, const GroupEntry &b) { return a.end - a.first > b.end - b.first; });
+    GroupProblem<RawOperand<true>, RawOperand<true>, kGroupSums, false> p;
+    p.epi = Epilogue{gw, nullptr, scale, 1.f, LONG_MAX, 0, in};
+    p.M = in; p.N = out; p.K = g.rows;
+    p.out_group = out * in;
+    launch_groups(p, bn2, entries, ((in + 255) / 256) * ((out + bn2 - 1) / bn2), [&](auto &q, int) {
+      attach_raw_map<kTf32>(q.a, xs.p, in, g.rows, xs.ld, TC_BM);
+      attach_raw_map<kTf32>(q.b, gs.p, out, g.rows, gs.ld, bn2 / 2);
+    });
+    return;
+  }
   SmallGroups p = {};
   p.a = small_operand(x, ldx); p.b = small_operand(gz, ldg);
   p.M = (int)in; p.N = (int)out; p.K = 0;
   p.c = gw; p.sm = 1; p.sn = in;
   p.alpha = scale; p.beta = 1.f;
   p.kind = kGroupSums;
-  const int bn = small_tile_width(out);
   p.column_tiles = ceil_div(out, bn);
   p.at = GroupPlaces{0, ldx, ldg, out * in, 0, 0};
-  small_groups(p, whole_groups(g), bn, false, false);
+  small_groups(p, entries, bn, false, false);
 }
 
 }  // namespace thc
