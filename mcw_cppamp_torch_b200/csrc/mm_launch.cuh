@@ -405,16 +405,20 @@ inline double small_product_us(long m, long n, long k, bool aligned) {
 // matrix stays in L2 many times over (a 4096 x 1000 one: 12.8 -> 9 us); beyond, the reads of the rows outweigh those
 // of the matrix and the MMA tiles win (8 rows against 4096 x 9216: 43 us, here 53).
 template <class P>
+static void launch_few_rows_kernel(const P &p, int rows, dim3 grid) {
+  const int ra = rows == 1 || (rows > 2 && rows <= 4) ? 4 : 8;
+  int groups = 8;   // sets of rows per block: as many as leave two blocks per SM, since they share the few rows
+  while (groups > 1 && ceil_div(p.M, ra * groups) * (long)grid.y < 2 * ctx().sm_count) groups /= 2;
+  grid.x = (unsigned)ceil_div(p.M, ra * groups);
+  if (rows == 1) pdl_launch(few_rows_kernel<1, 4, 2, P>, grid, 256, 0, p, groups);
+  else if (rows == 2) pdl_launch(few_rows_kernel<2, 8, 2, P>, grid, 256, 0, p, groups);
+  else if (rows <= 4) pdl_launch(few_rows_kernel<4, 4, 3, P>, grid, 256, 0, p, groups);
+  else pdl_launch(few_rows_kernel<8, 8, 1, P>, grid, 256, 0, p, groups);
+}
+template <class P>
 static bool launch_few_rows(const P &p, bool a_k, bool b_k) {
   if (!(a_k && b_k && p.a.vec4 && p.b.vec4 && p.K % 4 == 0 && p.K <= 1 << 30 && p.N <= 8 && (p.N <= 4 || (long)p.M * p.K <= 1l << 23))) return false;
-  const int ra = p.N == 1 || (p.N > 2 && p.N <= 4) ? 4 : 8;
-  int groups = 8;   // sets of rows per block: as many as leave two blocks per SM, since they share the few rows
-  while (groups > 1 && ceil_div(p.M, ra * groups) < 2 * ctx().sm_count) groups /= 2;
-  const unsigned blocks = (unsigned)ceil_div(p.M, ra * groups);
-  if (p.N == 1) pdl_launch(few_rows_kernel<1, 4, 2, P>, blocks, 256, 0, p, groups);
-  else if (p.N == 2) pdl_launch(few_rows_kernel<2, 8, 2, P>, blocks, 256, 0, p, groups);
-  else if (p.N <= 4) pdl_launch(few_rows_kernel<4, 4, 3, P>, blocks, 256, 0, p, groups);
-  else pdl_launch(few_rows_kernel<8, 8, 1, P>, blocks, 256, 0, p, groups);
+  launch_few_rows_kernel(p, p.N, dim3(1));
   check_launch("few_rows");
   return true;
 }

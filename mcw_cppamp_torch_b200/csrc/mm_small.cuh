@@ -437,8 +437,10 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant
 // 4096 -> 1000 (16 MB, which then stays in L2) 12.5 -> 6.5; 512 -> 512 5.0 -> 3.3.  With the matrix in DRAM: 32, 18 (4096 -> 4096) and
 // 11 us, i.e. 4.7, 3.7 and 1.5 TB/s: the shorter the launch, the more of it is its start.
 template <int R, int RA, int UNROLL, class P = SmallProblem>
-__global__ void __launch_bounds__(256) few_rows_kernel(const P p, int groups) {
+__global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ P whole, int groups) {
   pdl_begin();
+  int column = 0, k_tiles = 0;
+  const auto &p = whole.at_block(column, k_tiles);
   __shared__ float part[8][RA * R];
   const int stalled = *reinterpret_cast<const volatile int *>(p.stalled);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -88,6 +88,21 @@ static Choice choose_rows(const Groups &g, long features, long K, bool small_ali
   return best;
 }
 
+// A handful of rows in each group, K-major operands in whole 16-byte pieces: the weights' bytes are the bound (few_rows_kernel).
+static bool few_rows_groups(SmallGroups p, const Groups &g) {
+  if (!p.a.vec4 || !p.b.vec4 || p.K % 4) return false;
+  long most = 0;
+  for (int e = 0; e < g.n; e++) most = std::max(most, g.counts[e]);
+  if (most > 4) return false;
+  const std::vector<GroupEntry> entries = row_tiles(g, 4);
+  for (size_t i = 0; i < entries.size(); i += 65535) {
+    p.list = make_list(entries.data() + i, (int)std::min(entries.size() - i, (size_t)65535));
+    p.stalled = stall_ctl().dev_flag;
+    launch_few_rows_kernel(p, (int)most, dim3(1, (unsigned)p.list.count));
+    check_launch("few_rows");
+  }
+  return true;
+}
 // The warp-level engine over the groups: any size, pitch and alignment.
 static void small_groups(SmallGroups p, const std::vector<GroupEntry> &entries, int bn, bool a_k, bool b_k) {
   p.stalled = stall_ctl().dev_flag;
@@ -186,6 +201,16 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
       }))
     return;
   WsScope scope;
+  SmallGroups p = {};
+  p.a = small_operand(w, in); p.b = small_operand(x, ldx);
+  p.M = (int)out; p.N = 0; p.K = (int)in;
+  p.c = y; p.sm = 1; p.sn = out;
+  p.alpha = 1.f;
+  p.bias = b; p.bias_m = 1;
+  p.act = act; p.z = z;
+  p.kind = kGroupRows; p.column_tiles = 1;
+  p.at = GroupPlaces{out * in, 0, ldx, 0, out, out};
+  if (few_rows_groups(p, g)) return;
   const Lines ws{w, (long)g.n * out, in, in}, xs{x, g.rows, in, ldx};
   const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), encode_tiled_fn() != nullptr);
   if (c.engine) {
@@ -196,15 +221,6 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
     engine_rows<false, true>(g, ws, xs, out, in, c.width, epi, out, tail);
     return;
   }
-  SmallGroups p = {};
-  p.a = small_operand(w, in); p.b = small_operand(x, ldx);
-  p.M = (int)out; p.N = 0; p.K = (int)in;
-  p.c = y; p.sm = 1; p.sn = out;
-  p.alpha = 1.f;
-  p.bias = b; p.bias_m = 1;
-  p.act = act; p.z = z;
-  p.kind = kGroupRows; p.column_tiles = 1;
-  p.at = GroupPlaces{out * in, 0, ldx, 0, out, out};
   small_groups(p, row_tiles(g, c.width), c.width, true, true);
 }
 void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
