@@ -3,9 +3,9 @@
 //   mean = sum x / D,  var = sum (x - mean)^2 / D,  inv = 1 / sqrt(var + eps),  u = (x - mean) inv,  y = u w + b
 //   dx = inv (g w - mean(g w) - u mean(g w u)),  dw += scale sum_rows g u,  db += scale sum_rows g
 //
-// The least traffic is 8 bytes a value forward and 12 backward: everything here is bound by HBM.  So a row is read once and stays in
-// registers, whatever its length up to 65536 values: a warp has the rows of up to 512, a block those of up to 8192, and a cluster of two,
-// four or eight blocks the longer ones, each block a slice, whose sums meet through distributed shared memory.
+// The least traffic is 8 bytes a value forward and 12 backward: everything here is bound by HBM.  So rows of up to 8192 values are read once and
+// stay in registers, those of up to 512 in a warp's, the others in a block's.  Longer ones are cut into pieces: a launch sums over the pieces of all
+// rows and a second one, which reads them again (from L2 where they fit), joins a row's sums and finishes it.
 // The variance is taken around the mean, not as a difference of two sums: rows whose mean is large against their spread keep their bits.
 // With s1 = sum (x - m) left over from the rounding of m, mean = m + s1 / D and var = sum (x - m)^2 / D - (s1 / D)^2.
 #include <type_traits>
@@ -16,7 +16,7 @@
 namespace thc {
 
 // ---- rows in registers ------------------------------------------------------------------------------------------------
-// The share of a thread in a row (or a block's slice of one): 4 V of the T threads' 4 V T values, in 16-byte pieces where lengths and addresses
+// The share of a thread in a row (or a piece of one): 4 V of the T threads' 4 V T values, in 16-byte pieces where lengths and addresses
 // allow it (VEC), else T apart.
 template <int T, int V, bool VEC> struct Share {
   float v[4 * V];
@@ -84,50 +84,9 @@ template <int T> struct RowSums {
   }
 };
 
-constexpr int kMostBlocks = 8;   // of a cluster
-__device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ unsigned cluster_blocks() { unsigned n; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n)); return n; }
-// Every block of the cluster gets every block's two values, in the order of their ranks.  Two sets of places in turn: a block writes into one only
-// after the barrier of the other, which all have come to with the first one read.
-struct ClusterValues {
-  float2 (*sm)[kMostBlocks];
-  int turn = 0;
-  // Before the first exchange: a block may write into another's shared memory once that has started.
-  static __device__ __forceinline__ void begin() {
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-  }
-  __device__ __forceinline__ const float2 *exchange(float2 mine, unsigned rank, unsigned blocks) {
-    float2 *s = sm[turn];
-    turn ^= 1;
-    if (threadIdx.x < blocks) {
-      unsigned there;
-      const unsigned here = (unsigned)__cvta_generic_to_shared(s + rank);
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(threadIdx.x));
-      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(mine.x), "f"(mine.y) : "memory");
-    }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    return s;
-  }
-};
-// Forward.  A row by T threads of this block (BLOCK / T rows a block), or by all threads of a cluster's blocks.
-template <int T, int V, bool VEC, bool CLUSTER>
-static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_forward_kernel(const float *__restrict__ x, float *__restrict__ y, const float *__restrict__ w,
-                                                                              const float *__restrict__ b, float *mean, float *inv, long rows, int D, int slice,
-                                                                              float eps) {
-  pdl_begin();
-  constexpr int BLOCK = T < 128 ? 256 : T;
-  __shared__ float2 sm[2 * (BLOCK / 32)];
-  __shared__ float2 shared_values[2][kMostBlocks];
-  const int t = threadIdx.x % T;
-  const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_blocks() : 1;
-  const int first = (int)rank * slice, n = min(slice, D - first);
-  const long row = CLUSTER ? blockIdx.x / blocks : blockIdx.x * (long)(BLOCK / T) + threadIdx.x / T;
-  if (T == 32 && row >= rows) return;
-  RowSums<T> sums{sm};
-  Share<T, V, VEC> a;
-  a.template load<true>(x + row * D + first, t, n);
-  if constexpr (CLUSTER) ClusterValues::begin();
+// The row's sums of the block's (or warp's) values: mean = base + off, and the sum of the squares around it.
+struct RowStats { float base, off, square; };
+template <int T, int V, bool VEC> __device__ __forceinline__ RowStats row_stats(const Share<T, V, VEC> &a, RowSums<T> &sums, int t, int n) {
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < 4 * V; j++) s += a.v[j];
@@ -141,69 +100,71 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_forward_kernel(
     q.y = fmaf(c, c, q.y);
   }
   q = sums(q);
-  float base = m0, off = q.x / (float)n, square = fmaf(-off, q.x, q.y);   // mean = base + off; square: sum (x - mean)^2
-  if constexpr (CLUSTER) {
-    // of the slices' means m and squares q: mean = m_0 + sum n (m - m_0) / D, square = sum q + n (m - mean)^2
-    ClusterValues values{shared_values};
-    const float2 *all = values.exchange(make_float2(m0 + off, square), rank, blocks);
-    base = all[0].x;
-    float d = 0.f;
-    for (unsigned k = 1; k < blocks; k++) d = fmaf((float)min(slice, D - (int)k * slice), all[k].x - base, d);
-    off = d / (float)D;
-    square = 0.f;
-    for (unsigned k = 0; k < blocks; k++) {
-      const float e = (all[k].x - base) - off;
-      square += fmaf((float)min(slice, D - (int)k * slice) * e, e, all[k].y);
-    }
-  }
-  const float i = 1.f / sqrtf(square / (float)D + eps);
-  if (mean && rank == 0 && t == 0) { mean[row] = base + off; inv[row] = i; }
+  const float off = q.x / (float)n;
+  return RowStats{m0, off, fmaf(-off, q.x, q.y)};
+}
+// y = u w + b over a share, in place of x
+template <int T, int V, bool VEC>
+__device__ __forceinline__ void apply_norm(Share<T, V, VEC> &a, const RowStats &s, float inv, const float *w, const float *b, int t, int n) {
   if (w) {
-    Share<T, V, VEC> p;
-    p.template load<false>(w + first, t, n);
+    Share<T, V, VEC> p, c;
+    p.template load<false>(w, t, n);
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) p.v[j] *= i;      // (u w = (x - mean) (inv w))
-    Share<T, V, VEC> c;
-    c.template load<false>(b + first, t, n);
+    for (int j = 0; j < 4 * V; j++) p.v[j] *= inv;      // (u w = (x - mean) (inv w))
+    c.template load<false>(b, t, n);
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) a.v[j] = fmaf((a.v[j] - base) - off, p.v[j], c.v[j]);
+    for (int j = 0; j < 4 * V; j++) a.v[j] = fmaf((a.v[j] - s.base) - s.off, p.v[j], c.v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) a.v[j] = ((a.v[j] - base) - off) * i;
+    for (int j = 0; j < 4 * V; j++) a.v[j] = ((a.v[j] - s.base) - s.off) * inv;
   }
-  a.store(y + row * D + first, t, n);
 }
 
-// Backward.  The blocks stay, each with the rows team, team + teams, ... (a team: T threads, or a cluster), the next row on its way while one is
-// worked on, and with the sums of its columns for the weight's and the bias's gradient in registers, which part[block or cluster][2][D] gets.
-// gx or part may be null.
-template <int T, int V, bool VEC, bool CLUSTER>
+// Forward.  A row by T threads (BLOCK / T rows a block).
+template <int T, int V, bool VEC>
+static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_forward_kernel(const float *__restrict__ x, float *__restrict__ y, const float *__restrict__ w,
+                                                                              const float *__restrict__ b, float *mean, float *inv, long rows, int D, float eps) {
+  pdl_begin();
+  constexpr int BLOCK = T < 128 ? 256 : T;
+  __shared__ float2 sm[2 * (BLOCK / 32)];
+  const int t = threadIdx.x % T;
+  const long row = blockIdx.x * (long)(BLOCK / T) + threadIdx.x / T;
+  if (T == 32 && row >= rows) return;
+  RowSums<T> sums{sm};
+  Share<T, V, VEC> a;
+  a.template load<true>(x + row * D, t, D);
+  const RowStats s = row_stats(a, sums, t, D);
+  const float i = 1.f / sqrtf(s.square / (float)D + eps);
+  if (mean && t == 0) { mean[row] = s.base + s.off; inv[row] = i; }
+  apply_norm(a, s, i, w, b, t, D);
+  a.store(y + row * D, t, D);
+}
+
+// Backward.  The blocks stay, each with the rows team, team + teams, ... (a team: T threads), the next row on its way while one is worked on, and
+// with the sums of its columns for the weight's and the bias's gradient in registers, which part[block][2][D] gets.  gx or part may be null.
+// 16384 x 4096: 119 us, 6.7 TB/s.
+template <int T, int V, bool VEC>
 static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) norm_backward_kernel(const float *__restrict__ x, const float *__restrict__ g, float *__restrict__ gx,
                                                                                const float *__restrict__ w, const float *__restrict__ mean,
-                                                                               const float *__restrict__ inv, long rows, int D, int slice, float *part) {
+                                                                               const float *__restrict__ inv, long rows, int D, float *part) {
   pdl_begin();
   constexpr int BLOCK = T < 128 ? 256 : T, TEAMS = BLOCK / T;
   __shared__ float2 sm[2 * (BLOCK / 32)];
-  __shared__ float2 shared_values[2][kMostBlocks];
   const int t = threadIdx.x % T;
-  const unsigned rank = CLUSTER ? cluster_rank() : 0, blocks = CLUSTER ? cluster_blocks() : 1;
-  const int first = (int)rank * slice, n = min(slice, D - first);
-  const long team = CLUSTER ? blockIdx.x / blocks : blockIdx.x * (long)TEAMS + threadIdx.x / T, teams = CLUSTER ? gridDim.x / blocks : gridDim.x * (long)TEAMS;
+  const long team = blockIdx.x * (long)TEAMS + threadIdx.x / T, teams = gridDim.x * (long)TEAMS;
   RowSums<T> sums{sm};
-  ClusterValues values{shared_values};
   float gw[4 * V], gb[4 * V];
 #pragma unroll
   for (int j = 0; j < 4 * V; j++) gw[j] = gb[j] = 0.f;
   Share<T, V, VEC> xn, gn;
   float mn = 0.f, in = 0.f;
   auto fetch = [&](long r) {
-    xn.template load<true>(x + r * D + first, t, n);
-    gn.template load<true>(g + r * D + first, t, n);
+    xn.template load<true>(x + r * D, t, D);
+    gn.template load<true>(g + r * D, t, D);
     mn = __ldg(mean + r);
     in = __ldg(inv + r);
   };
   if (team < rows) fetch(team);
-  if constexpr (CLUSTER) ClusterValues::begin();
   for (long r = team; r < rows; r += teams) {
     Share<T, V, VEC> a = xn, c = gn;
     const float m = mn, i = in;
@@ -211,14 +172,14 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) nor
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) {
-      a.v[j] = a.in(j, t, n) ? (a.v[j] - m) * i : 0.f;
+      a.v[j] = a.in(j, t, D) ? (a.v[j] - m) * i : 0.f;
       gw[j] = fmaf(c.v[j], a.v[j], gw[j]);
       gb[j] += c.v[j];
     }
     if (!gx) continue;
     if (w) {
       Share<T, V, VEC> p;
-      p.template load<false>(w + first, t, n);
+      p.template load<false>(w, t, D);
 #pragma unroll
       for (int j = 0; j < 4 * V; j++) c.v[j] *= p.v[j];
     }
@@ -228,15 +189,10 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) nor
       s.y = fmaf(c.v[j], a.v[j], s.y);
     }
     s = sums(s);
-    if constexpr (CLUSTER) {
-      const float2 *all = values.exchange(s, rank, blocks);
-      s = all[0];
-      for (unsigned k = 1; k < blocks; k++) { s.x += all[k].x; s.y += all[k].y; }
-    }
     const float one = s.x / (float)D, two = s.y / (float)D;
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) a.v[j] = i * (c.v[j] - one - a.v[j] * two);
-    a.store(gx + r * D + first, t, n);
+    a.store(gx + r * D, t, D);
   }
   if (!part) return;
   if constexpr (TEAMS > 1) {   // the block's warps one after the other
@@ -261,101 +217,164 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) nor
     Share<T, V, VEC> o;
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) o.v[j] = gw[j];
-    o.store(part + 2 * team * D + first, t, n);
+    o.store(part + 2 * team * D, t, D);
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) o.v[j] = gb[j];
-    o.store(part + (2 * team + 1) * D + first, t, n);
+    o.store(part + (2 * team + 1) * D, t, D);
   }
 }
 
-// ---- rows of more than 65536 values -----------------------------------------------------------------------------------
-// Two sums over a block; every thread gets both.
-static __device__ __forceinline__ float2 block_sum2(float2 v, float2 *sm) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sm[0];
-  for (int i = 1; i < (int)(blockDim.x >> 5); i++) { v.x += sm[i].x; v.y += sm[i].y; }
-  __syncthreads();
-  return v;
-}
-
-// Rows of any length, a block each, from memory three times.
-static __global__ void __launch_bounds__(256) norm_rows_kernel(const float *__restrict__ x, float *y, const float *__restrict__ w, const float *__restrict__ b,
-                                                               float *mean, float *inv, long rows, long D, float eps) {
+// ---- rows cut into pieces ---------------------------------------------------------------------------------------------
+// 256 threads, up to 16 values each.  Block (a, b) has piece a of row b, b + gridDim.y, ...
+constexpr int kPiece = 4096;
+// part[row][piece] = mean and sum of squares around it
+template <bool VEC>
+static __global__ void __launch_bounds__(256) norm_pieces_kernel(const float *__restrict__ x, long rows, long D, float2 *part) {
   pdl_begin();
-  __shared__ float2 sm[8];
-  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float *xr = x + r * D;
-    float2 s = make_float2(0.f, 0.f);
-    for (long d = threadIdx.x; d < D; d += 256) s.x += xr[d];
-    const float m0 = block_sum2(s, sm).x / (float)D;
-    s = make_float2(0.f, 0.f);
-    for (long d = threadIdx.x; d < D; d += 256) {
-      const float c = xr[d] - m0;
-      s.x += c;
-      s.y = fmaf(c, c, s.y);
-    }
-    s = block_sum2(s, sm);
-    const float off = s.x / (float)D, m = m0 + off, i = 1.f / sqrtf(fmaf(-off, off, s.y / (float)D) + eps);
-    if (threadIdx.x == 0 && mean) { mean[r] = m; inv[r] = i; }
-    for (long d = threadIdx.x; d < D; d += 256) {
-      const float u = (xr[d] - m) * i;
-      y[r * D + d] = w ? fmaf(u, w[d], b[d]) : u;
-    }
+  __shared__ float2 sm[2 * 8];
+  RowSums<256> sums{sm};
+  const long c0 = blockIdx.x * (long)kPiece;
+  const int n = (int)min((long)kPiece, D - c0), t = threadIdx.x;
+  for (long r = blockIdx.y; r < rows; r += gridDim.y) {
+    Share<256, 4, VEC> a;
+    a.template load<true>(x + r * D + c0, t, n);
+    const RowStats s = row_stats(a, sums, t, n);
+    if (t == 0) part[r * gridDim.x + blockIdx.x] = make_float2(s.base + s.off, s.square);
   }
 }
-static __global__ void __launch_bounds__(256) norm_rows_grad_kernel(const float *__restrict__ x, const float *__restrict__ g, float *gx, const float *__restrict__ w,
-                                                                    const float *__restrict__ mean, const float *__restrict__ inv, long rows, long D) {
+// The row's mean and squares from its pieces': mean = m_0 + sum n (m - m_0) / D, squares = sum q + n (m - mean)^2, by the threads of a block.
+static __device__ __forceinline__ RowStats join_pieces(const float2 *part, int pieces, long D, RowSums<256> &sums) {
+  auto size = [&](int k) { return (float)min((long)kPiece, D - k * (long)kPiece); };
+  const float base = part[0].x;
+  float2 s = make_float2(0.f, 0.f);
+  for (int k = threadIdx.x; k < pieces; k += 256) s.x = fmaf(size(k), part[k].x - base, s.x);
+  const float off = sums(s).x / (float)D;
+  s = make_float2(0.f, 0.f);
+  for (int k = threadIdx.x; k < pieces; k += 256) {
+    const float e = (part[k].x - base) - off;
+    s.x += fmaf(size(k) * e, e, part[k].y);
+  }
+  return RowStats{base, off, sums(s).x};
+}
+template <bool VEC>
+static __global__ void __launch_bounds__(256) norm_apply_kernel(const float *__restrict__ x, float *__restrict__ y, const float *__restrict__ w,
+                                                                const float *__restrict__ b, float *mean, float *inv, long rows, long D, float eps,
+                                                                const float2 *__restrict__ part) {
   pdl_begin();
-  __shared__ float2 sm[8];
-  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float *xr = x + r * D, *gr = g + r * D;
+  __shared__ float2 sm[2 * 8];
+  RowSums<256> sums{sm};
+  const long c0 = blockIdx.x * (long)kPiece;
+  const int n = (int)min((long)kPiece, D - c0), t = threadIdx.x;
+  for (long r = blockIdx.y; r < rows; r += gridDim.y) {
+    Share<256, 4, VEC> a;
+    a.template load<true>(x + r * D + c0, t, n);
+    const RowStats s = join_pieces(part + r * gridDim.x, gridDim.x, D, sums);
+    const float i = 1.f / sqrtf(s.square / (float)D + eps);
+    if (mean && blockIdx.x == 0 && t == 0) { mean[r] = s.base + s.off; inv[r] = i; }
+    apply_norm(a, s, i, w ? w + c0 : nullptr, b ? b + c0 : nullptr, t, n);
+    a.store(y + r * D + c0, t, n);
+  }
+}
+// part[row][piece] = sums of g w and of g w u
+template <bool VEC>
+static __global__ void __launch_bounds__(256) norm_piece_sums_kernel(const float *__restrict__ x, const float *__restrict__ g, const float *__restrict__ w,
+                                                                     const float *__restrict__ mean, const float *__restrict__ inv, long rows, long D,
+                                                                     float2 *part) {
+  pdl_begin();
+  __shared__ float2 sm[2 * 8];
+  RowSums<256> sums{sm};
+  const long c0 = blockIdx.x * (long)kPiece;
+  const int n = (int)min((long)kPiece, D - c0), t = threadIdx.x;
+  for (long r = blockIdx.y; r < rows; r += gridDim.y) {
+    Share<256, 4, VEC> a, c;
+    a.template load<true>(x + r * D + c0, t, n);
+    c.template load<true>(g + r * D + c0, t, n);
     const float m = mean[r], i = inv[r];
+    if (w) {
+      Share<256, 4, VEC> p;
+      p.template load<false>(w + c0, t, n);
+#pragma unroll
+      for (int j = 0; j < 16; j++) c.v[j] *= p.v[j];
+    }
     float2 s = make_float2(0.f, 0.f);
-    for (long d = threadIdx.x; d < D; d += 256) {
-      const float gw = w ? gr[d] * w[d] : gr[d];
-      s.x += gw;
-      s.y = fmaf(gw, (xr[d] - m) * i, s.y);
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      if (!a.in(j, t, n)) continue;
+      s.x += c.v[j];
+      s.y = fmaf(c.v[j], (a.v[j] - m) * i, s.y);
     }
-    s = block_sum2(s, sm);
-    const float a = s.x / (float)D, c = s.y / (float)D;
-    for (long d = threadIdx.x; d < D; d += 256) {
-      const float gw = w ? gr[d] * w[d] : gr[d], u = (xr[d] - m) * i;
-      gx[r * D + d] = i * (gw - a - u * c);
-    }
+    s = sums(s);
+    if (t == 0) part[r * gridDim.x + blockIdx.x] = s;
   }
 }
-// Sums over a part of the rows (blockIdx.y) of 32 columns: part[blockIdx.y][2][D].
-static __global__ void __launch_bounds__(256) norm_columns_kernel(const float *__restrict__ x, const float *__restrict__ g, const float *__restrict__ mean,
-                                                                  const float *__restrict__ inv, long rows, long D, long per, float *part) {
+// The gradients of 1024 columns (blockIdx.x) over the rows [per * blockIdx.y, + per): gx, and the columns' sums in columns[blockIdx.y][2][D].
+// No thread waits for another: four rows are on the way.  The rows' sums over their pieces come first, kRowSums rows at a time.
+constexpr int kRowSums = 64;
+template <bool VEC>
+static __global__ void __launch_bounds__(256) norm_columns_kernel(const float *__restrict__ x, const float *__restrict__ g, float *__restrict__ gx,
+                                                                  const float *__restrict__ w, const float *__restrict__ mean, const float *__restrict__ inv,
+                                                                  long rows, long D, long per, const float2 *__restrict__ part, int pieces, float *columns) {
   pdl_begin();
-  __shared__ float2 sm[8][32];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long end = min(rows, (blockIdx.y + 1) * per);
-  for (long d0 = blockIdx.x * 32l; d0 < D; d0 += gridDim.x * 32l) {
-    const long d = d0 + tx;
-    float2 s = make_float2(0.f, 0.f);
-    if (d < D)
-      for (long r = blockIdx.y * per + ty; r < end; r += 8) {
-        const float gv = g[r * D + d];
-        s.x = fmaf(gv, (x[r * D + d] - mean[r]) * inv[r], s.x);
-        s.y += gv;
-      }
-    sm[ty][tx] = s;
+  __shared__ float4 row_sums[kRowSums];   // mean, inv, mean of g w, mean of g w u
+  const long c0 = blockIdx.x * 1024l, end = min(rows, (blockIdx.y + 1) * per);
+  const int n = (int)min(1024l, D - c0), t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  float gw[4] = {0.f, 0.f, 0.f, 0.f}, gb[4] = {0.f, 0.f, 0.f, 0.f};
+  Share<256, 1, VEC> p;
+#pragma unroll
+  for (int j = 0; j < 4; j++) p.v[j] = 1.f;
+  if (w) p.template load<false>(w + c0, t, n);
+  for (long r0 = blockIdx.y * per; r0 < end; r0 += kRowSums) {
+    const int some = (int)min((long)kRowSums, end - r0);
     __syncthreads();
-    if (ty == 0 && d < D) {
-      for (int i = 1; i < 8; i++) { s.x += sm[i][tx].x; s.y += sm[i][tx].y; }
-      part[(2l * blockIdx.y) * D + d] = s.x;
-      part[(2l * blockIdx.y + 1) * D + d] = s.y;
+    for (int k = warp; k < some; k += 8) {
+      float2 s = make_float2(0.f, 0.f);
+      if (gx)
+        for (int q = lane; q < pieces; q += 32) {
+          const float2 v = part[(r0 + k) * pieces + q];
+          s.x += v.x; s.y += v.y;
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+        s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+      }
+      if (lane == 0) row_sums[k] = make_float4(mean[r0 + k], inv[r0 + k], s.x / (float)D, s.y / (float)D);
     }
     __syncthreads();
+    constexpr int U = 4;
+    for (int k0 = 0; k0 < some; k0 += U) {
+      Share<256, 1, VEC> a[U], c[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (k0 + u < some) {
+          a[u].template load<true>(x + (r0 + k0 + u) * D + c0, t, n);
+          c[u].template load<true>(g + (r0 + k0 + u) * D + c0, t, n);
+        }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (k0 + u < some) {
+          const float4 q = row_sums[k0 + u];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float z = (a[u].v[j] - q.x) * q.y;
+            gw[j] = fmaf(c[u].v[j], z, gw[j]);
+            gb[j] += c[u].v[j];
+            a[u].v[j] = q.y * (c[u].v[j] * p.v[j] - q.z - z * q.w);
+          }
+          if (gx) a[u].store(gx + (r0 + k0 + u) * D + c0, t, n);
+        }
+    }
   }
+  if (!columns) return;
+  Share<256, 1, VEC> o;
+#pragma unroll
+  for (int j = 0; j < 4; j++) o.v[j] = gw[j];
+  o.store(columns + 2l * blockIdx.y * D + c0, t, n);
+#pragma unroll
+  for (int j = 0; j < 4; j++) o.v[j] = gb[j];
+  o.store(columns + (2l * blockIdx.y + 1) * D + c0, t, n);
 }
+
 // gw += scale * sum of part[.][0], gb += scale * sum of part[.][1]: LANES threads a column, which take every LANES-th part and meet in the order of
 // their places.
 template <int LANES>
@@ -382,51 +401,28 @@ static __global__ void __launch_bounds__(256) norm_fold_kernel(const float *__re
   *o = fmaf(scale, s, *o);
 }
 
-// How rows of D values are shared out.
-struct NormShape {
-  int blocks = 1, slice = 0;   // blocks of a cluster, values of a block's slice
-};
-constexpr long kRowMost = 65536;
-static NormShape norm_shape(long D) {
-  NormShape s;
-  while (s.blocks < kMostBlocks && (D + s.blocks - 1) / s.blocks > 8192) s.blocks *= 2;
-  s.slice = (int)((D + 4l * s.blocks - 1) / (4l * s.blocks) * 4);
-  return s;
+template <int T, int V> struct NormConfig { static constexpr int kT = T, kV = V; };
+constexpr long kRowMost = 8192;
+// f(config) for the narrowest threads' share that holds a row
+template <class F> static void with_norm_config(long D, F f) {
+  if (D <= 128) f(NormConfig<32, 1>());
+  else if (D <= 256) f(NormConfig<32, 2>());
+  else if (D <= 384) f(NormConfig<32, 3>());
+  else if (D <= 512) f(NormConfig<32, 4>());
+  else if (D <= 1024) f(NormConfig<128, 2>());
+  else if (D <= 2048) f(NormConfig<256, 2>());
+  else if (D <= 4096) f(NormConfig<256, 4>());
+  else f(NormConfig<512, 4>());
 }
-template <int T, int V, bool CLUSTER> struct NormConfig {
-  static constexpr int kT = T, kV = V;
-  static constexpr bool kCluster = CLUSTER;
-};
-// f(config) for the narrowest threads' share that holds a row, or a slice of one
-template <class F> static void with_norm_config(long D, const NormShape &s, F f) {
-  if (s.blocks > 1) f(NormConfig<512, 4, true>());
-  else if (D <= 128) f(NormConfig<32, 1, false>());
-  else if (D <= 256) f(NormConfig<32, 2, false>());
-  else if (D <= 384) f(NormConfig<32, 3, false>());
-  else if (D <= 512) f(NormConfig<32, 4, false>());
-  else if (D <= 1024) f(NormConfig<128, 2, false>());
-  else if (D <= 2048) f(NormConfig<256, 2, false>());
-  else if (D <= 4096) f(NormConfig<256, 4, false>());
-  else f(NormConfig<512, 4, false>());
+template <class F> static void with_vec(bool vec, F f) {
+  if (vec) f(std::true_type()); else f(std::false_type());
 }
-template <class... P, class... A>
-static void launch_rows(void (*kernel)(P...), long grid, int block, size_t smem, int cluster, A... args) {
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = stream();
-  cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);   // check_launch() picks an error up
-}
-template <int T, int V, bool VEC, bool CLUSTER> static int resident_blocks() {
+template <int T, int V, bool VEC> static int resident_blocks() {
   static PerDevice resident;
   constexpr int BLOCK = T < 128 ? 256 : T;
   return resident.get(ctx().device, [] {
     int n = 0;
-    THC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_backward_kernel<T, V, VEC, CLUSTER>, BLOCK, T < 128 ? 2 * T * 4 * V * 4 : 0));
+    THC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, norm_backward_kernel<T, V, VEC>, BLOCK, T < 128 ? 2 * T * 4 * V * 4 : 0));
     return std::max(n, 1);
   });
 }
@@ -465,44 +461,43 @@ static void norm_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTens
   if (gradInput) size_result(gradInput, input->nDimension, input->size, {input, gradOutput, weight, mean, invStd, gradWeight, gradBias}, 3);
   check_apart(gradWeight, {input, gradOutput, weight, mean, invStd, gradBias}, 5);
   check_apart(gradBias, {input, gradOutput, weight, mean, invStd}, 6);
+  if (!gradInput && !gradWeight) return;
   WsScope scope;
   TensorRef x(tensor_new_contiguous(input)), g(tensor_new_contiguous(gradOutput));
   const float *w = weight ? data_ptr(weight) : nullptr, *xp = data_ptr(x), *gp = data_ptr(g), *mp = data_ptr(mean), *ip = data_ptr(invStd);
   float *gx = gradInput ? data_ptr(gradInput) : nullptr, *part = nullptr;
   long parts = 0;
+  const bool vec = size % 4 == 0 && aligned({xp, gp, gx, w});
   if (size <= kRowMost) {
-    const NormShape s = norm_shape(size);
-    const bool vec = size % 4 == 0 && aligned({xp, gp, gx, w});
-    with_norm_config(size, s, [&](auto c) {
-      typedef decltype(c) Cfg;
-      auto go = [&](auto v) {
+    with_norm_config(size, [&](auto c) {
+      with_vec(vec, [&](auto v) {
         constexpr bool VEC = decltype(v)::value;
-        constexpr int T = Cfg::kT, V = Cfg::kV, BLOCK = T < 128 ? 256 : T, TEAMS = BLOCK / T;
-        // as many teams as are resident at once
-        const long blocks = std::min((rows + TEAMS - 1) / TEAMS * s.blocks, ctx().sm_count * (long)resident_blocks<T, V, VEC, Cfg::kCluster>() / s.blocks * s.blocks);
-        if (gradWeight) {
-          parts = blocks / s.blocks;
-          part = (float *)ws_alloc(sizeof(float) * 2 * size * parts);
-        }
-        launch_rows(norm_backward_kernel<T, V, VEC, Cfg::kCluster>, blocks, BLOCK, TEAMS > 1 ? sizeof(float) * 2 * T * 4 * V : 0, s.blocks, xp, gp, gx, w, mp, ip, rows,
-                    size, s.slice, part);
-      };
-      if (vec) go(std::true_type()); else go(std::false_type());
+        constexpr int T = decltype(c)::kT, V = decltype(c)::kV, BLOCK = T < 128 ? 256 : T, TEAMS = BLOCK / T;
+        parts = std::min((rows + TEAMS - 1) / TEAMS, ctx().sm_count * (long)resident_blocks<T, V, VEC>());   // as many as are resident at once
+        if (gradWeight) part = (float *)ws_alloc(sizeof(float) * 2 * size * parts);
+        pdl_launch(norm_backward_kernel<T, V, VEC>, (unsigned)parts, BLOCK, TEAMS > 1 ? sizeof(float) * 2 * T * 4 * V : 0, xp, gp, gx, w, mp, ip, rows, (int)size,
+                   part);
+      });
     });
     check_launch("LayerNorm_backward");
   } else {
-    if (gx) {
-      pdl_launch(norm_rows_grad_kernel, (unsigned)std::min(rows, ctx().sm_count * 64l), 256, 0, xp, gp, gx, w, mp, ip, rows, size);
-      check_launch("LayerNorm_backward");
-    }
-    if (gradWeight) {
-      const long columns = std::min<long>((size + 31) / 32, 1l << 20);
-      parts = std::max(1l, std::min(std::min((rows + 31) / 32, (ctx().sm_count * 8l + columns - 1) / columns), 65535l));
-      const long per = (rows + parts - 1) / parts;
-      part = (float *)ws_alloc(sizeof(float) * 2 * size * parts);
-      pdl_launch(norm_columns_kernel, dim3((unsigned)columns, (unsigned)parts), 256, 0, xp, gp, mp, ip, rows, size, per, part);
-      check_launch("LayerNorm_backward");
-    }
+    const long pieces = (size + kPiece - 1) / kPiece, columns = (size + 1023) / 1024;
+    // rows enough in each of the column sums' blocks, and eight blocks an SM
+    parts = std::max(1l, std::min(std::min((rows + 3) / 4, (ctx().sm_count * 8l + columns - 1) / columns), 65535l));
+    const long per = (rows + parts - 1) / parts;
+    parts = (rows + per - 1) / per;
+    float2 *sums = nullptr;
+    if (gradWeight) part = (float *)ws_alloc(sizeof(float) * 2 * size * parts);
+    with_vec(vec, [&](auto v) {
+      constexpr bool VEC = decltype(v)::value;
+      if (gx) {
+        sums = (float2 *)ws_alloc(sizeof(float2) * rows * pieces);
+        pdl_launch(norm_piece_sums_kernel<VEC>, dim3((unsigned)pieces, (unsigned)std::min(rows, 65535l)), 256, 0, xp, gp, w, mp, ip, rows, size, sums);
+        check_launch("LayerNorm_backward");
+      }
+      pdl_launch(norm_columns_kernel<VEC>, dim3((unsigned)columns, (unsigned)parts), 256, 0, xp, gp, gx, w, mp, ip, rows, size, per, sums, (int)pieces, part);
+    });
+    check_launch("LayerNorm_backward");
   }
   if (gradWeight) {
     // a thread a column where that fills the device or there is little to add up
@@ -543,21 +538,29 @@ THC_API int THGPUNN_LayerNorm_updateOutput(THGPUTensor *input, THGPUTensor *outp
   TensorRef x(tensor_new_contiguous(input));
   const float *xp = data_ptr(x), *w = weight ? data_ptr(weight) : nullptr, *bp = bias ? data_ptr(bias) : nullptr;
   float *y = data_ptr(output), *mp = mean ? data_ptr(mean) : nullptr, *ip = mean ? data_ptr(invStd) : nullptr;
-  if (size <= kRowMost && rows <= 1l << 27) {
-    const NormShape s = norm_shape(size);
-    const bool vec = size % 4 == 0 && aligned({xp, y, w, bp});
-    with_norm_config(size, s, [&](auto c) {
-      typedef decltype(c) Cfg;
-      auto go = [&](auto v) {
-        constexpr int T = Cfg::kT, BLOCK = T < 128 ? 256 : T, TEAMS = BLOCK / T;
-        launch_rows(norm_forward_kernel<T, Cfg::kV, decltype(v)::value, Cfg::kCluster>, (rows + TEAMS - 1) / TEAMS * s.blocks, BLOCK, 0, s.blocks, xp, y, w, bp, mp, ip,
-                    rows, size, s.slice, (float)eps);
-      };
-      if (vec) go(std::true_type()); else go(std::false_type());
-    });
-  } else {
-    pdl_launch(norm_rows_kernel, (unsigned)std::min(rows, ctx().sm_count * 64l), 256, 0, xp, y, w, bp, mp, ip, rows, size, (float)eps);
-  }
+  const bool vec = size % 4 == 0 && aligned({xp, y, w, bp});
+  WsScope scope;
+  with_vec(vec, [&](auto v) {
+    constexpr bool VEC = decltype(v)::value;
+    if (size <= kRowMost) {
+      with_norm_config(size, [&](auto c) {
+        constexpr int T = decltype(c)::kT, BLOCK = T < 128 ? 256 : T, TEAMS = BLOCK / T;
+        // (a launch has less than 2^31 blocks)
+        for (long r = 0; r < rows; r += 1l << 30) {
+          const long n = std::min(rows - r, 1l << 30);
+          pdl_launch(norm_forward_kernel<T, decltype(c)::kV, VEC>, (unsigned)((n + TEAMS - 1) / TEAMS), BLOCK, 0, xp + r * size, y + r * size, w, bp, mp ? mp + r : nullptr,
+                     ip ? ip + r : nullptr, n, (int)size, (float)eps);
+        }
+      });
+      return;
+    }
+    const long pieces = (size + kPiece - 1) / kPiece;
+    const dim3 grid((unsigned)pieces, (unsigned)std::min(rows, 65535l));
+    float2 *part = (float2 *)ws_alloc(sizeof(float2) * rows * pieces);
+    pdl_launch(norm_pieces_kernel<VEC>, grid, 256, 0, xp, rows, size, part);
+    check_launch("LayerNorm_updateOutput");
+    pdl_launch(norm_apply_kernel<VEC>, grid, 256, 0, xp, y, w, bp, mp, ip, rows, size, (float)eps, part);
+  });
   check_launch("LayerNorm_updateOutput");
   return 0;
   THC_END(1)
