@@ -304,8 +304,8 @@ THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *count
   const long ldgz = act ? out : g.ld;
   if (act || gradBias)
     act_grad(gr, g.p, g.ld, act ? data_ptr(preactivation) : nullptr, act ? data_ptr(gradPre) : nullptr, out, activation, gradBias ? data_ptr(gradBias) : nullptr, scale);
-  if (gradInput) group_grad_input(gr, gz, ldgz, in, out, data_ptr(weight), data_ptr(gradInput));
-  if (gradWeight) group_grad_weight(gr, x.p, x.ld, gz, ldgz, in, out, data_ptr(gradWeight), scale);
+  if (gradInput || gradWeight)
+    group_backward(gr, x.p, x.ld, gz, ldgz, in, out, data_ptr(weight), gradInput ? data_ptr(gradInput) : nullptr, gradWeight ? data_ptr(gradWeight) : nullptr, scale);
   return 0;
   THC_END(1)
 }

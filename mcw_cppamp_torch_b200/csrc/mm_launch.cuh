@@ -148,19 +148,31 @@ static void encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int size, 
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   THC_CHECK(r == CUDA_SUCCESS, "internal: cuTensorMapEncodeTiled failed");
 }
-// One matrix a group, one behind the other, their lines `ld` apart: `rows` x K as above.
-static void encode_groups(CUtensorMap *map, const float *base, bool mn, long groups, long rows, long K, long ld, int tile_rows) {
+// One matrix a group, one behind the other, their lines `ld` values apart: `rows` x K as above.
+static void encode_groups(CUtensorMap *map, CUtensorMapDataType type, int size, const void *base, bool mn, long groups, long rows, long K, long ld, int tile_rows) {
+  const cuuint32_t kv = 128 / (cuuint32_t)size;
   EncodeTiledFn enc = encode_tiled_fn();
   const long inner = mn ? rows : K, mid = mn ? K : rows;
-  THC_CHECK(enc && ((uintptr_t)base & 15) == 0 && ld % 4 == 0, "internal: matrices not addressable by TMA");
+  THC_CHECK(enc && ((uintptr_t)base & 15) == 0 && ld * size % 16 == 0, "internal: matrices not addressable by TMA");
   const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)mid, (cuuint64_t)groups};
-  const cuuint64_t strides[2] = {(cuuint64_t)ld * 4, (cuuint64_t)ld * mid * 4};
-  const cuuint32_t box[3] = {32, mn ? 32 : (cuuint32_t)tile_rows, 1};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * size, (cuuint64_t)ld * mid * size};
+  const cuuint32_t box[3] = {kv, mn ? kv : (cuuint32_t)tile_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         mn ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const CUresult r = enc(map, type, 3, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         mn && size == 4 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   THC_CHECK(r == CUDA_SUCCESS, "internal: cuTensorMapEncodeTiled failed");
+}
+// kPairs: as attach_raw_map.
+template <bool MN, int PREC>
+static void attach_group_map(GroupOperand<MN, PREC> &op, const void *base, long groups, long rows, long K, long ld, int tile_rows) {
+  if constexpr (PREC == kPairs) {
+    op.lo = (int)ld;
+    encode_groups(&op.tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, MN, groups, MN ? 2 * ld : rows, MN ? K : 2 * ld, 2 * ld, tile_rows);
+    encode_groups(&op.tmap_wide, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, MN, groups, rows, K, ld, tile_rows);
+  } else {
+    encode_groups(&op.tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, MN, groups, rows, K, ld, tile_rows);
+  }
 }
 // kPairs: `ld` is the padded length of a line's halves, whose FP32 form has that pitch.
 template <int PREC, bool MN>

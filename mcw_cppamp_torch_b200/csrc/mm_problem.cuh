@@ -407,7 +407,7 @@ struct FusedProblem : Problem<OpA_, OpB_, false, PREC_> {
 // Products where the rows of each group meet a matrix of their own, in one launch.  An entry is a piece of a group's rows: a tile of columns of
 // the result (rows [first, end), the tile's width or less), or (kGroupSums) all rows of the group, which are summed over.
 enum : int { kGroupRows = 1, kGroupSums = 2 };
-struct GroupEntry { int group, first, end; };
+struct GroupEntry { int group, first, end, shift; };   // row r of the operands is row r - shift of the results
 constexpr int kGroupEntries = 160;   // that travel with a launch; more of them lie in device memory
 struct GroupList {
   int count;
@@ -417,8 +417,8 @@ struct GroupList {
 };
 // For the two-SM engine.  kGroupRows: A is the groups' (GroupOperand), column n of the result is row n of B; the list's pieces are tiles wide.
 // kGroupSums: k is the rows, each entry has a result of its own.  Tiles of an entry: m fastest.
-template <class OpA_, class OpB_, int GROUPS_, bool FUSED_>
-struct GroupProblem : Problem<OpA_, OpB_> {
+template <class OpA_, class OpB_, int GROUPS_, bool FUSED_, int PREC_ = kTf32>
+struct GroupProblem : Problem<OpA_, OpB_, false, PREC_> {
   static constexpr int GROUPS = GROUPS_;
   static constexpr bool FUSED = FUSED_;
   LinearEpilogue tail;      // (FUSED)

@@ -111,6 +111,129 @@ static __global__ void __launch_bounds__(256) matrix_strays_kernel(const StraySi
   }
 }
 
+// ---- groups --------------------------------------------------------------------------------------------------------------
+// Where the groups' rows start: as they are, and with each group padded to whole k tiles of 64 rows.
+constexpr int kPaddedGroups = 160;
+struct GroupRows {
+  int n;
+  int real[kPaddedGroups + 1], padded[kPaddedGroups + 1];
+  // the group of a row; of several that start there the one that has rows
+  static __device__ __forceinline__ int find(const int *starts, int n, int row) {
+    int lo = 0, hi = n;   // starts[lo] <= row < starts[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+  }
+};
+// c(r, f) += sum over k of what the pairs have left out of w[group of r](f, k) and x(r, k).  w [groups][out][in]; features are its lines (`lines`) or
+// its columns.  A block owns the rows blockIdx.x, blockIdx.x + gridDim.x, ... and takes the strays in their listed order.
+struct GroupStrays { const float *w; long in, out; const float *x; long ldx, run; Measured mw, mx; };
+static __global__ void __launch_bounds__(256) group_row_strays_kernel(const GroupStrays g, bool lines, float *c, const Ranges ranges,
+                                                                      const __grid_constant__ GroupRows rows) {
+  pdl_begin();
+  const bool wide = ranges.wide();
+  const int nx = g.mx.strays(wide), nw = g.mw.strays(wide);
+  if (nx + nw == 0) return;
+  const long features = lines ? g.out : g.in;
+  for (int e = 0; e < nx; e++) {
+    const long at = g.mx.list[e].at, r = at / g.run, k = at - r * g.run;
+    if (r % gridDim.x != blockIdx.x) continue;
+    const float v = g.mx.list[e].v;
+    const float *w = g.w + (long)GroupRows::find(rows.real, rows.n, (int)r) * g.out * g.in;
+    for (long f = threadIdx.x; f < features; f += 256) c[r * features + f] += v * (lines ? w[f * g.in + k] : w[k * g.in + f]);
+    __syncthreads();   // (another thread may take the same result next)
+  }
+  __syncthreads();
+  const unsigned limit = stray_limit(g.mx.rec->max_bits) - 1u;
+  for (int e = 0; e < nw; e++) {
+    const long at = g.mw.list[e].at, line = at / g.in, i = at - line * g.in, group = line / g.out, o = line - group * g.out;
+    const long f = lines ? o : i, k = lines ? i : o;
+    const float v = g.mw.list[e].v;
+    for (long r = blockIdx.x + (long)threadIdx.x * gridDim.x; r < rows.real[group + 1]; r += 256l * gridDim.x) {
+      if (r < rows.real[group]) continue;
+      const float s = g.x[r * g.ldx + k];
+      if ((__float_as_uint(s) & 0x7fffffffu) - 1u >= limit) c[r * features + f] += v * s;   // (zeros pass)
+    }
+    __syncthreads();
+  }
+}
+// gw[group](o, i) += scale * what the pairs have left out of the sums of gz(r, o) x(r, i) over the group's rows.  A block owns the lines blockIdx.x, ... of
+// every group's matrix.
+static __global__ void __launch_bounds__(256) group_sum_strays_kernel(const float *x, long ldx, long in, const float *gz, long ldg, long out, float *gw, float scale,
+                                                                      const Measured mx, const Measured mg, const Ranges ranges,
+                                                                      const __grid_constant__ GroupRows rows) {
+  pdl_begin();
+  const bool wide = ranges.wide();
+  const int nx = mx.strays(wide), ng = mg.strays(wide);
+  if (nx + ng == 0) return;
+  for (int e = 0; e < nx; e++) {
+    const long at = mx.list[e].at, r = at / in, i = at - r * in;
+    const float v = scale * mx.list[e].v;
+    float *c = gw + (long)GroupRows::find(rows.real, rows.n, (int)r) * out * in;
+    for (long o = blockIdx.x + (long)threadIdx.x * gridDim.x; o < out; o += 256l * gridDim.x) c[o * in + i] += v * gz[r * ldg + o];
+    __syncthreads();
+  }
+  const unsigned limit = stray_limit(mx.rec->max_bits) - 1u;
+  for (int e = 0; e < ng; e++) {
+    const long at = mg.list[e].at, r = at / out, o = at - r * out;
+    if (o % gridDim.x != blockIdx.x) continue;
+    const float v = scale * mg.list[e].v;
+    float *c = gw + ((long)GroupRows::find(rows.real, rows.n, (int)r) * out + o) * in;
+    for (long i = threadIdx.x; i < in; i += 256) {
+      const float s = x[r * ldx + i];
+      if ((__float_as_uint(s) & 0x7fffffffu) - 1u >= limit) c[i] += v * s;
+    }
+    __syncthreads();
+  }
+}
+// Up to three matrices (blockIdx.y) as FP16 pairs, as split_matrix_kernel makes them: weights as they lie, rows (`grouped`) with each group padded by
+// zeros to whole k tiles.
+struct GroupPairJob : PairJob { int grouped; };
+static __global__ void __launch_bounds__(256) split_groups_kernel(const GroupPairJob a, const GroupPairJob b, const GroupPairJob c,
+                                                                  const __grid_constant__ GroupRows rows) {
+  pdl_begin();
+  const GroupPairJob &j = blockIdx.y == 0 ? a : blockIdx.y == 1 ? b : c;
+  const bool wide = j.ranges.wide();
+  const float scale = wide ? 1.f : pair_scale(*j.ranges.rec[0]);
+  const int lane = threadIdx.x & 31;
+  const long warps = (long)gridDim.x * 8, parts = (j.ldp + 511) / 512, lines = j.grouped ? rows.padded[rows.n] : j.lines;
+  for (long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5); w < lines * parts; w += warps) {
+    const long l = w / parts, c0 = (w - l * parts) * 512 + lane * 4;
+    long run = j.run, from = l;
+    if (j.grouped) {
+      const int e = GroupRows::find(rows.padded, rows.n, (int)l);
+      from = l - rows.padded[e] + rows.real[e];
+      if (from >= rows.real[e + 1]) run = 0;   // padding
+    }
+    const float *s = j.src + from * j.ld;
+    float4 v[4];
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const long c = c0 + g * 128;
+      if (j.vec && c + 4 <= run) v[g] = __ldg(reinterpret_cast<const float4 *>(s + c));
+      else v[g] = make_float4(c < run ? s[c] : 0.f, c + 1 < run ? s[c + 1] : 0.f, c + 2 < run ? s[c + 2] : 0.f, c + 3 < run ? s[c + 3] : 0.f);
+    }
+    float *d = reinterpret_cast<float *>(j.dst) + l * j.ldp;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const long c = c0 + g * 128;
+      if (c >= j.ldp) break;
+      if (wide) {
+        *reinterpret_cast<float4 *>(d + c) = v[g];
+      } else {
+        __half2 hi[2], lo[2];
+        split_pair(v[g].x * scale, v[g].y * scale, hi[0], lo[0]);
+        split_pair(v[g].z * scale, v[g].w * scale, hi[1], lo[1]);
+        uint2 *h = reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(d) + c);
+        h[0] = make_uint2(half2_bits(hi[0]), half2_bits(hi[1]));
+        h[j.ldp / 4] = make_uint2(half2_bits(lo[0]), half2_bits(lo[1]));
+      }
+    }
+  }
+}
+
 }  // namespace mm
 }  // namespace thc
 

@@ -277,7 +277,7 @@ struct Tc2rItem {
   long slot;   // partial-sum block of the workspace (tail items only)
   int num_k_tiles;
   int group, k_left;   // of a grouped product: the group, and the k of this item
-  long n_end;          // the end of this item's columns
+  long n_end, shift;   // the end of this item's columns, and how far they lie behind the result's
 };
 
 // Persistent: the launch has as many clusters as the device runs at once; cluster c starts with item c and takes
@@ -328,9 +328,9 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
       t.group = g.group;
       t.m_tile0 = (long)(r - nt * gm) * 256;
       if constexpr (P::GROUPS == kGroupRows) {
-        t.n_tile0 = g.first; t.n_end = g.end; t.k_begin = 0; t.k_left = (int)p.K;
+        t.n_tile0 = g.first; t.n_end = g.end; t.shift = g.shift; t.k_begin = 0; t.k_left = (int)p.K;
       } else {
-        t.n_tile0 = (long)nt * BN2; t.n_end = p.N; t.k_begin = g.first; t.k_left = g.end - g.first;
+        t.n_tile0 = (long)nt * BN2; t.n_end = p.N; t.shift = 0; t.k_begin = g.first; t.k_left = g.end - g.first;
       }
       t.num_k_tiles = (t.k_left + KV - 1) / KV;
       return t;
@@ -748,13 +748,15 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
           for (int j = 0; j < NCOL; j++) o[j * 256] = acc[j];
         } else if constexpr (P::GROUPS != 0) {
           ResultView view{p.epi, p.M, item.n_end};
+          const long n = item.n_tile0 + h * NCOL - item.shift;
+          view.N -= item.shift;
           if constexpr (P::GROUPS == kGroupRows) {
             if (view.epi.row_bias) view.epi.row_bias += item.group * p.bias_group;
           } else {
             view.epi.out += item.group * p.out_group;
           }
-          if constexpr (P::FUSED) tc2_store_linear(view, p.tail, false, acc, m, item.n_tile0 + h * NCOL);
-          else tc2_store_rows<ResultView, NCOL>(view, acc, m, item.n_tile0 + h * NCOL);
+          if constexpr (P::FUSED) tc2_store_linear(view, p.tail, PAIRS && p.tail.deferred(), acc, m, n);
+          else tc2_store_rows<ResultView, NCOL>(view, acc, m, n);
         } else if constexpr (P::FUSED) {
           tc2_store_linear(p, p.tail, PAIRS && p.tail.deferred(), acc, m, item.n_tile0 + h * NCOL);
         } else if constexpr (P::PAIR && BN2 == 128) {

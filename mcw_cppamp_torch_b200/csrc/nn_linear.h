@@ -18,6 +18,10 @@ struct LinearTail {
 // y = act(z) + residual with z = x w^T + b: x [rows][in] at pitch ldx, w [out][in], b may be null
 void linear_product(const float *x, long ldx, long rows, long in, long out, const float *w, const float *b, float *y, const LinearTail &tail);
 
+namespace mm { struct LinearEpilogue; }
+// y = act(z) + residual in a pass of its own; with the records of a product over pairs, only where that has left its sums in z
+void linear_tail(const float *z, float *y, long rows, long out, const LinearTail &tail, const mm::LinearEpilogue &product);
+
 // Rows of group e: the counts[e] from the sum of the counts before it on.
 struct Groups {
   const long *counts;
@@ -26,10 +30,8 @@ struct Groups {
 };
 // For the rows of each group e: y = act(z), z = x w[e]^T + b[e]
 void group_forward(const Groups &g, const float *x, long ldx, long in, long out, const float *w, const float *b, float *y, int act, float *z);
-// gx = gz w[e]
-void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx);
-// gw[e] += scale * gz^T x over the group's rows
-void group_grad_weight(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale);
+// gx = gz w[e], unless null, and gw[e] += scale * gz^T x over the group's rows, unless null
+void group_backward(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, const float *w, float *gx, float *gw, float scale);
 
 }  // namespace thc
 

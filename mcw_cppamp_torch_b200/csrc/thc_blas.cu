@@ -281,7 +281,7 @@ static __global__ void __launch_bounds__(256) linear_tail_kernel(const float *z,
     y[i] = v;
   }
 }
-static void linear_tail(const float *z, float *y, long rows, long out, const LinearTail &tail, const mm::LinearEpilogue &product) {
+void linear_tail(const float *z, float *y, long rows, long out, const LinearTail &tail, const mm::LinearEpilogue &product) {
   const bool vec = out % 4 == 0 && tail.ldr % 4 == 0 && (((uintptr_t)z | (uintptr_t)y | (uintptr_t)tail.residual) & 15) == 0;
   const long n = rows * out / (vec ? 4 : 1);
   with_activation(tail.act, [&](auto a) {

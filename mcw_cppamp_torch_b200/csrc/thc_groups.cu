@@ -44,14 +44,14 @@ static std::vector<GroupEntry> row_tiles(const Groups &g, int width) {
   std::vector<GroupEntry> v;
   long r = 0;
   for (int e = 0; e < g.n; r += g.counts[e++])
-    for (long i = 0; i < g.counts[e]; i += width) v.push_back(GroupEntry{e, (int)(r + i), (int)(r + std::min<long>(g.counts[e], i + width))});
+    for (long i = 0; i < g.counts[e]; i += width) v.push_back(GroupEntry{e, (int)(r + i), (int)(r + std::min<long>(g.counts[e], i + width)), 0});
   return v;
 }
 static std::vector<GroupEntry> whole_groups(const Groups &g) {
   std::vector<GroupEntry> v;
   long r = 0;
   for (int e = 0; e < g.n; r += g.counts[e++])
-    if (g.counts[e]) v.push_back(GroupEntry{e, (int)r, (int)(r + g.counts[e])});
+    if (g.counts[e]) v.push_back(GroupEntry{e, (int)r, (int)(r + g.counts[e]), 0});
   return v;
 }
 // The warp-level engine's time, by small_product_us()'s figures: `features` tiles of 64, times `tiles` along the groups' rows (or the other features), which
@@ -68,22 +68,30 @@ static long tiles_of(const Groups &g, long width) {
   for (int e = 0; e < g.n; e++) t += (g.counts[e] + width - 1) / width;
   return t;
 }
-struct Choice { bool engine; int width; };
-// For kGroupRows: the engine and the width of its tiles along the rows that finish first.  The two-SM engine takes all tiles round by round, with two k
-// tiles for a tile's epilogue and, where its operands have to be copied, `pack` bytes at 2 TB/s.
-static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, bool tma) {
-  Choice best{false, 64};
+enum Way { kSmall, kEngine, kEnginePairs };   // the warp-level engine; the two-SM one over FP32 values; over FP16 pairs
+struct Choice { Way way; int width; };
+// Passes over `values` values that make pairs of them, as pairs_are_faster() has it.
+static double pair_passes_us(double values) { return 14 + 4e-6 * values * (1 / 5.5 + 2 / 5.0); }
+static bool pairs_fit(const Groups &g, double values) { return ctx().math_mode == 0 && g.n <= kPaddedGroups && g.rows < 1l << 28 && 4 * values < 16e9 && encode_tiled_fn(); }
+// For kGroupRows: the way and the width of its tiles along the rows that finish first.  The two-SM engine takes all tiles round by round, with two k
+// tiles for a tile's epilogue and, where its operands have to be copied, `pack` bytes at 2 TB/s; pairs of the `values` of both operands take
+// their passes.
+static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, double values) {
+  Choice best{kSmall, 64};
   double least = 0;
-  const long ktiles = (K + 31) / 32;
+  const long ktiles = (K + 31) / 32, ktiles_half = (K + 63) / 64;
   for (int w : {64, 32, 16, 8}) {
     const double n = (double)tiles_of(g, w), us = small_groups_us((double)((features + 63) / 64), n, n * (double)ktiles, w, small_aligned);
-    if (!least || us < least) { best = Choice{false, w}; least = us; }
+    if (!least || us < least) { best = Choice{kSmall, w}; least = us; }
   }
-  if (!tma) return best;
+  if (!encode_tiled_fn()) return best;
+  const bool pairs = pairs_fit(g, values);
   for (int w : {256, 192, 128, 64}) {
-    const double tiles = (double)((features + 255) / 256) * (double)tiles_of(g, w);
-    const double us = 10 + std::ceil(tiles / (ctx().sm_count / 2)) * (double)(ktiles + 2) * group_tile_us(w) + (pack ? 5 + pack / 2e6 : 0);
-    if (us < least) { best = Choice{true, w}; least = us; }
+    const double rounds = std::ceil((double)((features + 255) / 256) * (double)tiles_of(g, w) / (ctx().sm_count / 2));
+    const double us = 10 + rounds * (double)(ktiles + 2) * group_tile_us(w) + (pack ? 5 + pack / 2e6 : 0);
+    if (us < least) { best = Choice{kEngine, w}; least = us; }
+    const double with_pairs = 10 + rounds * (double)(ktiles_half + 2) * tc2_tile_us(w, kPairs) + pair_passes_us(values);
+    if (pairs && with_pairs < least) { best = Choice{kEnginePairs, w}; least = with_pairs; }
   }
   return best;
 }
@@ -170,10 +178,14 @@ static void launch_groups(P p, int bn2, const std::vector<GroupEntry> &entries, 
   attach(p, bn2);
   auto go = [&](auto w) { launch_tc2r_kernel<P, decltype(w)::value>(p, p.items, false); };
   if (bn2 == 256) go(std::integral_constant<int, 256>());
-  else if (bn2 == 192) go(std::integral_constant<int, 192>());
   else if (bn2 == 128) go(std::integral_constant<int, 128>());
-  else go(std::integral_constant<int, 64>());
-  ctx().products[kTf32]++;
+  else if constexpr (P::PREC == kTf32 || !P::OpB::MN_MAJOR) {
+    if (bn2 == 192) go(std::integral_constant<int, 192>());
+    else go(std::integral_constant<int, 64>());
+  } else {
+    fail("internal: tile width %d for a problem that has none", bn2);
+  }
+  ctx().products[P::PREC]++;
 }
 
 // D(f, r) = sum_k A[e](f, k) B(r, k): the forward pass (the features are w's rows) and gradInput (its columns, MN).
@@ -186,9 +198,89 @@ static void engine_rows(const Groups &g, Lines a, Lines b, long features, long K
   p.bias_group = bias_group;
   p.tail = tail;
   launch_groups(p, width, row_tiles(g, width), (features + 255) / 256, [&](auto &q, int bn2) {
-    encode_groups(&q.a.tmap, a.p, MN, g.n, features, K, a.ld, TC_BM);
+    attach_group_map<MN, kTf32>(q.a, a.p, g.n, features, K, a.ld, TC_BM);
     attach_raw_map<kTf32>(q.b, b.p, g.rows, K, b.ld, bn2 / 2);
   });
+}
+
+// ---- the two-SM engine over pairs ------------------------------------------------------------------------------------
+// An operand as FP16 pairs (mm_problem.cuh): weights as they lie, rows with each group padded by zeros to whole k tiles, so that no k tile has two
+// groups' rows.
+struct PairSide {
+  const float *p;
+  long lines, run, ld;
+  bool grouped;
+  Measured m;
+  void *dst;
+  long ldp;
+};
+struct GroupPairs {
+  GroupRows rows;
+  PairSide *sides[3];
+  int n = 0;
+  Ranges ranges;      // of all sides: their form is decided together
+  long padded() const { return rows.padded[rows.n]; }
+};
+// False: there is no room for the pairs, and nothing has been done.
+static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<PairSide *> sides) {
+  gp.rows.n = g.n;
+  gp.rows.real[0] = gp.rows.padded[0] = 0;
+  for (int e = 0; e < g.n; e++) {
+    gp.rows.real[e + 1] = gp.rows.real[e] + (int)g.counts[e];
+    gp.rows.padded[e + 1] = gp.rows.padded[e] + (int)((g.counts[e] + 63) / 64 * 64);
+  }
+  double need = 96e6;
+  for (PairSide *s : sides) need += 4.1 * (double)(s->grouped ? gp.padded() : s->lines) * (double)(s->run + 64);
+  if (!ws_reserve((size_t)need)) return false;
+  RangeJob ranges[3];
+  GroupPairJob jobs[3] = {};
+  long pieces = 0;
+  for (PairSide *s : sides) {
+    const int i = gp.n++;
+    gp.sides[i] = s;
+    s->m = new_measured();
+    s->ldp = (s->run + 63) / 64 * 64;
+    const long lines = s->grouped ? gp.padded() : s->lines;
+    s->dst = ws_alloc(sizeof(float) * lines * s->ldp);
+    gp.ranges.rec[i] = s->m.rec;
+    ranges[i] = range_job(s->p, s->lines, s->run, s->ld, s->m);
+    static_cast<PairJob &>(jobs[i]) = PairJob{s->p, s->dst, s->lines, s->run, s->ld, s->ldp, ((uintptr_t)s->p & 15) == 0 && s->ld % 4 == 0, {}};
+    jobs[i].grouped = s->grouped;
+    pieces = std::max(pieces, lines * ((s->ldp + 511) / 512));
+  }
+  for (int i = 0; i < gp.n; i++)
+    for (int k = 0; k < gp.n; k++) jobs[i].ranges.rec[k] = gp.ranges.rec[(i + k) % gp.n];   // its own first
+  launch_ranges(ranges[0], &ranges[1]);
+  if (gp.n > 2) launch_ranges(ranges[2], nullptr);
+  pdl_launch(split_groups_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), (unsigned)gp.n), 256, 0, jobs[0], jobs[1], jobs[2], gp.rows);
+  check_launch("split_groups");
+  return true;
+}
+static std::vector<GroupEntry> padded(std::vector<GroupEntry> v, const GroupRows &rows) {
+  for (GroupEntry &e : v) {
+    e.shift = rows.padded[e.group] - rows.real[e.group];
+    e.first += e.shift; e.end += e.shift;
+  }
+  return v;
+}
+// As engine_rows, over the pairs of w and of the rows; what they leave out is added to `sums`.
+template <bool MN, bool FUSED>
+static void pairs_rows(const Groups &g, const GroupPairs &gp, const PairSide &w, const PairSide &x, long in, long out, int width, const Epilogue &epi, float *sums,
+                       const LinearEpilogue &tail) {
+  const long features = MN ? in : out, K = MN ? out : in;
+  GroupProblem<GroupOperand<MN, kPairs>, RawOperand<false, kPairs>, kGroupRows, FUSED, kPairs> p;
+  p.epi = epi;
+  p.M = features; p.N = gp.padded(); p.K = K;
+  p.bias_group = out;
+  p.tail = tail;
+  p.range_a = w.m.rec; p.range_b = x.m.rec; p.ranges = gp.ranges;
+  launch_groups(p, width, padded(row_tiles(g, width), gp.rows), (features + 255) / 256, [&](auto &q, int bn2) {
+    attach_group_map<MN, kPairs>(q.a, w.dst, g.n, features, K, w.ldp, TC_BM);
+    attach_raw_map<kPairs>(q.b, x.dst, gp.padded(), K, x.ldp, bn2 / 2);
+  });
+  pdl_launch(group_row_strays_kernel, (unsigned)std::min<long>(g.rows, ctx().sm_count), 256, 0, GroupStrays{w.p, in, out, x.p, x.ld, x.run, w.m, x.m}, !MN, sums, gp.ranges,
+             gp.rows);
+  check_launch("group_strays");
 }
 
 // ---- the passes -------------------------------------------------------------------------------------------------------
@@ -212,24 +304,38 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
   p.at = GroupPlaces{out * in, 0, ldx, 0, out, out};
   if (few_rows_groups(p, g)) return;
   const Lines ws{w, (long)g.n * out, in, in}, xs{x, g.rows, in, ldx};
-  const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), encode_tiled_fn() != nullptr);
-  if (c.engine) {
+  const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), (double)in * (double)(g.n * out + g.rows));
+  if (c.way != kSmall) {
     Epilogue epi{y, nullptr, 1.f, 0.f, LONG_MAX, 0, out};
     epi.row_bias = b;
     LinearEpilogue tail;
     tail.act = act; tail.z = z;
+    if (c.way == kEnginePairs) {
+      PairSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true};
+      GroupPairs gp;
+      if (make_pairs(gp, g, {&wp, &xp})) {
+        tail.a = wp.m.rec; tail.b = xp.m.rec; tail.ranges = gp.ranges;
+        float *sums = z ? z : y;
+        pairs_rows<false, true>(g, gp, wp, xp, in, out, c.width, epi, sums, tail);
+        LinearTail after;
+        after.act = act;
+        if (act != kActNone || z) linear_tail(sums, y, g.rows, out, after, tail);
+        return;
+      }
+    }
     engine_rows<false, true>(g, ws, xs, out, in, c.width, epi, out, tail);
     return;
   }
   small_groups(p, row_tiles(g, c.width), c.width, true, true);
 }
-void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
-  if (each_group(g, [&](int e, long r, long n) { gemm('n', 'n', in, n, out, 1.f, w + e * out * in, in, gz + r * ldg, ldg, 0.f, gx + r * in, in); })) return;
-  WsScope scope;
+static Choice choose_grad_input(const Groups &g, long ldg, const float *gz, long in, long out, const float *w) {
   const Lines ws{w, (long)g.n * out, in, in}, gs{gz, g.rows, out, ldg};
-  const Choice c = choose_rows(g, in, out, ws.ok() && gs.ok(), pack_bytes(ws, gs), encode_tiled_fn() != nullptr);
-  if (c.engine) {
-    engine_rows<true, false>(g, ws, gs, in, out, c.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, 0, {});
+  return choose_rows(g, in, out, ws.ok() && gs.ok(), pack_bytes(ws, gs), (double)out * (double)(g.n * in + g.rows));
+}
+static void grad_input(const Groups &g, const Choice &c, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
+  WsScope scope;
+  if (c.way != kSmall) {
+    engine_rows<true, false>(g, Lines{w, (long)g.n * out, in, in}, Lines{gz, g.rows, out, ldg}, in, out, c.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, 0, {});
     return;
   }
   SmallGroups p = {};
@@ -241,45 +347,106 @@ void group_grad_input(const Groups &g, const float *gz, long ldg, long in, long 
   p.at = GroupPlaces{out * in, 0, ldg, 0, in, 0};
   small_groups(p, row_tiles(g, c.width), c.width, false, true);
 }
-void group_grad_weight(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale) {
-  if (each_group(g, [&](int e, long r, long n) { gemm('n', 't', in, out, n, scale, x + r * ldx, ldx, gz + r * ldg, ldg, 1.f, gw + e * out * in, in); })) return;
-  WsScope scope;
-  Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
-  const int bn2 = tc2_tile_width(out), bn = small_tile_width(out);
-  long ktiles = 0, most = 0;
-  std::vector<GroupEntry> entries = whole_groups(g);
-  for (const GroupEntry &e : entries) {
-    const long t = (e.end - e.first + 31) / 32;
-    ktiles += t;
+// The largest first: the clusters take items as they finish, and short ones level the end.
+static std::vector<GroupEntry> largest_first(std::vector<GroupEntry> v) {
+  std::stable_sort(v.begin(), v.end(), [](const GroupEntry &a, const GroupEntry &b) { return a.end - a.first > b.end - b.first; });
+  return v;
+}
+static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &gs) {
+  const long in = xs.run, out = gs.run;
+  long ktiles = 0, halves = 0, most = 0, live = 0;
+  for (int e = 0; e < g.n; e++) {
+    const long t = (g.counts[e] + 31) / 32;
+    ktiles += t; halves += (g.counts[e] + 63) / 64; live += t > 0;
     most = std::max(most, t);
   }
-  const double bytes = pack_bytes(xs, gs), tiles = (double)((in + 255) / 256) * (double)((out + bn2 - 1) / bn2);
-  const double engine = 10 + std::max(tiles * (double)(ktiles + 2 * (long)entries.size()) / (ctx().sm_count / 2), (double)(most + 2)) * group_tile_us(bn2) +
-                        (bytes ? 5 + bytes / 2e6 : 0);
-  const double columns = (double)((out + bn - 1) / bn);
-  if (encode_tiled_fn() && engine < small_groups_us((double)((in + 63) / 64), columns * (double)entries.size(), columns * (double)ktiles, bn, xs.ok() && gs.ok())) {
+  const int bn = small_tile_width(out);
+  const double columns = (double)((out + bn - 1) / bn), bytes = pack_bytes(xs, gs), values = (double)g.rows * (double)(in + out);
+  Choice best{kSmall, bn};
+  double least = small_groups_us((double)((in + 63) / 64), columns * (double)live, columns * (double)ktiles, bn, xs.ok() && gs.ok());
+  if (!encode_tiled_fn()) return best;
+  for (int pairs = 0; pairs < (pairs_fit(g, values) ? 2 : 1); pairs++) {
+    const int w = tc2_tile_width(out, pairs);
+    const double tiles = (double)((in + 255) / 256) * (double)((out + w - 1) / w), k = (double)(pairs ? halves : ktiles), longest = (double)(pairs ? (most + 1) / 2 : most);
+    const double us = 10 + std::max(tiles * (k + 2 * (double)live) / (ctx().sm_count / 2), longest + 2) * (pairs ? tc2_tile_us(w, kPairs) : group_tile_us(w)) +
+                      (pairs ? pair_passes_us(values) : bytes ? 5 + bytes / 2e6 : 0);
+    if (us < least) { best = Choice{pairs ? kEnginePairs : kEngine, w}; least = us; }
+  }
+  return best;
+}
+template <class P> static void set_sums(P &p, long in, long out, float *gw, float scale) {
+  p.epi = Epilogue{gw, nullptr, scale, 1.f, LONG_MAX, 0, in};
+  p.M = in; p.N = out;
+  p.out_group = out * in;
+}
+static void grad_weight(const Groups &g, const Choice &c, Lines xs, Lines gs, float *gw, float scale) {
+  WsScope scope;
+  const long in = xs.run, out = gs.run;
+  if (c.way != kSmall) {
     pack(xs, gs);
-    // the largest first: the clusters take items as they finish, and short ones level the end
-    std::stable_sort(entries.begin(), entries.end(), [](const GroupEntry &a, const GroupEntry &b) { return a.end - a.first > b.end - b.first; });
     GroupProblem<RawOperand<true>, RawOperand<true>, kGroupSums, false> p;
-    p.epi = Epilogue{gw, nullptr, scale, 1.f, LONG_MAX, 0, in};
-    p.M = in; p.N = out; p.K = g.rows;
-    p.out_group = out * in;
-    launch_groups(p, bn2, entries, ((in + 255) / 256) * ((out + bn2 - 1) / bn2), [&](auto &q, int) {
+    set_sums(p, in, out, gw, scale);
+    p.K = g.rows;
+    const int bn2 = tc2_tile_width(out);
+    launch_groups(p, bn2, largest_first(whole_groups(g)), ((in + 255) / 256) * ((out + bn2 - 1) / bn2), [&](auto &q, int) {
       attach_raw_map<kTf32>(q.a, xs.p, in, g.rows, xs.ld, TC_BM);
       attach_raw_map<kTf32>(q.b, gs.p, out, g.rows, gs.ld, bn2 / 2);
     });
     return;
   }
   SmallGroups p = {};
-  p.a = small_operand(x, ldx); p.b = small_operand(gz, ldg);
+  p.a = small_operand(xs.p, xs.ld); p.b = small_operand(gs.p, gs.ld);
   p.M = (int)in; p.N = (int)out; p.K = 0;
   p.c = gw; p.sm = 1; p.sn = in;
   p.alpha = scale; p.beta = 1.f;
   p.kind = kGroupSums;
-  p.column_tiles = ceil_div(out, bn);
-  p.at = GroupPlaces{0, ldx, ldg, out * in, 0, 0};
-  small_groups(p, entries, bn, false, false);
+  p.column_tiles = ceil_div(out, c.width);
+  p.at = GroupPlaces{0, xs.ld, gs.ld, out * in, 0, 0};
+  small_groups(p, whole_groups(g), c.width, false, false);
+}
+static void pairs_sums(const Groups &g, const GroupPairs &gp, const PairSide &x, const PairSide &gz, float *gw, float scale) {
+  const long in = x.run, out = gz.run;
+  GroupProblem<RawOperand<true, kPairs>, RawOperand<true, kPairs>, kGroupSums, false, kPairs> p;
+  set_sums(p, in, out, gw, scale);
+  p.K = gp.padded();
+  p.range_a = x.m.rec; p.range_b = gz.m.rec; p.ranges = gp.ranges;
+  const int w = tc2_tile_width(out, true);
+  launch_groups(p, w, largest_first(padded(whole_groups(g), gp.rows)), ((in + 255) / 256) * ((out + w - 1) / w), [&](auto &q, int bn2) {
+    attach_raw_map<kPairs>(q.a, x.dst, in, gp.padded(), x.ldp, TC_BM);
+    attach_raw_map<kPairs>(q.b, gz.dst, out, gp.padded(), gz.ldp, bn2 / 2);
+  });
+  pdl_launch(group_sum_strays_kernel, (unsigned)std::min<long>(out, ctx().sm_count), 256, 0, x.p, x.ld, in, gz.p, gz.ld, out, gw, scale, x.m, gz.m, gp.ranges, gp.rows);
+  check_launch("group_strays");
+}
+
+// Which way a gradient takes depends on it alone, not on whether the other is asked for too; where both take pairs, gz is split once.
+void group_backward(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, const float *w, float *gx, float *gw, float scale) {
+  if (each_group(g, [&](int e, long r, long n) {
+        if (gx) gemm('n', 'n', in, n, out, 1.f, w + e * out * in, in, gz + r * ldg, ldg, 0.f, gx + r * in, in);
+        if (gw) gemm('n', 't', in, out, n, scale, x + r * ldx, ldx, gz + r * ldg, ldg, 1.f, gw + e * out * in, in);
+      }))
+    return;
+  WsScope scope;
+  const Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
+  const Choice ci = gx ? choose_grad_input(g, ldg, gz, in, out, w) : Choice{kSmall, 64}, cw = gw ? choose_grad_weight(g, xs, gs) : Choice{kSmall, 64};
+  const bool pi = gx && ci.way == kEnginePairs, pw = gw && cw.way == kEnginePairs;
+  if (pi || pw) {
+    PairSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true}, gp{gz, g.rows, out, ldg, true};
+    GroupPairs pairs;
+    const bool made = pi && pw ? make_pairs(pairs, g, {&gp, &wp, &xp}) : pi ? make_pairs(pairs, g, {&gp, &wp}) : make_pairs(pairs, g, {&gp, &xp});
+    if (made) {
+      if (pi) {
+        pairs_rows<true, false>(g, pairs, wp, gp, in, out, ci.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, gx, {});
+        gx = nullptr;
+      }
+      if (pw) {
+        pairs_sums(g, pairs, xp, gp, gw, scale);
+        gw = nullptr;
+      }
+    }
+  }
+  if (gx) grad_input(g, ci, gz, ldg, in, out, w, gx);
+  if (gw) grad_weight(g, cw, xs, gs, gw, scale);
 }
 
 }  // namespace thc

@@ -346,3 +346,79 @@ def test_a_group_keeps_to_itself(gt, I, O):
     for a, c in zip(*out):
         keep = rows if a.size(0) == T else groups
         assert torch.equal(a[keep], c[keep]) and torch.isfinite(c[keep]).all()
+
+
+@pytest.mark.parametrize("kind", ["plain", "strays", "wide", "odd"])
+@pytest.mark.parametrize("name", ["gelu", "none"])
+@pytest.mark.parametrize("large", [False, True])
+def test_groups_over_pairs(gt, kind, name, large):
+    """Products whose operands are split into FP16 halves: padded groups, values that halves do not hold (a few: added on their own; many: the same
+    launch multiplies FP32 values), in all three passes."""
+    counts, I, O = [1500, 0, 2300, 65, 1, 2230], 1536, 1600
+    if kind == "odd":
+        I, O = 1531, 1601
+    if large:                                                    # (gradInput stays in FP32 at the sizes above)
+        counts, I, O = [3000, 0, 4100, 65, 1, 2700], I + 512, O + 704
+    T, n = sum(counts), len(counts)
+    x, w, b, g = randn(1, T, I), randn(2, n, O, I) / I ** 0.5, 0.1 * randn(3, n, O), randn(4, T, O)
+    b[:, 3] = 0
+    if kind == "strays":
+        for r in (0, 1499, 1500, 3799, 3864, 3865, T - 1):       # rows with one value each, far below the largest
+            x[r] = 0
+            x[r, r % I] = 2.0 ** -38
+            g[r] = 0
+            g[r, r % O] = 2.0 ** -37
+        w[2, 3] = 0
+        w[2, 3, 7] = 2.0 ** -40                                  # a line of a weight
+        w[5, :, 11] = 0
+        w[5, 9, 11] = 2.0 ** -41                                 # a column of another
+        w[1, 0, 0] = 2.0 ** -42                                  # of a group without rows
+    if kind == "wide":
+        x = x * torch.exp2(-torch.linspace(0, 45, T, device="cuda").round())[:, None]
+        w = w * torch.exp2(-torch.linspace(0, 40, O, device="cuda").round())[None, :, None]
+    m = fill(gt, gt.nn.GroupedLinear(n, I, O, name), w, b)
+    X, W, B, G = x.double(), w.double(), b.double(), g.double()
+    ends = np.cumsum([0] + counts)
+    at = [slice(int(a), int(c)) for a, c in zip(ends[:-1], ends[1:])]
+    L = gt.lib()
+    before = L.THGPUProductCount(2)
+    m.forward([up(gt, x), counts])
+    z = torch.cat([X[p] @ W[e].t() + B[e] for e, p in enumerate(at)])
+    zt = torch.cat([rel_of(I) * (X[p].abs() @ W[e].abs().t() + B[e].abs()) for e, p in enumerate(at)])
+    y = act(z, name)
+    near(down(m.output), y, y_tolerance(z, zt, y, name))
+    if name != "none":
+        near(down(m.preactivation), z, zt)
+        m.preactivation.fill(30)                                 # slopes of one: the gradients' rows keep their sizes
+    m.gradWeight.zero(); m.gradBias.zero()
+    gi = down(m.backward([up(gt, x), counts], up(gt, g), 1.0)[0])
+    assert L.THGPUProductCount(2) - before >= (3 if large else 2)
+    near(gi, torch.cat([G[p] @ W[e] for e, p in enumerate(at)]), torch.cat([(rel_of(O) + 8 * E) * (G[p].abs() @ W[e].abs()) for e, p in enumerate(at)]))
+    gw = down(m.gradWeight)
+    for e, p in enumerate(at):
+        near(gw[e], G[p].t() @ X[p], (rel_of(counts[e]) + 8 * E) * (G[p].abs().t() @ X[p].abs()))
+    first = [t.clone() for t in (gi, gw)]
+    m.gradInput = gt.GPUTensor()
+    m.gradWeight.zero()
+    assert torch.equal(down(m.updateGradInput([up(gt, x), counts], up(gt, g))[0]), first[0])
+    m.accGradParameters([up(gt, x), counts], up(gt, g), 1.0)
+    assert torch.equal(down(m.gradWeight), first[1])
+
+
+def test_groups_with_infinite_rows_over_pairs(gt):
+    """An infinity makes the operands stay in FP32; its row's and its group's results are its own."""
+    counts, I, O = [2000, 2100, 1900], 1536, 1536
+    T = sum(counts)
+    x, w, b, g = randn(1, T, I), randn(2, 3, O, I) / I ** 0.5, randn(3, 3, O), randn(4, T, O)
+    m = fill(gt, gt.nn.GroupedLinear(3, I, O, "none"), w, b)
+    x[2500, 7] = float("inf")
+    y = down(m.forward([up(gt, x), counts]))
+    m.gradWeight.zero()
+    m.backward([up(gt, x), counts], up(gt, g))
+    rows = torch.arange(T, device="cuda") != 2500
+    X, W = x.double(), w.double()
+    for e, p in enumerate((slice(0, 2000), slice(2000, 4100), slice(4100, 6000))):
+        k = rows[p]
+        near(y[p][k], (X[p] @ W[e].t() + b[e].double())[k], (rel_of(I) * (X[p].abs() @ W[e].abs().t() + b[e].abs().double()))[k])
+        if e != 1:
+            near(down(m.gradWeight)[e], g[p].double().t() @ X[p], (rel_of(counts[e]) + 4 * E) * (g[p].abs().double().t() @ X[p].abs()))
