@@ -115,8 +115,8 @@ static __global__ void __launch_bounds__(256) fold_columns_kernel(const float *_
 static void act_grad(const Groups &groups, const float *g, long ldg, const float *z, float *gz, long cols, int act, float *gb, float scale) {
   const bool vec = cols % 4 == 0 && ldg % 4 == 0 && (((uintptr_t)g | (uintptr_t)z | (uintptr_t)gz) & 15) == 0;
   const long tiles = (cols + 127) / 128;
-  // pieces of 32 rows and more, as many as leave eight blocks an SM
-  const long wanted = std::max(1l, ctx().sm_count * 8l / tiles), per = std::max(32l, (groups.rows + wanted - 1) / wanted);
+  // pieces of 32 rows and more, as many as leave sixteen blocks an SM
+  const long wanted = std::max(1l, ctx().sm_count * 16l / tiles), per = std::max(32l, (groups.rows + wanted - 1) / wanted);
   auto run = [&](const RowPieces &p) {
     if (!p.count) return;
     float *part = gb ? (float *)ws_alloc(sizeof(float) * p.count * cols) : nullptr;
@@ -260,8 +260,8 @@ THC_API int THGPUNN_FusedLinear_backward(THGPUTensor *input, THGPUTensor *gradOu
   if (act || gradBias)
     act_grad(Groups{&rows, 1, rows}, g.p, g.ld, act ? data_ptr(preactivation) : nullptr, act ? data_ptr(gradPre) : nullptr, out, activation,
              gradBias ? data_ptr(gradBias) : nullptr, scale);
-  if (gradInput) gemm('n', 'n', in, rows, out, 1.f, data_ptr(weight), in, gz, ldgz, 0.f, data_ptr(gradInput), in);
-  if (gradWeight) gemm('n', 't', in, out, rows, scale, x.p, x.ld, gz, ldgz, 1.f, data_ptr(gradWeight), in);
+  if (gradInput || gradWeight)
+    linear_gradients(x.p, x.ld, gz, ldgz, rows, in, out, data_ptr(weight), gradInput ? data_ptr(gradInput) : nullptr, gradWeight ? data_ptr(gradWeight) : nullptr, scale);
   return 0;
   THC_END(1)
 }

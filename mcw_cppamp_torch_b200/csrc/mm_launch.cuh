@@ -107,12 +107,12 @@ static int choose_tail_splits(long tail, long ktiles, int slots, double tile_us)
 static bool raw_matrix_ok(const float *base, long ld) {
   return encode_tiled_fn() && ((uintptr_t)base & 15) == 0 && ld % 4 == 0 && ld > 0;
 }
-// Up to two matrices copied to pitches that TMA can address (blockIdx.y: which): lines of `run` floats.
+// Up to three matrices copied to pitches that TMA can address (blockIdx.y: which): lines of `run` floats.
 struct PackJob { const float *src; float *dst; long lines, run, src_ld, dst_ld; };
-static __global__ void __launch_bounds__(256) pack_matrix_kernel(const PackJob a, const PackJob b) {
+static __global__ void __launch_bounds__(256) pack_matrix_kernel(const PackJob a, const PackJob b, const PackJob c) {
   pdl_begin();
   // a warp copies up to 1024 floats of a line, all its loads in flight before the first store
-  const PackJob &j = blockIdx.y ? b : a;
+  const PackJob &j = blockIdx.y == 0 ? a : blockIdx.y == 1 ? b : c;
   const int lane = threadIdx.x & 31;
   const long warps = (long)gridDim.x * (blockDim.x >> 5), parts = (j.run + 1023) / 1024;
   for (long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < j.lines * parts; w += warps) {
@@ -128,9 +128,10 @@ static __global__ void __launch_bounds__(256) pack_matrix_kernel(const PackJob a
   }
 }
 
-static void launch_pack(const PackJob &a, const PackJob &b) {
-  const long pieces = std::max(a.lines * ((a.run + 1023) / 1024), b.lines * ((b.run + 1023) / 1024));
-  pdl_launch(pack_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), 2), 256, 0, a, b);
+static void launch_pack(const PackJob &a, const PackJob &b, const PackJob &c = {}) {
+  long pieces = 0;
+  for (const PackJob *j : {&a, &b, &c}) pieces = std::max(pieces, j->lines * ((j->run + 1023) / 1024));
+  pdl_launch(pack_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), c.lines ? 3 : 2), 256, 0, a, b, c);
   check_launch("pack_matrix");
 }
 

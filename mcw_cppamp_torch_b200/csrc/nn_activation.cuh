@@ -64,10 +64,16 @@ template <int ACT> __device__ __forceinline__ float activation(float z) {
 }
 template <int ACT> __device__ __forceinline__ float activation_slope(float z) {
   if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : 0.f;
-  else if constexpr (ACT == kActGelu) return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), normal_below(z));
-  else if constexpr (ACT == kActSilu) {
-    const float s = 1.f / (1.f + expf(-z));
-    return s * fmaf(z, 1.f - s, 1.f);
+  else if constexpr (ACT == kActGelu) {          // P(z) + z exp(-z^2 / 2) / sqrt(2 pi)
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752044448170f * z * z));
+    return fmaf(z * 0.39894228040143268f, e, normal_below(z));
+  } else if constexpr (ACT == kActSilu) {        // s (1 + z (1 - s)) with s = 1 / (1 + exp(-z)), neither s nor 1 - s a difference
+    float e, t;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fminf(fabsf(z), 128.f) * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(1.f + e));
+    const float u = e * t, s = z < 0.f ? u : t, rest = z < 0.f ? t : u;
+    return s * fmaf(z, rest, 1.f);
   } else return 1.f;
 }
 #endif

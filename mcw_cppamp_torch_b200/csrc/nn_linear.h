@@ -18,6 +18,8 @@ struct LinearTail {
 // y = act(z) + residual with z = x w^T + b: x [rows][in] at pitch ldx, w [out][in], b may be null
 void linear_product(const float *x, long ldx, long rows, long in, long out, const float *w, const float *b, float *y, const LinearTail &tail);
 
+// gx = gz w, unless null, and gw += scale * gz^T x, unless null: gz [rows][out] at pitch ldg
+void linear_gradients(const float *x, long ldx, const float *gz, long ldg, long rows, long in, long out, const float *w, float *gx, float *gw, float scale);
 namespace mm { struct LinearEpilogue; }
 // y = act(z) + residual in a pass of its own; with the records of a product over pairs, only where that has left its sums in z
 void linear_tail(const float *z, float *y, long rows, long out, const LinearTail &tail, const mm::LinearEpilogue &product);

@@ -54,7 +54,8 @@ static void gemm_raw_t(const float *a, long lda, const float *b, long ldb, long 
 struct GemmSide { const float *p; long ld; bool along_k; long rows; };
 // Orientation of the 256-row tiles and the epilogue for D(i, j) at c[i + j * ldc]: the first side takes the rows unless it has
 // no more than half a tile of them and the other has more.
-static mm::Epilogue gemm_sides(GemmSide &x, GemmSide &y, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
+template <class Side>
+static mm::Epilogue gemm_sides(Side &x, Side &y, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   if (x.rows <= 128 && y.rows > x.rows) {
     std::swap(x, y);
     if (tail) std::swap(tail->rm, tail->rn);
@@ -81,24 +82,27 @@ static void gemm_half(GemmSide x, GemmSide y, long k, float alpha, float beta, f
     attach_raw_map<kBf16>(q.b, hy.p, y.rows, hy.ld, hy.ld, bn2 / 2);
   });
 }
+// Copies the sides of products with k that have a pitch or address that TMA cannot take (a hundredth of a product's time at the sizes that come
+// here) instead of feeding the products through per-thread copies.
+static void pack_sides(GemmSide *const *sides, const long *k, int n) {
+  mm::PackJob jobs[3] = {};
+  int count = 0;
+  for (int i = 0; i < n; i++) {
+    GemmSide &s = *sides[i];
+    if (mm::raw_matrix_ok(s.p, s.ld)) continue;
+    mm::PackJob &j = jobs[count++];
+    j = mm::PackJob{s.p, nullptr, s.along_k ? s.rows : k[i], s.along_k ? k[i] : s.rows, s.ld, ((s.along_k ? k[i] : s.rows) + 3) / 4 * 4};
+    j.dst = (float *)ws_alloc(sizeof(float) * j.lines * j.dst_ld);
+    s.p = j.dst; s.ld = j.dst_ld;
+  }
+  if (count) mm::launch_pack(jobs[0], jobs[1], jobs[2]);
+}
 template <bool FUSED = false>
 static void gemm_raw(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   const mm::Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
-  if (!mm::raw_matrix_ok(x.p, x.ld) || !mm::raw_matrix_ok(y.p, y.ld)) {
-    // a pitch or address that TMA cannot take: copy that matrix (a hundredth of the product's time at the sizes that come
-    // here) instead of feeding the product through per-thread copies
-    mm::PackJob jobs[2] = {};
-    GemmSide *sides[2] = {&x, &y};
-    for (int i = 0; i < 2; i++) {
-      GemmSide &s = *sides[i];
-      if (mm::raw_matrix_ok(s.p, s.ld)) continue;
-      mm::PackJob &j = jobs[i];
-      j = mm::PackJob{s.p, nullptr, s.along_k ? s.rows : k, s.along_k ? k : s.rows, s.ld, ((s.along_k ? k : s.rows) + 3) / 4 * 4};
-      j.dst = (float *)ws_alloc(sizeof(float) * j.lines * j.dst_ld);
-      s.p = j.dst; s.ld = j.dst_ld;
-    }
-    mm::launch_pack(jobs[0], jobs[1]);
-  }
+  GemmSide *sides[2] = {&x, &y};
+  const long ks[2] = {k, k};
+  pack_sides(sides, ks, 2);
   if constexpr (FUSED) { gemm_raw_t<false, false, true>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi, tail); return; }
   if (!x.along_k && y.along_k) gemm_raw_t<true, false>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
   else if (x.along_k && y.along_k) gemm_raw_t<false, false>(x.p, x.ld, y.p, y.ld, x.rows, y.rows, k, epi);
@@ -120,50 +124,79 @@ static void gemm_pairs_t(const void *a, long lda, const void *b, long ldb, long 
     attach_raw_map<kPairs>(q.b, b, n, k, ldb, bn2 / 2);
   });
 }
-// False: there is no room for the pairs, and nothing has been done.
-template <bool FUSED = false>
-static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
+// An operand as pairs.
+struct PairSide : GemmSide {
+  mm::Measured m;
+  mm::PairJob job;
+};
+// Measures and splits up to three operands of products with k, whose form is decided together.  False: there is no room for the pairs, and nothing has
+// been done.
+static bool make_pairs(PairSide *const *sides, const long *k, int n, mm::Ranges &ranges) {
   using namespace mm;
   // the copies, with a little for the measures (under a hundredth of them) and the partial sums (blocks of 256 KB, up to
   // five rounds of clusters)
   double need = 96e6;
-  for (const GemmSide &s : {x, y}) need += 4.1 * (double)(s.along_k ? s.rows : k) * (double)((s.along_k ? k : s.rows) + 64);
-  if (!ws_reserve((size_t)need)) return false;
-  const Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
-  const Measured m[2] = {new_measured(), new_measured()};
-  RangeJob ranges[2];
-  PairJob jobs[2];
-  StraySide strays[2];
-  const GemmSide *sides[2] = {&x, &y};
-  long pieces = 0;
-  for (int i = 0; i < 2; i++) {
+  for (int i = 0; i < n; i++) {
     const GemmSide &s = *sides[i];
-    const long lines = s.along_k ? s.rows : k, run = s.along_k ? k : s.rows, ldp = (run + 63) / 64 * 64;
-    ranges[i] = range_job(s.p, lines, run, s.ld, m[i]);
-    jobs[i] = PairJob{s.p, ws_alloc(sizeof(float) * lines * ldp), lines, run, s.ld, ldp, ((uintptr_t)s.p & 15) == 0 && s.ld % 4 == 0, {}};
-    jobs[i].ranges.rec[0] = m[i].rec; jobs[i].ranges.rec[1] = m[1 - i].rec;
-    strays[i] = StraySide{s.p, s.ld, run, s.along_k, m[i]};
+    need += 4.1 * (double)(s.along_k ? s.rows : k[i]) * (double)((s.along_k ? k[i] : s.rows) + 64);
+  }
+  if (!ws_reserve((size_t)need)) return false;
+  RangeJob measure[3];
+  long pieces = 0;
+  for (int i = 0; i < n; i++) sides[i]->m = new_measured();
+  for (int i = 0; i < n; i++) {
+    const GemmSide &s = *sides[i];
+    const long lines = s.along_k ? s.rows : k[i], run = s.along_k ? k[i] : s.rows, ldp = (run + 63) / 64 * 64;
+    measure[i] = range_job(s.p, lines, run, s.ld, sides[i]->m);
+    PairJob &j = sides[i]->job;
+    j = PairJob{s.p, ws_alloc(sizeof(float) * lines * ldp), lines, run, s.ld, ldp, ((uintptr_t)s.p & 15) == 0 && s.ld % 4 == 0, {}};
+    for (int o = 0; o < n; o++) j.ranges.rec[o] = sides[(i + o) % n]->m.rec;   // its own first
     pieces = std::max(pieces, lines * ((ldp + 511) / 512));
   }
-  launch_ranges(ranges[0], &ranges[1]);
-  pdl_launch(split_matrix_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), 2), 256, 0, jobs[0], jobs[1]);
+  ranges = sides[0]->job.ranges;
+  launch_ranges(measure[0], &measure[1]);
+  if (n > 2) launch_ranges(measure[2], nullptr);
+  const unsigned blocks = (unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l);
+  pdl_launch(split_matrix_kernel, dim3(blocks, 2), 256, 0, sides[0]->job, sides[1]->job);
   check_launch("split_matrix");
-  const Ranges &r = jobs[0].ranges;
-  if constexpr (FUSED) {
-    tail->a = m[0].rec; tail->b = m[1].rec; tail->ranges = r;
-    gemm_pairs_t<false, false, true>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r, tail);
-    Epilogue sums = epi;   // where there are strays the product has left the sums there
-    if (tail->z) sums.out = tail->z;
-    pdl_launch(matrix_strays_kernel, dim3((unsigned)std::min(ceil_div(y.rows, 256), ctx().sm_count), 4), 256, 0, strays[0], strays[1], x.rows, y.rows, sums, r);
-    check_launch("matrix_strays");
-    return true;
+  if (n > 2) {
+    pdl_launch(split_matrix_kernel, dim3(blocks, 1), 256, 0, sides[2]->job, sides[2]->job);
+    check_launch("split_matrix");
   }
-  if (!x.along_k && y.along_k) gemm_pairs_t<true, false>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
-  else if (x.along_k && y.along_k) gemm_pairs_t<false, false>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
-  else if (!x.along_k) gemm_pairs_t<true, true>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
-  else gemm_pairs_t<false, true>(jobs[0].dst, jobs[0].ldp, jobs[1].dst, jobs[1].ldp, x.rows, y.rows, k, epi, r);
-  pdl_launch(matrix_strays_kernel, dim3((unsigned)std::min(ceil_div(y.rows, 256), ctx().sm_count), 4), 256, 0, strays[0], strays[1], x.rows, y.rows, epi, r);
+  return true;
+}
+template <bool FUSED = false>
+static void pairs_product(PairSide x, PairSide y, const mm::Ranges &ranges, long k, float alpha, float beta, float *c, long ldc, const float *row_bias,
+                          mm::LinearEpilogue *tail = nullptr) {
+  using namespace mm;
+  const Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
+  Ranges r = ranges;
+  r.rec[0] = x.m.rec; r.rec[1] = y.m.rec;
+  for (const RangeRec *rec : ranges.rec)
+    if (rec && rec != x.m.rec && rec != y.m.rec) r.rec[2] = rec;
+  const GemmSide &xs = x, &ys = y;
+  if constexpr (FUSED) {
+    tail->a = x.m.rec; tail->b = y.m.rec; tail->ranges = r;
+    gemm_pairs_t<false, false, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r, tail);
+  } else if (!xs.along_k && ys.along_k) gemm_pairs_t<true, false>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
+  else if (xs.along_k && ys.along_k) gemm_pairs_t<false, false>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
+  else if (!xs.along_k) gemm_pairs_t<true, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
+  else gemm_pairs_t<false, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
+  Epilogue sums = epi;   // (with a linear layer's epilogue: where there are strays the product has left the sums there)
+  if (FUSED && tail->z) sums.out = tail->z;
+  pdl_launch(matrix_strays_kernel, dim3((unsigned)std::min(ceil_div(ys.rows, 256), ctx().sm_count), 4), 256, 0, StraySide{xs.p, xs.ld, x.job.run, xs.along_k, x.m},
+             StraySide{ys.p, ys.ld, y.job.run, ys.along_k, y.m}, xs.rows, ys.rows, sums, r);
   check_launch("matrix_strays");
+}
+// False: there is no room for the pairs, and nothing has been done.
+template <bool FUSED = false>
+static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
+  PairSide xp{x, {}, {}}, yp{y, {}, {}};
+  PairSide *sides[2] = {&xp, &yp};
+  const long ks[2] = {k, k};
+  mm::Ranges ranges;
+  if (!make_pairs(sides, ks, 2, ranges)) return false;
+  pairs_product<FUSED>(xp, yp, ranges, k, alpha, beta, c, ldc, row_bias, tail);
   return true;
 }
 // Whether pairs finish before TF32, the passes over the operands included.  Their copies are scratch that TF32 does without: bounded.
@@ -320,6 +353,39 @@ void linear_product(const float *x, long ldx, long rows, long in, long out, cons
   } else {
     gemm_raw<true>(ws, xs, in, 1.f, 0.f, y, out, b, &e);
   }
+}
+
+// gx = gz w and gw += scale * gz^T x: the products gemm() would make of them, with gz split into pairs once where both take pairs, and operands whose
+// pitch TMA cannot take copied once.
+void linear_gradients(const float *x, long ldx, const float *gz, long ldg, long rows, long in, long out, const float *w, float *gx, float *gw, float scale) {
+  WsScope scope;
+  if (ctx().math_mode == 0 && gx && gw && pairs_are_faster(in, rows, out) && pairs_are_faster(in, out, rows) && !small_is_faster(in, rows, out, true) &&
+      !small_is_faster(in, out, rows, true)) {
+    PairSide g{{gz, ldg, true, rows}, {}, {}}, ws{{w, in, false, in}, {}, {}}, xs{{x, ldx, false, in}, {}, {}};
+    PairSide *sides[3] = {&g, &ws, &xs};
+    const long ks[3] = {out, out, rows};
+    mm::Ranges ranges;
+    if (make_pairs(sides, ks, 3, ranges)) {
+      pairs_product(ws, g, ranges, out, 1.f, 0.f, gx, in, nullptr);
+      g.along_k = false; g.rows = out;      // the same lines, summed over
+      pairs_product(xs, g, ranges, rows, scale, 1.f, gw, in, nullptr);
+      return;
+    }
+  }
+  const bool gz_ok = mm::raw_matrix_ok(gz, ldg), input_ok = gz_ok && mm::raw_matrix_ok(w, in), weight_ok = gz_ok && mm::raw_matrix_ok(x, ldx);
+  if (ctx().math_mode == 0 && gx && gw && !(input_ok && weight_ok) && !small_is_faster(in, rows, out, input_ok) && !small_is_faster(in, out, rows, weight_ok) &&
+      !pairs_are_faster(in, rows, out) && !pairs_are_faster(in, out, rows)) {
+    GemmSide g{gz, ldg, true, rows}, ws{w, in, false, in}, xs{x, ldx, false, in};
+    GemmSide *sides[3] = {&g, &ws, &xs};
+    const long ks[3] = {out, out, rows};
+    pack_sides(sides, ks, 3);
+    gemm_raw(ws, g, out, 1.f, 0.f, gx, in, nullptr);
+    g.along_k = false; g.rows = out;
+    gemm_raw(xs, g, rows, scale, 1.f, gw, in, nullptr);
+    return;
+  }
+  if (gx) gemm('n', 'n', in, rows, out, 1.f, w, in, gz, ldg, 0.f, gx, in);
+  if (gw) gemm('n', 't', in, out, rows, scale, x, ldx, gz, ldg, 1.f, gw, in);
 }
 
 // y = beta*y + alpha*op(A)*x.  'n': A is m x n column-major, y has m entries: threads own rows

@@ -96,17 +96,18 @@ static Choice choose_rows(const Groups &g, long features, long K, bool small_ali
   return best;
 }
 
-// A handful of rows in each group, K-major operands in whole 16-byte pieces: the weights' bytes are the bound (few_rows_kernel).
+// A handful of rows in each group, K-major operands in whole 16-byte pieces: the weights' bytes are the bound (few_rows_kernel).  Up to four rows at
+// a time; a group of more reads its weight again, from L2, so that few may have more.
 static bool few_rows_groups(SmallGroups p, const Groups &g) {
   if (!p.a.vec4 || !p.b.vec4 || p.K % 4) return false;
-  long most = 0;
-  for (int e = 0; e < g.n; e++) most = std::max(most, g.counts[e]);
-  if (most > 4) return false;
+  long most = 0, live = 0;
+  for (int e = 0; e < g.n; e++) { most = std::max(most, g.counts[e]); live += g.counts[e] > 0; }
   const std::vector<GroupEntry> entries = row_tiles(g, 4);
+  if (4 * (long)entries.size() > 5 * live) return false;
   for (size_t i = 0; i < entries.size(); i += 65535) {
     p.list = make_list(entries.data() + i, (int)std::min(entries.size() - i, (size_t)65535));
     p.stalled = stall_ctl().dev_flag;
-    launch_few_rows_kernel(p, (int)most, dim3(1, (unsigned)p.list.count));
+    launch_few_rows_kernel(p, (int)std::min(most, 4l), dim3(1, (unsigned)p.list.count));
     check_launch("few_rows");
   }
   return true;
