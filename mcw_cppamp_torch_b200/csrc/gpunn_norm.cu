@@ -142,6 +142,8 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T) norm_forward_kernel(
 
 // Backward.  The blocks stay, each with the rows team, team + teams, ... (a team: T threads), the next row on its way while one is worked on, and
 // with the sums of its columns for the weight's and the bias's gradient in registers, which part[block][2][D] gets.  gx or part may be null.
+// gx is summed without fused multiply-adds: of a row of two values the formula leaves eps / (var + eps) of its terms, which then is the same
+// whatever else evaluates it step by step in FP32.
 // 16384 x 4096: 119 us, 6.7 TB/s.
 template <int T, int V, bool VEC>
 static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) norm_backward_kernel(const float *__restrict__ x, const float *__restrict__ g, float *__restrict__ gx,
@@ -186,12 +188,12 @@ static __global__ void __launch_bounds__(T < 128 ? 256 : T, T < 512 ? 2 : 1) nor
 #pragma unroll
     for (int j = 0; j < 4 * V; j++) {
       s.x += c.v[j];
-      s.y = fmaf(c.v[j], a.v[j], s.y);
+      s.y = __fadd_rn(s.y, __fmul_rn(c.v[j], a.v[j]));
     }
     s = sums(s);
     const float one = s.x / (float)D, two = s.y / (float)D;
 #pragma unroll
-    for (int j = 0; j < 4 * V; j++) a.v[j] = i * (c.v[j] - one - a.v[j] * two);
+    for (int j = 0; j < 4 * V; j++) a.v[j] = i * __fsub_rn(c.v[j] - one, __fmul_rn(a.v[j], two));
     a.store(gx + r * D, t, D);
   }
   if (!part) return;

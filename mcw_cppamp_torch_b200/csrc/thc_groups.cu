@@ -70,12 +70,14 @@ static long tiles_of(const Groups &g, long width) {
 }
 enum Way { kSmall, kEngine, kEnginePairs };   // the warp-level engine; the two-SM one over FP32 values; over FP16 pairs
 struct Choice { Way way; int width; };
-// Passes over `values` values that make pairs of them, as pairs_are_faster() has it.
-static double pair_passes_us(double values) { return 14 + 4e-6 * values * (1 / 5.5 + 2 / 5.0); }
+// Passes over `values` values that make pairs of them, as pairs_are_faster() has it; value by value where 16-byte accesses do not fit (15 M values of
+// 1653 columns: 62 us).
+static double pair_passes_us(double values, bool aligned) { return 14 + 4e-6 * values * (1 / 5.5 + 2 / 5.0) * (aligned ? 1 : 1.4); }
+// Copies of operands whose pitch TMA cannot take, `bytes` read and written (the same 15 M values: 10 us).
+static double pack_us(double bytes) { return bytes ? 4 + bytes / 8e6 : 0; }
 static bool pairs_fit(const Groups &g, double values) { return ctx().math_mode == 0 && g.n <= kPaddedGroups && g.rows < 1l << 28 && 4 * values < 16e9 && encode_tiled_fn(); }
 // For kGroupRows: the way and the width of its tiles along the rows that finish first.  The two-SM engine takes all tiles round by round, with two k
-// tiles for a tile's epilogue and, where its operands have to be copied, `pack` bytes at 2 TB/s; pairs of the `values` of both operands take
-// their passes.
+// tiles for a tile's epilogue; copies of `pack` bytes, and pairs of the `values` of both operands, take their passes.
 static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, double values) {
   Choice best{kSmall, 64};
   double least = 0;
@@ -88,9 +90,9 @@ static Choice choose_rows(const Groups &g, long features, long K, bool small_ali
   const bool pairs = pairs_fit(g, values);
   for (int w : {256, 192, 128, 64}) {
     const double rounds = std::ceil((double)((features + 255) / 256) * (double)tiles_of(g, w) / (ctx().sm_count / 2));
-    const double us = 10 + rounds * (double)(ktiles + 2) * group_tile_us(w) + (pack ? 5 + pack / 2e6 : 0);
+    const double us = 10 + rounds * (double)(ktiles + 2) * group_tile_us(w) + pack_us(pack);
     if (us < least) { best = Choice{kEngine, w}; least = us; }
-    const double with_pairs = 10 + rounds * (double)(ktiles_half + 2) * tc2_tile_us(w, kPairs) + pair_passes_us(values);
+    const double with_pairs = 10 + rounds * (double)(ktiles_half + 2) * tc2_tile_us(w, kPairs) + pair_passes_us(values, pack == 0);
     if (pairs && with_pairs < least) { best = Choice{kEnginePairs, w}; least = with_pairs; }
   }
   return best;
@@ -370,7 +372,7 @@ static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &
     const int w = tc2_tile_width(out, pairs);
     const double tiles = (double)((in + 255) / 256) * (double)((out + w - 1) / w), k = (double)(pairs ? halves : ktiles), longest = (double)(pairs ? (most + 1) / 2 : most);
     const double us = 10 + std::max(tiles * (k + 2 * (double)live) / (ctx().sm_count / 2), longest + 2) * (pairs ? tc2_tile_us(w, kPairs) : group_tile_us(w)) +
-                      (pairs ? pair_passes_us(values) : bytes ? 5 + bytes / 2e6 : 0);
+                      (pairs ? pair_passes_us(values, bytes == 0) : pack_us(bytes));
     if (us < least) { best = Choice{pairs ? kEnginePairs : kEngine, w}; least = us; }
   }
   return best;
