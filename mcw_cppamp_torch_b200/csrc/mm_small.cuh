@@ -82,7 +82,7 @@ struct SmallGroups : SmallFused {
       p.N = g.end - g.first;
     } else {
       p.K = g.end - g.first;
-      k_tiles = (p.K + TC_BK - 1) / TC_BK;
+      k_tiles = ((p.K + TC_BK - 1) / TC_BK + slices - 1) / slices;
     }
     return p;
   }

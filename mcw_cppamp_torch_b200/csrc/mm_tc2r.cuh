@@ -277,6 +277,7 @@ struct Tc2rItem {
   long slot;   // partial-sum block of the workspace (tail items only)
   int num_k_tiles;
   int group, k_left;   // of a grouped product: the group, and the k of this item
+  int width;           // of its tile: the columns there are, in whole steps
   long n_end, shift;   // the end of this item's columns, and how far they lie behind the result's
 };
 
@@ -333,6 +334,10 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         t.n_tile0 = (long)nt * BN2; t.n_end = p.N; t.shift = 0; t.k_begin = g.first; t.k_left = g.end - g.first;
       }
       t.num_k_tiles = (t.k_left + KV - 1) / KV;
+      // The MMAs take as many columns as the tile has, in steps of 64 (of 128 where each CTA's rows of B come in blocks of 64 values): each CTA
+      // then has half of those.  The last tiles of a few hundred rows a group, at full width, were a fifth of all MMAs.
+      constexpr int STEP = HALF && P::OpB::MN_MAJOR ? 128 : 64;
+      t.width = (int)min((long)BN2, (t.n_end - t.n_tile0 + STEP - 1) / STEP * STEP);
       return t;
     }
     uint32_t tile = w;
@@ -486,6 +491,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         const int k_left = P::GROUPS == kGroupSums ? item.k_left - 32 * it : 32;
 #pragma unroll
         for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+          if (P::GROUPS != 0 && i0 * GT * 16 >= Cfg::A_BYTES + item.width / 2 * 128) break;   // rows of B that no MMA reads
           uint4 v[BATCH];
 #pragma unroll
           for (int i = 0; i < BATCH; i++) v[i] = lds128(src + (uint32_t)((i0 + i) * GT * 16));
@@ -515,7 +521,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
     if (HALF && warp == T2_MMA_WARP && rank == 0) {
       // ---------------------------------------------------------- MMA issuer of 16-bit operands: one warp, CHAIN k tiles per buffer
       constexpr bool A_MN = P::OpA::MN_MAJOR, B_MN = P::OpB::MN_MAJOR;
-      constexpr uint32_t idesc = PAIRS ? umma2_idesc_f16(BN2, A_MN, B_MN) : umma2_idesc_bf16(BN2, A_MN, B_MN);
+      uint32_t idesc = PAIRS ? umma2_idesc_f16(BN2, A_MN, B_MN) : umma2_idesc_bf16(BN2, A_MN, B_MN);
       const uint32_t ring = smem_u32(smem);
       uint32_t s = 0, phase = 0, buf = 0, acc_phase = 0;
       for (uint32_t n = 0; ok; n++) {
@@ -525,7 +531,9 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         w = __shfl_sync(0xffffffffu, w, 0);
         if (lane == 0) sched.done(n);
         if (w == T2R_NO_ITEM) break;
-        const int nk = item_at(w).num_k_tiles;
+        const Tc2rItem item = item_at(w);
+        const int nk = item.num_k_tiles;
+        if constexpr (P::GROUPS != 0) idesc = umma2_idesc_f16(item.width, A_MN, B_MN);
         for (int it = 0; it < nk; it++) {
           const bool first = it % CHAIN == 0, last = it % CHAIN == CHAIN - 1 || it == nk - 1;
           const uint32_t d = tmem_base + buf * BN2;
@@ -584,7 +592,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
       // A scheme in which a warp skips whole revolutions (alternate ITEMS instead of alternate tiles) loses that
       // guarantee and stalls.
       constexpr bool A_MN = P::OpA::MN_MAJOR, B_MN = P::OpB::MN_MAJOR;
-      constexpr uint32_t idesc = umma2_idesc_tf32(BN2, A_MN, B_MN);
+      uint32_t idesc = umma2_idesc_tf32(BN2, A_MN, B_MN);
       const int mine = warp == T2_MMA_WARP ? 0 : 1;
       int g0 = 0;
       for (uint32_t n = 0; ok; n++) {
@@ -594,7 +602,9 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         w = __shfl_sync(0xffffffffu, w, 0);
         if (lane == 0) sched.done(n);
         if (w == T2R_NO_ITEM) break;
-        const int nk = item_at(w).num_k_tiles;
+        const Tc2rItem item = item_at(w);
+        const int nk = item.num_k_tiles;
+        if constexpr (P::GROUPS != 0) idesc = umma2_idesc_tf32(item.width, A_MN, B_MN);
         for (int it = (g0 + mine) & 1; it < nk; it += 2) {
           const int g = g0 + it;
           const int s = g % R, ls = g % LM, buf = ACCS == 2 ? mine : g % ACCS;
@@ -646,7 +656,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         if (rank == 0 && lane == 0) mbar_arrive_local(bar_sched_go);   // item n is under way: time to fetch the number of item n + 1
         const Tc2rItem item = item_at(w);
         auto load_a = make_loader<TileLoader<TC_BM, PREC, WIDE, typename P::OpA>>(p.a, item.m_tile0 + (long)rank * TC_BM, item.k_begin, item.group);   // (gathered: nothing)
-        TileLoader<BH, PREC, WIDE, typename P::OpB> load_b(p.b, item.n_tile0 + (long)rank * BH, item.k_begin);
+        TileLoader<BH, PREC, WIDE, typename P::OpB> load_b(p.b, item.n_tile0 + (long)rank * (P::GROUPS != 0 ? item.width / 2 : BH), item.k_begin);
         for (int t = 0; ok && t < item.num_k_tiles; t++) {
 #pragma unroll
           for (int part = 0; part < PARTS; part++) {
@@ -724,6 +734,7 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
         const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN2 + (pair_lines ? h * 32 : h * NCOL));
 #pragma unroll
         for (int c0 = 0; c0 < NCOL; c0 += 32) {
+          if (P::GROUPS != 0 && h * NCOL + c0 >= item.width) continue;   // columns that nobody has written
           uint32_t v[32];
           tmem_ld32_nowait(t0 + (pair_lines ? 2 * c0 : c0), v);
           tmem_ld_wait();

@@ -7,6 +7,8 @@
 // A launch per group, as gemm() would have it, leaves most of the device idle behind each (37 groups of some 40 rows, 333 -> 515: three products
 // took 785 us); here the pieces of all groups are a launch's work items.  The 64-row (or 256-row) side of a tile is the features', so that a weight
 // that meets few rows is read once, in tiles as narrow as the rows.
+#include <map>
+
 #include "mm_launch.cuh"
 #include "nn_linear.h"
 
@@ -47,6 +49,12 @@ static std::vector<GroupEntry> row_tiles(const Groups &g, int width) {
     for (long i = 0; i < g.counts[e]; i += width) v.push_back(GroupEntry{e, (int)(r + i), (int)(r + std::min<long>(g.counts[e], i + width)), 0});
   return v;
 }
+// The same with the pieces that are not full behind those that are, the largest first: the clusters take items as they finish, and short ones level
+// the end.
+static std::vector<GroupEntry> largest_first(std::vector<GroupEntry> v) {
+  std::stable_sort(v.begin(), v.end(), [](const GroupEntry &a, const GroupEntry &b) { return a.end - a.first > b.end - b.first; });
+  return v;
+}
 static std::vector<GroupEntry> whole_groups(const Groups &g) {
   std::vector<GroupEntry> v;
   long r = 0;
@@ -61,8 +69,48 @@ static double small_groups_us(double features, double tiles, double steps, int b
   const double step = bn == 64 ? 1.35 + 0.4 * resident : bn == 32 ? 1.3 + 0.15 * resident : bn == 16 ? 0.6 + 0.15 * resident : 0.45 + 0.15 * resident;
   return 5 + (aligned ? 1.0 : 1.3) * step * features * (steps + 3 * tiles) / ctx().sm_count / resident;
 }
-// The two-SM engine's k tile over FP32 values: 16 groups of 512 rows, 1024 -> 4096, 298 / 342 / 336 / 495 us with tiles of 256 / 192 / 128 / 64 columns.
-static double group_tile_us(int width) { return width == 256 ? 1.25 : width == 192 ? 0.91 : width == 128 ? 0.71 : 0.52; }
+// The two-SM engine's k tile of `columns` columns in tiles of up to `width`.  FP32 values: 16 groups of 512 rows, 1024 -> 4096, 298 / 342 / 336 / 495 us
+// with tiles of 256 / 192 / 128 / 64 columns; fewer columns spare the MMAs, but the loads and most of the splitting go on (32 groups of
+// some 16 rows, 1024 -> 2048: 145 / 121 / 99 / 92 us).
+static double group_tile_us(int columns, int width, bool pairs) {
+  if (pairs) return std::max(tc2_tile_us(columns, kPairs), 0.75 * tc2_tile_us(width, kPairs));
+  const double mma = columns == 256 ? 1.25 : columns == 192 ? 0.91 : columns == 128 ? 0.71 : 0.52;
+  return std::max(mma, width == 256 ? 0.95 : width == 192 ? 0.8 : width == 128 ? 0.65 : 0.58);
+}
+// Work items of a launch, the longest first: how many take how long.
+struct Items {
+  double us[5] = {};
+  long n[5] = {};
+};
+// When the last cluster is done if each takes the next item as it finishes one.
+static double makespan_us(const Items &items) {
+  std::map<double, long> done;     // clusters by the time they are free
+  done[0] = ctx().sm_count / 2;
+  for (int i = 0; i < 5; i++)
+    for (long n = items.n[i]; n > 0;) {
+      const auto first = *done.begin();
+      const long take = std::min(first.second, n);
+      done.erase(done.begin());
+      if (take < first.second) done[first.first] = first.second - take;
+      done[first.first + items.us[i]] += take;
+      n -= take;
+    }
+  return 10 + done.rbegin()->first;
+}
+// Adds the tiles along `n` columns, at most `width` each, the last as wide as it has to be, `features` times; k tiles of one of them.
+static void add_tiles(Items &items, long n, int width, int step, long features, double k, bool pairs) {
+  items.us[0] = k * group_tile_us(width, width, pairs);
+  items.n[0] += n / width * features;
+  const int rest = (int)((n % width + step - 1) / step * step);
+  if (!rest) return;
+  const int i = rest == width ? 0 : 5 - rest / 64;
+  items.us[i] = k * group_tile_us(rest, width, pairs);
+  items.n[i] += features;
+}
+static double columns_us(long n, int width, int step, bool pairs) {
+  const long rest = (n % width + step - 1) / step * step;
+  return (double)(n / width) * group_tile_us(width, width, pairs) + (rest ? group_tile_us((int)rest, width, pairs) : 0);
+}
 static long tiles_of(const Groups &g, long width) {
   long t = 0;
   for (int e = 0; e < g.n; e++) t += (g.counts[e] + width - 1) / width;
@@ -76,9 +124,9 @@ static double pair_passes_us(double values, bool aligned) { return 14 + 4e-6 * v
 // Copies of operands whose pitch TMA cannot take, `bytes` read and written (the same 15 M values: 10 us).
 static double pack_us(double bytes) { return bytes ? 4 + bytes / 8e6 : 0; }
 static bool pairs_fit(const Groups &g, double values) { return ctx().math_mode == 0 && g.n <= kPaddedGroups && g.rows < 1l << 28 && 4 * values < 16e9 && encode_tiled_fn(); }
-// For kGroupRows: the way and the width of its tiles along the rows that finish first.  The two-SM engine takes all tiles round by round, with two k
-// tiles for a tile's epilogue; copies of `pack` bytes, and pairs of the `values` of both operands, take their passes.
-static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, double values) {
+// For kGroupRows: the way and the width of its tiles along the rows that finish first.  The two-SM engine takes two k
+// tiles' time for a tile's epilogue, and more where that has exponentials; copies of `pack` bytes, and pairs of the `values` of both operands, take their passes.
+static Choice choose_rows(const Groups &g, long features, long K, bool small_aligned, double pack, double values, int act = kActNone) {
   Choice best{kSmall, 64};
   double least = 0;
   const long ktiles = (K + 31) / 32, ktiles_half = (K + 63) / 64;
@@ -87,13 +135,15 @@ static Choice choose_rows(const Groups &g, long features, long K, bool small_ali
     if (!least || us < least) { best = Choice{kSmall, w}; least = us; }
   }
   if (!encode_tiled_fn()) return best;
-  const bool pairs = pairs_fit(g, values);
-  for (int w : {256, 192, 128, 64}) {
-    const double rounds = std::ceil((double)((features + 255) / 256) * (double)tiles_of(g, w) / (ctx().sm_count / 2));
-    const double us = 10 + rounds * (double)(ktiles + 2) * group_tile_us(w) + pack_us(pack);
-    if (us < least) { best = Choice{kEngine, w}; least = us; }
-    const double with_pairs = 10 + rounds * (double)(ktiles_half + 2) * tc2_tile_us(w, kPairs) + pair_passes_us(values, pack == 0);
-    if (pairs && with_pairs < least) { best = Choice{kEnginePairs, w}; least = with_pairs; }
+  for (bool pairs : {false, true}) {
+    if (pairs && !pairs_fit(g, values)) break;
+    for (int w : {256, 192, 128, 64}) {
+      Items items;
+      const double k = (double)(pairs ? ktiles_half : ktiles) + 2 + (act >= kActGelu ? w / 64 : 0);
+      for (int e = 0; e < g.n; e++) add_tiles(items, g.counts[e], w, 64, (features + 255) / 256, k, pairs);
+      const double us = makespan_us(items) + (pairs ? pair_passes_us(values, pack == 0) : pack_us(pack));
+      if (us < least) { best = Choice{pairs ? kEnginePairs : kEngine, w}; least = us; }
+    }
   }
   return best;
 }
@@ -121,18 +171,16 @@ static void small_groups(SmallGroups p, const std::vector<GroupEntry> &entries, 
   for (size_t i = 0; i < entries.size(); i += most) {
     const int n = (int)std::min(entries.size() - i, (size_t)most);
     p.list = make_list(entries.data() + i, n);
-    p.slices = 1;
-    p.tiles_per_slice = INT_MAX;
     p.ws = nullptr;
-    if (p.kind == kGroupRows) {
-      const long tiles = (long)ceil_div(p.M, 64) * n, ktiles = ceil_div(p.K, TC_BK);
-      const long slices = small_slices(tiles, ktiles, bn);
-      p.tiles_per_slice = ceil_div(ktiles, slices);
-      p.slices = ceil_div(ktiles, p.tiles_per_slice);
-      if (p.slices > 1) {
-        p.ws = (float *)ws_alloc(sizeof(float) * tiles * p.slices * 64 * bn);
-        p.tickets = zero_words();
-      }
+    long k = p.K;     // of the longest
+    if (p.kind == kGroupSums)
+      for (int q = 0; q < n; q++) k = std::max<long>(k, entries[i + q].end - entries[i + q].first);
+    const long tiles = (long)ceil_div(p.M, 64) * n * p.column_tiles, ktiles = ceil_div(k, TC_BK), slices = tiles > 2 * ctx().sm_count ? 1 : small_slices(tiles, ktiles, bn);
+    p.tiles_per_slice = ceil_div(ktiles, slices);
+    p.slices = ceil_div(ktiles, p.tiles_per_slice);
+    if (p.slices > 1) {
+      p.ws = (float *)ws_alloc(sizeof(float) * tiles * p.slices * 64 * bn);
+      p.tickets = zero_words();
     }
     launch_small_width(p, bn, a_k, b_k);
   }
@@ -200,7 +248,7 @@ static void engine_rows(const Groups &g, Lines a, Lines b, long features, long K
   p.M = features; p.N = g.rows; p.K = K;
   p.bias_group = bias_group;
   p.tail = tail;
-  launch_groups(p, width, row_tiles(g, width), (features + 255) / 256, [&](auto &q, int bn2) {
+  launch_groups(p, width, largest_first(row_tiles(g, width)), (features + 255) / 256, [&](auto &q, int bn2) {
     attach_group_map<MN, kTf32>(q.a, a.p, g.n, features, K, a.ld, TC_BM);
     attach_raw_map<kTf32>(q.b, b.p, g.rows, K, b.ld, bn2 / 2);
   });
@@ -277,7 +325,7 @@ static void pairs_rows(const Groups &g, const GroupPairs &gp, const PairSide &w,
   p.bias_group = out;
   p.tail = tail;
   p.range_a = w.m.rec; p.range_b = x.m.rec; p.ranges = gp.ranges;
-  launch_groups(p, width, padded(row_tiles(g, width), gp.rows), (features + 255) / 256, [&](auto &q, int bn2) {
+  launch_groups(p, width, padded(largest_first(row_tiles(g, width)), gp.rows), (features + 255) / 256, [&](auto &q, int bn2) {
     attach_group_map<MN, kPairs>(q.a, w.dst, g.n, features, K, w.ldp, TC_BM);
     attach_raw_map<kPairs>(q.b, x.dst, gp.padded(), K, x.ldp, bn2 / 2);
   });
@@ -307,7 +355,7 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
   p.at = GroupPlaces{out * in, 0, ldx, 0, out, out};
   if (few_rows_groups(p, g)) return;
   const Lines ws{w, (long)g.n * out, in, in}, xs{x, g.rows, in, ldx};
-  const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), (double)in * (double)(g.n * out + g.rows));
+  const Choice c = choose_rows(g, out, in, ws.ok() && xs.ok(), pack_bytes(ws, xs), (double)in * (double)(g.n * out + g.rows), act);
   if (c.way != kSmall) {
     Epilogue epi{y, nullptr, 1.f, 0.f, LONG_MAX, 0, out};
     epi.row_bias = b;
@@ -350,11 +398,6 @@ static void grad_input(const Groups &g, const Choice &c, const float *gz, long l
   p.at = GroupPlaces{out * in, 0, ldg, 0, in, 0};
   small_groups(p, row_tiles(g, c.width), c.width, false, true);
 }
-// The largest first: the clusters take items as they finish, and short ones level the end.
-static std::vector<GroupEntry> largest_first(std::vector<GroupEntry> v) {
-  std::stable_sort(v.begin(), v.end(), [](const GroupEntry &a, const GroupEntry &b) { return a.end - a.first > b.end - b.first; });
-  return v;
-}
 static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &gs) {
   const long in = xs.run, out = gs.run;
   long ktiles = 0, halves = 0, most = 0, live = 0;
@@ -368,12 +411,18 @@ static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &
   Choice best{kSmall, bn};
   double least = small_groups_us((double)((in + 63) / 64), columns * (double)live, columns * (double)ktiles, bn, xs.ok() && gs.ok());
   if (!encode_tiled_fn()) return best;
-  for (int pairs = 0; pairs < (pairs_fit(g, values) ? 2 : 1); pairs++) {
-    const int w = tc2_tile_width(out, pairs);
-    const double tiles = (double)((in + 255) / 256) * (double)((out + w - 1) / w), k = (double)(pairs ? halves : ktiles), longest = (double)(pairs ? (most + 1) / 2 : most);
-    const double us = 10 + std::max(tiles * (k + 2 * (double)live) / (ctx().sm_count / 2), longest + 2) * (pairs ? tc2_tile_us(w, kPairs) : group_tile_us(w)) +
-                      (pairs ? pair_passes_us(values, bytes == 0) : pack_us(bytes));
-    if (us < least) { best = Choice{pairs ? kEnginePairs : kEngine, w}; least = us; }
+  for (bool pairs : {false, true}) {
+    if (pairs && !pairs_fit(g, values)) break;
+    for (int w : {256, 192, 128, 64}) {
+      if (pairs && w % 128) continue;
+      const long tiles = (in + 255) / 256 * ((out + w - 1) / w);
+      const double per = (double)((in + 255) / 256), total = per * columns_us(out, w, pairs ? 128 : 64, pairs) * ((double)(pairs ? halves : ktiles) + (pairs ? 6 : 2) * (double)live);
+      const double longest = ((double)(pairs ? (most + 1) / 2 : most) + 2) * group_tile_us(w, w, pairs);
+      // items of many lengths, the longest first: level but for what the last are long.  (Accumulating a tile takes as long as six k tiles of pairs.)
+      const double us = 10 + std::max(total / (ctx().sm_count / 2) + 0.25 * total / (double)(tiles * std::max(live, 1l)), longest) +
+                        (pairs ? pair_passes_us(values, bytes == 0) : pack_us(bytes));
+      if (us < least) { best = Choice{pairs ? kEnginePairs : kEngine, w}; least = us; }
+    }
   }
   return best;
 }
@@ -390,7 +439,7 @@ static void grad_weight(const Groups &g, const Choice &c, Lines xs, Lines gs, fl
     GroupProblem<RawOperand<true>, RawOperand<true>, kGroupSums, false> p;
     set_sums(p, in, out, gw, scale);
     p.K = g.rows;
-    const int bn2 = tc2_tile_width(out);
+    const int bn2 = c.width;
     launch_groups(p, bn2, largest_first(whole_groups(g)), ((in + 255) / 256) * ((out + bn2 - 1) / bn2), [&](auto &q, int) {
       attach_raw_map<kTf32>(q.a, xs.p, in, g.rows, xs.ld, TC_BM);
       attach_raw_map<kTf32>(q.b, gs.p, out, g.rows, gs.ld, bn2 / 2);
@@ -407,13 +456,12 @@ static void grad_weight(const Groups &g, const Choice &c, Lines xs, Lines gs, fl
   p.at = GroupPlaces{0, xs.ld, gs.ld, out * in, 0, 0};
   small_groups(p, whole_groups(g), c.width, false, false);
 }
-static void pairs_sums(const Groups &g, const GroupPairs &gp, const PairSide &x, const PairSide &gz, float *gw, float scale) {
+static void pairs_sums(const Groups &g, const GroupPairs &gp, int w, const PairSide &x, const PairSide &gz, float *gw, float scale) {
   const long in = x.run, out = gz.run;
   GroupProblem<RawOperand<true, kPairs>, RawOperand<true, kPairs>, kGroupSums, false, kPairs> p;
   set_sums(p, in, out, gw, scale);
   p.K = gp.padded();
   p.range_a = x.m.rec; p.range_b = gz.m.rec; p.ranges = gp.ranges;
-  const int w = tc2_tile_width(out, true);
   launch_groups(p, w, largest_first(padded(whole_groups(g), gp.rows)), ((in + 255) / 256) * ((out + w - 1) / w), [&](auto &q, int bn2) {
     attach_raw_map<kPairs>(q.a, x.dst, in, gp.padded(), x.ldp, TC_BM);
     attach_raw_map<kPairs>(q.b, gz.dst, out, gp.padded(), gz.ldp, bn2 / 2);
@@ -443,7 +491,7 @@ void group_backward(const Groups &g, const float *x, long ldx, const float *gz, 
         gx = nullptr;
       }
       if (pw) {
-        pairs_sums(g, pairs, xp, gp, gw, scale);
+        pairs_sums(g, pairs, cw.width, xp, gp, gw, scale);
         gw = nullptr;
       }
     }
