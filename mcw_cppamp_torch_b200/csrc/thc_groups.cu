@@ -172,10 +172,20 @@ static void small_groups(SmallGroups p, const std::vector<GroupEntry> &entries, 
     const int n = (int)std::min(entries.size() - i, (size_t)most);
     p.list = make_list(entries.data() + i, n);
     p.ws = nullptr;
-    long k = p.K;     // of the longest
-    if (p.kind == kGroupSums)
-      for (int q = 0; q < n; q++) k = std::max<long>(k, entries[i + q].end - entries[i + q].first);
-    const long tiles = (long)ceil_div(p.M, 64) * n * p.column_tiles, ktiles = ceil_div(k, TC_BK), slices = tiles > 2 * ctx().sm_count ? 1 : small_slices(tiles, ktiles, bn);
+    const long tiles = (long)ceil_div(p.M, 64) * n * p.column_tiles;
+    long ktiles = ceil_div(p.K, TC_BK), slices = 1;
+    if (p.kind == kGroupRows) {
+      if (tiles <= 2 * ctx().sm_count) slices = small_slices(tiles, ktiles, bn);
+    } else if (tiles <= kZeroWords) {
+      // groups of unlike lengths: none longer than a block's share of all k tiles, or than sixteen
+      long all = 0;
+      for (int q = 0; q < n; q++) {
+        const long t = ceil_div(entries[i + q].end - entries[i + q].first, TC_BK);
+        all += t * (tiles / n);
+        ktiles = std::max(ktiles, t);
+      }
+      slices = std::min(32l, (long)ceil_div(ktiles, std::max(16l, all / (3l * ctx().sm_count))));
+    }
     p.tiles_per_slice = ceil_div(ktiles, slices);
     p.slices = ceil_div(ktiles, p.tiles_per_slice);
     if (p.slices > 1) {
@@ -206,19 +216,17 @@ struct Lines {
 static double pack_bytes(const Lines &a, const Lines &b) {
   return (a.ok() ? 0 : 8. * (double)a.lines * (double)a.run) + (b.ok() ? 0 : 8. * (double)b.lines * (double)b.run);
 }
-static void pack(Lines &a, Lines &b) {
-  PackJob jobs[2] = {};
-  Lines *l[2] = {&a, &b};
-  bool any = false;
-  for (int i = 0; i < 2; i++) {
-    if (l[i]->ok()) continue;
-    any = true;
-    const long ld = (l[i]->run + 3) / 4 * 4;
-    float *to = (float *)ws_alloc(sizeof(float) * l[i]->lines * ld);
-    jobs[i] = PackJob{l[i]->p, to, l[i]->lines, l[i]->run, l[i]->ld, ld};
-    l[i]->p = to; l[i]->ld = ld;
+static void pack(Lines &a, Lines &b, Lines *c = nullptr) {
+  PackJob jobs[3] = {};
+  int n = 0;
+  for (Lines *l : {&a, &b, c}) {
+    if (!l || l->ok()) continue;
+    const long ld = (l->run + 3) / 4 * 4;
+    float *to = (float *)ws_alloc(sizeof(float) * l->lines * ld);
+    jobs[n++] = PackJob{l->p, to, l->lines, l->run, l->ld, ld};
+    l->p = to; l->ld = ld;
   }
-  if (any) launch_pack(jobs[0], jobs[1]);
+  if (n) launch_pack(jobs[0], jobs[1], jobs[2]);
 }
 template <class P, class Attach>
 static void launch_groups(P p, int bn2, const std::vector<GroupEntry> &entries, long tiles_of_entry, Attach attach) {
@@ -383,19 +391,19 @@ static Choice choose_grad_input(const Groups &g, long ldg, const float *gz, long
   const Lines ws{w, (long)g.n * out, in, in}, gs{gz, g.rows, out, ldg};
   return choose_rows(g, in, out, ws.ok() && gs.ok(), pack_bytes(ws, gs), (double)out * (double)(g.n * in + g.rows));
 }
-static void grad_input(const Groups &g, const Choice &c, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
+static void grad_input(const Groups &g, const Choice &c, const Lines &gz, long in, long out, const Lines &w, float *gx) {
   WsScope scope;
   if (c.way != kSmall) {
-    engine_rows<true, false>(g, Lines{w, (long)g.n * out, in, in}, Lines{gz, g.rows, out, ldg}, in, out, c.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, 0, {});
+    engine_rows<true, false>(g, w, gz, in, out, c.width, Epilogue{gx, nullptr, 1.f, 0.f, LONG_MAX, 0, in}, 0, {});
     return;
   }
   SmallGroups p = {};
-  p.a = small_operand(w, in); p.b = small_operand(gz, ldg);
+  p.a = small_operand(w.p, w.ld); p.b = small_operand(gz.p, gz.ld);
   p.M = (int)in; p.N = 0; p.K = (int)out;
   p.c = gx; p.sm = 1; p.sn = in;
   p.alpha = 1.f;
   p.kind = kGroupRows; p.column_tiles = 1;
-  p.at = GroupPlaces{out * in, 0, ldg, 0, in, 0};
+  p.at = GroupPlaces{out * w.ld, 0, gz.ld, 0, in, 0};
   small_groups(p, row_tiles(g, c.width), c.width, false, true);
 }
 static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &gs) {
@@ -478,7 +486,7 @@ void group_backward(const Groups &g, const float *x, long ldx, const float *gz, 
       }))
     return;
   WsScope scope;
-  const Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
+  Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
   const Choice ci = gx ? choose_grad_input(g, ldg, gz, in, out, w) : Choice{kSmall, 64}, cw = gw ? choose_grad_weight(g, xs, gs) : Choice{kSmall, 64};
   const bool pi = gx && ci.way == kEnginePairs, pw = gw && cw.way == kEnginePairs;
   if (pi || pw) {
@@ -496,7 +504,9 @@ void group_backward(const Groups &g, const float *x, long ldx, const float *gz, 
       }
     }
   }
-  if (gx) grad_input(g, ci, gz, ldg, in, out, w, gx);
+  Lines ws{w, (long)g.n * out, in, in};
+  if (gx && gw && ci.way != kSmall && cw.way != kSmall) pack(gs, ws, &xs);   // once for both
+  if (gx) grad_input(g, ci, gs, in, out, ws, gx);
   if (gw) grad_weight(g, cw, xs, gs, gw, scale);
 }
 
