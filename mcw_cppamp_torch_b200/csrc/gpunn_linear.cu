@@ -220,6 +220,7 @@ using namespace thc;
 THC_API int THGPUNN_FusedLinear_updateOutput(THGPUTensor *input, THGPUTensor *residual, THGPUTensor *output, THGPUTensor *preactivation, THGPUTensor *weight,
                                              THGPUTensor *bias, int activation) {
   THC_BEGIN
+  THC_ARG(input && output && weight, 1, "tensors expected");
   check_act(activation, 7);
   check_here({input, residual, output, preactivation, weight, bias});
   check_forward(input, weight, bias, 0, 5);
@@ -246,6 +247,7 @@ THC_API int THGPUNN_FusedLinear_updateOutput(THGPUTensor *input, THGPUTensor *re
 THC_API int THGPUNN_FusedLinear_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *preactivation, THGPUTensor *gradPre,
                                          THGPUTensor *weight, THGPUTensor *gradWeight, THGPUTensor *gradBias, int activation, float scale) {
   THC_BEGIN
+  THC_ARG(input && gradOutput && weight, 1, "tensors expected");
   check_act(activation, 9);
   check_here({input, gradOutput, gradInput, preactivation, gradPre, weight, gradWeight, gradBias});
   check_backward(input, gradOutput, gradInput, preactivation, gradPre, weight, gradWeight, gradBias, activation, 0, 1);
@@ -269,6 +271,7 @@ THC_API int THGPUNN_FusedLinear_backward(THGPUTensor *input, THGPUTensor *gradOu
 THC_API int THGPUNN_GroupedLinear_updateOutput(THGPUTensor *input, const long *counts, int groups, THGPUTensor *output, THGPUTensor *preactivation,
                                                THGPUTensor *weight, THGPUTensor *bias, int activation) {
   THC_BEGIN
+  THC_ARG(input && output && weight, 1, "tensors expected");
   check_act(activation, 8);
   const long rows = nelem(input) ? input->size[0] : 0;
   check_counts(counts, groups, rows, 2);
@@ -289,6 +292,7 @@ THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *count
                                            THGPUTensor *preactivation, THGPUTensor *gradPre, THGPUTensor *weight, THGPUTensor *gradWeight, THGPUTensor *gradBias,
                                            int activation, float scale) {
   THC_BEGIN
+  THC_ARG(input && gradOutput && weight, 1, "tensors expected");
   check_act(activation, 11);
   const long rows = nelem(input) ? input->size[0] : 0;
   check_counts(counts, groups, rows, 2);

@@ -445,6 +445,7 @@ static long rows_of(const THGPUTensor *t, long size, int argn) {
 
 static void norm_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *weight, THGPUTensor *gradWeight,
                           THGPUTensor *gradBias, THGPUTensor *mean, THGPUTensor *invStd, long size, float scale) {
+  THC_ARG(input && gradOutput && mean && invStd, 1, "tensors expected");
   THC_ARG(size > 0, 9, "size must be positive");
   THC_ARG(THGPUTensor_isSameSizeAs(input, gradOutput), 2, "gradOutput has the wrong size");
   THC_ARG(!weight || (nelem(weight) == size && is_contiguous(weight)), 4, "contiguous weight of the normalised size expected");
@@ -518,6 +519,7 @@ using namespace thc;
 THC_API int THGPUNN_LayerNorm_updateOutput(THGPUTensor *input, THGPUTensor *output, THGPUTensor *weight, THGPUTensor *bias, THGPUTensor *mean,
                                            THGPUTensor *invStd, long size, double eps) {
   THC_BEGIN
+  THC_ARG(input && output, 1, "tensors expected");
   THC_ARG(size > 0, 7, "size must be positive");
   THC_ARG(eps >= 0, 8, "eps must not be negative");
   THC_ARG(!weight == !bias, 4, "both or neither of weight and bias expected");

@@ -428,6 +428,11 @@ def _activation(name):
     return ACTIVATIONS[name]
 
 
+def _need_kept(m):
+    if not m._kept:
+        raise RuntimeError("%s: the last forward pass has kept nothing for a backward pass (it ran after evaluate())" % type(m).__name__)
+
+
 class LayerNorm(Module):
     """Rows normalised to mean zero and variance one over the trailing `sizes`, times `weight` plus `bias` (one of each for every place
     in a row); with affine=False the normalised rows themselves.  `mean` and `invStd` keep each row's statistics for the backward
@@ -435,7 +440,7 @@ class LayerNorm(Module):
 
     def __init__(self, *sizes, eps=1e-5, affine=True):
         super().__init__()
-        self.size, self.eps, self.train = math.prod(sizes), eps, True
+        self.size, self.eps, self.train, self._kept = math.prod(sizes), eps, True, True
         if not sizes or min(sizes) < 1:
             raise ValueError("LayerNorm: positive sizes expected")
         self.mean, self.invStd = GPUTensor(), GPUTensor()
@@ -453,10 +458,12 @@ class LayerNorm(Module):
         _need_gpu(input, "LayerNorm")
         w, b = self._affine()
         keep = (self.mean._p, self.invStd._p) if self.train else (None, None)
+        self._kept = self.train
         lib().THGPUNN_LayerNorm_updateOutput(input._p, self.output._p, w, b, keep[0], keep[1], self.size, self.eps)
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
+        _need_kept(self)
         lib().THGPUNN_LayerNorm_backward(input._p, gradOutput._p, gradInput, self._affine()[0], gradWeight, gradBias, self.mean._p, self.invStd._p,
                                          self.size, scale)
 
@@ -486,7 +493,7 @@ class FusedLinear(Linear):
 
     def __init__(self, inputSize, outputSize, activation="none", rng=None):
         super().__init__(inputSize, outputSize, rng=rng)
-        self.activation, self.train = activation, True
+        self.activation, self.train, self._kept = activation, True, True
         self._code = _activation(activation)
         self.preactivation, self.gradPreactivation = GPUTensor(), GPUTensor()
 
@@ -500,12 +507,14 @@ class FusedLinear(Linear):
         x, residual = self._split(input)
         _need_gpu(self.weight, "FusedLinear.weight")
         keep = self.preactivation._p if self.train and self._code else None
+        self._kept = self.train or not self._code
         lib().THGPUNN_FusedLinear_updateOutput(x._p, residual._p if residual is not None else None, self.output._p, keep, self.weight._p, self.bias._p,
                                                self._code)
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
         x, residual = self._split(input)
+        _need_kept(self)
         lib().THGPUNN_FusedLinear_backward(x._p, gradOutput._p, gradInput, self.preactivation._p, self.gradPreactivation._p, self.weight._p, gradWeight,
                                            gradBias, self._code, scale)
         return residual
@@ -543,7 +552,7 @@ class GroupedLinear(Module):
 
     def __init__(self, groups, inputSize, outputSize, activation="none", rng=None):
         super().__init__()
-        self.groups, self.activation, self.train = groups, activation, True
+        self.groups, self.activation, self.train, self._kept = groups, activation, True, True
         self._code = _activation(activation)
         self.weight = np.empty((groups, outputSize, inputSize), np.float32)
         self.bias = np.empty((groups, outputSize), np.float32)
@@ -577,11 +586,13 @@ class GroupedLinear(Module):
         x, counts = self._split(input)
         _need_gpu(self.weight, "GroupedLinear.weight")
         keep = self.preactivation._p if self.train and self._code else None
+        self._kept = self.train or not self._code
         lib().THGPUNN_GroupedLinear_updateOutput(x._p, counts, self.groups, self.output._p, keep, self.weight._p, self.bias._p, self._code)
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
         x, counts = self._split(input)
+        _need_kept(self)
         lib().THGPUNN_GroupedLinear_backward(x._p, counts, self.groups, gradOutput._p, gradInput, self.preactivation._p, self.gradPreactivation._p,
                                              self.weight._p, gradWeight, gradBias, self._code, scale)
 

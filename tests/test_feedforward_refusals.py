@@ -206,3 +206,30 @@ def test_tensors_of_another_device(fake):
     m.weight = fake(3, 4, 6, device=2)
     with pytest.raises(gt.THCError, match="Invalid argument 6: tensor of device 2"):
         m.forward([here, [2, 0, 3]])
+
+
+def test_missing_tensors():
+    L = gt.lib()
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_LayerNorm_updateOutput(None, None, None, None, None, None, 4, 1e-5)
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_LayerNorm_backward(None, None, None, None, None, None, None, None, 4, 1.0)
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_FusedLinear_updateOutput(None, None, None, None, None, None, 0)
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_FusedLinear_backward(None, None, None, None, None, None, None, None, 0, 1.0)
+    counts = np.zeros(2, np.int64)
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_GroupedLinear_updateOutput(None, counts, 2, None, None, None, None, 0)
+    with pytest.raises(gt.THCError, match="tensors expected"):
+        L.THGPUNN_GroupedLinear_backward(None, counts, 2, None, None, None, None, None, None, None, 0, 1.0)
+
+
+def test_a_backward_pass_behind_an_evaluation(fake):
+    """After evaluate() a forward pass keeps nothing, and what an earlier one kept is another input's."""
+    for m in (norm(fake), linear(fake), grouped(fake)):
+        m._kept = False
+        x = fake(5, 8) if isinstance(m, nn.LayerNorm) else [fake(5, 6), [2, 0, 3]] if isinstance(m, nn.GroupedLinear) else fake(5, 6)
+        for call in (m.backward, m.updateGradInput, m.accGradParameters):
+            with pytest.raises(RuntimeError, match="kept nothing"):
+                call(x, fake(5, 8) if isinstance(m, nn.LayerNorm) else fake(5, 4))
