@@ -455,55 +455,75 @@ template <int ACT, int NCOL> __device__ __forceinline__ void tc2_activate(float 
     }
   }
 }
-// Columns [0, left) of the row at o, `st` apart.
+// Columns [0, left) of the row at o, `st` apart: one pointer that moves on, since addresses worked out ahead would spill.
 template <int NCOL> __device__ __forceinline__ void tc2_put(float *o, long st, int left, const float (&acc)[NCOL]) {
   if (st == 1 && left >= NCOL && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
 #pragma unroll
     for (int j = 0; j < NCOL; j += 4) *reinterpret_cast<float4 *>(o + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-  } else if (left >= NCOL) {
+    return;
+  }
+  if (left >= NCOL) {
 #pragma unroll
-    for (int j = 0; j < NCOL; j++) o[j * st] = acc[j];
-  } else {
+    for (int j = 0; j < NCOL; j++) { *o = acc[j]; o += st; }
+    return;
+  }
 #pragma unroll
-    for (int j = 0; j < NCOL; j++)
-      if (j < left) o[j * st] = acc[j];
+  for (int j = 0; j < NCOL; j++) {
+    if (j < left) *o = acc[j];
+    o += st;
   }
 }
-template <class V, int NCOL>
+// The residual of a drain warp's 32 rows (from m on in its first lane) and NCOL columns on its way to L2, while the tile is still being multiplied.
+template <int NCOL>
+__device__ __forceinline__ void tc2_fetch_residual(const LinearEpilogue &l, long M, long N, long m, long nb) {
+  if (!l.residual) return;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < NCOL / 32; i++) {
+    const bool rows = l.rm == 1;     // a line holds the rows of a column, or columns of a row
+    const long row = rows ? m - lane : m, n = rows ? nb + 32 * i + lane : nb + 32 * i;
+    if (row < M && n < N) asm volatile("prefetch.global.L2 [%0];" ::"l"(l.residual + row * l.rm + n * l.rn));
+  }
+}
+// ROWS: the bias is the rows' and there is no residual (a grouped layer's).
+template <bool ROWS, class V, int NCOL>
 __device__ __forceinline__ void tc2_store_linear(const V &p, const LinearEpilogue &l, bool deferred, float (&acc)[NCOL], long m, long nb) {
   const int left = m < p.M ? (int)max(0l, min((long)NCOL, p.N - nb)) : 0;
   if (left == 0) return;
   const long st = p.epi.nstride, o = p.epi.template moff<false>(m) + nb * st;
-  if (p.epi.bias) {
-    const float *bias = p.epi.bias + nb;
+  const float row_b = p.epi.rb(m);
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int j = 0; j < NCOL; j++) acc[j] += row_b;
+  } else {
+    const float *bias = p.epi.bias ? p.epi.bias + nb : nullptr;
 #pragma unroll
     for (int j0 = 0; j0 < NCOL; j0 += 16) {
       float b[16];
 #pragma unroll
-      for (int j = 0; j < 16; j++) b[j] = j0 + j < left ? __ldg(bias + j0 + j) : 0.f;
+      for (int j = 0; j < 16; j++) b[j] = bias && j0 + j < left ? __ldg(bias + j0 + j) : row_b;
 #pragma unroll
       for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
     }
-  } else {
-    const float row_b = p.epi.rb(m);
-#pragma unroll
-    for (int j = 0; j < NCOL; j++) acc[j] += row_b;
   }
   if (deferred || l.z) tc2_put(deferred && !l.z ? p.epi.out + o : l.z + o, st, left, acc);
   if (deferred) return;
   if (l.act == kActRelu) tc2_activate<kActRelu>(acc);
   else if (l.act == kActGelu) tc2_activate<kActGelu>(acc);
   else if (l.act == kActSilu) tc2_activate<kActSilu>(acc);
-  if (l.residual) {
+  if (!ROWS && l.residual) {
     const float *r = l.residual + m * l.rm + nb * l.rn;
     const long rn = l.rn;
 #pragma unroll
-    for (int j0 = 0; j0 < NCOL; j0 += 16) {
-      float b[16];
+    for (int j0 = 0; j0 < NCOL; j0 += 32) {
+      float b[32];
 #pragma unroll
-      for (int j = 0; j < 16; j++) b[j] = j0 + j < left ? __ldg(r + (j0 + j) * rn) : 0.f;
+      for (int j = 0; j < 32; j++) {
+        b[j] = j0 + j < left ? __ldg(r) : 0.f;
+        r += rn;
+      }
 #pragma unroll
-      for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
+      for (int j = 0; j < 32; j++) acc[j0 + j] += b[j];
     }
   }
   tc2_put(p.epi.out + o, st, left, acc);

@@ -722,6 +722,9 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
       float acc[NCOL];
 #pragma unroll
       for (int j = 0; j < NCOL; j++) acc[j] = 0.f;
+      if constexpr (P::FUSED && P::GROUPS == 0) {
+        if (item.z < 0) tc2_fetch_residual<NCOL>(p.tail, p.M, p.N, item.m_tile0 + (long)rank * TC_BM + q * 32 + lane, item.n_tile0 + h * NCOL);
+      }
       const int folds = HALF ? (item.num_k_tiles + CHAIN - 1) / CHAIN : item.num_k_tiles;   // accumulators of this item
       for (int it = 0; it < folds; it++) {
         const int g = g0 + it;
@@ -766,10 +769,10 @@ __device__ __forceinline__ void tc2r_run(const P &p, const StallCtl &ctl, unsign
           } else {
             view.epi.out += item.group * p.out_group;
           }
-          if constexpr (P::FUSED) tc2_store_linear(view, p.tail, PAIRS && p.tail.deferred(), acc, m, n);
+          if constexpr (P::FUSED) tc2_store_linear<true>(view, p.tail, PAIRS && p.tail.deferred(), acc, m, n);
           else tc2_store_rows<ResultView, NCOL>(view, acc, m, n);
         } else if constexpr (P::FUSED) {
-          tc2_store_linear(p, p.tail, PAIRS && p.tail.deferred(), acc, m, item.n_tile0 + h * NCOL);
+          tc2_store_linear<false>(p, p.tail, PAIRS && p.tail.deferred(), acc, m, item.n_tile0 + h * NCOL);
         } else if constexpr (P::PAIR && BN2 == 128) {
           if (pair_lines) tc2_store_pair_rows<P>(p, acc, m, h * 32);
           else tc2_store_rows<P, NCOL>(p, acc, m, item.n_tile0 + h * NCOL);

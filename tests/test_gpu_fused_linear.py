@@ -97,6 +97,7 @@ def check_linear(gt, R, I, O, name, residual=False, mode="fp32x3", views=lambda 
     m.training()
     if not backward:
         return
+    m.forward(inp)
     # the backward pass goes by what the forward pass has kept
     zk = down(m.preactivation).double() if name != "none" else z
     s = slope(zk, name)
@@ -261,8 +262,10 @@ def check_groups(gt, counts, I, O, name, scale=0.5, views=lambda gt, t: up(gt, t
     m.evaluate()
     m.output = gt.GPUTensor()
     assert torch.equal(down(m.forward([xin, counts])), train)
+    m.training()
     if not backward:
         return
+    m.forward([xin, counts])
     zk = down(m.preactivation).double() if name != "none" else z
     gz = G * slope(zk, name)
     gzt = (16 * E * G.abs() * (1 + zk.abs().clamp(max=8)) if name in ("gelu", "silu") else torch.zeros_like(G)) + E * gz.abs()
