@@ -16,10 +16,16 @@ namespace thc {
 
 using namespace mm;
 
-// Entries that do not travel with a launch.
-static __global__ void __launch_bounds__(256) group_list_kernel(const __grid_constant__ GroupList piece, GroupEntry *to) {
+// Entries that do not travel with a launch go ahead of it, as many at a time as a kernel's 32 KB of parameters hold: by value, so that a recording has
+// its own.
+struct GroupUpload {
+  static constexpr int kMost = 2000;
+  int count;
+  GroupEntry at[kMost];
+};
+static __global__ void __launch_bounds__(256) group_list_kernel(const __grid_constant__ GroupUpload piece, GroupEntry *to) {
   pdl_begin();
-  for (int i = threadIdx.x; i < piece.count; i += 256) to[i] = piece.few[i];
+  for (int i = threadIdx.x; i < piece.count; i += 256) to[i] = piece.at[i];
 }
 static GroupList make_list(const GroupEntry *e, int n) {
   GroupList l;
@@ -30,11 +36,10 @@ static GroupList make_list(const GroupEntry *e, int n) {
     return l;
   }
   GroupEntry *to = (GroupEntry *)ws_alloc(sizeof(GroupEntry) * n);
-  for (int i = 0; i < n; i += kGroupEntries) {
-    GroupList piece;
-    piece.count = std::min(n - i, kGroupEntries);
-    piece.more = nullptr;
-    std::copy(e + i, e + i + piece.count, piece.few);
+  GroupUpload piece;
+  for (int i = 0; i < n; i += GroupUpload::kMost) {
+    piece.count = std::min(n - i, GroupUpload::kMost);
+    std::copy(e + i, e + i + piece.count, piece.at);
     pdl_launch(group_list_kernel, 1, 256, 0, piece, to + i);
     check_launch("group_list");
   }
@@ -173,7 +178,7 @@ static void small_groups(SmallGroups p, const std::vector<GroupEntry> &entries, 
     p.list = make_list(entries.data() + i, n);
     p.ws = nullptr;
     const long tiles = (long)ceil_div(p.M, 64) * n * p.column_tiles;
-    long ktiles = ceil_div(p.K, TC_BK), slices = 1;
+    long ktiles = std::max(1, ceil_div(p.K, TC_BK)), slices = 1;
     if (p.kind == kGroupRows) {
       if (tiles <= 2 * ctx().sm_count) slices = small_slices(tiles, ktiles, bn);
     } else if (tiles <= kZeroWords) {
@@ -419,6 +424,7 @@ static Choice choose_grad_weight(const Groups &g, const Lines &xs, const Lines &
   Choice best{kSmall, bn};
   double least = small_groups_us((double)((in + 63) / 64), columns * (double)live, columns * (double)ktiles, bn, xs.ok() && gs.ok());
   if (!encode_tiled_fn()) return best;
+  if (columns > 65535) least = 1e30;   // more tiles than a launch of that engine has
   for (bool pairs : {false, true}) {
     if (pairs && !pairs_fit(g, values)) break;
     for (int w : {256, 192, 128, 64}) {

@@ -426,3 +426,22 @@ def test_groups_with_infinite_rows_over_pairs(gt):
         near(y[p][k], (X[p] @ W[e].t() + b[e].double())[k], (rel_of(I) * (X[p].abs() @ W[e].abs().t() + b[e].abs().double()))[k])
         if e != 1:
             near(down(m.gradWeight)[e], g[p].double().t() @ X[p], (rel_of(counts[e]) + 4 * E) * (g[p].abs().double().t() @ X[p].abs()))
+
+
+@pytest.mark.parametrize("n,I,O", [(20000, 8, 8), (17000, 3, 5), (3000, 64, 32), (2, 1, 4200000)])
+def test_many_groups_and_many_columns(gt, n, I, O):
+    """More groups, or more columns, than a launch has of blocks to count them by."""
+    counts = np.arange(n) % 3
+    e = torch.from_numpy(np.repeat(np.arange(n), counts)).cuda()
+    T = len(e)
+    x, w, b, g = randn(1, T, I), randn(2, n, O, I) / I ** 0.5, 0.1 * randn(3, n, O), randn(4, T, O)
+    m = fill(gt, gt.nn.GroupedLinear(n, I, O), w, b)
+    X, W, B, G = x.double(), w.double()[e], b.double()[e], g.double()
+    near(down(m.forward([up(gt, x), counts])), torch.einsum("ti,toi->to", X, W) + B, rel_of(I) * (torch.einsum("ti,toi->to", X.abs(), W.abs()) + B.abs()))
+    m.gradWeight.fill(0.25); m.gradBias.fill(-0.5)
+    gi = m.backward([up(gt, x), counts], up(gt, g), 0.5)[0]
+    near(down(gi), torch.einsum("to,toi->ti", G, W), rel_of(O) * torch.einsum("to,toi->ti", G.abs(), W.abs()))
+    for k, (got, start, terms) in enumerate(((down(m.gradWeight), 0.25, G[:, :, None] * X[:, None, :]), (down(m.gradBias), -0.5, G))):
+        sums = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
+        want, size = sums.index_add(0, e, terms), sums.index_add(0, e, terms.abs())
+        near(got, start + 0.5 * want, 0.5 * rel_of(2) * size + 2 * E * (abs(start) + 0.5 * want.abs()))
