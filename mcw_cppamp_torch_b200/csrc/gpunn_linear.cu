@@ -19,6 +19,8 @@ struct RowPieces {
   long per;          // rows of a piece, where there is one group
   int groups;        // 1: pieces of `per` rows; else `at`
   long rows;
+  int live;          // groups among the pieces: the i-th has [first[i], first[i + 1])
+  short first[kRowPieces + 1];
   RowPiece at[kRowPieces];
   __device__ __forceinline__ RowPiece piece(int i) const {
     if (groups > 1) return at[i];
@@ -87,18 +89,16 @@ static __global__ void __launch_bounds__(256) act_grad_kernel(const float *__res
   }
 }
 // out[group] += scale * sum of the group's parts: eight threads a column, which take every eighth part and meet in the order of their places.  Block
-// (a, b) has 32 columns of the group that starts with piece b.
+// (a, b) has 32 columns of the b-th group.
 static __global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ part, long cols, float *out, float scale,
                                                                   const __grid_constant__ RowPieces pieces) {
   pdl_begin();
   __shared__ float sm[8][32];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, first = blockIdx.y;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const bool one = pieces.groups == 1;
+  const int first = one ? 0 : pieces.first[blockIdx.y], end = one ? pieces.count : pieces.first[blockIdx.y + 1];
   const long c = blockIdx.x * 32l + tx;
-  const int group = pieces.piece(first).group;
-  if (first > 0 && pieces.piece(first - 1).group == group) return;
-  int end = pieces.count;
-  if (pieces.groups > 1)
-    for (end = first + 1; end < pieces.count && pieces.at[end].group == group;) end++;
+  const int group = one ? 0 : pieces.at[first].group;
   float s = 0.f;
   if (c < cols) {
 #pragma unroll 4
@@ -127,11 +127,11 @@ static void act_grad(const Groups &groups, const float *g, long ldg, const float
     });
     check_launch("activation gradient");
     if (!gb) return;
-    pdl_launch(fold_columns_kernel, dim3((unsigned)ceil_div(cols, 32), p.groups == 1 ? 1u : (unsigned)p.count), 256, 0, part, cols, gb, scale, p);
+    pdl_launch(fold_columns_kernel, dim3((unsigned)ceil_div(cols, 32), p.groups == 1 ? 1u : (unsigned)p.live), 256, 0, part, cols, gb, scale, p);
     check_launch("bias gradient");
   };
   RowPieces p;
-  p.groups = groups.n; p.rows = groups.rows; p.per = per; p.count = 0;
+  p.groups = groups.n; p.rows = groups.rows; p.per = per; p.count = p.live = 0;
   if (groups.n == 1) {
     p.count = (int)((groups.rows + per - 1) / per);
     run(p);
@@ -141,8 +141,11 @@ static void act_grad(const Groups &groups, const float *g, long ldg, const float
   long r = 0;
   for (int e = 0; e < groups.n; r += groups.counts[e++]) {
     const long n = groups.counts[e], step = std::max(per, (n + kRowPieces - 1) / kRowPieces);
-    if (p.count + (n + step - 1) / step > kRowPieces) { run(p); p.count = 0; }
+    if (n == 0) continue;
+    if (p.count + (n + step - 1) / step > kRowPieces) { run(p); p.count = p.live = 0; }
+    p.first[p.live++] = (short)p.count;
     for (long i = 0; i < n; i += step) p.at[p.count++] = RowPiece{e, (int)(r + i), (int)(r + std::min(n, i + step))};
+    p.first[p.live] = (short)p.count;
   }
   run(p);
 }
