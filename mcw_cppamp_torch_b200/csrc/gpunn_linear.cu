@@ -11,7 +11,7 @@ namespace thc {
 
 // gz = g act'(z) over [first, end) of the rows, a piece of a group (blockIdx.y), with the sums of 128 columns over them: part[blockIdx.y][cols].  gz or
 // part may be null.  12 bytes a value: bound by HBM, or by latency where there are few rows.  A thread has four neighbouring columns (VEC), or one
-// of each 32, and every eighth row, four rows on the way.
+// of each 32, and every eighth row, four rows on the way.  2048 x 4096, gelu: 25 us, 4 TB/s (100 MB, from cold caches).
 struct RowPiece { int group, first, end; };
 constexpr int kRowPieces = 256;
 struct RowPieces {
@@ -89,7 +89,7 @@ static __global__ void __launch_bounds__(256) act_grad_kernel(const float *__res
   }
 }
 // out[group] += scale * sum of the group's parts: eight threads a column, which take every eighth part and meet in the order of their places.  Block
-// (a, b) has 32 columns of the b-th group.
+// (a, b) has 32 columns of the b-th group.  192 pieces of 8 groups, 1408 columns: a block for every piece took 12 us, most of them to find nothing.
 static __global__ void __launch_bounds__(256) fold_columns_kernel(const float *__restrict__ part, long cols, float *out, float scale,
                                                                   const __grid_constant__ RowPieces pieces) {
   pdl_begin();

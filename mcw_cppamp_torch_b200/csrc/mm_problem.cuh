@@ -433,28 +433,8 @@ struct ResultView {
   long M, N;
 };
 
-// Epilogue of one drain thread with a linear layer's tail.  The tensor pipe waits for it once all accumulators are full.  The activations run in a loop
-// over the columns, kLinearStep at a time in the first registers and all columns moved on by as many: straight-line code for 128 values at some
-// 25 instructions each, 50 KB of it, runs at the pace that instructions arrive from L2 (50 us a 256 x 256 tile).  What is stored is
-// stored in straight lines with one pointer and a constant stride, as in tc2_store_rows.
+// Epilogue of one drain thread with a linear layer's tail.  The tensor pipe waits for it once all accumulators are full.
 constexpr int kLinearStep = 16;
-template <int ACT, int NCOL> __device__ __forceinline__ void tc2_activate(float (&acc)[NCOL]) {
-  if constexpr (ACT == kActRelu) {
-#pragma unroll
-    for (int j = 0; j < NCOL; j++) acc[j] = activation<ACT>(acc[j]);
-  } else if constexpr (ACT != kActNone) {
-#pragma unroll 1
-    for (int i = 0; i < NCOL; i += kLinearStep) {
-      float v[kLinearStep];
-#pragma unroll
-      for (int j = 0; j < kLinearStep; j++) v[j] = activation<ACT>(acc[j]);
-#pragma unroll
-      for (int j = 0; j + kLinearStep < NCOL; j++) acc[j] = acc[j + kLinearStep];
-#pragma unroll
-      for (int j = 0; j < kLinearStep; j++) acc[NCOL - kLinearStep + j] = v[j];
-    }
-  }
-}
 // Columns [0, left) of the row at o, `st` apart: one pointer that moves on, since addresses worked out ahead would spill.
 template <int NCOL> __device__ __forceinline__ void tc2_put(float *o, long st, int left, const float (&acc)[NCOL]) {
   if (st == 1 && left >= NCOL && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
@@ -485,33 +465,76 @@ __device__ __forceinline__ void tc2_fetch_residual(const LinearEpilogue &l, long
     if (row < M && n < N) asm volatile("prefetch.global.L2 [%0];" ::"l"(l.residual + row * l.rm + n * l.rn));
   }
 }
-// ROWS: the bias is the rows' and there is no residual (a grouped layer's).
+// An activation of more than an instruction: kLinearStep columns at a time in the first registers and all columns moved on by as many, since
+// straight-line code for 128 values at some 25 instructions each, 50 KB of it, runs at the pace that instructions arrive from L2 (50 us a 256 x 256
+// tile).  With a residual the values go on into acc (RESIDUAL), else to the result.
+template <int ACT, bool RESIDUAL, bool ROWS, int NCOL>
+__device__ __forceinline__ void tc2_linear_steps(float (&acc)[NCOL], int left, float *out, float *z, long st, const float *bias, float row_b) {
+  constexpr int S = kLinearStep;
+#pragma unroll 1
+  for (int i = 0; i < (RESIDUAL ? NCOL : left); i += S) {
+    float v[S];
+#pragma unroll
+    for (int j = 0; j < S; j++) v[j] = acc[j] + (!ROWS && bias && i + j < left ? __ldg(bias + i + j) : row_b);
+    if (z) {
+      tc2_put(z, st, left - i, v);
+      z += S * st;
+    }
+#pragma unroll
+    for (int j = 0; j < S; j++) v[j] = activation<ACT>(v[j]);
+    if constexpr (!RESIDUAL) {
+      tc2_put(out, st, left - i, v);
+      out += S * st;
+    }
+#pragma unroll
+    for (int j = 0; j + S < NCOL; j++) acc[j] = acc[j + S];
+    if constexpr (RESIDUAL) {
+#pragma unroll
+      for (int j = 0; j < S; j++) acc[NCOL - S + j] = v[j];
+    }
+  }
+}
+// What costs nothing beside its loads and stores: in straight lines with one pointer and a constant stride, as in tc2_store_rows, a residual 32 values
+// at a time (16, one step of the loop above ahead: 8192 x 8192 results 115 us more).  ROWS: the bias is the rows' and there is no residual (a
+// grouped layer's).
 template <bool ROWS, class V, int NCOL>
 __device__ __forceinline__ void tc2_store_linear(const V &p, const LinearEpilogue &l, bool deferred, float (&acc)[NCOL], long m, long nb) {
   const int left = m < p.M ? (int)max(0l, min((long)NCOL, p.N - nb)) : 0;
   if (left == 0) return;
   const long st = p.epi.nstride, o = p.epi.template moff<false>(m) + nb * st;
-  const float row_b = p.epi.rb(m);
-  if constexpr (ROWS) {
-#pragma unroll
-    for (int j = 0; j < NCOL; j++) acc[j] += row_b;
+  const float row_b = p.epi.rb(m), *bias = !ROWS && p.epi.bias ? p.epi.bias + nb : nullptr;
+  float *out = p.epi.out + o, *z = l.z ? l.z + o : nullptr;
+  const bool residual = !ROWS && l.residual;
+  if (!deferred && l.act >= kActGelu) {
+    auto steps = [&](auto a) {
+      if (ROWS || !residual) tc2_linear_steps<decltype(a)::value, false, ROWS>(acc, left, out, z, st, bias, row_b);
+      else tc2_linear_steps<decltype(a)::value, true, ROWS>(acc, left, out, z, st, bias, row_b);
+    };
+    if (l.act == kActGelu) steps(std::integral_constant<int, kActGelu>());
+    else steps(std::integral_constant<int, kActSilu>());
+    if (ROWS || !residual) return;
   } else {
-    const float *bias = p.epi.bias ? p.epi.bias + nb : nullptr;
+    if constexpr (ROWS) {
 #pragma unroll
-    for (int j0 = 0; j0 < NCOL; j0 += 16) {
-      float b[16];
+      for (int j = 0; j < NCOL; j++) acc[j] += row_b;
+    } else {
 #pragma unroll
-      for (int j = 0; j < 16; j++) b[j] = bias && j0 + j < left ? __ldg(bias + j0 + j) : row_b;
+      for (int j0 = 0; j0 < NCOL; j0 += 16) {
+        float b[16];
 #pragma unroll
-      for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
+        for (int j = 0; j < 16; j++) b[j] = bias && j0 + j < left ? __ldg(bias + j0 + j) : row_b;
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[j0 + j] += b[j];
+      }
+    }
+    if (deferred || z) tc2_put(deferred && !z ? out : z, st, left, acc);
+    if (deferred) return;
+    if (l.act == kActRelu) {
+#pragma unroll
+      for (int j = 0; j < NCOL; j++) acc[j] = activation<kActRelu>(acc[j]);
     }
   }
-  if (deferred || l.z) tc2_put(deferred && !l.z ? p.epi.out + o : l.z + o, st, left, acc);
-  if (deferred) return;
-  if (l.act == kActRelu) tc2_activate<kActRelu>(acc);
-  else if (l.act == kActGelu) tc2_activate<kActGelu>(acc);
-  else if (l.act == kActSilu) tc2_activate<kActSilu>(acc);
-  if (!ROWS && l.residual) {
+  if (!ROWS && residual) {
     const float *r = l.residual + m * l.rm + nb * l.rn;
     const long rn = l.rn;
 #pragma unroll
@@ -526,7 +549,7 @@ __device__ __forceinline__ void tc2_store_linear(const V &p, const LinearEpilogu
       for (int j = 0; j < 32; j++) acc[j0 + j] += b[j];
     }
   }
-  tc2_put(p.epi.out + o, st, left, acc);
+  tc2_put(out, st, left, acc);
 }
 
 // Epilogue of one drain thread: its row m of the tile, NCOL columns from nb on.

@@ -7,6 +7,14 @@
 // A launch per group, as gemm() would have it, leaves most of the device idle behind each (37 groups of some 40 rows, 333 -> 515: three products
 // took 785 us); here the pieces of all groups are a launch's work items.  The 64-row (or 256-row) side of a tile is the features', so that a weight
 // that meets few rows is read once, in tiles as narrow as the rows.
+//
+// What each way measured (forward; a product of FP32 accuracy is three of halves, 555 TFLOP/s at the rate of library products):
+//   few rows        64 groups, 24 rows, 1024 -> 2048: 35 us, 168 MB of weights at 4.8 TB/s; the warp-level engine took 129
+//   warp-level      37 groups, 1537 rows, gradInput of 333 -> 515: 42 us, 12 TFLOP/s; operands of odd pitch come in 4-byte pieces, 17 k tiles in turn
+//   two-SM, FP32    16 groups, 8192 rows, 1024 -> 4096: 382 us with gelu, 180 TFLOP/s; 8 groups, 6000 rows, 2048 -> 1408: 190, 182.  The splitters and
+//                   the MMAs (tensor pipe 57 - 63 %) share the SM's memory
+//   two-SM, pairs   at twice that rate, but the weights are read twice and written once to make them: for the first of these 454 us in all against 429,
+//                   for gradWeight of the second 2 % less, with both gradients in pairs 3 %; they pay where rows are many for each weight
 #include <map>
 
 #include "mm_launch.cuh"
