@@ -419,7 +419,7 @@ THC_API int THGPUNN_SpatialAveragePooling_updateGradInput(THGPUTensor *input, TH
  *   output = (x - mean) * invStd * weight + bias,  invStd = 1 / sqrt(variance + eps), the variance over `size` values.
  * weight and bias are both given or both NULL; so are mean and invStd, which receive one value a row for the backward pass.
  * backward: gradInput (skipped when NULL), and gradWeight += scale * ..., gradBias += scale * ... (both or neither).  Sums are in FP32, in
- * an order that the sizes alone decide.  Results may not share memory with operands. */
+ * an order that the sizes and the device decide.  Results may not share memory with operands. */
 THC_API int THGPUNN_LayerNorm_updateOutput(THGPUTensor *input, THGPUTensor *output, THGPUTensor *weight, THGPUTensor *bias,
     THGPUTensor *mean, THGPUTensor *invStd, long size, double eps);
 THC_API int THGPUNN_LayerNorm_backward(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *weight,

@@ -53,9 +53,10 @@
 // The kernel is persistent: see tc2r_kernel.
 //
 // A linear layer's epilogue (FUSED): the drain warps add the bias, keep the sum where it is asked for, apply the activation and add a residual whose rows
-// were fetched to L2 while the tile was multiplied.  Products of FP32 values have more, narrower accumulators there (tc2r_deep), which take up the
-// MMAs of the next tile while a tile's results go through an exponential.  2048 rows, 4096 -> 4096 with gelu, residual and kept sums: 205 us, where the
-// plain product of that size takes 167 and the passes it saves 60.
+// were fetched to L2 while the tile was multiplied.  Products of FP32 values in tiles of up to 128 columns have four accumulators there (tc2r_deep), which
+// take the MMAs of the next tile meanwhile; wider ones, and pairs of 256 columns, have two k tiles of slack.  In a loop, 8192 rows, 1024 -> 8192: 400 us, with
+// gelu 462, with its sums kept and a residual 625 (268 MB each, 41 us at the copy rate); 4096 -> 8192 with gelu and its sums 1610, where a product and a pass
+// behind it take 1650 - 1690.
 // Groups (GroupProblem): an item is a tile of one group's rows, as wide as they are in steps of 64 (its MMAs are that narrow too), or a tile of one
 // group's weight gradient, whose k tiles end with the group: the rows of the next group in the last tile are zeroed by the splitters, pairs are padded
 // in memory.  Items come longest first.  Figures: thc_groups.cu.

@@ -34,6 +34,8 @@ struct Groups {
 void group_forward(const Groups &g, const float *x, long ldx, long in, long out, const float *w, const float *b, float *y, int act, float *z);
 // gx = gz w[e], unless null, and gw[e] += scale * gz^T x over the group's rows, unless null
 void group_backward(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, const float *w, float *gx, float *gw, float scale);
+// gw[e] += scale * gz^T x in FP32 where no group has more than a handful of rows; false: some has, and nothing has been done
+bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale);
 
 }  // namespace thc
 

@@ -359,6 +359,7 @@ void linear_product(const float *x, long ldx, long rows, long in, long out, cons
 // pitch TMA cannot take copied once.
 void linear_gradients(const float *x, long ldx, const float *gz, long ldg, long rows, long in, long out, const float *w, float *gx, float *gw, float scale) {
   WsScope scope;
+  if (gw && ctx().math_mode != 1 && few_rows_sums(Groups{&rows, 1, rows}, x, ldx, gz, ldg, in, out, gw, scale)) gw = nullptr;
   if (ctx().math_mode == 0 && gx && gw && pairs_are_faster(in, rows, out) && pairs_are_faster(in, out, rows) && !small_is_faster(in, rows, out, true) &&
       !small_is_faster(in, out, rows, true)) {
     PairSide g{{gz, ldg, true, rows}, {}, {}}, ws{{w, in, false, in}, {}, {}}, xs{{x, ldx, false, in}, {}, {}};

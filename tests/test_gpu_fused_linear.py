@@ -428,20 +428,35 @@ def test_groups_with_infinite_rows_over_pairs(gt):
             near(down(m.gradWeight)[e], g[p].double().t() @ X[p], (rel_of(counts[e]) + 4 * E) * (g[p].abs().double().t() @ X[p].abs()))
 
 
-@pytest.mark.parametrize("n,I,O", [(20000, 8, 8), (17000, 3, 5), (3000, 64, 32), (2, 1, 4200000)])
-def test_many_groups_and_many_columns(gt, n, I, O):
-    """More groups, or more columns, than a launch has of blocks to count them by."""
+@pytest.mark.parametrize("last", [0, 1, 16, 40])
+@pytest.mark.parametrize("n,I,O", [(20000, 8, 8), (70000, 3, 5), (3000, 64, 32), (2, 1, 4200000)])
+def test_many_groups_and_many_columns(gt, n, I, O, last):
+    """More groups, or more columns, than a launch has of blocks to count them by; `last`: rows of the last group, few or not (an empty tensor has no
+    dimensions)."""
     counts = np.arange(n) % 3
+    counts[-1] = last
     e = torch.from_numpy(np.repeat(np.arange(n), counts)).cuda()
     T = len(e)
     x, w, b, g = randn(1, T, I), randn(2, n, O, I) / I ** 0.5, 0.1 * randn(3, n, O), randn(4, T, O)
     m = fill(gt, gt.nn.GroupedLinear(n, I, O), w, b)
     X, W, B, G = x.double(), w.double()[e], b.double()[e], g.double()
-    near(down(m.forward([up(gt, x), counts])), torch.einsum("ti,toi->to", X, W) + B, rel_of(I) * (torch.einsum("ti,toi->to", X.abs(), W.abs()) + B.abs()))
+    near(down(m.forward([up(gt, x), counts])).reshape(T, O), torch.einsum("ti,toi->to", X, W) + B, rel_of(I) * (torch.einsum("ti,toi->to", X.abs(), W.abs()) + B.abs()))
     m.gradWeight.fill(0.25); m.gradBias.fill(-0.5)
     gi = m.backward([up(gt, x), counts], up(gt, g), 0.5)[0]
-    near(down(gi), torch.einsum("to,toi->ti", G, W), rel_of(O) * torch.einsum("to,toi->ti", G.abs(), W.abs()))
+    near(down(gi).reshape(T, I), torch.einsum("to,toi->ti", G, W), rel_of(O) * torch.einsum("to,toi->ti", G.abs(), W.abs()))
     for k, (got, start, terms) in enumerate(((down(m.gradWeight), 0.25, G[:, :, None] * X[:, None, :]), (down(m.gradBias), -0.5, G))):
         sums = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
         want, size = sums.index_add(0, e, terms), sums.index_add(0, e, terms.abs())
         near(got, start + 0.5 * want, 0.5 * rel_of(2) * size + 2 * E * (abs(start) + 0.5 * want.abs()))
+
+
+@pytest.mark.parametrize("R", [1, 2, 4, 7, 15, 16, 17])
+@pytest.mark.parametrize("I,O", [(1, 1), (4, 9), (130, 64), (333, 515), (1024, 70), (1100, 33), (5000, 3)])
+def test_weight_gradients_of_few_rows(gt, R, I, O):
+    """Rows of all strides, pitches that 16-byte accesses take and others, columns of one block and of several, empty groups around."""
+    def wide(gt, t):
+        return up(gt, torch.cat([t, t.flip(0)], 1)).narrow(2, 1, t.shape[1])
+
+    for views in (lambda gt, t: up(gt, t), wide, lambda gt, t: up(gt, t.t().contiguous()).t()):
+        check_linear(gt, R, I, O, "none", views=views)
+        check_groups(gt, [0, R, 1, 0, 2, R], I, O, "none", views=views)
