@@ -247,9 +247,21 @@ static __global__ void __launch_bounds__(256) few_rows_sums_kernel(const float *
     }
   }
 }
+// f(R as a constant, list) for the groups with rows, as many as a launch has blocks for along z.
+template <int MOST, class F> static void each_few(const Groups &g, long most, F f) {
+  const std::vector<GroupEntry> entries = whole_groups(g);
+  for (size_t i = 0; i < entries.size(); i += 65535) {
+    const GroupList list = make_list(entries.data() + i, (int)std::min(entries.size() - i, (size_t)65535));
+    if (most <= 1) f(std::integral_constant<int, 1>(), list);
+    else if (most <= 2) f(std::integral_constant<int, 2>(), list);
+    else if (most <= 4) f(std::integral_constant<int, 4>(), list);
+    else if (MOST == 8 || most <= 8) f(std::integral_constant<int, 8>(), list);
+    else f(std::integral_constant<int, MOST>(), list);
+  }
+}
+static long most_rows(const Groups &g) { return *std::max_element(g.counts, g.counts + g.n); }
 bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, float *gw, float scale) {
-  long most = 0;
-  for (int e = 0; e < g.n; e++) most = std::max(most, g.counts[e]);
+  const long most = most_rows(g);
   if (most > kFewSums) return false;
   const bool vec = in % 4 == 0 && ldx % 4 == 0 && (((uintptr_t)x | (uintptr_t)gw) & 15) == 0;
   int T = 32;
@@ -257,21 +269,128 @@ bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, l
   const long columns = (in + 4 * T - 1) / (4 * T), rows = 8 * (256 / T), tiles = (out + rows - 1) / rows;
   if (tiles > 65535) return false;
   WsScope scope;
-  const std::vector<GroupEntry> entries = whole_groups(g);
-  auto go = [&](auto r, auto v, const GroupList &list) {
-    pdl_launch(few_rows_sums_kernel<decltype(r)::value, decltype(v)::value>, dim3((unsigned)columns, (unsigned)tiles, (unsigned)list.count), 256, 0, x, ldx, gz, ldg, in, out,
-               gw, scale, T, list);
+  each_few<kFewSums>(g, most, [&](auto r, const GroupList &list) {
+    const dim3 grid((unsigned)columns, (unsigned)tiles, (unsigned)list.count);
+    if (vec) pdl_launch(few_rows_sums_kernel<decltype(r)::value, true>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, list);
+    else pdl_launch(few_rows_sums_kernel<decltype(r)::value, false>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, list);
     check_launch("few_rows_sums");
-  };
-  for (size_t i = 0; i < entries.size(); i += 65535) {
-    const GroupList list = make_list(entries.data() + i, (int)std::min(entries.size() - i, (size_t)65535));
-    auto width = [&](auto r) { vec ? go(r, std::true_type(), list) : go(r, std::false_type(), list); };
-    if (most <= 1) width(std::integral_constant<int, 1>());
-    else if (most <= 2) width(std::integral_constant<int, 2>());
-    else if (most <= 4) width(std::integral_constant<int, 4>());
-    else if (most <= 8) width(std::integral_constant<int, 8>());
-    else width(std::integral_constant<int, kFewSums>());
+  });
+  return true;
+}
+
+// gradInput of eight groups and more where none has more than eight rows: w[e] is read once, along its rows, and multiply-adds in FP32 keep up.  A warp has 128 columns (VEC: four neighbours a lane, else 32
+// apart) and eight rows of w on their way; the eight warps of a block take eight rows each in turn of the block's `run` rows of w and meet in shared memory,
+// the blocks of a column tile in memory, where the last one adds their sums up in their order.  kFewRun rows' gradients lie in shared memory at a time.
+// A backward call of 64 groups, 1024 -> 2048 with 24 rows, 333 -> 515 with 100: 174 and 64 us, with the warp-level engine 208 and 76.  One
+// matrix, which has to be cut along its rows for blocks enough, stays with that engine (7 rows, 5716 -> 5630: 131 and 112).
+constexpr int kFewRun = 512, kFewBack = 8;
+template <int R, bool VEC>
+static __global__ void __launch_bounds__(256) few_rows_back_kernel(const float *__restrict__ w, const float *__restrict__ gz, long ldg, long in, long out, float *__restrict__ gx,
+                                                                   int run, float *part, unsigned *tickets, const __grid_constant__ GroupList list) {
+  pdl_begin();
+  constexpr int U = 8, Q = R < 4 ? R : 4;
+  __shared__ __align__(16) float sm[R * kFewRun > 8 * Q * 128 ? R * kFewRun : 8 * Q * 128];
+  __shared__ bool last;
+  const GroupEntry e = list.at(blockIdx.z);
+  const int n = e.end - e.first, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long c0 = blockIdx.x * 128l, o0 = (long)blockIdx.y * run;
+  const int all_rows = (int)min((long)run, out - o0);
+  w += (e.group * out + o0) * in;
+  auto column = [&](int j) { return c0 + (VEC ? 4 * lane + j : lane + 32 * j); };
+  float acc[R][4];
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[r][j] = 0.f;
+  for (int from = 0; from < all_rows; from += kFewRun) {
+    const int rows = min(kFewRun, all_rows - from);
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * kFewRun; i += 256) {
+      const int r = i / kFewRun, o = i % kFewRun;
+      if (o < (rows + 7) / 8 * 8) sm[i] = r < n && o < rows ? __ldg(gz + (e.first + r) * ldg + o0 + from + o) : 0.f;
+    }
+    __syncthreads();
+    for (int o = warp * U; o < rows; o += 8 * U) {
+      float v[U][4];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const float *p = w + (long)(o + u) * in;
+        if constexpr (VEC) {
+          const float4 q = o + u < rows && column(0) < in ? __ldg(reinterpret_cast<const float4 *>(p + column(0))) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[u][j] = o + u < rows && column(j) < in ? __ldg(p + column(j)) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float4 g0 = *reinterpret_cast<const float4 *>(sm + r * kFewRun + o), g1 = *reinterpret_cast<const float4 *>(sm + r * kFewRun + o + 4);
+        const float gs[U] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[r][j] = fmaf(gs[u], v[u][j], acc[r][j]);
+      }
+    }
+    w += (long)kFewRun * in;
   }
+  const long tile = (long)blockIdx.z * gridDim.x + blockIdx.x;
+  float *mine = part + (tile * gridDim.y + blockIdx.y) * (R * 128);
+#pragma unroll
+  for (int r0 = 0; r0 < R; r0 += Q) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) sm[(warp * Q + q) * 128 + (VEC ? 4 * lane + j : lane + 32 * j)] = acc[r0 + q][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < Q * 128; i += 256) {
+      float s = sm[i];
+#pragma unroll
+      for (int k = 1; k < 8; k++) s += sm[k * Q * 128 + i];
+      const int r = r0 + i / 128;
+      if (gridDim.y > 1) mine[r * 128 + i % 128] = s;
+      else if (r < n && c0 + i % 128 < in) gx[(e.first + r) * in + c0 + i % 128] = s;
+    }
+  }
+  if (gridDim.y == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicAdd(tickets + tile, 1u) == gridDim.y - 1;
+    if (last) tickets[tile] = 0;   // ready for the next launch on this stream
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float *all = part + tile * gridDim.y * (R * 128);
+  for (int i = threadIdx.x; i < n * 128; i += 256) {
+    if (c0 + i % 128 >= in) continue;
+    float s = 0.f;
+#pragma unroll 8
+    for (int z = 0; z < (int)gridDim.y; z++) s += __ldcg(all + (long)z * (R * 128) + i);
+    gx[(e.first + i / 128) * in + c0 + i % 128] = s;
+  }
+}
+static bool few_rows_back(const Groups &g, const float *gz, long ldg, long in, long out, const float *w, float *gx) {
+  const long most = most_rows(g);
+  if (most > kFewBack || g.n - std::count(g.counts, g.counts + g.n, 0l) < 8) return false;
+  const bool vec = in % 4 == 0 && ((uintptr_t)w & 15) == 0;
+  const long columns = (in + 127) / 128;
+  WsScope scope;
+  each_few<kFewBack>(g, most, [&](auto r, const GroupList &list) {
+    constexpr int R = decltype(r)::value;
+    // as many blocks as are resident at once, rows of w in whole eights for each warp
+    constexpr long kResident = R <= 2 ? 4 : 2;
+    const long tiles = columns * list.count, wanted = std::max(1l, ctx().sm_count * kResident / tiles);
+    const long run = std::max(64l, ((out + wanted - 1) / wanted + 63) / 64 * 64), splits = (out + run - 1) / run;
+    const dim3 grid((unsigned)columns, (unsigned)splits, (unsigned)list.count);
+    float *part = splits > 1 ? (float *)ws_alloc(sizeof(float) * tiles * splits * R * 128) : nullptr;
+    if (vec) pdl_launch(few_rows_back_kernel<R, true>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), list);
+    else pdl_launch(few_rows_back_kernel<R, false>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), list);
+    check_launch("few_rows_back");
+  });
   return true;
 }
 // The warp-level engine over the groups: any size, pitch and alignment.
@@ -597,6 +716,7 @@ void group_backward(const Groups &g, const float *x, long ldx, const float *gz, 
       }))
     return;
   WsScope scope;
+  if (gx && few_rows_back(g, gz, ldg, in, out, w, gx)) gx = nullptr;
   if (gw && few_rows_sums(g, x, ldx, gz, ldg, in, out, gw, scale)) gw = nullptr;
   Lines xs{x, g.rows, in, ldx}, gs{gz, g.rows, out, ldg};
   const Choice ci = gx ? choose_grad_input(g, ldg, gz, in, out, w) : Choice{kSmall, 64}, cw = gw ? choose_grad_weight(g, xs, gs) : Choice{kSmall, 64};

@@ -460,3 +460,10 @@ def test_weight_gradients_of_few_rows(gt, R, I, O):
     for views in (lambda gt, t: up(gt, t), wide, lambda gt, t: up(gt, t.t().contiguous()).t()):
         check_linear(gt, R, I, O, "none", views=views)
         check_groups(gt, [0, R, 1, 0, 2, R], I, O, "none", views=views)
+
+
+@pytest.mark.parametrize("counts", [[1] * 8, [2, 0, 1, 2] * 3, [4, 3, 0, 1, 2] * 2, [1] * 40 + [0] * 5 + [4], [8, 1, 7, 5] * 2, [9] + [1] * 9, [3] * 7])
+@pytest.mark.parametrize("I,O", [(1, 1), (130, 64), (128, 513), (333, 515), (260, 2049), (5000, 70)])
+def test_input_gradients_of_few_rows(gt, counts, I, O):
+    """Rows of weights that a block's pieces divide and others, one piece of them and several, columns of one tile and of several."""
+    check_groups(gt, counts, I, O, "silu")
