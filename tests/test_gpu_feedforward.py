@@ -206,6 +206,56 @@ def test_recorded_and_replayed(gt, rows, width, inner):
         gt.lib().THGPUSetStream(None)
 
 
+@pytest.mark.parametrize("groups,most", [(12, 3), (12, 9), (500, 3), (500, 9), (500, 40)])
+def test_routed_layers_recorded_and_replayed(gt, groups, most):
+    """Lists of groups that travel with a launch and that lie in memory, rows of a group few and not; other counts between the replays."""
+    m = gt.nn.GroupedLinear(groups, 72, 600, "gelu").gpu()
+    counts, others = np.arange(groups) % most, (np.arange(groups) * 5 + 1) % (most + 3)
+    rows, more = int(counts.sum()), int(others.sum())
+    x, g = torch.zeros(rows, 72, device="cuda"), torch.zeros(rows, 600, device="cuda")
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    gt.lib().THGPUSetStream(ctypes.c_void_p(stream.cuda_stream))
+    try:
+        X, G, X2, G2 = wrap(gt, x), wrap(gt, g), up(gt, randn(5, more, 72)), up(gt, randn(6, more, 600))
+
+        def step():
+            m.zeroGradParameters()
+            m.forward([X, counts])
+            m.backward([X, counts], G)
+
+        def results():
+            return [down(t).clone() for t in (m.output, m.gradInput[0], m.gradWeight, m.gradBias)]
+        for _ in range(2):
+            step()
+        gt.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        kept = (m.output, m.gradInput, m.preactivation, m.gradPreactivation)
+        for seed in (1, 2):
+            x.copy_(randn(seed, rows, 72)); g.copy_(randn(seed + 10, rows, 600))
+            torch.cuda.synchronize()
+            step()
+            gt.synchronize()
+            want = results()
+            m.output, m.gradInput, m.preactivation, m.gradPreactivation = (gt.GPUTensor() for _ in range(4))
+            m.forward([X2, others])
+            m.backward([X2, others], G2)
+            m.output, m.gradInput, m.preactivation, m.gradPreactivation = kept
+            m.gradWeight.fill(float("nan")); m.output.fill(float("nan"))
+            gt.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            gt.synchronize()
+            for a, b in zip(results(), want):
+                assert torch.equal(a, b)
+        del graph
+    finally:
+        gt.synchronize()
+        gt.lib().THGPUSetStream(None)
+
+
 def test_two_threads(gt):
     """Two threads, each on its own stream of the device, at the same time: the results of each alone."""
     def work(out, seed):
