@@ -407,7 +407,7 @@ struct FusedProblem : Problem<OpA_, OpB_, false, PREC_> {
 // Products where the rows of each group meet a matrix of their own, in one launch.  An entry is a piece of a group's rows: a tile of columns of
 // the result (rows [first, end), the tile's width or less), or (kGroupSums) all rows of the group, which are summed over.
 enum : int { kGroupRows = 1, kGroupSums = 2 };
-struct GroupEntry { int group, first, end, shift; };   // row r of the operands is row r - shift of the results
+struct GroupEntry { int group, first, end, shift; };   // row r of the operands is row r - shift of the results (the warp-level engine's sums: the entry's slice of k)
 constexpr int kGroupEntries = 160;   // that travel with a launch; more of them lie in device memory
 struct GroupList {
   int count;

@@ -43,7 +43,7 @@ struct SmallProblem {
   unsigned *tickets;         // one zero word per tile
   const int *stalled;        // the stream's stall flag (StallCtl::dev_flag): behind a stalled kernel nothing is written
   static constexpr bool FUSED = false, GROUPS = false;
-  __device__ __forceinline__ const SmallProblem &at_block(int &, int &) const { return *this; }
+  __device__ __forceinline__ const SmallProblem &at_block(int &, int &, int &) const { return *this; }
 };
 // The same with D = act(A B^T + bias) + residual; z, unless null, gets the sum that the activation is taken of, laid out as D.  beta == 0.
 struct SmallFused : SmallProblem {
@@ -52,7 +52,7 @@ struct SmallFused : SmallProblem {
   long rm = 0, rn = 0;
   float *z = nullptr;
   static constexpr bool FUSED = true;
-  __device__ __forceinline__ const SmallFused &at_block(int &, int &) const { return *this; }
+  __device__ __forceinline__ const SmallFused &at_block(int &, int &, int &) const { return *this; }
 };
 
 // ---- groups ----------------------------------------------------------------------------------------------------------
@@ -60,14 +60,19 @@ struct SmallFused : SmallProblem {
 struct GroupPlaces {
   long a_group, a_row, b_row, c_group, c_row, bias_group;
 };
+// kGroupSums: a group of more than tiles_per_slice k tiles is cut along k into as few even slices as have no more than that.  Its entries stand one
+// behind the other, one for each slice (`shift`: which), before those of all groups that are not cut, so that memory for partial sums and tickets is
+// theirs alone.  (kGroupRows: k is the same for all, `slices` of the launch.)
 struct SmallGroups : SmallFused {
   int kind;                  // kGroupRows: A belongs to the group, B's rows and D's columns to the entry; kGroupSums: k belongs to the entry, D to the group
   int column_tiles;          // of an entry
+  int tile_floats;           // of a tile's partial sums
   GroupPlaces at;
   GroupList list;
   static constexpr bool GROUPS = true;
-  // This block's product, with its first column.
-  __device__ __forceinline__ SmallFused at_block(int &column, int &k_tiles) const {
+  __host__ __device__ static int slices_of(int rows, int tiles_per_slice) { return ((rows + TC_BK - 1) / TC_BK + tiles_per_slice - 1) / tiles_per_slice; }
+  // This block's product, with its first column and its slice.
+  __device__ __forceinline__ SmallFused at_block(int &column, int &k_tiles, int &slice) const {
     SmallFused p = *this;
     const int e = (int)blockIdx.y / column_tiles;
     const GroupEntry g = list.at(e);
@@ -78,11 +83,20 @@ struct SmallGroups : SmallFused {
     if (p.z) p.z += c;
     if (p.bias) p.bias += g.group * at.bias_group;
     column = (int)blockIdx.y - e * column_tiles;
+    int first = e, slots = e * slices;   // entries whose tickets, and whose partial sums, come before this group's
     if (kind == kGroupRows) {
       p.N = g.end - g.first;
     } else {
       p.K = g.end - g.first;
-      k_tiles = ((p.K + TC_BK - 1) / TC_BK + slices - 1) / slices;
+      p.slices = slices_of(p.K, tiles_per_slice);
+      k_tiles = ((p.K + TC_BK - 1) / TC_BK + p.slices - 1) / p.slices;
+      slice = g.shift;
+      first = slots = e - slice;
+    }
+    if (p.slices > 1) {
+      const long tiles = (long)column_tiles * gridDim.x;
+      p.tickets += first * tiles;
+      p.ws += slots * tiles * tile_floats;
     }
     return p;
   }
@@ -198,8 +212,8 @@ __device__ __forceinline__ float fp32_sum(const SmallProblem &p, long m, long n,
 template <int BM, int BN, int WM, int WN, bool A_K, bool B_K, class P = SmallProblem>
 __global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant__ P whole) {
   pdl_begin();
-  int column = blockIdx.y, tiles_per_slice = whole.tiles_per_slice;
-  const auto &p = whole.at_block(column, tiles_per_slice);
+  int column = blockIdx.y, tiles_per_slice = whole.tiles_per_slice, slice = blockIdx.z;
+  const auto &p = whole.at_block(column, tiles_per_slice, slice);
   static_assert(WM * WN * 32 == SM_THREADS && BM % (16 * WM) == 0 && BN % (8 * WN) == 0, "warp layout");
   constexpr int MT = BM / WM / 16, NT = BN / WN / 8;
   constexpr int A_FLOATS = SmallTile<BM, A_K>::FLOATS, B_FLOATS = SmallTile<BN, B_K>::FLOATS, STAGE = A_FLOATS + B_FLOATS;
@@ -209,7 +223,7 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.x * BM, n0 = column * BN;
   const int wm = (warp % WM) * (BM / WM), wn = (warp / WM) * (BN / WN);
-  const int kt0 = blockIdx.z * tiles_per_slice;
+  const int kt0 = slice * tiles_per_slice;
   const int nk = min(tiles_per_slice, (p.K + TC_BK - 1) / TC_BK - kt0);
   // the rows a thread's fragment registers stand for: fragment row r = 16 i + g + 8 e (A) or 8 j + g (B) of a warp's share
   // is this row of it
@@ -324,9 +338,9 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant
         }
   }
   if (p.slices > 1) {
-    const long tile = (long)blockIdx.y * gridDim.x + blockIdx.x;
+    const long tile = (long)column * gridDim.x + blockIdx.x;
     constexpr int NV = MT * NT * 4;
-    float *mine = p.ws + (tile * p.slices + blockIdx.z) * (NV * SM_THREADS) + tid;
+    float *mine = p.ws + (tile * p.slices + slice) * (NV * SM_THREADS) + tid;
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -450,8 +464,8 @@ __global__ void __launch_bounds__(SM_THREADS) small_kernel(const __grid_constant
 template <int R, int RA, int UNROLL, class P = SmallProblem>
 __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ P whole, int groups) {
   pdl_begin();
-  int column = 0, k_tiles = 0;
-  const auto &p = whole.at_block(column, k_tiles);
+  int column = 0, k_tiles = 0, k_slice = 0;
+  const auto &p = whole.at_block(column, k_tiles, k_slice);
   __shared__ float part[8][RA * R];
   const int stalled = *reinterpret_cast<const volatile int *>(p.stalled);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -393,32 +393,53 @@ static bool few_rows_back(const Groups &g, const float *gz, long ldg, long in, l
   });
   return true;
 }
+// Entries of sums with the groups of more than `most` k tiles cut into slices, those first.  `cut`: how many entries they are.
+static std::vector<GroupEntry> cut_groups(const std::vector<GroupEntry> &groups, int most, long &cut) {
+  std::vector<GroupEntry> v;
+  for (GroupEntry e : groups) {
+    const int slices = SmallGroups::slices_of(e.end - e.first, most);
+    for (e.shift = 0; slices > 1 && e.shift < slices; e.shift++) v.push_back(e);
+  }
+  cut = (long)v.size();
+  for (const GroupEntry &e : groups)
+    if (SmallGroups::slices_of(e.end - e.first, most) <= 1) v.push_back(e);
+  return v;
+}
 // The warp-level engine over the groups: any size, pitch and alignment.
-static void small_groups(SmallGroups p, const std::vector<GroupEntry> &entries, int bn, bool a_k, bool b_k) {
+static void small_groups(SmallGroups p, std::vector<GroupEntry> entries, int bn, bool a_k, bool b_k) {
   p.stalled = stall_ctl().dev_flag;
+  p.tile_floats = 64 * bn;
   const int most = std::max(1, 65535 / p.column_tiles);
+  const long tiles = (long)ceil_div(p.M, 64) * p.column_tiles;   // of an entry
+  long cut = 0;
+  if (p.kind == kGroupSums) {
+    // no slice longer than a block's share of all k tiles (three blocks an SM), or than sixteen, but no more than 32 slices.  So fewer than six tiles an SM
+    // keep partial sums (15 MB), however uneven the groups are.  128 groups, 256 -> 256, 13800 rows in one and 20 in each of the others: 88 us; with all
+    // of them in as many slices as the longest, 528 us and 738 MB.
+    long all = 0, longest = 1;
+    for (const GroupEntry &e : entries) {
+      const long t = ceil_div(e.end - e.first, TC_BK);
+      all += t * tiles;
+      longest = std::max(longest, t);
+    }
+    const long share = 3l * ctx().sm_count;
+    p.tiles_per_slice = (int)std::max(std::max(16l, (all + share - 1) / share), (longest + 31) / 32);
+    entries = cut_groups(entries, p.tiles_per_slice, cut);
+    THC_CHECK(cut <= most && cut * tiles <= kZeroWords, "internal: grouped sums cut into too many slices");
+  }
   for (size_t i = 0; i < entries.size(); i += most) {
     const int n = (int)std::min(entries.size() - i, (size_t)most);
     p.list = make_list(entries.data() + i, n);
     p.ws = nullptr;
-    const long tiles = (long)ceil_div(p.M, 64) * n * p.column_tiles;
-    long ktiles = std::max(1, ceil_div(p.K, TC_BK)), slices = 1;
+    p.slices = 1;
     if (p.kind == kGroupRows) {
-      if (tiles <= 2 * ctx().sm_count) slices = small_slices(tiles, ktiles, bn);
-    } else if (tiles <= kZeroWords) {
-      // groups of unlike lengths: none longer than a block's share of all k tiles, or than sixteen
-      long all = 0;
-      for (int q = 0; q < n; q++) {
-        const long t = ceil_div(entries[i + q].end - entries[i + q].first, TC_BK);
-        all += t * (tiles / n);
-        ktiles = std::max(ktiles, t);
-      }
-      slices = std::min(32l, (long)ceil_div(ktiles, std::max(16l, all / (3l * ctx().sm_count))));
+      const long ktiles = std::max(1, ceil_div(p.K, TC_BK)), slices = n * tiles <= 2 * ctx().sm_count ? small_slices(n * tiles, ktiles, bn) : 1;
+      p.tiles_per_slice = ceil_div(ktiles, slices);
+      p.slices = ceil_div(ktiles, p.tiles_per_slice);
     }
-    p.tiles_per_slice = ceil_div(ktiles, slices);
-    p.slices = ceil_div(ktiles, p.tiles_per_slice);
-    if (p.slices > 1) {
-      p.ws = (float *)ws_alloc(sizeof(float) * tiles * p.slices * 64 * bn);
+    const long slots = p.kind == kGroupRows ? (p.slices > 1 ? n * p.slices : 0) : i ? 0 : cut;
+    if (slots) {
+      p.ws = (float *)ws_alloc(sizeof(float) * slots * tiles * p.tile_floats);
       p.tickets = zero_words();
     }
     launch_small_width(p, bn, a_k, b_k);
