@@ -184,8 +184,10 @@ static bool few_rows_groups(SmallGroups p, const Groups &g) {
 constexpr int kFewSums = 16;
 template <int R, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_sums_kernel(const float *__restrict__ x, long ldx, const float *__restrict__ gz, long ldg, long in, long out,
-                                                                   float *__restrict__ gw, float scale, int T, const __grid_constant__ GroupList list) {
+                                                                   float *__restrict__ gw, float scale, int T, const int *stalled_flag,
+                                                                   const __grid_constant__ GroupList list) {
   pdl_begin();
+  const int stalled = *reinterpret_cast<const volatile int *>(stalled_flag);   // as SmallProblem::stalled
   constexpr int U = 4, ROWS = 8;
   __shared__ __align__(16) float g[8 * ROWS][R];
   const GroupEntry e = list.at(blockIdx.z);
@@ -209,7 +211,7 @@ static __global__ void __launch_bounds__(256) few_rows_sums_kernel(const float *
     }
   }
   __syncthreads();
-  if (column(0) >= in) return;
+  if (column(0) >= in || stalled) return;
   float *to = gw + e.group * out * in;
 #pragma unroll
   for (int u0 = 0; u0 < ROWS; u0 += U) {
@@ -269,10 +271,11 @@ bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, l
   const long columns = (in + 4 * T - 1) / (4 * T), rows = 8 * (256 / T), tiles = (out + rows - 1) / rows;
   if (tiles > 65535) return false;
   WsScope scope;
+  const int *stalled = stall_ctl().dev_flag;
   each_few<kFewSums>(g, most, [&](auto r, const GroupList &list) {
     const dim3 grid((unsigned)columns, (unsigned)tiles, (unsigned)list.count);
-    if (vec) pdl_launch(few_rows_sums_kernel<decltype(r)::value, true>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, list);
-    else pdl_launch(few_rows_sums_kernel<decltype(r)::value, false>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, list);
+    if (vec) pdl_launch(few_rows_sums_kernel<decltype(r)::value, true>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, stalled, list);
+    else pdl_launch(few_rows_sums_kernel<decltype(r)::value, false>, grid, 256, 0, x, ldx, gz, ldg, in, out, gw, scale, T, stalled, list);
     check_launch("few_rows_sums");
   });
   return true;
@@ -286,8 +289,10 @@ bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, l
 constexpr int kFewRun = 512, kFewBack = 8;
 template <int R, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_back_kernel(const float *__restrict__ w, const float *__restrict__ gz, long ldg, long in, long out, float *__restrict__ gx,
-                                                                   int run, float *part, unsigned *tickets, const __grid_constant__ GroupList list) {
+                                                                   int run, float *part, unsigned *tickets, const int *stalled_flag,
+                                                                   const __grid_constant__ GroupList list) {
   pdl_begin();
+  const int stalled = *reinterpret_cast<const volatile int *>(stalled_flag);   // as SmallProblem::stalled
   constexpr int U = 8, Q = R < 4 ? R : 4;
   __shared__ __align__(16) float sm[R * kFewRun > 8 * Q * 128 ? R * kFewRun : 8 * Q * 128];
   __shared__ bool last;
@@ -335,6 +340,7 @@ static __global__ void __launch_bounds__(256) few_rows_back_kernel(const float *
     }
     w += (long)kFewRun * in;
   }
+  if (stalled) return;   // (all blocks: no ticket is taken)
   const long tile = (long)blockIdx.z * gridDim.x + blockIdx.x;
   float *mine = part + (tile * gridDim.y + blockIdx.y) * (R * 128);
 #pragma unroll
@@ -378,6 +384,7 @@ static bool few_rows_back(const Groups &g, const float *gz, long ldg, long in, l
   if (most > kFewBack || g.n - std::count(g.counts, g.counts + g.n, 0l) < 8) return false;
   const bool vec = in % 4 == 0 && ((uintptr_t)w & 15) == 0;
   const long columns = (in + 127) / 128;
+  const int *stalled = stall_ctl().dev_flag;
   WsScope scope;
   each_few<kFewBack>(g, most, [&](auto r, const GroupList &list) {
     constexpr int R = decltype(r)::value;
@@ -387,8 +394,8 @@ static bool few_rows_back(const Groups &g, const float *gz, long ldg, long in, l
     const long run = std::max(64l, ((out + wanted - 1) / wanted + 63) / 64 * 64), splits = (out + run - 1) / run;
     const dim3 grid((unsigned)columns, (unsigned)splits, (unsigned)list.count);
     float *part = splits > 1 ? (float *)ws_alloc(sizeof(float) * tiles * splits * R * 128) : nullptr;
-    if (vec) pdl_launch(few_rows_back_kernel<R, true>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), list);
-    else pdl_launch(few_rows_back_kernel<R, false>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), list);
+    if (vec) pdl_launch(few_rows_back_kernel<R, true>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), stalled, list);
+    else pdl_launch(few_rows_back_kernel<R, false>, grid, 256, 0, w, gz, ldg, in, out, gx, (int)run, part, zero_words(), stalled, list);
     check_launch("few_rows_back");
   });
   return true;
