@@ -175,13 +175,13 @@ static void attach_group_map(GroupOperand<MN, PREC> &op, const void *base, long 
     encode_groups(&op.tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, MN, groups, rows, K, ld, tile_rows);
   }
 }
-// kPairs: `ld` is the padded length of a line's halves, whose FP32 form has that pitch.
+// kPairs: `ld` is the padded length of a line's halves, whose FP32 form has that pitch; it lies in `wide`, or (null) in the halves' place.
 template <int PREC, bool MN>
-static void attach_raw_map(RawOperand<MN, PREC> &op, const void *base, long rows, long K, long ld, int tile_rows) {
+static void attach_raw_map(RawOperand<MN, PREC> &op, const void *base, long rows, long K, long ld, int tile_rows, const void *wide = nullptr) {
   if constexpr (PREC == kPairs) {
     op.lo = (int)ld;
     encode_matrix(&op.tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, MN, MN ? 2 * ld : rows, MN ? K : 2 * ld, 2 * ld, tile_rows);
-    encode_matrix(&op.tmap_wide, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, MN, rows, K, ld, tile_rows);
+    encode_matrix(&op.tmap_wide, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, wide ? wide : base, MN, rows, K, ld, tile_rows);
   } else if (PREC == kBf16) {
     encode_matrix(&op.tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, MN, rows, K, ld, tile_rows);
   } else {

@@ -894,12 +894,48 @@ static __global__ void __launch_bounds__(256) unfold_grad_input_kernel(const flo
 
 // Up to two matrices (blockIdx.y) as FP16 pairs: lines of `run` values become [hi: ldp][lo: ldp], ldp = run padded with zeros to whole
 // spans, or lines of ldp FP32 values.  A warp takes 512 values of a line, all loads in flight before the first store.
-struct PairJob { const float *src; void *dst; long lines, run, ld, ldp; int vec; Ranges ranges; };
+// An operand of two products has the form that each of them takes: where these differ, pairs in dst and FP32 values in `wide`.
+struct PairJob {
+  const float *src;
+  void *dst;
+  long lines, run, ld, ldp;
+  int vec;
+  Ranges ranges;           // of a product's operands, this one's first
+  float *wide = nullptr;   // (null: dst, and there is no other product)
+  Ranges other = {};       // of the second product's
+};
+struct SplitForm {
+  bool pairs, wide;
+  float scale;
+  __device__ __forceinline__ explicit SplitForm(const PairJob &j) {
+    const bool one = j.ranges.wide(), two = j.wide ? j.other.wide() : one;
+    wide = one || two;
+    pairs = !(one && two);
+    scale = pairs ? pair_scale(*j.ranges.rec[0]) : 1.f;
+  }
+  // 16 values of line l of the result: four from column c0 on, and each 128 further.
+  __device__ __forceinline__ void store(const PairJob &j, long l, long c0, const float4 (&v)[4]) const {
+    float *d = reinterpret_cast<float *>(j.dst) + l * j.ldp, *f = j.wide ? j.wide + l * j.ldp : d;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const long c = c0 + g * 128;
+      if (c >= j.ldp) break;
+      if (wide) *reinterpret_cast<float4 *>(f + c) = v[g];
+      if (pairs) {
+        __half2 hi[2], lo[2];
+        split_pair(v[g].x * scale, v[g].y * scale, hi[0], lo[0]);
+        split_pair(v[g].z * scale, v[g].w * scale, hi[1], lo[1]);
+        uint2 *h = reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(d) + c);
+        h[0] = make_uint2(half2_bits(hi[0]), half2_bits(hi[1]));
+        h[j.ldp / 4] = make_uint2(half2_bits(lo[0]), half2_bits(lo[1]));
+      }
+    }
+  }
+};
 static __global__ void __launch_bounds__(256) split_matrix_kernel(const PairJob a, const PairJob b) {
   pdl_begin();
   const PairJob &j = blockIdx.y ? b : a;
-  const bool wide = j.ranges.wide();
-  const float scale = wide ? 1.f : pair_scale(*j.ranges.rec[0]);
+  const SplitForm form(j);
   const int lane = threadIdx.x & 31;
   const long warps = (long)gridDim.x * 8, parts = (j.ldp + 511) / 512;
   for (long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5); w < j.lines * parts; w += warps) {
@@ -912,22 +948,7 @@ static __global__ void __launch_bounds__(256) split_matrix_kernel(const PairJob 
       if (j.vec && c + 4 <= j.run) v[g] = __ldg(reinterpret_cast<const float4 *>(s + c));
       else v[g] = make_float4(c < j.run ? s[c] : 0.f, c + 1 < j.run ? s[c + 1] : 0.f, c + 2 < j.run ? s[c + 2] : 0.f, c + 3 < j.run ? s[c + 3] : 0.f);
     }
-    float *d = reinterpret_cast<float *>(j.dst) + l * j.ldp;
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const long c = c0 + g * 128;
-      if (c >= j.ldp) break;
-      if (wide) {
-        *reinterpret_cast<float4 *>(d + c) = v[g];
-      } else {
-        __half2 hi[2], lo[2];
-        split_pair(v[g].x * scale, v[g].y * scale, hi[0], lo[0]);
-        split_pair(v[g].z * scale, v[g].w * scale, hi[1], lo[1]);
-        uint2 *h = reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(d) + c);
-        h[0] = make_uint2(half2_bits(hi[0]), half2_bits(hi[1]));
-        h[j.ldp / 4] = make_uint2(half2_bits(lo[0]), half2_bits(lo[1]));
-      }
-    }
+    form.store(j, l, c0, v);
   }
 }
 

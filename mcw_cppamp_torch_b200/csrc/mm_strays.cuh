@@ -195,8 +195,7 @@ static __global__ void __launch_bounds__(256) split_groups_kernel(const GroupPai
                                                                   const __grid_constant__ GroupRows rows) {
   pdl_begin();
   const GroupPairJob &j = blockIdx.y == 0 ? a : blockIdx.y == 1 ? b : c;
-  const bool wide = j.ranges.wide();
-  const float scale = wide ? 1.f : pair_scale(*j.ranges.rec[0]);
+  const SplitForm form(j);
   const int lane = threadIdx.x & 31;
   const long warps = (long)gridDim.x * 8, parts = (j.ldp + 511) / 512, lines = j.grouped ? rows.padded[rows.n] : j.lines;
   for (long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5); w < lines * parts; w += warps) {
@@ -215,22 +214,7 @@ static __global__ void __launch_bounds__(256) split_groups_kernel(const GroupPai
       if (j.vec && c + 4 <= run) v[g] = __ldg(reinterpret_cast<const float4 *>(s + c));
       else v[g] = make_float4(c < run ? s[c] : 0.f, c + 1 < run ? s[c + 1] : 0.f, c + 2 < run ? s[c + 2] : 0.f, c + 3 < run ? s[c + 3] : 0.f);
     }
-    float *d = reinterpret_cast<float *>(j.dst) + l * j.ldp;
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const long c = c0 + g * 128;
-      if (c >= j.ldp) break;
-      if (wide) {
-        *reinterpret_cast<float4 *>(d + c) = v[g];
-      } else {
-        __half2 hi[2], lo[2];
-        split_pair(v[g].x * scale, v[g].y * scale, hi[0], lo[0]);
-        split_pair(v[g].z * scale, v[g].w * scale, hi[1], lo[1]);
-        uint2 *h = reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(d) + c);
-        h[0] = make_uint2(half2_bits(hi[0]), half2_bits(hi[1]));
-        h[j.ldp / 4] = make_uint2(half2_bits(lo[0]), half2_bits(lo[1]));
-      }
-    }
+    form.store(j, l, c0, v);
   }
 }
 

@@ -111,8 +111,8 @@ static void gemm_raw(GemmSide x, GemmSide y, long k, float alpha, float beta, fl
 }
 // The same over FP16 pairs: a pass measures both operands and one splits them, each as it lies in memory.
 template <bool A_MN, bool B_MN, bool FUSED = false>
-static void gemm_pairs_t(const void *a, long lda, const void *b, long ldb, long m, long n, long k, const mm::Epilogue &epi,
-                         const mm::Ranges &ranges, const mm::LinearEpilogue *tail = nullptr) {
+static void gemm_pairs_t(const mm::PairJob &a, const mm::PairJob &b, long m, long n, long k, const mm::Epilogue &epi, const mm::Ranges &ranges,
+                         const mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
   typename MatrixProblem<A_MN, B_MN, kPairs, FUSED>::type p;
   p.epi = epi;
@@ -120,8 +120,8 @@ static void gemm_pairs_t(const void *a, long lda, const void *b, long ldb, long 
   p.M = m; p.N = n; p.K = k;
   p.range_a = ranges.rec[0]; p.range_b = ranges.rec[1]; p.ranges = ranges;
   launch_raw(p, [&](auto &q, int bn2) {
-    attach_raw_map<kPairs>(q.a, a, m, k, lda, TC_BM);
-    attach_raw_map<kPairs>(q.b, b, n, k, ldb, bn2 / 2);
+    attach_raw_map<kPairs>(q.a, a.dst, m, k, a.ldp, TC_BM, a.wide);
+    attach_raw_map<kPairs>(q.b, b.dst, n, k, b.ldp, bn2 / 2, b.wide);
   });
 }
 // An operand as pairs.
@@ -129,16 +129,16 @@ struct PairSide : GemmSide {
   mm::Measured m;
   mm::PairJob job;
 };
-// Measures and splits up to three operands of products with k, whose form is decided together.  False: there is no room for the pairs, and nothing has
-// been done.
-static bool make_pairs(PairSide *const *sides, const long *k, int n, mm::Ranges &ranges) {
+// Measures and splits both operands of a product with k; or of two products, with the first operand in each, whose forms are decided product by product.
+// False: there is no room for the pairs, and nothing has been done.
+static bool make_pairs(PairSide *const *sides, const long *k, int n) {
   using namespace mm;
   // the copies, with a little for the measures (under a hundredth of them) and the partial sums (blocks of 256 KB, up to
   // five rounds of clusters)
   double need = 96e6;
   for (int i = 0; i < n; i++) {
     const GemmSide &s = *sides[i];
-    need += 4.1 * (double)(s.along_k ? s.rows : k[i]) * (double)((s.along_k ? k[i] : s.rows) + 64);
+    need += 4.1 * (double)(s.along_k ? s.rows : k[i]) * (double)((s.along_k ? k[i] : s.rows) + 64) * (n > 2 && i == 0 ? 2 : 1);
   }
   if (!ws_reserve((size_t)need)) return false;
   RangeJob measure[3];
@@ -150,10 +150,15 @@ static bool make_pairs(PairSide *const *sides, const long *k, int n, mm::Ranges 
     measure[i] = range_job(s.p, lines, run, s.ld, sides[i]->m);
     PairJob &j = sides[i]->job;
     j = PairJob{s.p, ws_alloc(sizeof(float) * lines * ldp), lines, run, s.ld, ldp, ((uintptr_t)s.p & 15) == 0 && s.ld % 4 == 0, {}};
-    for (int o = 0; o < n; o++) j.ranges.rec[o] = sides[(i + o) % n]->m.rec;   // its own first
+    j.ranges.rec[0] = sides[i]->m.rec;
+    j.ranges.rec[1] = sides[i ? 0 : 1]->m.rec;
+    if (n > 2 && i == 0) {
+      j.wide = (float *)ws_alloc(sizeof(float) * lines * ldp);
+      j.other.rec[0] = sides[0]->m.rec;
+      j.other.rec[1] = sides[2]->m.rec;
+    }
     pieces = std::max(pieces, lines * ((ldp + 511) / 512));
   }
-  ranges = sides[0]->job.ranges;
   launch_ranges(measure[0], &measure[1]);
   if (n > 2) launch_ranges(measure[2], nullptr);
   const unsigned blocks = (unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l);
@@ -166,22 +171,19 @@ static bool make_pairs(PairSide *const *sides, const long *k, int n, mm::Ranges 
   return true;
 }
 template <bool FUSED = false>
-static void pairs_product(PairSide x, PairSide y, const mm::Ranges &ranges, long k, float alpha, float beta, float *c, long ldc, const float *row_bias,
-                          mm::LinearEpilogue *tail = nullptr) {
+static void pairs_product(PairSide x, PairSide y, long k, float alpha, float beta, float *c, long ldc, const float *row_bias, mm::LinearEpilogue *tail = nullptr) {
   using namespace mm;
   const Epilogue epi = gemm_sides(x, y, alpha, beta, c, ldc, row_bias, tail);
-  Ranges r = ranges;
+  Ranges r;
   r.rec[0] = x.m.rec; r.rec[1] = y.m.rec;
-  for (const RangeRec *rec : ranges.rec)
-    if (rec && rec != x.m.rec && rec != y.m.rec) r.rec[2] = rec;
   const GemmSide &xs = x, &ys = y;
   if constexpr (FUSED) {
     tail->a = x.m.rec; tail->b = y.m.rec; tail->ranges = r;
-    gemm_pairs_t<false, false, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r, tail);
-  } else if (!xs.along_k && ys.along_k) gemm_pairs_t<true, false>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
-  else if (xs.along_k && ys.along_k) gemm_pairs_t<false, false>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
-  else if (!xs.along_k) gemm_pairs_t<true, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
-  else gemm_pairs_t<false, true>(x.job.dst, x.job.ldp, y.job.dst, y.job.ldp, xs.rows, ys.rows, k, epi, r);
+    gemm_pairs_t<false, false, true>(x.job, y.job, xs.rows, ys.rows, k, epi, r, tail);
+  } else if (!xs.along_k && ys.along_k) gemm_pairs_t<true, false>(x.job, y.job, xs.rows, ys.rows, k, epi, r);
+  else if (xs.along_k && ys.along_k) gemm_pairs_t<false, false>(x.job, y.job, xs.rows, ys.rows, k, epi, r);
+  else if (!xs.along_k) gemm_pairs_t<true, true>(x.job, y.job, xs.rows, ys.rows, k, epi, r);
+  else gemm_pairs_t<false, true>(x.job, y.job, xs.rows, ys.rows, k, epi, r);
   Epilogue sums = epi;   // (with a linear layer's epilogue: where there are strays the product has left the sums there)
   if (FUSED && tail->z) sums.out = tail->z;
   pdl_launch(matrix_strays_kernel, dim3((unsigned)std::min(ceil_div(ys.rows, 256), ctx().sm_count), 4), 256, 0, StraySide{xs.p, xs.ld, x.job.run, xs.along_k, x.m},
@@ -194,9 +196,8 @@ static bool gemm_pairs(GemmSide x, GemmSide y, long k, float alpha, float beta, 
   PairSide xp{x, {}, {}}, yp{y, {}, {}};
   PairSide *sides[2] = {&xp, &yp};
   const long ks[2] = {k, k};
-  mm::Ranges ranges;
-  if (!make_pairs(sides, ks, 2, ranges)) return false;
-  pairs_product<FUSED>(xp, yp, ranges, k, alpha, beta, c, ldc, row_bias, tail);
+  if (!make_pairs(sides, ks, 2)) return false;
+  pairs_product<FUSED>(xp, yp, k, alpha, beta, c, ldc, row_bias, tail);
   return true;
 }
 // Whether pairs finish before TF32, the passes over the operands included.  Their copies are scratch that TF32 does without: bounded.
@@ -360,22 +361,20 @@ void linear_product(const float *x, long ldx, long rows, long in, long out, cons
 void linear_gradients(const float *x, long ldx, const float *gz, long ldg, long rows, long in, long out, const float *w, float *gx, float *gw, float scale) {
   WsScope scope;
   if (gw && ctx().math_mode != 1 && few_rows_sums(Groups{&rows, 1, rows}, x, ldx, gz, ldg, in, out, gw, scale)) gw = nullptr;
-  if (ctx().math_mode == 0 && gx && gw && pairs_are_faster(in, rows, out) && pairs_are_faster(in, out, rows) && !small_is_faster(in, rows, out, true) &&
-      !small_is_faster(in, out, rows, true)) {
+  const bool gz_ok = mm::raw_matrix_ok(gz, ldg), input_ok = gz_ok && mm::raw_matrix_ok(w, in), weight_ok = gz_ok && mm::raw_matrix_ok(x, ldx);
+  const bool engine = ctx().math_mode == 0 && gx && gw && !small_is_faster(in, rows, out, input_ok) && !small_is_faster(in, out, rows, weight_ok);   // for both
+  if (engine && pairs_are_faster(in, rows, out) && pairs_are_faster(in, out, rows)) {
     PairSide g{{gz, ldg, true, rows}, {}, {}}, ws{{w, in, false, in}, {}, {}}, xs{{x, ldx, false, in}, {}, {}};
     PairSide *sides[3] = {&g, &ws, &xs};
     const long ks[3] = {out, out, rows};
-    mm::Ranges ranges;
-    if (make_pairs(sides, ks, 3, ranges)) {
-      pairs_product(ws, g, ranges, out, 1.f, 0.f, gx, in, nullptr);
+    if (make_pairs(sides, ks, 3)) {
+      pairs_product(ws, g, out, 1.f, 0.f, gx, in, nullptr);
       g.along_k = false; g.rows = out;      // the same lines, summed over
-      pairs_product(xs, g, ranges, rows, scale, 1.f, gw, in, nullptr);
+      pairs_product(xs, g, rows, scale, 1.f, gw, in, nullptr);
       return;
     }
   }
-  const bool gz_ok = mm::raw_matrix_ok(gz, ldg), input_ok = gz_ok && mm::raw_matrix_ok(w, in), weight_ok = gz_ok && mm::raw_matrix_ok(x, ldx);
-  if (ctx().math_mode == 0 && gx && gw && !(input_ok && weight_ok) && !small_is_faster(in, rows, out, input_ok) && !small_is_faster(in, out, rows, weight_ok) &&
-      !pairs_are_faster(in, rows, out) && !pairs_are_faster(in, out, rows)) {
+  if (engine && !(input_ok && weight_ok) && !pairs_are_faster(in, rows, out) && !pairs_are_faster(in, out, rows)) {
     GemmSide g{gz, ldg, true, rows}, ws{w, in, false, in}, xs{x, ldx, false, in};
     GemmSide *sides[3] = {&g, &ws, &xs};
     const long ks[3] = {out, out, rows};

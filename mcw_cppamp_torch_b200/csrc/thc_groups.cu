@@ -529,16 +529,22 @@ struct PairSide {
   Measured m;
   void *dst;
   long ldp;
+  float *wide = nullptr;   // (PairJob)
 };
+static Ranges ranges_of(const PairSide &own, const PairSide &other) {
+  Ranges r;
+  r.rec[0] = own.m.rec; r.rec[1] = other.m.rec;
+  return r;
+}
 struct GroupPairs {
   GroupRows rows;
-  PairSide *sides[3];
-  int n = 0;
-  Ranges ranges;      // of all sides: their form is decided together
   long padded() const { return rows.padded[rows.n]; }
 };
-// False: there is no room for the pairs, and nothing has been done.
-static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<PairSide *> sides) {
+// Both operands of a product, or of two, with the first operand in each, whose forms are decided product by product.  False: there is no room for the
+// pairs, and nothing has been done.
+static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<PairSide *> list) {
+  const int n = (int)list.size();
+  PairSide *const *sides = list.begin();
   gp.rows.n = g.n;
   gp.rows.real[0] = gp.rows.padded[0] = 0;
   for (int e = 0; e < g.n; e++) {
@@ -546,29 +552,31 @@ static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<Pa
     gp.rows.padded[e + 1] = gp.rows.padded[e] + (int)((g.counts[e] + 63) / 64 * 64);
   }
   double need = 96e6;
-  for (PairSide *s : sides) need += 4.1 * (double)(s->grouped ? gp.padded() : s->lines) * (double)(s->run + 64);
+  for (int i = 0; i < n; i++) need += 4.1 * (double)(sides[i]->grouped ? gp.padded() : sides[i]->lines) * (double)(sides[i]->run + 64) * (n > 2 && i == 0 ? 2 : 1);
   if (!ws_reserve((size_t)need)) return false;
   RangeJob ranges[3];
   GroupPairJob jobs[3] = {};
   long pieces = 0;
-  for (PairSide *s : sides) {
-    const int i = gp.n++;
-    gp.sides[i] = s;
-    s->m = new_measured();
-    s->ldp = (s->run + 63) / 64 * 64;
-    const long lines = s->grouped ? gp.padded() : s->lines;
-    s->dst = ws_alloc(sizeof(float) * lines * s->ldp);
-    gp.ranges.rec[i] = s->m.rec;
-    ranges[i] = range_job(s->p, s->lines, s->run, s->ld, s->m);
-    static_cast<PairJob &>(jobs[i]) = PairJob{s->p, s->dst, s->lines, s->run, s->ld, s->ldp, ((uintptr_t)s->p & 15) == 0 && s->ld % 4 == 0, {}};
-    jobs[i].grouped = s->grouped;
-    pieces = std::max(pieces, lines * ((s->ldp + 511) / 512));
+  for (int i = 0; i < n; i++) sides[i]->m = new_measured();
+  for (int i = 0; i < n; i++) {
+    PairSide &s = *sides[i];
+    s.ldp = (s.run + 63) / 64 * 64;
+    const long lines = s.grouped ? gp.padded() : s.lines;
+    s.dst = ws_alloc(sizeof(float) * lines * s.ldp);
+    ranges[i] = range_job(s.p, s.lines, s.run, s.ld, s.m);
+    GroupPairJob &j = jobs[i];
+    static_cast<PairJob &>(j) = PairJob{s.p, s.dst, s.lines, s.run, s.ld, s.ldp, ((uintptr_t)s.p & 15) == 0 && s.ld % 4 == 0, {}};
+    j.grouped = s.grouped;
+    j.ranges = ranges_of(s, *sides[i ? 0 : 1]);
+    if (n > 2 && i == 0) {
+      j.wide = s.wide = (float *)ws_alloc(sizeof(float) * lines * s.ldp);
+      j.other = ranges_of(s, *sides[2]);
+    }
+    pieces = std::max(pieces, lines * ((s.ldp + 511) / 512));
   }
-  for (int i = 0; i < gp.n; i++)
-    for (int k = 0; k < gp.n; k++) jobs[i].ranges.rec[k] = gp.ranges.rec[(i + k) % gp.n];   // its own first
   launch_ranges(ranges[0], &ranges[1]);
-  if (gp.n > 2) launch_ranges(ranges[2], nullptr);
-  pdl_launch(split_groups_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), (unsigned)gp.n), 256, 0, jobs[0], jobs[1], jobs[2], gp.rows);
+  if (n > 2) launch_ranges(ranges[2], nullptr);
+  pdl_launch(split_groups_kernel, dim3((unsigned)std::min<long>((pieces + 7) / 8, ctx().sm_count * 8l), (unsigned)n), 256, 0, jobs[0], jobs[1], jobs[2], gp.rows);
   check_launch("split_groups");
   return true;
 }
@@ -589,12 +597,12 @@ static void pairs_rows(const Groups &g, const GroupPairs &gp, const PairSide &w,
   p.M = features; p.N = gp.padded(); p.K = K;
   p.bias_group = out;
   p.tail = tail;
-  p.range_a = w.m.rec; p.range_b = x.m.rec; p.ranges = gp.ranges;
+  p.range_a = w.m.rec; p.range_b = x.m.rec; p.ranges = ranges_of(w, x);
   launch_groups(p, width, padded(largest_first(row_tiles(g, width)), gp.rows), (features + 255) / 256, [&](auto &q, int bn2) {
     attach_group_map<MN, kPairs>(q.a, w.dst, g.n, features, K, w.ldp, TC_BM);
-    attach_raw_map<kPairs>(q.b, x.dst, gp.padded(), K, x.ldp, bn2 / 2);
+    attach_raw_map<kPairs>(q.b, x.dst, gp.padded(), K, x.ldp, bn2 / 2, x.wide);
   });
-  pdl_launch(group_row_strays_kernel, (unsigned)std::min<long>(g.rows, ctx().sm_count), 256, 0, GroupStrays{w.p, in, out, x.p, x.ld, x.run, w.m, x.m}, !MN, sums, gp.ranges,
+  pdl_launch(group_row_strays_kernel, (unsigned)std::min<long>(g.rows, ctx().sm_count), 256, 0, GroupStrays{w.p, in, out, x.p, x.ld, x.run, w.m, x.m}, !MN, sums, p.ranges,
              gp.rows);
   check_launch("group_strays");
 }
@@ -630,7 +638,7 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
       PairSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true};
       GroupPairs gp;
       if (make_pairs(gp, g, {&wp, &xp})) {
-        tail.a = wp.m.rec; tail.b = xp.m.rec; tail.ranges = gp.ranges;
+        tail.a = wp.m.rec; tail.b = xp.m.rec; tail.ranges = ranges_of(wp, xp);
         float *sums = z ? z : y;
         pairs_rows<false, true>(g, gp, wp, xp, in, out, c.width, epi, sums, tail);
         LinearTail after;
@@ -727,12 +735,12 @@ static void pairs_sums(const Groups &g, const GroupPairs &gp, int w, const PairS
   GroupProblem<RawOperand<true, kPairs>, RawOperand<true, kPairs>, kGroupSums, false, kPairs> p;
   set_sums(p, in, out, gw, scale);
   p.K = gp.padded();
-  p.range_a = x.m.rec; p.range_b = gz.m.rec; p.ranges = gp.ranges;
+  p.range_a = x.m.rec; p.range_b = gz.m.rec; p.ranges = ranges_of(x, gz);
   launch_groups(p, w, largest_first(padded(whole_groups(g), gp.rows)), ((in + 255) / 256) * ((out + w - 1) / w), [&](auto &q, int bn2) {
     attach_raw_map<kPairs>(q.a, x.dst, in, gp.padded(), x.ldp, TC_BM);
-    attach_raw_map<kPairs>(q.b, gz.dst, out, gp.padded(), gz.ldp, bn2 / 2);
+    attach_raw_map<kPairs>(q.b, gz.dst, out, gp.padded(), gz.ldp, bn2 / 2, gz.wide);
   });
-  pdl_launch(group_sum_strays_kernel, (unsigned)std::min<long>(out, ctx().sm_count), 256, 0, x.p, x.ld, in, gz.p, gz.ld, out, gw, scale, x.m, gz.m, gp.ranges, gp.rows);
+  pdl_launch(group_sum_strays_kernel, (unsigned)std::min<long>(out, ctx().sm_count), 256, 0, x.p, x.ld, in, gz.p, gz.ld, out, gw, scale, x.m, gz.m, p.ranges, gp.rows);
   check_launch("group_strays");
 }
 
