@@ -435,14 +435,16 @@ def _need_kept(m):
 
 class LayerNorm(Module):
     """Rows normalised to mean zero and variance one over the trailing `sizes`, times `weight` plus `bias` (one of each for every place
-    in a row); with affine=False the normalised rows themselves.  `mean` and `invStd` keep each row's statistics for the backward
-    pass; after evaluate() they are left alone."""
+    in a row); with affine=False the normalised rows themselves.  An input may have neighbours among the sizes as one dimension, or one of
+    them as several.  `mean` and `invStd` keep each row's statistics for the backward pass; after evaluate() they are left alone."""
+    sizes = ()
 
     def __init__(self, *sizes, eps=1e-5, affine=True):
         super().__init__()
         self.size, self.eps, self.train, self._kept = math.prod(sizes), eps, True, True
         if not sizes or min(sizes) < 1:
             raise ValueError("LayerNorm: positive sizes expected")
+        self.sizes = sizes
         self.mean, self.invStd = GPUTensor(), GPUTensor()
         self.weight = self.bias = self.gradWeight = self.gradBias = None
         if affine:
@@ -454,8 +456,22 @@ class LayerNorm(Module):
             return None, None
         return _need_gpu(self.weight, "LayerNorm.weight")._p, self.bias._p
 
+    def _ends(self, sizes):
+        """How many values each of the last dimensions has with those behind it, up to a row's."""
+        n, ends = 1, set()
+        for k in reversed(sizes):
+            if n >= self.size:
+                break
+            n *= k
+            ends.add(n)
+        return ends
+
     def updateOutput(self, input):
         _need_gpu(input, "LayerNorm")
+        if len(self.sizes) > 1:
+            mine, its = self._ends(self.sizes), self._ends(input.size())
+            if not (mine <= its or its <= mine):
+                raise ValueError("LayerNorm: trailing sizes %s expected, not those of %s" % (self.sizes, tuple(input.size())))
         w, b = self._affine()
         keep = (self.mean._p, self.invStd._p) if self.train else (None, None)
         self._kept = self.train

@@ -1,0 +1,40 @@
+"""What the modules LayerNorm, FusedLinear and GroupedLinear do on the host around their library calls.  Tensors are shapes over memory that nothing reads,
+as in tests/test_feedforward_refusals.py, but for the tests that are marked."""
+import pytest
+
+from mcw_cppamp_torch_b200 import nn
+from test_feedforward_refusals import fake, norm  # noqa: F401
+
+
+@pytest.mark.parametrize("sizes,shape", [((6, 5), (4, 5, 6)), ((6, 5), (5, 6)), ((6, 5), (4, 3, 10)), ((4, 6, 5), (2, 4, 5, 6)), ((4, 6, 5), (6, 4, 5)),
+                                         ((2, 8), (3, 4, 4)), ((3, 4), (4, 1, 3))])
+def test_layer_norm_refuses_other_sizes_of_the_same_product(fake, sizes, shape):  # noqa: F811
+    m = norm(fake, sizes[0])
+    m.__init__(*sizes)
+    m.weight, m.bias = fake(m.size), fake(m.size)
+    with pytest.raises(ValueError, match="trailing sizes"):
+        m.forward(fake(*shape))
+
+
+@pytest.mark.parametrize("sizes,shape", [((6, 5), (4, 6, 5)), ((6, 5), (6, 5)), ((6, 5), (7, 30)), ((6, 5), (30,)), ((6, 5), (3, 2, 3, 5)), ((30,), (4, 5, 6)),
+                                         ((30,), (4, 30)), ((4, 6, 5), (3, 24, 5)), ((4, 6, 5), (4, 30)), ((6, 1, 5), (6, 5)), ((6, 5), (6, 1, 5)), ((1, 1), (4, 3)),
+                                         ((6, 5), (6, 5, 1)), ((1, 6, 5), (2, 6, 5))])
+def test_layer_norm_takes_merged_and_split_sizes(fake, monkeypatch, sizes, shape):  # noqa: F811
+    calls = []
+
+    class Library:
+        def THGPUNN_LayerNorm_updateOutput(self, *args):
+            calls.append(args)
+    m = nn.LayerNorm(*sizes)
+    m.weight, m.bias = fake(m.size), fake(m.size)
+    x = fake(*shape)
+    monkeypatch.setattr(nn, "lib", Library)
+    m.forward(x)
+    assert len(calls) == 1 and calls[0][6] == m.size
+
+
+def test_layer_norm_refuses_sizes_that_make_no_row(fake):  # noqa: F811
+    m = nn.LayerNorm(6, 5)
+    m.weight, m.bias = fake(30), fake(30)
+    with pytest.raises(ValueError, match="trailing sizes"):
+        m.forward(fake(4, 7))
