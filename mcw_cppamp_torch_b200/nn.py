@@ -474,8 +474,8 @@ class LayerNorm(Module):
                 raise ValueError("LayerNorm: trailing sizes %s expected, not those of %s" % (self.sizes, tuple(input.size())))
         w, b = self._affine()
         keep = (self.mean._p, self.invStd._p) if self.train else (None, None)
-        self._kept = self.train
         lib().THGPUNN_LayerNorm_updateOutput(input._p, self.output._p, w, b, keep[0], keep[1], self.size, self.eps)
+        self._kept = self.train
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
@@ -523,9 +523,9 @@ class FusedLinear(Linear):
         x, residual = self._split(input)
         _need_gpu(self.weight, "FusedLinear.weight")
         keep = self.preactivation._p if self.train and self._code else None
-        self._kept = self.train or not self._code
         lib().THGPUNN_FusedLinear_updateOutput(x._p, residual._p if residual is not None else None, self.output._p, keep, self.weight._p, self.bias._p,
                                                self._code)
+        self._kept = self.train or not self._code
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):
@@ -602,8 +602,8 @@ class GroupedLinear(Module):
         x, counts = self._split(input)
         _need_gpu(self.weight, "GroupedLinear.weight")
         keep = self.preactivation._p if self.train and self._code else None
-        self._kept = self.train or not self._code
         lib().THGPUNN_GroupedLinear_updateOutput(x._p, counts, self.groups, self.output._p, keep, self.weight._p, self.bias._p, self._code)
+        self._kept = self.train or not self._code
         return self.output
 
     def _back(self, input, gradOutput, gradInput, gradWeight, gradBias, scale):

@@ -2,8 +2,9 @@
 as in tests/test_feedforward_refusals.py, but for the tests that are marked."""
 import pytest
 
+import mcw_cppamp_torch_b200 as gt
 from mcw_cppamp_torch_b200 import nn
-from test_feedforward_refusals import fake, norm  # noqa: F401
+from test_feedforward_refusals import fake, grouped, linear, norm  # noqa: F401
 
 
 @pytest.mark.parametrize("sizes,shape", [((6, 5), (4, 5, 6)), ((6, 5), (5, 6)), ((6, 5), (4, 3, 10)), ((4, 6, 5), (2, 4, 5, 6)), ((4, 6, 5), (6, 4, 5)),
@@ -38,3 +39,14 @@ def test_layer_norm_refuses_sizes_that_make_no_row(fake):  # noqa: F811
     m.weight, m.bias = fake(30), fake(30)
     with pytest.raises(ValueError, match="trailing sizes"):
         m.forward(fake(4, 7))
+
+
+@pytest.mark.parametrize("make,bad", [(norm, lambda f: f(5, 9)), (linear, lambda f: f(5, 7)), (grouped, lambda f: [f(5, 7), [2, 0, 3]])])
+@pytest.mark.parametrize("kept", [True, False])
+def test_a_refused_forward_pass_changes_nothing_about_what_is_kept(fake, make, bad, kept):  # noqa: F811
+    """Behind an evaluation, a training pass that is refused leaves the module with nothing to go back by; and one that evaluates leaves what there was."""
+    m = make(fake)
+    m._kept, m.train = kept, not kept
+    with pytest.raises(gt.THCError):
+        m.forward(bad(fake))
+    assert m._kept is kept
