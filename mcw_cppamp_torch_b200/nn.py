@@ -505,7 +505,8 @@ class FusedLinear(Linear):
     """activation(input * weight^T + bias), or that plus a residual for the input [rows, residual], in one product whose epilogue does the
     rest.  activation: "none", "relu", "gelu" (of the normal distribution's integral) or "silu".  `preactivation` keeps the sum that the
     activation is taken of for the backward pass; after evaluate() forward passes leave it alone.
-    With a residual gradInput is [the rows' gradient, gradOutput]: the second is the given tensor itself."""
+    With a residual gradInput is [the rows' gradient, gradOutput]: the second is the given tensor itself, which is not saved or cloned with the
+    module."""
 
     def __init__(self, inputSize, outputSize, activation="none", rng=None):
         super().__init__(inputSize, outputSize, rng=rng)
@@ -538,6 +539,9 @@ class FusedLinear(Linear):
     def _grad_rows(self):
         """The rows' gradient in `gradInput`, which is a pair after a call with a residual."""
         return self.gradInput[0] if isinstance(self.gradInput, list) else self.gradInput
+
+    def __getstate__(self):
+        return dict(self.__dict__, gradInput=self._grad_rows())
 
     def updateGradInput(self, input, gradOutput):
         gi = self._grad_rows()

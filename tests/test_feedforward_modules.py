@@ -1,5 +1,6 @@
 """What the modules LayerNorm, FusedLinear and GroupedLinear do on the host around their library calls.  Tensors are shapes over memory that nothing reads,
 as in tests/test_feedforward_refusals.py, but for the tests that are marked."""
+import numpy as np
 import pytest
 
 import mcw_cppamp_torch_b200 as gt
@@ -50,3 +51,26 @@ def test_a_refused_forward_pass_changes_nothing_about_what_is_kept(fake, make, b
     with pytest.raises(gt.THCError):
         m.forward(bad(fake))
     assert m._kept is kept
+
+
+def test_the_callers_gradient_is_not_saved(fake):  # noqa: F811
+    m, rows = linear(fake), fake(5, 6)
+    for gradInput, want in (([rows, fake(5, 4)], rows), (rows, rows), (None, None)):
+        m.gradInput = gradInput
+        state = m.__getstate__()
+        assert state["gradInput"] is want and m.gradInput is gradInput and set(state) == set(m.__dict__)
+
+
+@pytest.mark.gpu
+def test_a_clone_behind_a_call_with_a_residual():
+    m = nn.FusedLinear(6, 4, "gelu").gpu()
+    rs = np.random.RandomState(0)
+    x, r, g = (gt.gpu(rs.randn(5, n).astype(np.float32)) for n in (6, 4, 4))
+    m.zeroGradParameters()
+    m.forward([x, r])
+    rows = m.backward([x, r], g)[0].float()
+    twin = m.clone()
+    assert isinstance(twin.gradInput, gt.GPUTensor) and np.array_equal(twin.gradInput.float(), rows)
+    assert np.array_equal(twin.forward([x, r]).float(), m.output.float())
+    first, second = twin.backward([x, r], g)
+    assert second is g and np.array_equal(first.float(), rows)
