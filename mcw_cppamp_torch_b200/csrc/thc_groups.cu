@@ -522,7 +522,7 @@ static void engine_rows(const Groups &g, Lines a, Lines b, long features, long K
 // ---- the two-SM engine over pairs ------------------------------------------------------------------------------------
 // An operand as FP16 pairs (mm_problem.cuh): weights as they lie, rows with each group padded by zeros to whole k tiles, so that no k tile has two
 // groups' rows.
-struct PairSide {
+struct GroupSide {
   const float *p;
   long lines, run, ld;
   bool grouped;
@@ -531,7 +531,7 @@ struct PairSide {
   long ldp;
   float *wide = nullptr;   // (PairJob)
 };
-static Ranges ranges_of(const PairSide &own, const PairSide &other) {
+static Ranges ranges_of(const GroupSide &own, const GroupSide &other) {
   Ranges r;
   r.rec[0] = own.m.rec; r.rec[1] = other.m.rec;
   return r;
@@ -542,9 +542,9 @@ struct GroupPairs {
 };
 // Both operands of a product, or of two, with the first operand in each, whose forms are decided product by product.  False: there is no room for the
 // pairs, and nothing has been done.
-static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<PairSide *> list) {
+static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<GroupSide *> list) {
   const int n = (int)list.size();
-  PairSide *const *sides = list.begin();
+  GroupSide *const *sides = list.begin();
   gp.rows.n = g.n;
   gp.rows.real[0] = gp.rows.padded[0] = 0;
   for (int e = 0; e < g.n; e++) {
@@ -559,7 +559,7 @@ static bool make_pairs(GroupPairs &gp, const Groups &g, std::initializer_list<Pa
   long pieces = 0;
   for (int i = 0; i < n; i++) sides[i]->m = new_measured();
   for (int i = 0; i < n; i++) {
-    PairSide &s = *sides[i];
+    GroupSide &s = *sides[i];
     s.ldp = (s.run + 63) / 64 * 64;
     const long lines = s.grouped ? gp.padded() : s.lines;
     s.dst = ws_alloc(sizeof(float) * lines * s.ldp);
@@ -589,7 +589,7 @@ static std::vector<GroupEntry> padded(std::vector<GroupEntry> v, const GroupRows
 }
 // As engine_rows, over the pairs of w and of the rows; what they leave out is added to `sums`.
 template <bool MN, bool FUSED>
-static void pairs_rows(const Groups &g, const GroupPairs &gp, const PairSide &w, const PairSide &x, long in, long out, int width, const Epilogue &epi, float *sums,
+static void pairs_rows(const Groups &g, const GroupPairs &gp, const GroupSide &w, const GroupSide &x, long in, long out, int width, const Epilogue &epi, float *sums,
                        const LinearEpilogue &tail) {
   const long features = MN ? in : out, K = MN ? out : in;
   GroupProblem<GroupOperand<MN, kPairs>, RawOperand<false, kPairs>, kGroupRows, FUSED, kPairs> p;
@@ -635,7 +635,7 @@ void group_forward(const Groups &g, const float *x, long ldx, long in, long out,
     LinearEpilogue tail;
     tail.act = act; tail.z = z;
     if (c.way == kEnginePairs) {
-      PairSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true};
+      GroupSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true};
       GroupPairs gp;
       if (make_pairs(gp, g, {&wp, &xp})) {
         tail.a = wp.m.rec; tail.b = xp.m.rec; tail.ranges = ranges_of(wp, xp);
@@ -730,7 +730,7 @@ static void grad_weight(const Groups &g, const Choice &c, Lines xs, Lines gs, fl
   p.at = GroupPlaces{0, xs.ld, gs.ld, out * in, 0, 0};
   small_groups(p, whole_groups(g), c.width, false, false);
 }
-static void pairs_sums(const Groups &g, const GroupPairs &gp, int w, const PairSide &x, const PairSide &gz, float *gw, float scale) {
+static void pairs_sums(const Groups &g, const GroupPairs &gp, int w, const GroupSide &x, const GroupSide &gz, float *gw, float scale) {
   const long in = x.run, out = gz.run;
   GroupProblem<RawOperand<true, kPairs>, RawOperand<true, kPairs>, kGroupSums, false, kPairs> p;
   set_sums(p, in, out, gw, scale);
@@ -758,7 +758,7 @@ void group_backward(const Groups &g, const float *x, long ldx, const float *gz, 
   const Choice ci = gx ? choose_grad_input(g, ldg, gz, in, out, w) : Choice{kSmall, 64}, cw = gw ? choose_grad_weight(g, xs, gs) : Choice{kSmall, 64};
   const bool pi = gx && ci.way == kEnginePairs, pw = gw && cw.way == kEnginePairs;
   if (pi || pw) {
-    PairSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true}, gp{gz, g.rows, out, ldg, true};
+    GroupSide wp{w, (long)g.n * out, in, in, false}, xp{x, g.rows, in, ldx, true}, gp{gz, g.rows, out, ldg, true};
     GroupPairs pairs;
     const bool made = pi && pw ? make_pairs(pairs, g, {&gp, &wp, &xp}) : pi ? make_pairs(pairs, g, {&gp, &wp}) : make_pairs(pairs, g, {&gp, &xp});
     if (made) {
