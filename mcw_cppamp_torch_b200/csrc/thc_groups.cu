@@ -167,8 +167,8 @@ static bool few_rows_groups(SmallGroups p, const Groups &g) {
   if (!p.a.vec4 || !p.b.vec4 || p.K % 4) return false;
   long most = 0, live = 0;
   for (int e = 0; e < g.n; e++) { most = std::max(most, g.counts[e]); live += g.counts[e] > 0; }
+  if (4 * tiles_of(g, 4) > 5 * live) return false;
   const std::vector<GroupEntry> entries = row_tiles(g, 4);
-  if (4 * (long)entries.size() > 5 * live) return false;
   for (size_t i = 0; i < entries.size(); i += 65535) {
     p.list = make_list(entries.data() + i, (int)std::min(entries.size() - i, (size_t)65535));
     p.stalled = stall_ctl().dev_flag;
