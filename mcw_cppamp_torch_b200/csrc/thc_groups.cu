@@ -285,7 +285,10 @@ bool few_rows_sums(const Groups &g, const float *x, long ldx, const float *gz, l
 // apart) and eight rows of w on their way; the eight warps of a block take eight rows each in turn of the block's `run` rows of w and meet in shared memory,
 // the blocks of a column tile in memory, where the last one adds their sums up in their order.  kFewRun rows' gradients lie in shared memory at a time.
 // A backward call of 64 groups, 1024 -> 2048 with 24 rows, 333 -> 515 with 100: 174 and 64 us, with the warp-level engine 208 and 76.  One
-// matrix, which has to be cut along its rows for blocks enough, stays with that engine (7 rows, 5716 -> 5630: 131 and 112).
+// matrix, which has to be cut along its rows for blocks enough, stays with that engine (7 rows, 5716 -> 5630: 131 and 112).  gradInput alone, this way / that
+// engine: 8 groups of four rows 13.8 / 21.0 us (1024 -> 2048), 132 / 150 (4096 -> 4096), 7.0 / 9.5 (333 -> 515), 16 groups 38 / 44, 174 / 208, 9.9 / 11.6; with
+// eight rows the shared memory's reads show: 22.6 / 21.1, 168 / 150, 10.4 / 9.6, and 50 / 43, 329 / 209, 14.0 / 11.7.  Below eight groups, four rows:
+// four groups 8.8 / 12.9, 70 / 76, 6.3 / 8.1, two 8.2 / 10.6, 39 / 37, 6.3 / 7.3.
 constexpr int kFewRun = 512, kFewBack = 8;
 template <int R, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_back_kernel(const float *__restrict__ w, const float *__restrict__ gz, long ldg, long in, long out, float *__restrict__ gx,
@@ -744,7 +747,8 @@ static void pairs_sums(const Groups &g, const GroupPairs &gp, int w, const Group
   check_launch("group_strays");
 }
 
-// Which way a gradient takes depends on it alone, not on whether the other is asked for too; where both take pairs, gz is split once.
+// Which way a gradient takes, and over pairs its form, depends on it and its operands alone, not on whether the other is asked for too; where both take pairs,
+// gz is measured and split once.
 void group_backward(const Groups &g, const float *x, long ldx, const float *gz, long ldg, long in, long out, const float *w, float *gx, float *gw, float scale) {
   if (each_group(g, [&](int e, long r, long n) {
         if (gx) gemm('n', 'n', in, n, out, 1.f, w + e * out * in, in, gz + r * ldg, ldg, 0.f, gx + r * in, in);
