@@ -1,11 +1,14 @@
 """nn.GroupedLinear where one group has most of the rows: results, and the device memory that a call takes for itself."""
+import ctypes
 import os
 import subprocess
 import sys
 
 import pytest
+import torch
 
-from test_gpu_fused_linear import check_groups, gt  # noqa: F401
+from test_gpu_feedforward import wrap
+from test_gpu_fused_linear import check_groups, down, gt, randn, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +57,42 @@ def test_scratch_of_weight_gradients(sizes):
     r = subprocess.run([sys.executable, "-c", MEMORY % (sizes,)], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert int(r.stdout.split()[-1]) <= 128 << 20
+
+
+def test_recorded_and_replayed(gt):  # noqa: F811
+    """Tickets and partial sums of cut groups inside a recording, with calls of other counts between its runs."""
+    counts, others = uneven(30, 18, {3: 5000, 20: 1500}), uneven(30, 600, {29: 9})
+    rows, more = sum(counts), sum(others)
+    m = gt.nn.GroupedLinear(30, 70, 90).gpu()
+    x, g = torch.zeros(rows, 70, device="cuda"), torch.zeros(rows, 90, device="cuda")
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    gt.lib().THGPUSetStream(ctypes.c_void_p(stream.cuda_stream))
+    try:
+        X, G, X2, G2 = wrap(gt, x), wrap(gt, g), up(gt, randn(5, more, 70)), up(gt, randn(6, more, 90))
+
+        def step():
+            m.gradWeight.fill(0.25)
+            m.accGradParameters([X, counts], G)
+        for _ in range(2):
+            step()
+        gt.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for seed in (1, 2, 3):
+            x.copy_(randn(seed, rows, 70)); g.copy_(randn(seed + 10, rows, 90))
+            torch.cuda.synchronize()
+            step()
+            gt.synchronize()
+            want = down(m.gradWeight).clone()
+            m.accGradParameters([X2, others], G2)
+            gt.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            gt.synchronize()
+            assert torch.equal(down(m.gradWeight), want)
+        del graph
+    finally:
+        gt.synchronize()
+        gt.lib().THGPUSetStream(None)
