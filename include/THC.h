@@ -444,6 +444,51 @@ THC_API int THGPUNN_GroupedLinear_updateOutput(THGPUTensor *input, const long *c
 THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *counts, int groups, THGPUTensor *gradOutput,
     THGPUTensor *gradInput, THGPUTensor *preactivation, THGPUTensor *gradPre, THGPUTensor *weight, THGPUTensor *gradWeight,
     THGPUTensor *gradBias, int activation, float scale);
+/* Router (no counterpart in the reference): the k largest of each row's scores and softmax weights over them.  input [R, E]; weights and
+ * experts [R, k], in descending order of the scores, equal ones by their place; experts are counted from 1.  A score of minus infinity is a closed
+ * expert's, which is never chosen: slots for which a row has no open expert left have the number 0 and the weight 0.  A NaN counts as the largest
+ * score and makes its row's weights NaN.  normalize: the weights of a row's chosen experts sum to one; else they are those of the softmax over all
+ * its scores.  E <= 1024, k <= 32 and k <= E.
+ * updateGradInput: gradInput [R, E] from gradWeights [R, k] and what updateOutput left; gradWeights of slots without an expert are not looked at.  With
+ * normalize only input's size is. */
+THC_API int THGPUNN_Router_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *experts, int k, int normalize);
+THC_API int THGPUNN_Router_updateGradInput(THGPUTensor *input, THGPUTensor *gradWeights, THGPUTensor *gradInput, THGPUTensor *weights,
+    THGPUTensor *experts, int normalize);
+/* Dispatch (no counterpart in the reference): a copy of a token's row for each of its slots that names an expert, sorted by expert, then by
+ * token and slot.  input [T, D], experts [T, k] with numbers from 1 to `groups`, 0 for none; output [R, D], R the slots that name one; positions
+ * [T, k] receives the place of each slot's row, from 1, 0 where there is none; counts: HOST array of `groups` numbers, receives the rows of each, which
+ * are what GroupedLinear takes.  The call waits until the counts have come (not for the copies), and so cannot be recorded.  Other
+ * numbers among the experts count as none, and the call then returns an error after its work.  T * k <= 2^24, groups <= 4096, D <= 2^23.
+ * updateGradInput: gradInput [T, D] receives the sum of each token's rows of gradOutput [R, D]. */
+THC_API int THGPUNN_Dispatch_updateOutput(THGPUTensor *input, THGPUTensor *experts, THGPUTensor *output, THGPUTensor *positions, long *counts,
+    int groups);
+THC_API int THGPUNN_Dispatch_updateGradInput(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *positions);
+/* Combine (no counterpart in the reference): output [T, size] receives residual + the sum of each token's rows of input [R, size] times their
+ * weights [T, k] (NULL: all one); positions as Dispatch leaves them: every row has one slot.  residual [T, size] or NULL.  Slots without a row, whose
+ * position is 0 or none of the rows', add nothing whatever their weight.
+ * backward: gradInput [R, size] receives each row's weight times its token's gradOutput, gradWeights [T, k] the products <gradOutput, row>, zero for slots
+ * without a row; each is skipped when NULL.  The residual's gradient is gradOutput itself. */
+THC_API int THGPUNN_Combine_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *residual,
+    THGPUTensor *output, long size);
+THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *gradOutput,
+    THGPUTensor *gradInput, THGPUTensor *gradWeights);
+/* AdamW over n tensors at once (not in the reference): with t = step[0] + 1
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   w = w (1 - lr * decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps),  step[0] = t.
+ * Arrays of n tensors each, contiguous, of one size an index.  `step` has two values: steps taken, and a word that the kernel works with, zero between
+ * calls.  It lies on the device, so that a recorded step counts on when it is replayed.  Tensors that are written may not share memory with any other.
+ * AdamW8: the moments in 8 bits.  meanCodes and rootCodes hold codes of m and of sqrt(v), four to a float, 256 to a block, and scales two values a block (of m,
+ * of sqrt(v)): 64, 64 and 2 floats for each 256 values of a tensor or part of them, zero at the start.  A code c stands for
+ * (f(b + c * 2^s) - f(b)) * scale, f(i) the float of the bits i, b those of 2^-16; codes of m have a sign bit above 7 others and s = 20, those of
+ * sqrt(v) 8 bits and s = 19.  Values are rounded up or down at random by their distance from the codes beside them, by a hash of the place, the tensor's index, the
+ * step and `seed`: the same call on the same state gives the same bits.  A gradient that is not finite makes its block's moments so.
+ * AdamW8_moments: what the codes stand for, m and v. */
+THC_API int THGPUNN_AdamW_update(int n, THGPUTensor **weights, THGPUTensor **grads, THGPUTensor **means, THGPUTensor **squares, THGPUTensor *step,
+    double lr, double beta1, double beta2, double eps, double decay);
+THC_API int THGPUNN_AdamW8_update(int n, THGPUTensor **weights, THGPUTensor **grads, THGPUTensor **meanCodes, THGPUTensor **rootCodes,
+    THGPUTensor **scales, THGPUTensor *step, double lr, double beta1, double beta2, double eps, double decay, long seed);
+THC_API int THGPUNN_AdamW8_moments(int n, THGPUTensor **meanCodes, THGPUTensor **rootCodes, THGPUTensor **scales, THGPUTensor **means,
+    THGPUTensor **squares);
 /* Parameter update over flat buffers.  momentum == 0: w -= lr*g, i.e. Module:updateParameters
  * (mcw_nn/Module.lua:75-82).  momentum != 0: v = momentum*v + g; w -= lr*v (not in the reference). */
 THC_API int THGPUNN_SGD_update(THGPUTensor *weight, THGPUTensor *grad, THGPUTensor *velocity,

@@ -99,6 +99,7 @@ class THGPUCommBackend(C.Structure):
 
 
 TP = C.POINTER(THGPUTensor)
+TPP = C.POINTER(TP)
 SP = C.POINTER(THGPUStorage)
 LSP = C.POINTER(THLongStorage)
 FTP = C.POINTER(THFloatTensor)
@@ -106,6 +107,7 @@ FSP = C.POINTER(THFloatStorage)
 f, l, i, d, vp, ch = C.c_float, C.c_long, C.c_int, C.c_double, C.c_void_p, C.c_char
 fp = C.POINTER(C.c_float)
 COUNTS = np.ctypeslib.ndpointer(np.int64, ndim=1, flags="C_CONTIGUOUS")   # a host array of whole numbers
+COUNTS_OUT = np.ctypeslib.ndpointer(np.int64, ndim=1, flags="C_CONTIGUOUS,WRITEABLE")
 
 # name -> (restype, argtypes); every symbol include/THC.h declares
 SIGNATURES = {
@@ -200,6 +202,12 @@ SIGNATURES = {
     "THGPUNN_FusedLinear_backward": (i, [TP, TP, TP, TP, TP, TP, TP, TP, i, f]),
     "THGPUNN_GroupedLinear_updateOutput": (i, [TP, COUNTS, i, TP, TP, TP, TP, i]),
     "THGPUNN_GroupedLinear_backward": (i, [TP, COUNTS, i, TP, TP, TP, TP, TP, TP, TP, i, f]),
+    "THGPUNN_Router_updateOutput": (i, [TP, TP, TP, i, i]), "THGPUNN_Router_updateGradInput": (i, [TP, TP, TP, TP, TP, i]),
+    "THGPUNN_Dispatch_updateOutput": (i, [TP, TP, TP, TP, COUNTS_OUT, i]), "THGPUNN_Dispatch_updateGradInput": (i, [TP, TP, TP, TP]),
+    "THGPUNN_Combine_updateOutput": (i, [TP, TP, TP, TP, TP, l]), "THGPUNN_Combine_backward": (i, [TP, TP, TP, TP, TP, TP]),
+    "THGPUNN_AdamW_update": (i, [i, TPP, TPP, TPP, TPP, TP, d, d, d, d, d]),
+    "THGPUNN_AdamW8_update": (i, [i, TPP, TPP, TPP, TPP, TPP, TP, d, d, d, d, d, l]),
+    "THGPUNN_AdamW8_moments": (i, [i, TPP, TPP, TPP, TPP, TPP]),
 }
 
 for _n, (_np, _st, _tn) in HOST_TYPES.items():

@@ -1,0 +1,523 @@
+// nn.Dispatch and nn.Combine: rows copied to the experts they go to, sorted by expert, and each token's rows summed again.
+//
+//   slot (t, i) of T tokens with k slots each names an expert, from 1, or none: 0.  Slots sorted by expert, then by t k + i, are the rows; pos(t, i) is
+//   the place of the slot's row, from 1, 0 where it has none.
+//   Dispatch  rows[pos(t, i)] = x[t];                    dx[t] = sum_i drows[pos(t, i)]
+//   Combine   y[t] = residual[t] + sum_i w(t, i) rows[pos(t, i)];  drows[pos(t, i)] = w(t, i) dy[t],  dw(t, i) = <dy[t], rows[pos(t, i)]>
+//
+// A row is D values of 4 bytes and is read or written once: all of it is bound by HBM, in small calls by launches.  Each thread of a token's team takes the
+// same columns of all its rows, so that nothing but the dot products crosses threads, and every result has one writer and one order.
+#include <cstring>
+#include <type_traits>
+
+#include "nn_args.h"
+#include "per_device.h"
+
+namespace thc {
+
+constexpr long kMostSlots = 1l << 24;     // positions are floats
+constexpr int kMostGroups = 4096;
+constexpr long kMostValues = 1l << 23;    // of a row: its pieces are a dimension of the grid
+constexpr long kFewSlots = 2048;          // up to here every block ranks its token's slots by itself
+
+// The expert of a slot, from 1; 0: none; -1: the number stands for no expert.
+static __device__ __forceinline__ int slot_expert(float e, int groups) {
+  return e >= 0.f && e <= (float)groups && e == truncf(e) ? (int)e : -1;
+}
+// The row at a place, or -1: a place that stands for none of the `rows` is passed over.
+static __device__ __forceinline__ long row_at(float place, long rows) { return place >= 1.f && place <= (float)rows ? (long)place - 1 : -1; }
+
+// What the host is told: rows of each group in out[0 .. groups), the slots whose number stands for no expert in out[groups].
+struct SlotCounts {
+  int *out;
+  ScalarSlot *slot;
+  unsigned long long seq;
+};
+
+// ---- where the rows go -------------------------------------------------------------------------------------------------
+// Many slots: in `chunks` pieces of `per`, a block each.  The first launch counts: hist[group][chunk], the bad numbers as one more group.  In the second one
+// a block adds up what lies before its own piece, counts its warps' shares of it, and each warp goes through its share 32 slots at a time.
+static __global__ void __launch_bounds__(256) slots_count_kernel(const float *__restrict__ experts, long slots, int per, int groups, int *__restrict__ hist) {
+  pdl_begin();
+  extern __shared__ int count[];   // [groups + 1]
+  for (int g = threadIdx.x; g <= groups; g += 256) count[g] = 0;
+  __syncthreads();
+  const long from = blockIdx.x * (long)per, to = min(slots, from + per);
+  for (long s = from + threadIdx.x; s < to; s += 256) {
+    const int e = slot_expert(experts[s], groups);
+    if (e != 0) atomicAdd(&count[e > 0 ? e - 1 : groups], 1);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g <= groups; g += 256) hist[(long)g * gridDim.x + blockIdx.x] = count[g];
+}
+
+static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__restrict__ experts, long slots, int per, int groups, const int *__restrict__ hist,
+                                                                 float *__restrict__ positions, SlotCounts tell) {
+  pdl_begin();
+  extern __shared__ int place[];                   // [8 warps][groups]: rows before the warp's next one of a group
+  int *total = place + 8 * groups, *before = total + groups;   // [groups]: a group's rows, and those of the pieces before this one
+  __shared__ int sums[256];
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, chunks = gridDim.x;
+  const long from = blockIdx.x * (long)per, to = min(slots, from + per);
+  const int share = (per / 8 + 31) & ~31;
+  const long mine = from + (long)warp * share, end = min(to, mine + share);
+  for (int g = t; g < 8 * groups; g += 256) place[g] = 0;
+  __syncthreads();
+  for (long s = mine + lane; s < end; s += 32) {
+    const int e = slot_expert(experts[s], groups);
+    if (e > 0) atomicAdd(&place[warp * groups + e - 1], 1);
+  }
+  for (int g = warp; g <= groups; g += 8) {
+    int all = 0, ahead = 0;
+    for (int c = lane; c < chunks; c += 32) {
+      const int n = hist[(long)g * chunks + c];
+      all += n;
+      if (c < (int)blockIdx.x) ahead += n;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (lane == 0) {
+      if (g < groups) { total[g] = all; before[g] = ahead; }
+      if (blockIdx.x == 0) tell.out[g] = all;
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && t == 0) scalar_deliver(tell.slot, 0.0, tell.seq);   // its system fence comes after every warp's counts, through the barrier
+  // the groups' first rows: each thread has some neighbouring groups
+  const int some = (groups + 255) / 256, g0 = min(groups, t * some), g1 = min(groups, g0 + some);
+  int own = 0;
+  for (int g = g0; g < g1; g++) own += total[g];
+  sums[t] = own;
+  __syncthreads();
+  if (warp == 0) {
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += sums[lane * 8 + i];
+    int run = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    run -= s;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int n = sums[lane * 8 + i];
+      sums[lane * 8 + i] = run;
+      run += n;
+    }
+  }
+  __syncthreads();
+  int first = sums[t];
+  for (int g = g0; g < g1; g++) {
+    int at = first + before[g];
+    for (int w = 0; w < 8; w++) {
+      const int n = place[w * groups + g];
+      place[w * groups + g] = at;
+      at += n;
+    }
+    first += total[g];
+  }
+  __syncthreads();
+  for (long s = mine; s < end; s += 32) {
+    const int e = s + lane < end ? max(0, slot_expert(experts[s + lane], groups)) : 0;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    int at = 0;
+    if (e > 0) at = place[warp * groups + e - 1];
+    __syncwarp();
+    if (e > 0 && lane == __ffs(same) - 1) place[warp * groups + e - 1] = at + __popc(same);
+    __syncwarp();
+    if (s + lane < end) positions[s + lane] = e > 0 ? (float)(at + __popc(same & ((1u << lane) - 1)) + 1) : 0.f;
+  }
+}
+
+// ---- copying and summing rows ------------------------------------------------------------------------------------------
+// Blocks of 256 threads in teams of T, a team for each token (blockIdx.x) and T U W of its columns (blockIdx.y): U pieces of W = 4 values, or one where
+// lengths or addresses do not allow it, a thread.
+template <int T, int U, bool VEC> struct Columns {
+  static constexpr int W = VEC ? 4 : 1;
+  float v[U * W];
+  int c;                                              // the thread's first column; its u-th piece is u T W further on
+  __device__ __forceinline__ Columns(long piece) : c((int)(piece * (T * U * W)) + (int)(threadIdx.x % T) * W) {}
+  static __device__ __forceinline__ long token() { return blockIdx.x * (long)(256 / T) + threadIdx.x / T; }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < U * W; j++) v[j] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float *__restrict__ row, int n) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = c + u * T * W;
+      if constexpr (VEC) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at < n) q = __ldg(reinterpret_cast<const float4 *>(row + at));
+        v[4 * u] = q.x; v[4 * u + 1] = q.y; v[4 * u + 2] = q.z; v[4 * u + 3] = q.w;
+      } else v[u] = at < n ? __ldg(row + at) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(float *__restrict__ row, int n) const {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = c + u * T * W;
+      if (at >= n) continue;
+      if constexpr (VEC) *reinterpret_cast<float4 *>(row + at) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+      else row[at] = v[u];
+    }
+  }
+};
+
+struct Rows {            // a matrix of rows at a distance
+  const float *p;
+  long ld;
+};
+
+// rows[pos(t, i)] = x[t]
+template <int T, int U, bool VEC>
+static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const float *__restrict__ positions, float *__restrict__ rows, long tokens, int k, int D, long most) {
+  pdl_begin();
+  typedef Columns<T, U, VEC> Cols;
+  const long t = Cols::token();
+  if (t >= tokens) return;
+  Cols a(blockIdx.y);
+  a.load(x.p + t * x.ld, D);
+  for (int i = 0; i < k; i++) {
+    const long r = row_at(__ldg(positions + t * k + i), most);
+    if (r >= 0) a.store(rows + r * D, D);
+  }
+}
+
+// The same for few slots, with the ranking: a block for a token and 256 U W of its columns.  A slot's place is the number of slots that name a lower expert,
+// or the same and come before it.
+template <int U, bool VEC>
+static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const float *__restrict__ experts, float *__restrict__ positions, float *__restrict__ rows, int k,
+                                                                  int D, int slots, int groups, SlotCounts tell) {
+  pdl_begin();
+  extern __shared__ int expert[];       // [slots], the token's rows [k], and in the first block the counts [groups + 1]
+  int *mine = expert + slots, *count = mine + k;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const long token = blockIdx.x;
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+  Columns<256, U, VEC> a(blockIdx.y);
+  a.load(x.p + token * x.ld, D);
+  if (first)
+    for (int g = t; g <= groups; g += 256) count[g] = 0;
+  for (int s = t; s < slots; s += 256) expert[s] = slot_expert(experts[s], groups);
+  __syncthreads();
+  if (first)
+    for (int s = t; s < slots; s += 256)
+      if (expert[s] != 0) atomicAdd(&count[expert[s] > 0 ? expert[s] - 1 : groups], 1);
+  for (int i = warp; i < k; i += 8) {
+    const int at = (int)token * k + i, e = expert[at];
+    int before = 0;
+    for (int s = lane; s < slots; s += 32) before += expert[s] > 0 && (expert[s] < e || (expert[s] == e && s < at));
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+      mine[i] = e > 0 ? before : -1;
+      if (blockIdx.y == 0) positions[at] = e > 0 ? (float)(before + 1) : 0.f;
+    }
+  }
+  __syncthreads();
+  if (first) {
+    for (int g = t; g <= groups; g += 256) tell.out[g] = count[g];
+    __syncthreads();
+    if (t == 0) scalar_deliver(tell.slot, 0.0, tell.seq);
+  }
+  for (int i = 0; i < k; i++)
+    if (mine[i] >= 0) a.store(rows + mine[i] * (long)D, D);
+}
+
+// y[t] = residual[t] + sum_i w(t, i) rows[pos(t, i)]; w and the residual may be null
+template <int T, int U, bool VEC>
+static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const float *__restrict__ w, const float *__restrict__ positions, Rows residual,
+                                                              float *__restrict__ y, long tokens, int k, int D, long most) {
+  pdl_begin();
+  typedef Columns<T, U, VEC> Cols;
+  const long t = Cols::token();
+  if (t >= tokens) return;
+  Cols a(blockIdx.y), b(blockIdx.y);
+  if (residual.p) a.load(residual.p + t * residual.ld, D);
+  else a.zero();
+  for (int i = 0; i < k; i++) {
+    const long r = row_at(__ldg(positions + t * k + i), most);
+    if (r < 0) continue;
+    const float f = w ? __ldg(w + t * k + i) : 1.f;
+    b.load(rows.p + r * rows.ld, D);
+#pragma unroll
+    for (int j = 0; j < U * Cols::W; j++) a.v[j] = fmaf(f, b.v[j], a.v[j]);
+  }
+  a.store(y + t * D, D);
+}
+
+// drows[pos(t, i)] = w(t, i) dy[t] and dw(t, i) = <dy[t], rows[pos(t, i)]>, either of them unless null; w may be null.  A team has all columns of its token.
+constexpr int kDotSlots = 32;
+template <int T, int U, bool VEC>
+static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows, const float *__restrict__ w, const float *__restrict__ positions, Rows dy,
+                                                                       float *__restrict__ drows, float *__restrict__ dw, long tokens, int k, int D, long most) {
+  pdl_begin();
+  typedef Columns<T, U, VEC> Cols;
+  __shared__ float dots[256 / T][T / 32][kDotSlots];
+  const long t = Cols::token();
+  const int team = threadIdx.x / T, warp = threadIdx.x % T / 32, lane = threadIdx.x & 31, pieces = (D + T * U * Cols::W - 1) / (T * U * Cols::W);
+  const bool live = t < tokens;
+  Cols g(0);
+  if (live && pieces == 1) g.load(dy.p + t * dy.ld, D);
+  for (int i0 = 0; i0 < k; i0 += kDotSlots) {
+    const int n = min(kDotSlots, k - i0);
+    for (int i = 0; live && i < n; i++) {
+      const long r = row_at(__ldg(positions + t * k + i0 + i), most);
+      float dot = 0.f;
+      if (r >= 0) {
+        const float f = w ? __ldg(w + t * k + i0 + i) : 1.f;
+        for (int p = 0; p < pieces; p++) {
+          Cols b(p), o(p);
+          if (dw) b.load(rows.p + r * rows.ld, D);
+          if (pieces > 1) {
+            g.c = b.c;
+            g.load(dy.p + t * dy.ld, D);
+          }
+#pragma unroll
+          for (int j = 0; j < U * Cols::W; j++) {
+            if (dw) dot = fmaf(g.v[j], b.v[j], dot);
+            o.v[j] = f * g.v[j];
+          }
+          if (drows) o.store(drows + r * D, D);
+        }
+      }
+      if (dw) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (lane == 0) dots[team][warp][i] = dot;
+      }
+    }
+    if (!dw) continue;
+    if constexpr (T > 32) __syncthreads();
+    else __syncwarp();
+    if (live && threadIdx.x % T < n) {
+      float s = dots[team][0][threadIdx.x % T];
+#pragma unroll
+      for (int o = 1; o < T / 32; o++) s += dots[team][o][threadIdx.x % T];
+      dw[t * k + i0 + threadIdx.x % T] = s;
+    }
+    if constexpr (T > 32) __syncthreads();
+    else __syncwarp();
+  }
+}
+
+// f(integral constants T, U, VEC) for rows of D values: teams as wide as a row, at most a block; one piece a thread where the rows are few
+template <class F> static void with_columns(long tokens, int D, bool vec, bool whole, F f) {
+  auto go = [&](auto VEC, auto U) {
+    constexpr int per = (decltype(VEC)::value ? 4 : 1) * decltype(U)::value;
+    if (D <= 32 * per) f(std::integral_constant<int, 32>(), U, VEC);
+    else if (D <= 64 * per) f(std::integral_constant<int, 64>(), U, VEC);
+    else if (D <= 128 * per) f(std::integral_constant<int, 128>(), U, VEC);
+    else f(std::integral_constant<int, 256>(), U, VEC);
+  };
+  const bool few = !whole && tokens * (long)D < ctx().sm_count * 4096l;
+  auto with_u = [&](auto VEC) {
+    if (few) go(VEC, std::integral_constant<int, 1>());
+    else go(VEC, std::integral_constant<int, 4>());
+  };
+  if (vec) with_u(std::true_type());
+  else with_u(std::false_type());
+}
+
+static bool pieces_of_four(std::initializer_list<Rows> all, int D) {
+  bool ok = D % 4 == 0;
+  for (const Rows &r : all) ok = ok && ((uintptr_t)r.p & 15) == 0 && r.ld % 4 == 0;
+  return ok;
+}
+// ---- launches
+// Whether slots may be ranked block by block.
+static bool are_few(long slots, int k) { return slots <= kFewSlots && k <= 64; }
+
+static void dispatch(Rows x, const float *experts, long tokens, int k, int D, int groups, float *positions, float *rows, const SlotCounts &tell) {
+  const long slots = tokens * k;
+  const bool vec = pieces_of_four({x, Rows{rows, D}}, D);
+  if (are_few(slots, k)) {
+    const size_t smem = sizeof(int) * (slots + k + groups + 1);
+    if (vec) pdl_launch(few_rows_out_kernel<1, true>, dim3((unsigned)tokens, (unsigned)ceil_div(D, 1024)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
+    else pdl_launch(few_rows_out_kernel<1, false>, dim3((unsigned)tokens, (unsigned)ceil_div(D, 256)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
+    check_launch("Dispatch_updateOutput");
+    return;
+  }
+  const int sms = ctx().sm_count;
+  const int per = (int)std::max(1024l, (slots + sms * 256l - 1) / (sms * 256l) * 256), chunks = ceil_div(slots, per);
+  int *hist = (int *)ws_alloc(sizeof(int) * (groups + 1) * chunks);
+  pdl_launch(slots_count_kernel, (unsigned)chunks, 256, sizeof(int) * (groups + 1), experts, slots, per, groups, hist);
+  check_launch("Dispatch_updateOutput");
+  constexpr size_t most = sizeof(int) * 10 * kMostGroups;
+  static PerDevice allowed;
+  allowed.get(ctx().device, [&] {
+    THC_CUDA(cudaFuncSetAttribute(slots_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    return 1;
+  });
+  pdl_launch(slots_place_kernel, (unsigned)chunks, 256, sizeof(int) * 10 * groups, experts, slots, per, groups, hist, positions, tell);
+  check_launch("Dispatch_updateOutput");
+  with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
+    constexpr int t = decltype(T)::value, u = decltype(U)::value, width = t * u * (decltype(VEC)::value ? 4 : 1);
+    pdl_launch(rows_out_kernel<t, u, decltype(VEC)::value>, dim3((unsigned)ceil_div(tokens, 256 / t), (unsigned)ceil_div(D, width)), 256, 0, x, positions, rows, tokens, k,
+               D, slots);
+  });
+  check_launch("Dispatch_updateOutput");
+}
+
+static void sum_rows(Rows rows, long most, const float *w, const float *positions, Rows residual, float *y, long tokens, int k, int D, const char *what) {
+  const bool vec = pieces_of_four({rows, residual, Rows{y, D}}, D);
+  with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
+    constexpr int t = decltype(T)::value, u = decltype(U)::value, width = t * u * (decltype(VEC)::value ? 4 : 1);
+    pdl_launch(rows_sum_kernel<t, u, decltype(VEC)::value>, dim3((unsigned)ceil_div(tokens, 256 / t), (unsigned)ceil_div(D, width)), 256, 0, rows, w, positions, residual,
+               y, tokens, k, D, most);
+  });
+  check_launch(what);
+}
+
+// ---- checks
+// Slots of `tokens` tokens: [tokens][k]
+static bool slots_fit(const THGPUTensor *t, long tokens, long k) {
+  return tokens ? t->nDimension == 2 && t->size[0] == tokens && t->size[1] == k : nelem(t) == 0;
+}
+static void check_slots(const THGPUTensor *t, int argn) {
+  THC_ARG(nelem(t) == 0 || t->nDimension == 2, argn, "matrix of a row of slots for each token expected");
+  THC_ARG(nelem(t) <= kMostSlots, argn, "at most 2^24 slots");
+}
+static void check_rows(const THGPUTensor *t, int argn) {
+  THC_ARG(nelem(t) == 0 || t->nDimension == 2, argn, "matrix of rows expected");
+  THC_ARG(nelem(t) == 0 || t->size[1] <= kMostValues, argn, "at most 2^23 values a row expected");
+}
+
+}  // namespace thc
+
+using namespace thc;
+
+THC_API int THGPUNN_Dispatch_updateOutput(THGPUTensor *input, THGPUTensor *experts, THGPUTensor *output, THGPUTensor *positions, long *counts, int groups) {
+  THC_BEGIN
+  THC_ARG(input && experts && output && positions, 1, "tensors expected");
+  THC_ARG(counts, 5, "room for a count of each group expected");
+  THC_ARG(groups >= 1 && groups <= kMostGroups, 6, "between 1 and 4096 groups expected");
+  check_here({input, experts, output, positions});
+  check_rows(input, 1);
+  check_slots(experts, 2);
+  const long tokens = nelem(input) ? input->size[0] : 0, D = tokens ? input->size[1] : 0, k = nelem(experts) ? experts->size[1] : 0;
+  THC_ARG(slots_fit(experts, tokens, k), 2, "a row of slots for each row of the input expected");
+  check_apart(output, {input, experts, positions}, 3);
+  check_apart(positions, {input, experts}, 4);
+  if (tokens) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    THC_CUDA(cudaStreamIsCapturing(stream(), &capture));
+    THC_CHECK(capture == cudaStreamCaptureStatusNone, "Dispatch hands its counts to the host, which cannot be recorded: call it before, and record what follows");
+  }
+  const long ps[2] = {tokens, k}, room[2] = {tokens * k, D};
+  size_result(positions, 2, ps, {input, experts}, 4);
+  size_result(output, 2, room, {input, experts, positions}, 3);
+  std::memset(counts, 0, sizeof(long) * groups);
+  if (tokens == 0) return 0;
+  WsScope scope;
+  DenseRows x(input);
+  TensorRef e(tensor_new_contiguous(experts));
+  Context &c = ctx();
+  static_assert(kMostGroups < kSmallStage, "the counts travel through the stage of small downloads");
+  const SlotCounts tell{(int *)c.small_stage_dev, c.scalar_slot_dev, scalar_expect()};
+  dispatch(Rows{x.p, x.ld}, data_ptr(e), tokens, (int)k, (int)D, groups, data_ptr(positions), data_ptr(output), tell);
+  scalar_wait(tell.seq);
+  const int *told = (const int *)c.small_stage;
+  long rows = 0;
+  for (int g = 0; g < groups; g++) rows += counts[g] = told[g];
+  const long s[2] = {rows, D};
+  resize_nd(output, 2, s, nullptr);
+  if (told[groups]) fail("Invalid argument 2: %d slots hold something else than a whole number from 0 to %d", told[groups], groups);
+  return 0;
+  THC_END(1)
+}
+
+THC_API int THGPUNN_Dispatch_updateGradInput(THGPUTensor *input, THGPUTensor *gradOutput, THGPUTensor *gradInput, THGPUTensor *positions) {
+  THC_BEGIN
+  THC_ARG(input && gradOutput && gradInput && positions, 1, "tensors expected");
+  check_here({input, gradOutput, gradInput, positions});
+  check_rows(input, 1);
+  check_slots(positions, 4);
+  check_rows(gradOutput, 2);
+  const long tokens = nelem(input) ? input->size[0] : 0, D = tokens ? input->size[1] : 0, k = nelem(positions) ? positions->size[1] : 0;
+  const long rows = nelem(gradOutput) ? gradOutput->size[0] : 0;
+  THC_ARG(slots_fit(positions, tokens, k), 4, "positions of this input, as updateOutput left them, expected");
+  THC_ARG(rows == 0 || (gradOutput->size[1] == D && rows <= tokens * k), 2, "gradOutput has the wrong size");
+  const long s[2] = {tokens, D};
+  size_result(gradInput, 2, s, {input, gradOutput, positions}, 3);
+  if (tokens == 0) return 0;
+  TensorRef p(tensor_new_contiguous(positions));
+  auto run = [&](Rows g) { sum_rows(g, rows, nullptr, data_ptr(p), Rows{nullptr, 0}, data_ptr(gradInput), tokens, (int)k, (int)D, "Dispatch_updateGradInput"); };
+  if (rows == 0) run(Rows{nullptr, 0});
+  else {
+    DenseRows g(gradOutput);
+    run(Rows{g.p, g.ld});
+  }
+  return 0;
+  THC_END(1)
+}
+
+THC_API int THGPUNN_Combine_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *residual, THGPUTensor *output, long size) {
+  THC_BEGIN
+  THC_ARG(input && positions && output, 1, "tensors expected");
+  THC_ARG(size >= 1 && size <= kMostValues, 6, "size must be positive and at most 2^23");
+  check_here({input, weights, positions, residual, output});
+  check_rows(input, 1);
+  check_slots(positions, 3);
+  const long rows = nelem(input) ? input->size[0] : 0, tokens = nelem(positions) ? positions->size[0] : 0, k = tokens ? positions->size[1] : 0;
+  THC_ARG(rows == 0 || input->size[1] == size, 1, "rows of the given size expected");
+  if (weights) THC_ARG(slots_fit(weights, tokens, k), 2, "a weight for each slot expected");
+  if (residual) THC_ARG(tokens ? residual->nDimension == 2 && residual->size[0] == tokens && residual->size[1] == size : nelem(residual) == 0, 4,
+                        "residual of the output's size expected");
+  const long s[2] = {tokens, size};
+  size_result(output, 2, s, {input, weights, positions, residual}, 5);
+  if (tokens == 0) return 0;
+  TensorRef p(tensor_new_contiguous(positions)), w(weights ? tensor_new_contiguous(weights) : nullptr);
+  THGPUTensor *some = rows ? input : output;      // (without rows nothing is read through it)
+  DenseRows x(some);
+  auto run = [&](Rows r) {
+    sum_rows(Rows{x.p, x.ld}, rows, weights ? data_ptr(w) : nullptr, data_ptr(p), r, data_ptr(output), tokens, (int)k, (int)size, "Combine_updateOutput");
+  };
+  if (residual) {
+    DenseRows r(residual);
+    run(Rows{r.p, r.ld});
+  } else run(Rows{nullptr, 0});
+  return 0;
+  THC_END(1)
+}
+
+THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *gradOutput, THGPUTensor *gradInput,
+                                     THGPUTensor *gradWeights) {
+  THC_BEGIN
+  THC_ARG(input && positions && gradOutput, 1, "tensors expected");
+  THC_ARG(weights || !gradWeights, 6, "weights have a gradient where there are weights");
+  check_here({input, weights, positions, gradOutput, gradInput, gradWeights});
+  check_rows(input, 1);
+  check_slots(positions, 3);
+  check_rows(gradOutput, 4);
+  const long rows = nelem(input) ? input->size[0] : 0, tokens = nelem(positions) ? positions->size[0] : 0, k = tokens ? positions->size[1] : 0;
+  const long D = nelem(gradOutput) ? gradOutput->size[1] : rows ? input->size[1] : 0;
+  if (weights) THC_ARG(slots_fit(weights, tokens, k), 2, "a weight for each slot expected");
+  THC_ARG(tokens ? nelem(gradOutput) && gradOutput->size[0] == tokens : nelem(gradOutput) == 0, 4, "gradOutput has the wrong size");
+  THC_ARG(rows == 0 || input->size[1] == D, 1, "rows of gradOutput's size expected");
+  const long xs[2] = {rows, D}, ws[2] = {tokens, k};
+  if (gradInput) size_result(gradInput, 2, xs, {input, weights, positions, gradOutput, gradWeights}, 5);
+  if (gradWeights) size_result(gradWeights, 2, ws, {input, weights, positions, gradOutput, gradInput}, 6);
+  if (tokens == 0 || (!gradInput && !gradWeights)) return 0;
+  TensorRef p(tensor_new_contiguous(positions)), w(weights ? tensor_new_contiguous(weights) : nullptr);
+  DenseRows g(gradOutput);
+  auto run = [&](Rows x) {
+    float *gx = gradInput && rows ? data_ptr(gradInput) : nullptr, *gw = gradWeights ? data_ptr(gradWeights) : nullptr;
+    const bool vec = pieces_of_four({x, Rows{g.p, g.ld}, Rows{gx, D}}, (int)D);
+    with_columns(tokens, (int)D, vec, true, [&](auto T, auto U, auto VEC) {
+      constexpr int t = decltype(T)::value, u = decltype(U)::value;
+      pdl_launch(rows_sum_backward_kernel<t, u, decltype(VEC)::value>, (unsigned)ceil_div(tokens, 256 / t), 256, 0, x, weights ? data_ptr(w) : nullptr, data_ptr(p),
+                 Rows{g.p, g.ld}, gx, gw, tokens, (int)k, (int)D, rows);
+    });
+    check_launch("Combine_backward");
+  };
+  if (rows == 0) run(Rows{nullptr, 0});
+  else {
+    DenseRows x(input);
+    run(Rows{x.p, x.ld});
+  }
+  return 0;
+  THC_END(1)
+}

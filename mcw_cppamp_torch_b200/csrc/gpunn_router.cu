@@ -1,0 +1,231 @@
+// nn.Router: the k largest of a row's E scores and softmax weights over them, or over all open ones.
+//
+//   order: descending, equal scores by their place; a score of minus infinity is a closed expert's and is never chosen; a NaN counts as the largest
+//   w_i = exp(s_i - max) / sum exp(s_j - max), j over the chosen (normalize) or over all
+//   ds_j = w_j (g_j - sum_i g_i w_i) on the chosen and zero elsewhere (normalize), else p_j ([j chosen] g_j - sum_i g_i w_i) with p the whole softmax
+//
+// A row is read once, by a warp, and stays in its registers: 4 E bytes a row and 8 k out.
+#include <type_traits>
+
+#include "nn_args.h"
+
+namespace thc {
+
+constexpr int kRouterScores = 1024, kRouterChosen = 32;   // most scores a row, most of them chosen: what a warp's registers and lanes hold
+
+// ---- a row in a warp's registers: V values a lane, in pieces of four where lengths and addresses allow it
+template <int V, bool VEC> struct WarpRow {
+  static __device__ __forceinline__ int at(int j, int lane) { return VEC ? ((j >> 2) * 32 + lane) * 4 + (j & 3) : j * 32 + lane; }
+  static __device__ __forceinline__ void load(const float *__restrict__ p, int lane, int n, float (&v)[V]) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at(j, lane) < n) q = __ldg(reinterpret_cast<const float4 *>(p + at(j, lane)));
+        v[j] = q.x; v[j + 1] = q.y; v[j + 2] = q.z; v[j + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] = at(j, lane) < n ? __ldg(p + at(j, lane)) : -INFINITY;
+    }
+  }
+  static __device__ __forceinline__ void store(float *__restrict__ p, int lane, int n, const float (&v)[V]) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        if (at(j, lane) < n) *reinterpret_cast<float4 *>(p + at(j, lane)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (at(j, lane) < n) p[at(j, lane)] = v[j];
+    }
+  }
+};
+static __device__ __forceinline__ float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Whole numbers in the order of the scores they stand for (both zeros alike, a NaN above all), and back.
+static __device__ __forceinline__ unsigned score_key(float s) {
+  const unsigned u = __float_as_uint(s + 0.f);
+  if (s != s) return 0xffffffffu;
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+static __device__ __forceinline__ float key_score(unsigned k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);     // (all ones: a NaN)
+}
+constexpr unsigned kClosedKey = 0x007fffffu;    // of minus infinity
+
+template <int V, bool VEC>
+static __global__ void __launch_bounds__(256) router_forward_kernel(const float *__restrict__ x, long ld, float *__restrict__ weights, float *__restrict__ experts,
+                                                                    long rows, int E, int k, bool normalize) {
+  pdl_begin();
+  typedef WarpRow<V, VEC> Row;
+  const int lane = threadIdx.x & 31;
+  const long row = blockIdx.x * 8l + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float v[V];
+  Row::load(x + row * ld, lane, E, v);
+  unsigned key[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) key[j] = score_key(v[j]);
+  float score = -INFINITY, top = -INFINITY;
+  int expert = 0;
+  for (int i = 0; i < k; i++) {
+    unsigned best = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) best = max(best, key[j]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (best <= kClosedKey) break;
+    unsigned mine = 0xffffffffu;
+#pragma unroll
+    for (int j = V - 1; j >= 0; j--)
+      if (key[j] == best) mine = Row::at(j, lane);
+    const unsigned place = __reduce_min_sync(0xffffffffu, mine);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if ((unsigned)Row::at(j, lane) == place) key[j] = 0;
+    if (lane == i) { score = key_score(best); expert = (int)place + 1; }
+    if (i == 0) top = key_score(best);
+  }
+  const float e = expert ? expf(score - top) : 0.f;
+  float total = 0.f;
+  if (normalize) total = e;
+  else if (top != -INFINITY) {
+#pragma unroll
+    for (int j = 0; j < V; j++) total += expf(v[j] - top);
+  }
+  total = warp_total(total);
+  if (lane < k) {
+    weights[row * k + lane] = expert ? e / total : 0.f;
+    experts[row * k + lane] = (float)expert;
+  }
+}
+
+// The gradient of a row's scores.  x is read where the weights are of the whole softmax, and may else be null.
+template <int V, bool VEC>
+static __global__ void __launch_bounds__(256) router_backward_kernel(const float *__restrict__ x, long ldx, const float *__restrict__ g, long ldg,
+                                                                     const float *__restrict__ weights, const float *__restrict__ experts, float *__restrict__ gx,
+                                                                     long rows, int E, int k) {
+  pdl_begin();
+  typedef WarpRow<V, VEC> Row;
+  const int lane = threadIdx.x & 31;
+  const long row = blockIdx.x * 8l + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float w = 0.f, d = 0.f;
+  int expert = -1;
+  if (lane < k) {
+    expert = (int)experts[row * k + lane] - 1;
+    if (expert >= 0) { w = weights[row * k + lane]; d = g[row * ldg + lane]; }
+  }
+  const float spread = warp_total(w * d);
+  float out[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) out[j] = 0.f;
+  const float mine = x ? d : w * (d - spread);
+  for (int i = 0; i < k; i++) {
+    const int to = __shfl_sync(0xffffffffu, expert, i);
+    const float add = __shfl_sync(0xffffffffu, mine, i);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (Row::at(j, lane) == to) out[j] += add;
+  }
+  if (x) {
+    float v[V], top = -INFINITY, total = 0.f;
+    Row::load(x + row * ldx, lane, E, v);
+#pragma unroll
+    for (int j = 0; j < V; j++) top = fmaxf(top, v[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      v[j] = v[j] == -INFINITY ? 0.f : expf(v[j] - top);
+      total += v[j];
+    }
+    total = warp_total(total);
+#pragma unroll
+    for (int j = 0; j < V; j++) out[j] = v[j] == 0.f ? 0.f : v[j] / total * (out[j] - spread);
+  }
+  Row::store(gx + row * E, lane, E, out);
+}
+
+// f(integral constant V, bool constant VEC) for rows of E scores
+template <class F> static void with_row(int E, bool vec, F f) {
+  const int v = (E + 31) / 32;
+  auto go = [&](auto V) {
+    if constexpr (decltype(V)::value >= 4) {
+      if (vec) return f(V, std::true_type());
+    }
+    f(V, std::false_type());
+  };
+  if (v <= 1) go(std::integral_constant<int, 1>());
+  else if (v <= 2) go(std::integral_constant<int, 2>());
+  else if (v <= 4) go(std::integral_constant<int, 4>());
+  else if (v <= 8) go(std::integral_constant<int, 8>());
+  else if (v <= 16) go(std::integral_constant<int, 16>());
+  else go(std::integral_constant<int, 32>());
+}
+static bool in_pieces(const float *p, long ld, int E) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && E % 4 == 0; }
+
+}  // namespace thc
+
+using namespace thc;
+
+THC_API int THGPUNN_Router_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *experts, int k, int normalize) {
+  THC_BEGIN
+  THC_ARG(input && weights && experts, 1, "tensors expected");
+  check_here({input, weights, experts});
+  const long rows = nelem(input) ? input->size[0] : 0;
+  if (rows) THC_ARG(input->nDimension == 2, 1, "batch of rows of scores expected");
+  const long E = rows ? input->size[1] : kRouterScores;
+  THC_ARG(E <= kRouterScores, 1, "at most 1024 scores a row");
+  THC_ARG(k >= 1 && k <= kRouterChosen && k <= E, 4, "between 1 and 32 experts a row, and no more than there are, expected");
+  const long s[2] = {rows, k};
+  size_result(weights, 2, s, {input, experts}, 2);
+  size_result(experts, 2, s, {input, weights}, 3);
+  if (rows == 0) return 0;
+  DenseRows x(input);
+  with_row((int)E, in_pieces(x.p, x.ld, (int)E), [&](auto V, auto VEC) {
+    pdl_launch(router_forward_kernel<decltype(V)::value, decltype(VEC)::value>, (unsigned)ceil_div(rows, 8), 256, 0, x.p, x.ld, data_ptr(weights), data_ptr(experts),
+               rows, (int)E, k, normalize != 0);
+  });
+  check_launch("Router_updateOutput");
+  return 0;
+  THC_END(1)
+}
+
+THC_API int THGPUNN_Router_updateGradInput(THGPUTensor *input, THGPUTensor *gradWeights, THGPUTensor *gradInput, THGPUTensor *weights, THGPUTensor *experts,
+                                           int normalize) {
+  THC_BEGIN
+  THC_ARG(input && gradWeights && gradInput && weights && experts, 1, "tensors expected");
+  check_here({input, gradWeights, gradInput, weights, experts});
+  const long rows = nelem(input) ? input->size[0] : 0;
+  if (rows) THC_ARG(input->nDimension == 2, 1, "batch of rows of scores expected");
+  const long E = rows ? input->size[1] : 0;
+  THC_ARG(E <= kRouterScores, 1, "at most 1024 scores a row");
+  const long k = rows && weights->nDimension == 2 ? weights->size[1] : 0;
+  auto fits = [&](const THGPUTensor *t) { return rows ? t->nDimension == 2 && t->size[0] == rows && t->size[1] == k : nelem(t) == 0; };
+  THC_ARG(fits(weights) && is_contiguous(weights) && k <= kRouterChosen, 4, "weights of this input, as updateOutput left them, expected");
+  THC_ARG(fits(experts) && is_contiguous(experts), 5, "experts of this input, as updateOutput left them, expected");
+  THC_ARG(fits(gradWeights), 2, "gradWeights has the wrong size");
+  const long s[2] = {rows, E};
+  size_result(gradInput, 2, s, {input, gradWeights, weights, experts}, 3);
+  if (rows == 0) return 0;
+  DenseRows g(gradWeights);
+  auto run = [&](const float *x, long ldx) {
+    const bool vec = in_pieces(data_ptr(gradInput), E, (int)E) && (!x || in_pieces(x, ldx, (int)E));
+    with_row((int)E, vec, [&](auto V, auto VEC) {
+      pdl_launch(router_backward_kernel<decltype(V)::value, decltype(VEC)::value>, (unsigned)ceil_div(rows, 8), 256, 0, x, ldx, g.p, g.ld, data_ptr(weights),
+                 data_ptr(experts), data_ptr(gradInput), rows, (int)E, (int)k);
+    });
+  };
+  if (normalize) run(nullptr, 0);
+  else {
+    DenseRows x(input);
+    run(x.p, x.ld);
+  }
+  check_launch("Router_updateGradInput");
+  return 0;
+  THC_END(1)
+}

@@ -565,8 +565,8 @@ class FusedLinear(Linear):
 
 class GroupedLinear(Module):
     """activation(input * weight[e]^T + bias[e]) for the rows of group e: a layer of experts.  The input is [rows, counts], the rows sorted by
-    group and `counts` a host sequence with the number of rows of each group (zeros among them).  GPUTensor.index with the sorted rows'
-    positions brings rows into that order and indexCopy brings results back.  weight is [groups, outputSize, inputSize], bias
+    group and `counts` a host sequence with the number of rows of each group (zeros among them): what Dispatch makes of rows and their experts'
+    numbers, and Combine joins again.  weight is [groups, outputSize, inputSize], bias
     [groups, outputSize]; gradients of groups without rows stay as they are.  gradInput is [the rows' gradient, None].
     `activation`, `preactivation` and evaluate() as for FusedLinear.  In the "bf16" math mode the products stay FP32-accurate."""
 
@@ -637,6 +637,109 @@ class GroupedLinear(Module):
         if gi is not None:
             self.gradInput = [gi, None]
         return self.gradInput
+
+
+class Router(Module):
+    """The k largest of each row's scores and softmax weights over them: output is [weights, experts], [rows, k] each, in descending order of the
+    scores, equal ones by their place.  Experts are counted from 1.  A score of minus infinity closes its expert to the row; slots for which there is no open expert
+    left, as in the rows of a padded batch, have the number 0 and the weight 0.  normalize: a row's weights sum to one, else they are those of the
+    softmax over all its scores.  gradOutput is the weights' gradient, or [the weights' gradient, None]."""
+
+    def __init__(self, k, normalize=True):
+        super().__init__()
+        if k < 1:
+            raise ValueError("Router: at least one expert a row expected")
+        self.k, self.normalize = k, normalize
+        self.output = [GPUTensor(), GPUTensor()]
+
+    def updateOutput(self, input):
+        _need_gpu(input, "Router")
+        lib().THGPUNN_Router_updateOutput(input._p, self.output[0]._p, self.output[1]._p, self.k, int(self.normalize))
+        return self.output
+
+    def updateGradInput(self, input, gradOutput):
+        if self.gradInput is None:
+            return None
+        g = gradOutput[0] if isinstance(gradOutput, (list, tuple)) else gradOutput
+        lib().THGPUNN_Router_updateGradInput(_need_gpu(input, "Router")._p, _need_gpu(g, "Router")._p, self.gradInput._p, self.output[0]._p, self.output[1]._p,
+                                             int(self.normalize))
+        return self.gradInput
+
+
+class Dispatch(Module):
+    """Rows sorted by the experts they go to: of the input [rows, experts], experts [rows, k] as Router leaves them (numbers from 1 to `groups`, 0: none),
+    output is [a copy of a row for each of its experts, counts], sorted by expert, then by row, with the number of rows of each expert as a host array: GroupedLinear's
+    input.  `positions` [rows, k] keeps the place of each copy, from 1 (0: none), for Combine and the backward pass.  A forward pass waits for the counts, so that
+    it cannot be recorded.  gradOutput is [the copies' gradient, None] or that gradient itself; gradInput is [the rows' gradient, None]."""
+
+    def __init__(self, groups):
+        super().__init__()
+        if groups < 1:
+            raise ValueError("Dispatch: at least one group expected")
+        self.groups = groups
+        self.rows, self.positions, self.gradRows = GPUTensor(), GPUTensor(), GPUTensor()
+
+    def updateOutput(self, input):
+        x, experts = input
+        counts = np.zeros(self.groups, np.int64)
+        lib().THGPUNN_Dispatch_updateOutput(_need_gpu(x, "Dispatch")._p, _need_gpu(experts, "Dispatch experts")._p, self.rows._p, self.positions._p, counts, self.groups)
+        self.output = [self.rows, counts]
+        return self.output
+
+    def updateGradInput(self, input, gradOutput):
+        if self.gradInput is None:
+            return None
+        g = gradOutput[0] if isinstance(gradOutput, (list, tuple)) else gradOutput
+        lib().THGPUNN_Dispatch_updateGradInput(_need_gpu(input[0], "Dispatch")._p, _need_gpu(g, "Dispatch")._p, self.gradRows._p, self.positions._p)
+        self.gradInput = [self.gradRows, None]
+        return self.gradInput
+
+
+class Combine(Module):
+    """The sum of each token's rows times their weights: of the input [rows, weights, positions] or [rows, weights, positions, residual], rows sorted as by
+    Dispatch and weights and positions [tokens, k] (weights None: all one), plus the residual [tokens, size].  Slots whose position is 0 add nothing.
+    `size` is needed where there may be no rows at all and no residual.
+    gradInput is [the rows' gradient, the weights', None] or with a residual [the rows' gradient, the weights', None, gradOutput], the last the
+    given tensor itself, which is not saved or cloned with the module."""
+
+    def __init__(self, size=None):
+        super().__init__()
+        self.size = size
+        self.gradRows, self.gradWeights = GPUTensor(), GPUTensor()
+
+    def _split(self, input):
+        rows, weights, positions, residual = input if len(input) == 4 else (*input, None)
+        if weights is not None:
+            _need_gpu(weights, "Combine weights")
+        if residual is not None:
+            _need_gpu(residual, "Combine residual")
+        return _need_gpu(rows, "Combine"), weights, _need_gpu(positions, "Combine positions"), residual
+
+    def updateOutput(self, input):
+        rows, weights, positions, residual = self._split(input)
+        size = self.size
+        if size is None:
+            sizes = rows.size() or (residual.size() if residual is not None else ())
+            if len(sizes) != 2:
+                if positions.dim():
+                    raise ValueError("Combine: a matrix of rows expected, or the size of one in their place")
+                sizes = (0, 1)                   # nothing to sum
+            size = sizes[1]
+        lib().THGPUNN_Combine_updateOutput(rows._p, weights._p if weights is not None else None, positions._p, residual._p if residual is not None else None,
+                                           self.output._p, size)
+        return self.output
+
+    def updateGradInput(self, input, gradOutput):
+        if self.gradInput is None:
+            return None
+        rows, weights, positions, residual = self._split(input)
+        lib().THGPUNN_Combine_backward(rows._p, weights._p if weights is not None else None, positions._p, _need_gpu(gradOutput, "Combine")._p, self.gradRows._p,
+                                       self.gradWeights._p if weights is not None else None)
+        self.gradInput = [self.gradRows, self.gradWeights if weights is not None else None, None] + ([gradOutput] if residual is not None else [])
+        return self.gradInput
+
+    def __getstate__(self):
+        return dict(self.__dict__, gradInput=self.gradInput[:3] if isinstance(self.gradInput, list) else self.gradInput)
 
 
 class LogSoftMax(Module):
