@@ -50,26 +50,22 @@ struct AdamStep {
   unsigned seed;
   int number;                // of the table's first tensor
 };
-// What a step's number decides: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).
+// What a step's number decides: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).  1 - b^t loses a float's digits for small t: in 64 bits.
 struct AdamFactors {
   float rate, root;
   unsigned step;
 };
-static __device__ __forceinline__ double whole_power(double b, unsigned t) {
-  double p = 1.0;
-  for (; t; t >>= 1, b *= b)
+// By threads 0 and 1 into shared memory; a barrier has to follow.
+static __device__ __forceinline__ void adam_factors(const AdamStep &s, AdamFactors &f) {
+  if (threadIdx.x > 1) return;
+  const unsigned step = (unsigned)s.step[0] + 1;
+  double b = threadIdx.x ? s.b2 : s.b1, p = 1.0;
+  for (unsigned t = step; t; t >>= 1, b *= b)
     if (t & 1) p *= b;
-  return p;
-}
-static __device__ __forceinline__ AdamFactors adam_factors(const AdamStep &s, AdamFactors *shared) {
   if (threadIdx.x == 0) {
-    const unsigned t = (unsigned)s.step[0] + 1;
-    shared->rate = (float)(s.lr / (1.0 - whole_power(s.b1, t)));
-    shared->root = (float)(1.0 / sqrt(1.0 - whole_power(s.b2, t)));
-    shared->step = t;
-  }
-  __syncthreads();
-  return *shared;
+    f.rate = (float)(s.lr / (1.0 - p));
+    f.step = step;
+  } else f.root = (float)(1.0 / sqrt(1.0 - p));
 }
 // The last block of the last launch counts the step: by then every block has read its number.
 static __device__ __forceinline__ void adam_count(const AdamStep &s, unsigned step) {
@@ -95,17 +91,39 @@ template <int N> static __device__ __forceinline__ int tensor_of(const AdamTable
 }
 
 // ---- moments in 32 bits
+static __device__ __forceinline__ float reciprocal(float v) {     // within a step
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+static __device__ __forceinline__ float square_root(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+static __device__ __forceinline__ float adam_weight(float w, float m, float root, const AdamStep &s, const AdamFactors &f) {
+  return fmaf(-f.rate, m * reciprocal(fmaf(root, f.root, s.eps)), w * s.keep);
+}
 static __device__ __forceinline__ void adam_value(float &w, float g, float &m, float &v, const AdamStep &s, const AdamFactors &f) {
   m = fmaf(s.beta1, m, s.rest1 * g);
   v = fmaf(s.beta2, v, s.rest2 * (g * g));
-  w = fmaf(-f.rate, m / fmaf(sqrtf(v), f.root, s.eps), w * s.keep);
+  w = adam_weight(w, m, square_root(v), s, f);
 }
+// Eight values a thread: all of a turn's loads are on their way before the first is needed, in the first turn before the step's factors are made.
 template <int N>
-static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
+static __global__ void __launch_bounds__(256, 4) adam_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
   __shared__ AdamFactors shared;
-  const AdamFactors f = adam_factors(s, &shared);
+  AdamFactors f;
   const unsigned chunks = table.first[table.count];
+  bool started = false;
+  auto start = [&] {
+    if (started) return;
+    adam_factors(s, shared);
+    __syncthreads();
+    f = shared;
+    started = true;
+  };
   for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int i = tensor_of(table, chunk);
     const AdamTensor &a = table.t[i];
@@ -123,6 +141,7 @@ static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant_
         mm[j] = reinterpret_cast<float4 *>(m)[at];
         vv[j] = reinterpret_cast<float4 *>(v)[at];
       }
+      start();
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const int at = j * 256 + threadIdx.x;
@@ -141,6 +160,7 @@ static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant_
         const int at = j * 256 + threadIdx.x;
         if (at < n) { ww[j] = w[at]; gg[j] = g[at]; mm[j] = m[at]; vv[j] = v[at]; }
       }
+      start();
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const int at = j * 256 + threadIdx.x;
@@ -151,6 +171,7 @@ static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant_
       }
     }
   }
+  start();
   adam_count(s, f.step);
 }
 
@@ -158,18 +179,20 @@ static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant_
 static __device__ __forceinline__ float code_value(unsigned code, int shift, float scale) {
   return __fmul_rn(__fadd_rn(__uint_as_float(kCodeBits + (code << shift)), -kCodeFloor), scale);
 }
+// The code of x >= 0 with `noise` below 2^shift on its bits.
 static __device__ __forceinline__ unsigned value_code(float x, float inverse, int shift, unsigned noise, unsigned most) {
-  const int bits = (int)(__float_as_uint(__fadd_rn(__fmul_rn(x, inverse), kCodeFloor)) - kCodeBits);
-  return min((unsigned)((bits + (int)(noise << (shift - 16)) + (1 << (shift - 17))) >> shift), most);
+  return min((__float_as_uint(__fadd_rn(__fmul_rn(x, inverse), kCodeFloor)) + noise - (kCodeBits - (1u << (shift - 17)))) >> shift, most);
 }
-// 32 random bits of a place: products with odd numbers (the fractions of the golden ratio, e and 2 e as in 32-bit words) between shifts
-static __device__ __forceinline__ unsigned place_bits(unsigned place, unsigned key) {
-  unsigned h = place * 0x9e3779b9u + key;
+// 32 random bits of a place, but for the last step of the hash, h ^ h >> 16, which is taken along with the halves: products with odd numbers (the fractions of
+// the golden ratio, of e and of 2 e as words) between shifts
+static __device__ __forceinline__ unsigned place_bits(unsigned h) {
   h = (h ^ (h >> 16)) * 0xb7e15163u;
-  h = (h ^ (h >> 15)) * 0xadf85459u;
-  return h ^ (h >> 16);
+  return (h ^ (h >> 15)) * 0xadf85459u;
 }
-static __device__ __forceinline__ unsigned step_key(unsigned seed, unsigned step, unsigned number) { return (seed ^ step * 0x9e3779b9u) + number * 0x6a09e667u; }
+constexpr unsigned kPlaceStep = 0x9e3779b9u;
+static __device__ __forceinline__ unsigned mean_noise(unsigned h) { return ((h << 4) ^ (h >> 12)) & 0xffff0u; }     // 16 bits below 2^kMeanShift
+static __device__ __forceinline__ unsigned root_noise(unsigned h) { return (h >> 13) & 0x7fff8u; }                  // and below 2^kRootShift
+static __device__ __forceinline__ unsigned step_key(unsigned seed, unsigned step, unsigned number) { return (seed ^ step * kPlaceStep) + number * 0x6a09e667u; }
 // The larger of two, a NaN being the largest.
 static __device__ __forceinline__ float larger(float a, float b) {
   float r;
@@ -177,9 +200,9 @@ static __device__ __forceinline__ float larger(float a, float b) {
   return r;
 }
 static __device__ __forceinline__ float warp_largest(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 // Four values of a warp's 256: those from 4 lane on, in either half.
 static __device__ __forceinline__ void load_four(float (&v)[4], const float *p, int n, bool vec) {
@@ -200,11 +223,21 @@ static __device__ __forceinline__ void store_four(float *p, const float (&v)[4],
   }
 }
 
+// The words of codes of a block's places: those behind its values are zero.
+static __device__ __forceinline__ unsigned codes_of(const unsigned *codes, int h, int lane, int n) {
+  unsigned q = codes[h * 32 + lane];
+  const int left = n - (h * 128 + lane * 4);
+  if (left < 4) q = left > 0 ? q & ((1u << (8 * left)) - 1) : 0;
+  return q;
+}
+// A warp for a block of 256 values, eight a lane.
 template <int N>
-static __global__ void __launch_bounds__(256) adam8_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
+static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
   __shared__ AdamFactors shared;
-  const AdamFactors f = adam_factors(s, &shared);
+  adam_factors(s, shared);
+  __syncthreads();
+  const AdamFactors f = shared;
   const unsigned chunks = table.first[table.count];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
@@ -217,7 +250,7 @@ static __global__ void __launch_bounds__(256) adam8_kernel(const __grid_constant
     const float *g = a.g + from;
     unsigned *mc = (unsigned *)a.m + block * 64, *rc = (unsigned *)a.v + block * 64;
     const bool whole = n == kAdamBlock, vw = whole && ((uintptr_t)w & 15) == 0, vg = whole && ((uintptr_t)g & 15) == 0;
-    float ww[2][4], m[2][4], r[2][4];
+    float m[2][4], r[2][4], ww[2][4];
     unsigned mq[2], rq[2];
     const float2 scale = *reinterpret_cast<const float2 *>(a.scales + 2 * block);
 #pragma unroll
@@ -225,25 +258,25 @@ static __global__ void __launch_bounds__(256) adam8_kernel(const __grid_constant
       const int at = h * 128 + lane * 4;
       load_four(m[h], g + at, n - at, vg);
       load_four(ww[h], w + at, n - at, vw);
-      mq[h] = mc[h * 32 + lane];
-      rq[h] = rc[h * 32 + lane];
+      mq[h] = codes_of(mc, h, lane, n);
+      rq[h] = codes_of(rc, h, lane, n);
     }
     float top_m = 0.f, top_r = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < 2; h++) {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const bool in = whole || h * 128 + lane * 4 + j < n;
-        const unsigned cm = mq[h] >> (8 * j) & 255u, cr = rq[h] >> (8 * j) & 255u;
-        const float gj = m[h][j], was = code_value(cm & 127u, kMeanShift, scale.x), root = code_value(cr, kRootShift, scale.y);
-        m[h][j] = __fadd_rn(__fmul_rn(s.beta1, cm & 128u ? -was : was), __fmul_rn(s.rest1, gj));
+        const float gj = m[h][j];
+        const float was = code_value(mq[h] >> (8 * j) & 127u, kMeanShift, scale.x), root = code_value(rq[h] >> (8 * j) & 255u, kRootShift, scale.y);
+        const float sign = __uint_as_float(__float_as_uint(was) ^ (mq[h] << (24 - 8 * j) & 0x80000000u));
+        m[h][j] = __fadd_rn(__fmul_rn(s.beta1, sign), __fmul_rn(s.rest1, gj));
         r[h][j] = __fsqrt_rn(__fadd_rn(__fmul_rn(s.beta2, __fmul_rn(root, root)), __fmul_rn(s.rest2, __fmul_rn(gj, gj))));
-        if (in) {
-          top_m = larger(top_m, fabsf(m[h][j]));
-          top_r = larger(top_r, r[h][j]);
-        }
-        ww[h][j] = fmaf(-f.rate, m[h][j] / fmaf(r[h][j], f.root, s.eps), ww[h][j] * s.keep);
+        top_m = larger(top_m, fabsf(m[h][j]));
+        top_r = larger(top_r, r[h][j]);
+        ww[h][j] = adam_weight(ww[h][j], m[h][j], r[h][j], s, f);
       }
+      store_four(w + h * 128 + lane * 4, ww[h], n - (h * 128 + lane * 4), vw);
+    }
     top_m = warp_largest(top_m);
     top_r = warp_largest(top_r);
     // (a NaN stays one, and makes the block's values NaN)
@@ -251,24 +284,19 @@ static __global__ void __launch_bounds__(256) adam8_kernel(const __grid_constant
     if (scale_m < 0x1p-126f) scale_m = 0.f;
     if (scale_r < 0x1p-126f) scale_r = 0.f;
     const float inverse_m = scale_m == 0.f ? 0.f : __fdiv_rn(1.f, scale_m), inverse_r = scale_r == 0.f ? 0.f : __fdiv_rn(1.f, scale_r);
-    const unsigned key = step_key(s.seed, f.step, (unsigned)(s.number + i));
+    const unsigned key = step_key(s.seed, f.step, (unsigned)(s.number + i)) + (unsigned)(from + lane * 4) * kPlaceStep;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       mq[h] = rq[h] = 0;
-      const int at = h * 128 + lane * 4;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const unsigned bits = place_bits((unsigned)(from + at + j), key);
-        const unsigned cm = value_code(fabsf(m[h][j]), inverse_m, kMeanShift, bits & 0xffffu, 127u) | (m[h][j] < 0.f ? 128u : 0u);
-        const unsigned cr = value_code(r[h][j], inverse_r, kRootShift, bits >> 16, 255u);
-        if (whole || at + j < n) {
-          mq[h] |= cm << (8 * j);
-          rq[h] |= cr << (8 * j);
-        }
+      for (int j = 0; j < 4; j++) {                       // (zeros, those behind the values among them, have the code zero whatever the noise)
+        const unsigned bits = place_bits(key + (unsigned)(h * 128 + j) * kPlaceStep);
+        const unsigned cm = value_code(fabsf(m[h][j]), inverse_m, kMeanShift, mean_noise(bits), 127u) + (m[h][j] < 0.f ? 128u : 0u);
+        mq[h] += cm << (8 * j);
+        rq[h] += value_code(r[h][j], inverse_r, kRootShift, root_noise(bits), 255u) << (8 * j);
       }
       mc[h * 32 + lane] = mq[h];
       rc[h * 32 + lane] = rq[h];
-      store_four(w + at, ww[h], n - at, vw);
     }
     if (lane == 0) *reinterpret_cast<float2 *>(a.scales + 2 * block) = make_float2(scale_m, scale_r);
   }
@@ -328,7 +356,7 @@ template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTe
       table.count++;
     }
     s.last = i == all.size();
-    const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, (unsigned)ctx().sm_count * 8));
+    const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, kind == kAdamMoments ? 1u << 30 : (unsigned)ctx().sm_count * 4));
     if (kind == kAdam32) pdl_launch(adam_kernel<N>, blocks, 256, 0, table, s);
     else if (kind == kAdam8) pdl_launch(adam8_kernel<N>, blocks, 256, 0, table, s);
     else pdl_launch(adam8_moments_kernel<N>, blocks, 256, 0, table);
@@ -341,11 +369,16 @@ static void adam_launch(AdamKind kind, const std::vector<AdamTensor> &all, const
 }
 
 // ---- checks
-// Memory that a call writes may share nothing with the rest of its tensors.
+// Memory that a call writes may share nothing with the rest of its tensors.  Tensors of a kind often lie side by side in one storage: neighbours come together as
+// they are added, so that few spans are left to sort.
 class Spans {
  public:
   void add(const void *p, long values, bool written) {
-    if (values) spans_.push_back(Span{(uintptr_t)p, (uintptr_t)p + 4 * (uintptr_t)values, written});
+    if (!values) return;
+    const Span s{(uintptr_t)p, (uintptr_t)p + 4 * (uintptr_t)values, written};
+    if (!spans_.empty() && spans_.back().written == written && (spans_.back().to == s.from || (!written && spans_.back().from <= s.from && s.from < spans_.back().to)))
+      spans_.back().to = std::max(spans_.back().to, s.to);
+    else spans_.push_back(s);
   }
   void check() {
     if (!std::is_sorted(spans_.begin(), spans_.end())) std::sort(spans_.begin(), spans_.end());
@@ -368,11 +401,19 @@ class Spans {
 static void check_flat(const THGPUTensor *t, long n, int argn, int i, const char *what) {
   if (!t || nelem(t) != n || !is_contiguous(t)) fail("Invalid argument %d: contiguous %s of %ld values expected for tensor %d", argn, what, n, i + 1);
 }
+static void add_codes(Spans &spans, const std::vector<AdamTensor> &all, bool codes_written, bool g_written) {
+  auto blocks = [](const AdamTensor &t) { return (t.n + kAdamBlock - 1) / kAdamBlock; };
+  for (const AdamTensor &t : all) spans.add(t.w, t.n, true);
+  for (const AdamTensor &t : all) spans.add(t.g, t.n, g_written);
+  for (const AdamTensor &t : all) spans.add(t.m, 64 * blocks(t), codes_written);
+  for (const AdamTensor &t : all) spans.add(t.v, 64 * blocks(t), codes_written);
+  for (const AdamTensor &t : all) spans.add(t.scales, 2 * blocks(t), codes_written);
+}
 static void check_rates(double lr, double beta1, double beta2, double eps, double decay, int argn) {
   THC_ARG(std::isfinite(lr) && lr >= 0, argn, "learning rate must be finite and not negative");
   THC_ARG(beta1 >= 0 && beta1 < 1, argn + 1, "beta1 must be in [0, 1)");
   THC_ARG(beta2 >= 0 && beta2 < 1, argn + 2, "beta2 must be in [0, 1)");
-  THC_ARG(std::isfinite(eps) && eps > 0, argn + 3, "epsilon must be positive");
+  THC_ARG(std::isfinite(eps) && eps >= 0x1p-126 && eps < 0x1p126, argn + 3, "epsilon must be positive and within the range of a float's normal values");
   THC_ARG(std::isfinite(decay) && decay >= 0, argn + 4, "weight decay must be finite and not negative");
 }
 static AdamStep adam_step(THGPUTensor *step, double lr, double beta1, double beta2, double eps, double decay, long seed) {
@@ -412,11 +453,11 @@ THC_API int THGPUNN_AdamW_update(int n, THGPUTensor **weights, THGPUTensor **gra
     check_flat(squares[i], k, 5, i, "squares");
     check_here({nullptr, weights[i], grads[i], means[i], squares[i]});
     all.push_back(AdamTensor{data_ptr(weights[i]), data_ptr(grads[i]), data_ptr(means[i]), data_ptr(squares[i]), nullptr, k});
-    spans.add(all[i].w, k, true);
-    spans.add(all[i].g, k, false);
-    spans.add(all[i].m, k, true);
-    spans.add(all[i].v, k, true);
   }
+  for (const AdamTensor &t : all) spans.add(t.w, t.n, true);
+  for (const AdamTensor &t : all) spans.add(t.g, t.n, false);
+  for (const AdamTensor &t : all) spans.add(t.m, t.n, true);
+  for (const AdamTensor &t : all) spans.add(t.v, t.n, true);
   spans.check();
   adam_launch(kAdam32, all, adam_step(step, lr, beta1, beta2, eps, decay, 0));
   return 0;
@@ -446,12 +487,8 @@ THC_API int THGPUNN_AdamW8_update(int n, THGPUTensor **weights, THGPUTensor **gr
     check_here({nullptr, weights[i], grads[i], meanCodes[i], rootCodes[i], scales[i]});
     all.push_back(AdamTensor{data_ptr(weights[i]), data_ptr(grads[i]), data_ptr(meanCodes[i]), data_ptr(rootCodes[i]), data_ptr(scales[i]), k});
     THC_ARG(((uintptr_t)all[i].scales & 7) == 0, 6, "scales on a boundary of 8 bytes expected");
-    spans.add(all[i].w, k, true);
-    spans.add(all[i].g, k, false);
-    spans.add(all[i].m, 64 * blocks, true);
-    spans.add(all[i].v, 64 * blocks, true);
-    spans.add(all[i].scales, 2 * blocks, true);
   }
+  add_codes(spans, all, true, false);
   spans.check();
   adam_launch(kAdam8, all, adam_step(step, lr, beta1, beta2, eps, decay, seed));
   return 0;
@@ -476,12 +513,8 @@ THC_API int THGPUNN_AdamW8_moments(int n, THGPUTensor **meanCodes, THGPUTensor *
     check_here({nullptr, meanCodes[i], rootCodes[i], scales[i], means[i], squares[i]});
     all.push_back(AdamTensor{data_ptr(means[i]), data_ptr(squares[i]), data_ptr(meanCodes[i]), data_ptr(rootCodes[i]), data_ptr(scales[i]), k});
     THC_ARG(((uintptr_t)all[i].scales & 7) == 0, 4, "scales on a boundary of 8 bytes expected");
-    spans.add(all[i].w, k, true);
-    spans.add(all[i].g, k, true);
-    spans.add(all[i].m, 64 * blocks, false);
-    spans.add(all[i].v, 64 * blocks, false);
-    spans.add(all[i].scales, 2 * blocks, false);
   }
+  add_codes(spans, all, false, true);
   spans.check();
   if (n) adam_launch(kAdamMoments, all, AdamStep{});
   return 0;

@@ -9,6 +9,7 @@
 // same columns of all its rows, so that nothing but the dot products crosses threads, and every result has one writer and one order.
 #include <cstring>
 #include <type_traits>
+#include <vector>
 
 #include "nn_args.h"
 #include "per_device.h"
@@ -18,7 +19,9 @@ namespace thc {
 constexpr long kMostSlots = 1l << 24;     // positions are floats
 constexpr int kMostGroups = 4096;
 constexpr long kMostValues = 1l << 23;    // of a row: its pieces are a dimension of the grid
-constexpr long kFewSlots = 2048;          // up to here every block ranks its token's slots by itself
+constexpr long kFewSlots = 2048;          // up to here every block ranks its token's slots by itself,
+constexpr long kRankedSlots = 32768;      // and up to here a launch of its own ranks them, where the groups are
+constexpr int kRankedGroups = 1024;       // no more than these
 
 // The expert of a slot, from 1; 0: none; -1: the number stands for no expert.
 static __device__ __forceinline__ int slot_expert(float e, int groups) {
@@ -27,12 +30,7 @@ static __device__ __forceinline__ int slot_expert(float e, int groups) {
 // The row at a place, or -1: a place that stands for none of the `rows` is passed over.
 static __device__ __forceinline__ long row_at(float place, long rows) { return place >= 1.f && place <= (float)rows ? (long)place - 1 : -1; }
 
-// What the host is told: rows of each group in out[0 .. groups), the slots whose number stands for no expert in out[groups].
-struct SlotCounts {
-  int *out;
-  ScalarSlot *slot;
-  unsigned long long seq;
-};
+// The host is told the rows of each group, and as one more group the slots whose number stands for no expert, by the first block.
 
 // ---- where the rows go -------------------------------------------------------------------------------------------------
 // Many slots: in `chunks` pieces of `per`, a block each.  The first launch counts: hist[group][chunk], the bad numbers as one more group.  In the second one
@@ -52,7 +50,7 @@ static __global__ void __launch_bounds__(256) slots_count_kernel(const float *__
 }
 
 static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__restrict__ experts, long slots, int per, int groups, const int *__restrict__ hist,
-                                                                 float *__restrict__ positions, SlotCounts tell) {
+                                                                 float *__restrict__ positions, CountStage tell) {
   pdl_begin();
   extern __shared__ int place[];                   // [8 warps][groups]: rows before the warp's next one of a group
   int *total = place + 8 * groups, *before = total + groups;   // [groups]: a group's rows, and those of the pieces before this one
@@ -78,11 +76,10 @@ static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__
     ahead = __reduce_add_sync(0xffffffffu, ahead);
     if (lane == 0) {
       if (g < groups) { total[g] = all; before[g] = ahead; }
-      if (blockIdx.x == 0) tell.out[g] = all;
+      if (blockIdx.x == 0) count_deliver(tell, g, all);
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0 && t == 0) scalar_deliver(tell.slot, 0.0, tell.seq);   // its system fence comes after every warp's counts, through the barrier
   // the groups' first rows: each thread has some neighbouring groups
   const int some = (groups + 255) / 256, g0 = min(groups, t * some), g1 = min(groups, g0 + some);
   int own = 0;
@@ -131,6 +128,57 @@ static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__
   }
 }
 
+// In one launch, where every block can as well count all slots by itself: 1024 threads with a slot each.
+static __global__ void __launch_bounds__(1024) slots_rank_kernel(const float *__restrict__ experts, int slots, int groups, float *__restrict__ positions,
+                                                                 CountStage tell) {
+  pdl_begin();
+  extern __shared__ int ahead[];                                  // [32 warps][groups]: rows of a group in the warps, then before them
+  int *before = ahead + 32 * groups, *after = before + groups;    // [groups]: rows of the slots before the block's, and behind them
+  __shared__ int sums[32], wrong;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, from = blockIdx.x * 1024, mine = from + t;
+  for (int g = t; g < 34 * groups; g += 1024) ahead[g] = 0;
+  if (t == 0) wrong = 0;
+  const int e = mine < slots ? slot_expert(experts[mine], groups) : 0;
+  __syncthreads();
+  const unsigned same = __match_any_sync(0xffffffffu, e);
+  const bool leads = lane == __ffs(same) - 1;
+  if (leads && e > 0) ahead[warp * groups + e - 1] = __popc(same);
+  if (leads && e < 0) atomicAdd(&wrong, __popc(same));
+#pragma unroll 4
+  for (int s0 = 0; s0 < slots; s0 += 1024) {
+    if (s0 == from) continue;
+    const int s = s0 + t, x = s < slots ? slot_expert(experts[s], groups) : 0;
+    if (x > 0) atomicAdd(&(s0 < from ? before : after)[x - 1], 1);
+    else if (x < 0) atomicAdd(&wrong, 1);
+  }
+  __syncthreads();
+  int total = 0;                                                  // thread g: group g, at most 1024 of them
+  if (t < groups) {
+    int at = before[t];
+    for (int w = 0; w < 32; w++) {
+      const int n = ahead[w * groups + t];
+      ahead[w * groups + t] = at;
+      at += n;
+    }
+    total = at + after[t];
+    if (blockIdx.x == 0) count_deliver(tell, t, total);
+  }
+  if (blockIdx.x == 0 && t == 0) count_deliver(tell, groups, wrong);
+  int run = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) sums[warp] = run;
+  __syncthreads();
+  int base = run - total;
+  for (int w = 0; w < warp; w++) base += sums[w];
+  if (t < groups) before[t] = base;
+  __syncthreads();
+  if (mine < slots) positions[mine] = e > 0 ? (float)(before[e - 1] + ahead[warp * groups + e - 1] + __popc(same & ((1u << lane) - 1)) + 1) : 0.f;
+}
+
 // ---- copying and summing rows ------------------------------------------------------------------------------------------
 // Blocks of 256 threads in teams of T, a team for each token (blockIdx.x) and T U W of its columns (blockIdx.y): U pieces of W = 4 values, or one where
 // lengths or addresses do not allow it, a thread.
@@ -138,7 +186,8 @@ template <int T, int U, bool VEC> struct Columns {
   static constexpr int W = VEC ? 4 : 1;
   float v[U * W];
   int c;                                              // the thread's first column; its u-th piece is u T W further on
-  __device__ __forceinline__ Columns(long piece) : c((int)(piece * (T * U * W)) + (int)(threadIdx.x % T) * W) {}
+  Columns() = default;
+  __device__ __forceinline__ explicit Columns(long piece) : c((int)(piece * (T * U * W)) + (int)(threadIdx.x % T) * W) {}
   static __device__ __forceinline__ long token() { return blockIdx.x * (long)(256 / T) + threadIdx.x / T; }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -190,7 +239,7 @@ static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const floa
 // or the same and come before it.
 template <int U, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const float *__restrict__ experts, float *__restrict__ positions, float *__restrict__ rows, int k,
-                                                                  int D, int slots, int groups, SlotCounts tell) {
+                                                                  int D, int slots, int groups, CountStage tell) {
   pdl_begin();
   extern __shared__ int expert[];       // [slots], the token's rows [k], and in the first block the counts [groups + 1]
   int *mine = expert + slots, *count = mine + k;
@@ -217,11 +266,8 @@ static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const 
     }
   }
   __syncthreads();
-  if (first) {
-    for (int g = t; g <= groups; g += 256) tell.out[g] = count[g];
-    __syncthreads();
-    if (t == 0) scalar_deliver(tell.slot, 0.0, tell.seq);
-  }
+  if (first)
+    for (int g = t; g <= groups; g += 256) count_deliver(tell, g, count[g]);
   for (int i = 0; i < k; i++)
     if (mine[i] >= 0) a.store(rows + mine[i] * (long)D, D);
 }
@@ -234,16 +280,30 @@ static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const f
   typedef Columns<T, U, VEC> Cols;
   const long t = Cols::token();
   if (t >= tokens) return;
-  Cols a(blockIdx.y), b(blockIdx.y);
+  Cols a(blockIdx.y);
   if (residual.p) a.load(residual.p + t * residual.ld, D);
   else a.zero();
-  for (int i = 0; i < k; i++) {
-    const long r = row_at(__ldg(positions + t * k + i), most);
-    if (r < 0) continue;
-    const float f = w ? __ldg(w + t * k + i) : 1.f;
-    b.load(rows.p + r * rows.ld, D);
+  constexpr int B = U * Cols::W <= 4 ? 8 : 2;      // rows on their way at once
+  for (int i0 = 0; i0 < k; i0 += B) {
+    long r[B];
+    float f[B];
+    Cols b[B];
 #pragma unroll
-    for (int j = 0; j < U * Cols::W; j++) a.v[j] = fmaf(f, b.v[j], a.v[j]);
+    for (int i = 0; i < B; i++) {
+      r[i] = i0 + i < k ? row_at(__ldg(positions + t * k + i0 + i), most) : -1;
+      f[i] = r[i] < 0 ? 0.f : w ? __ldg(w + t * k + i0 + i) : 1.f;
+    }
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+      b[i].c = a.c;
+      b[i].zero();
+      if (r[i] >= 0) b[i].load(rows.p + r[i] * rows.ld, D);
+    }
+#pragma unroll
+    for (int i = 0; i < B; i++) {
+#pragma unroll
+      for (int j = 0; j < U * Cols::W; j++) a.v[j] = fmaf(f[i], b[i].v[j], a.v[j]);
+    }
   }
   a.store(y + t * D, D);
 }
@@ -303,13 +363,22 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
   }
 }
 
-// f(integral constants T, U, VEC) for rows of D values: teams as wide as a row, at most a block; one piece a thread where the rows are few
+// f(integral constants T, U, VEC) for rows of D values: the widest team that leaves the fewest columns over, or (whole) one as wide as a row, at most a block; one
+// piece a thread where the rows are few, so that they are spread over all SMs.
 template <class F> static void with_columns(long tokens, int D, bool vec, bool whole, F f) {
   auto go = [&](auto VEC, auto U) {
     constexpr int per = (decltype(VEC)::value ? 4 : 1) * decltype(U)::value;
-    if (D <= 32 * per) f(std::integral_constant<int, 32>(), U, VEC);
-    else if (D <= 64 * per) f(std::integral_constant<int, 64>(), U, VEC);
-    else if (D <= 128 * per) f(std::integral_constant<int, 128>(), U, VEC);
+    int team = 256;
+    if (whole) {
+      while (team > 32 && D <= team / 2 * per) team /= 2;
+    } else {
+      auto width = [&](int t) { return (long)ceil_div(D, t * per) * t; };
+      for (int t = 128; t >= 32; t /= 2)
+        if (width(t) < width(team)) team = t;
+    }
+    if (team == 32) f(std::integral_constant<int, 32>(), U, VEC);
+    else if (team == 64) f(std::integral_constant<int, 64>(), U, VEC);
+    else if (team == 128) f(std::integral_constant<int, 128>(), U, VEC);
     else f(std::integral_constant<int, 256>(), U, VEC);
   };
   const bool few = !whole && tokens * (long)D < ctx().sm_count * 4096l;
@@ -326,11 +395,12 @@ static bool pieces_of_four(std::initializer_list<Rows> all, int D) {
   for (const Rows &r : all) ok = ok && ((uintptr_t)r.p & 15) == 0 && r.ld % 4 == 0;
   return ok;
 }
+
 // ---- launches
 // Whether slots may be ranked block by block.
 static bool are_few(long slots, int k) { return slots <= kFewSlots && k <= 64; }
 
-static void dispatch(Rows x, const float *experts, long tokens, int k, int D, int groups, float *positions, float *rows, const SlotCounts &tell) {
+static void dispatch(Rows x, const float *experts, long tokens, int k, int D, int groups, float *positions, float *rows, const CountStage &tell) {
   const long slots = tokens * k;
   const bool vec = pieces_of_four({x, Rows{rows, D}}, D);
   if (are_few(slots, k)) {
@@ -341,18 +411,28 @@ static void dispatch(Rows x, const float *experts, long tokens, int k, int D, in
     return;
   }
   const int sms = ctx().sm_count;
-  const int per = (int)std::max(1024l, (slots + sms * 256l - 1) / (sms * 256l) * 256), chunks = ceil_div(slots, per);
-  int *hist = (int *)ws_alloc(sizeof(int) * (groups + 1) * chunks);
-  pdl_launch(slots_count_kernel, (unsigned)chunks, 256, sizeof(int) * (groups + 1), experts, slots, per, groups, hist);
-  check_launch("Dispatch_updateOutput");
-  constexpr size_t most = sizeof(int) * 10 * kMostGroups;
-  static PerDevice allowed;
-  allowed.get(ctx().device, [&] {
-    THC_CUDA(cudaFuncSetAttribute(slots_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
-    return 1;
-  });
-  pdl_launch(slots_place_kernel, (unsigned)chunks, 256, sizeof(int) * 10 * groups, experts, slots, per, groups, hist, positions, tell);
-  check_launch("Dispatch_updateOutput");
+  if (slots <= kRankedSlots && groups <= kRankedGroups) {
+    static PerDevice allowed;
+    allowed.get(ctx().device, [&] {
+      THC_CUDA(cudaFuncSetAttribute(slots_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(int) * 34 * kRankedGroups));
+      return 1;
+    });
+    pdl_launch(slots_rank_kernel, (unsigned)ceil_div(slots, 1024), 1024, sizeof(int) * 34 * groups, experts, (int)slots, groups, positions, tell);
+    check_launch("Dispatch_updateOutput");
+  } else {
+    const int per = (int)std::max(1024l, (slots + sms * 256l - 1) / (sms * 256l) * 256), chunks = ceil_div(slots, per);
+    int *hist = (int *)ws_alloc(sizeof(int) * (groups + 1) * chunks);
+    pdl_launch(slots_count_kernel, (unsigned)chunks, 256, sizeof(int) * (groups + 1), experts, slots, per, groups, hist);
+    check_launch("Dispatch_updateOutput");
+    constexpr size_t most = sizeof(int) * 10 * kMostGroups;
+    static PerDevice allowed;
+    allowed.get(ctx().device, [&] {
+      THC_CUDA(cudaFuncSetAttribute(slots_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+      return 1;
+    });
+    pdl_launch(slots_place_kernel, (unsigned)chunks, 256, sizeof(int) * 10 * groups, experts, slots, per, groups, hist, positions, tell);
+    check_launch("Dispatch_updateOutput");
+  }
   with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
     constexpr int t = decltype(T)::value, u = decltype(U)::value, width = t * u * (decltype(VEC)::value ? 4 : 1);
     pdl_launch(rows_out_kernel<t, u, decltype(VEC)::value>, dim3((unsigned)ceil_div(tokens, 256 / t), (unsigned)ceil_div(D, width)), 256, 0, x, positions, rows, tokens, k,
@@ -414,12 +494,11 @@ THC_API int THGPUNN_Dispatch_updateOutput(THGPUTensor *input, THGPUTensor *exper
   WsScope scope;
   DenseRows x(input);
   TensorRef e(tensor_new_contiguous(experts));
-  Context &c = ctx();
-  static_assert(kMostGroups < kSmallStage, "the counts travel through the stage of small downloads");
-  const SlotCounts tell{(int *)c.small_stage_dev, c.scalar_slot_dev, scalar_expect()};
+  static_assert(kMostGroups < kCountStage, "a word for each group and one more");
+  const CountStage tell = counts_expect();
   dispatch(Rows{x.p, x.ld}, data_ptr(e), tokens, (int)k, (int)D, groups, data_ptr(positions), data_ptr(output), tell);
-  scalar_wait(tell.seq);
-  const int *told = (const int *)c.small_stage;
+  std::vector<int> told(groups + 1);
+  counts_wait(tell, told.data(), groups + 1);
   long rows = 0;
   for (int g = 0; g < groups; g++) rows += counts[g] = told[g];
   const long s[2] = {rows, D};

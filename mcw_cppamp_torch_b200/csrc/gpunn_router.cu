@@ -57,21 +57,23 @@ static __device__ __forceinline__ float key_score(unsigned k) {
 }
 constexpr unsigned kClosedKey = 0x007fffffu;    // of minus infinity
 
-template <int V, bool VEC>
-static __global__ void __launch_bounds__(256) router_forward_kernel(const float *__restrict__ x, long ld, float *__restrict__ weights, float *__restrict__ experts,
-                                                                    long rows, int E, int k, bool normalize) {
-  pdl_begin();
-  typedef WarpRow<V, VEC> Row;
-  const int lane = threadIdx.x & 31;
-  const long row = blockIdx.x * 8l + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  float v[V];
-  Row::load(x + row * ld, lane, E, v);
+static __device__ __forceinline__ float warp_max(float v) {      // a NaN if there is one
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The chosen score of a lane, if it has one.
+struct Chosen {
+  float score;
+  int expert, slot;      // expert from 1, 0: none
+};
+// The k largest one after the other: the largest of each lane's, of the warp's, its first place; lane i has the i-th.
+template <int V> static __device__ __forceinline__ Chosen choose_in_turn(const float (&v)[V], int lane, int k) {
   unsigned key[V];
 #pragma unroll
   for (int j = 0; j < V; j++) key[j] = score_key(v[j]);
-  float score = -INFINITY, top = -INFINITY;
-  int expert = 0;
+  Chosen c{-INFINITY, 0, lane};
   for (int i = 0; i < k; i++) {
     unsigned best = 0;
 #pragma unroll
@@ -81,15 +83,77 @@ static __global__ void __launch_bounds__(256) router_forward_kernel(const float 
     unsigned mine = 0xffffffffu;
 #pragma unroll
     for (int j = V - 1; j >= 0; j--)
-      if (key[j] == best) mine = Row::at(j, lane);
+      if (key[j] == best) mine = j * 32 + lane;
     const unsigned place = __reduce_min_sync(0xffffffffu, mine);
 #pragma unroll
     for (int j = 0; j < V; j++)
-      if ((unsigned)Row::at(j, lane) == place) key[j] = 0;
-    if (lane == i) { score = key_score(best); expert = (int)place + 1; }
-    if (i == 0) top = key_score(best);
+      if ((unsigned)(j * 32 + lane) == place) key[j] = 0;
+    if (lane == i) { c.score = key_score(best); c.expert = (int)place + 1; }
   }
-  const float e = expert ? expf(score - top) : 0.f;
+  return c;
+}
+// The k largest at once.  The k-th largest of the lanes' largest is no more than the k-th of all, so that those from it on, some 32 log(32 / (32 - k)) of scores in
+// random order, are all that is left to rank: each is compared with each.  False where they are more than the lanes, with nothing done.
+constexpr int kFewChosen = 16;      // 22 scores are left on average, at 20 they are 31
+struct Candidates {
+  float score[32];
+  int expert[32];
+};
+template <int V> static __device__ __forceinline__ bool choose_at_once(const float (&v)[V], float most, float top, Candidates &left, int lane, int k, Chosen &c) {
+  float bound = top;
+  for (int i = 1; i < k; i++) {
+    most = most == bound ? -INFINITY : most;
+    bound = warp_max(most);
+  }
+  bound = fmaxf(bound, -3.402823466e+38f);      // (an open score)
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    const bool in = v[j] >= bound;
+    const unsigned all = __ballot_sync(0xffffffffu, in);
+    const int at = n + __popc(all & ((1u << lane) - 1));
+    if (in && at < 32) {
+      left.score[at] = v[j];
+      left.expert[at] = j * 32 + lane + 1;
+    }
+    n += __popc(all);
+  }
+  if (n > 32) return false;
+  __syncwarp();
+  c = Chosen{-INFINITY, 0, lane};
+  if (lane < n) {
+    c.score = left.score[lane];
+    c.slot = 0;
+  }
+  for (int i = 0; i < n; i++) {
+    const float o = left.score[i];
+    if (lane < n) c.slot += o > c.score || (o == c.score && i < lane);
+  }
+  if (lane < n && c.slot < k) c.expert = left.expert[lane];
+  return true;
+}
+
+template <int V>
+static __global__ void __launch_bounds__(256) router_forward_kernel(const float *__restrict__ x, long ld, float *__restrict__ weights, float *__restrict__ experts,
+                                                                    long rows, int E, int k, bool normalize) {
+  pdl_begin();
+  __shared__ Candidates left[V >= 4 ? 8 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long row = blockIdx.x * 8l + warp;
+  if (row >= rows) return;
+  float v[V];
+  WarpRow<V, false>::load(x + row * ld, lane, E, v);
+  float most = v[0];
+#pragma unroll
+  for (int j = 1; j < V; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(v[j]));
+  const float top = warp_max(most);
+  Chosen c;
+  bool done = false;
+  if constexpr (V >= 4) {
+    if (k <= kFewChosen && top == top) done = choose_at_once<V>(v, most, top, left[warp], lane, k, c);
+  }
+  if (!done) c = choose_in_turn<V>(v, lane, k);
+  const float e = c.expert ? expf(c.score - top) : 0.f;
   float total = 0.f;
   if (normalize) total = e;
   else if (top != -INFINITY) {
@@ -97,9 +161,9 @@ static __global__ void __launch_bounds__(256) router_forward_kernel(const float 
     for (int j = 0; j < V; j++) total += expf(v[j] - top);
   }
   total = warp_total(total);
-  if (lane < k) {
-    weights[row * k + lane] = expert ? e / total : 0.f;
-    experts[row * k + lane] = (float)expert;
+  if (c.slot < k) {
+    weights[row * k + c.slot] = c.expert ? e / total : 0.f;
+    experts[row * k + c.slot] = (float)c.expert;
   }
 }
 
@@ -186,8 +250,8 @@ THC_API int THGPUNN_Router_updateOutput(THGPUTensor *input, THGPUTensor *weights
   size_result(experts, 2, s, {input, weights}, 3);
   if (rows == 0) return 0;
   DenseRows x(input);
-  with_row((int)E, in_pieces(x.p, x.ld, (int)E), [&](auto V, auto VEC) {
-    pdl_launch(router_forward_kernel<decltype(V)::value, decltype(VEC)::value>, (unsigned)ceil_div(rows, 8), 256, 0, x.p, x.ld, data_ptr(weights), data_ptr(experts),
+  with_row((int)E, false, [&](auto V, auto) {
+    pdl_launch(router_forward_kernel<decltype(V)::value>, (unsigned)ceil_div(rows, 8), 256, 0, x.p, x.ld, data_ptr(weights), data_ptr(experts),
                rows, (int)E, k, normalize != 0);
   });
   check_launch("Router_updateOutput");

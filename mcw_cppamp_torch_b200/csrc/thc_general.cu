@@ -78,7 +78,10 @@ static void init_device(Context &c, int device) {
     THC_CUDA(cudaHostAlloc((void **)&c.scalar_slot, sizeof(ScalarSlot), cudaHostAllocMapped | cudaHostAllocPortable));
     c.scalar_slot->seq = 0;
     THC_CUDA(cudaHostAlloc((void **)&c.small_stage, sizeof(float) * kSmallStage, cudaHostAllocMapped | cudaHostAllocPortable));
+    THC_CUDA(cudaHostAlloc((void **)&c.count_stage, sizeof(*c.count_stage) * kCountStage, cudaHostAllocMapped | cudaHostAllocPortable));
+    std::fill(c.count_stage, c.count_stage + kCountStage, 0ull);
   }
+  THC_CUDA(cudaHostGetDevicePointer((void **)&c.count_stage_dev, c.count_stage, 0));
   THC_CUDA(cudaHostGetDevicePointer((void **)&c.small_stage_dev, c.small_stage, 0));
   THC_CUDA(cudaHostGetDevicePointer((void **)&c.scalar_slot_dev, c.scalar_slot, 0));
   if (!c.stall_host) {
@@ -209,6 +212,30 @@ double scalar_wait(unsigned long long seq) {
   const double v = slot->value;
   check_stall();
   return v;
+}
+CountStage counts_expect() {
+  Context &c = ctx();
+  return CountStage{c.count_stage_dev, ++c.count_seq};
+}
+void counts_wait(const CountStage &stage, int *values, int n) {
+  Context &c = ctx();
+  volatile unsigned long long *words = c.count_stage;
+  for (int i = 0; i < n; i++) {
+    unsigned long long w;
+    for (unsigned polls = 1; (w = words[i]) >> 32 != stage.seq; polls++) {
+      if ((polls & 4095) == 0) {   // a failed launch never delivers: ask the stream now and then
+        const cudaError_t e = cudaStreamQuery(c.stream);
+        if (e == cudaErrorNotReady) continue;
+        THC_CUDA(e);
+        THC_CHECK(words[i] >> 32 == stage.seq, "internal: a count was not delivered");
+      }
+#if defined(__x86_64__)
+      __builtin_ia32_pause();
+#endif
+    }
+    values[i] = (int)(unsigned)w;
+  }
+  check_stall();
 }
 int device_if_initialised() { return g_ctx.device; }
 

@@ -56,6 +56,7 @@ struct ScalarSlot {
 };
 
 constexpr long kSmallStage = 16384;
+constexpr int kCountStage = 4608;
 
 struct Context {
   int device = -1;            // current device of this host thread, -1 = not yet initialised
@@ -73,6 +74,9 @@ struct Context {
   float *small_stage = nullptr;           // kSmallStage floats of mapped pinned memory behind small downloads
   float *small_stage_dev = nullptr;
   unsigned long long scalar_seq = 0;      // number of the last scalar asked for
+  unsigned long long *count_stage = nullptr;      // kCountStage words of mapped pinned memory behind counts, and their device alias
+  unsigned long long *count_stage_dev = nullptr;
+  unsigned count_seq = 0;
   // stall flags of the tensor-core kernels (see mm::StallCtl)
   int *stall_host = nullptr;      // mapped pinned host word
   int *stall_host_dev = nullptr;  // its device alias
@@ -105,12 +109,25 @@ void check_stall();               // the check alone, for callers that have just
 // on the stream before that kernel is then complete too, and a pipeline stall is reported as by sync_stream.
 unsigned long long scalar_expect();
 double scalar_wait(unsigned long long seq);
+// Several whole numbers the same way, each in one word with the number of the call: they need no order among them, so that the kernel has no fence to wait for.
+// counts_wait returns when all n have come.  The caller sees to it that the stream is not being recorded.
+struct CountStage {
+  unsigned long long *out;
+  unsigned seq;
+};
+CountStage counts_expect();
+void counts_wait(const CountStage &stage, int *values, int n);
 #ifdef __CUDACC__
 __device__ __forceinline__ void scalar_deliver(ScalarSlot *slot, double v, unsigned long long seq) {
   volatile ScalarSlot *s = slot;
   s->value = v;
   __threadfence_system();
   s->seq = seq;
+}
+#endif
+#ifdef __CUDACC__
+__device__ __forceinline__ void count_deliver(const CountStage &s, int i, int value) {
+  static_cast<volatile unsigned long long *>(s.out)[i] = (unsigned long long)s.seq << 32 | (unsigned)value;
 }
 #endif
 mm::StallCtl stall_ctl();         // kernel parameter of the tensor-core kernels

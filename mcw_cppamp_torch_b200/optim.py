@@ -6,11 +6,29 @@ BLOCK = 256     # values under one scale of the 8-bit moments
 
 
 def _tensors(t, what):
-    t = [t] if isinstance(t, GPUTensor) else list(t)
+    t = (t,) if isinstance(t, GPUTensor) else tuple(t)
     for v in t:
         if not isinstance(v, GPUTensor):
             raise TypeError("%s: torch.GPUTensor expected (call :gpu() on the module first)" % what)
     return t
+
+
+def _array(tensors):
+    return (TP * max(1, len(tensors)))(*[t._p for t in tensors])
+
+
+class _Tensors:
+    """A sequence of tensors as a field: kept as a tuple, so that the array of them that the library takes is made once for each that is put there."""
+
+    def __set_name__(self, owner, name):
+        self.name = name
+
+    def __get__(self, obj, owner=None):
+        return self if obj is None else obj._lists[self.name][0]
+
+    def __set__(self, obj, tensors):
+        tensors = _tensors(tensors, "AdamW " + self.name)
+        obj._lists[self.name] = tensors, _array(tensors)
 
 
 class AdamW:
@@ -24,15 +42,17 @@ class AdamW:
     instead of 8, rounded at random by `seed`; moments() gives what they stand for.  `step` holds the number of steps taken, on the device (up to 2^24), so that a
     recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Gradients may share memory, what a step writes may not."""
 
+    weights, gradWeights, mean, square, meanCodes, rootCodes, scales = (_Tensors() for _ in range(7))      # tuples: a list put there becomes one
+
     def __init__(self, weights, gradWeights, learningRate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, bits=32, seed=0):
-        self.weights, self.gradWeights = _tensors(weights, "AdamW"), _tensors(gradWeights, "AdamW gradients")
+        self._lists = {}
+        self.weights, self.gradWeights = weights, gradWeights
         if len(self.weights) != len(self.gradWeights):
             raise ValueError("AdamW: a gradient for each tensor expected")
         if bits not in (8, 32):
             raise ValueError("AdamW: moments are held in 8 or in 32 bits")
         self.learningRate, self.beta1, self.beta2, self.epsilon, self.weightDecay = learningRate, beta1, beta2, epsilon, weightDecay
         self.bits, self.seed = bits, seed
-        self._arrays = {}
         self.step = GPUTensor(2).zero()
         if bits == 32:
             self.mean, self.square = ([_zeros(*w.size()) for w in self.weights] for _ in range(2))
@@ -41,28 +61,25 @@ class AdamW:
             self.meanCodes, self.rootCodes = ([_zeros(b * BLOCK // 4) for b in blocks] for _ in range(2))
             self.scales = [_zeros(2 * b) for b in blocks]
 
-    def _array(self, name, tensors):
-        """The tensors as the library takes them, made again when others have come to the list."""
-        if len(tensors) != len(self.weights):
+    def _arrays(self, *names):
+        if any(len(self._lists[n][0]) != len(self.weights) for n in names):
             raise ValueError("AdamW: a tensor of each kind for each of the weights expected")
-        held, array = self._arrays.get(name, (None, None))
-        if held != tensors:
-            held = list(tensors)
-            array = (TP * max(1, len(held)))(*[t._p for t in held])
-            self._arrays[name] = held, array
-        return array
+        return [self._lists[n][1] for n in names]
 
     def __getstate__(self):
-        return dict(self.__dict__, _arrays={})
+        return dict(self.__dict__, _lists={n: t for n, (t, _) in self._lists.items()})
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _lists={})
+        for n, t in state["_lists"].items():
+            setattr(self, n, t)
 
     def update(self):
-        names = ("weights", "gradWeights") + (("mean", "square") if self.bits == 32 else ("meanCodes", "rootCodes", "scales"))
-        call = (len(self.weights),) + tuple(self._array(n, getattr(self, n)) for n in names)
-        call += (self.step._p, float(self.learningRate), float(self.beta1), float(self.beta2), float(self.epsilon), float(self.weightDecay))
+        rates = (self.step._p, float(self.learningRate), float(self.beta1), float(self.beta2), float(self.epsilon), float(self.weightDecay))
         if self.bits == 32:
-            lib().THGPUNN_AdamW_update(*call)
+            lib().THGPUNN_AdamW_update(len(self.weights), *self._arrays("weights", "gradWeights", "mean", "square"), *rates)
         else:
-            lib().THGPUNN_AdamW8_update(*call, int(self.seed))
+            lib().THGPUNN_AdamW8_update(len(self.weights), *self._arrays("weights", "gradWeights", "meanCodes", "rootCodes", "scales"), *rates, int(self.seed))
 
     def moments(self, mean=None, square=None):
         """The moments as lists of tensors: those that update() keeps, or with 8 bits what their codes stand for, in `mean` and `square` where these are given."""
@@ -71,8 +88,9 @@ class AdamW:
                 raise ValueError("AdamW: moments of 32 bits are not copied")
             return self.mean, self.square
         mean, square = ([GPUTensor(*w.size()) for w in self.weights] if t is None else _tensors(t, "AdamW moments") for t in (mean, square))
-        lists = [self._array(n, getattr(self, n)) for n in ("meanCodes", "rootCodes", "scales")] + [self._array("mean", mean), self._array("square", square)]
-        lib().THGPUNN_AdamW8_moments(len(self.weights), *lists)
+        if not len(mean) == len(square) == len(self.weights):
+            raise ValueError("AdamW: a tensor for each of the weights expected")
+        lib().THGPUNN_AdamW8_moments(len(mean), *self._arrays("meanCodes", "rootCodes", "scales"), _array(mean), _array(square))
         return mean, square
 
 

@@ -184,8 +184,8 @@ def test_combine_saves_no_caller_tensor(fake):  # noqa: F811
 
 def adamw(fake, bits=32, sizes=((7, 3), (256,), (300,))):  # noqa: F811
     m = object.__new__(optim.AdamW)
-    m.__dict__.update(weights=[fake(*s) for s in sizes], gradWeights=[fake(*s) for s in sizes], learningRate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8,
-                      weightDecay=0.01, bits=bits, seed=0, step=fake(2), _arrays={})
+    m.__dict__.update(learningRate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, bits=bits, seed=0, step=fake(2), _lists={})
+    m.weights, m.gradWeights = ([fake(*s) for s in sizes] for _ in range(2))
     n = [int(np.prod(s)) for s in sizes]
     blocks = [-(-k // 256) for k in n]
     m.mean, m.square = ([fake(k) for k in n] for _ in range(2))
@@ -196,7 +196,7 @@ def adamw(fake, bits=32, sizes=((7, 3), (256,), (300,))):  # noqa: F811
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw(fake, bits):  # noqa: F811
     for name, values in (("learningRate", (-1e-3, float("nan"), float("inf"))), ("beta1", (-0.1, 1.0, float("nan"))), ("beta2", (-0.1, 1.0, 1.5)),
-                         ("epsilon", (0.0, -1e-8, float("nan"))), ("weightDecay", (-0.1, float("inf")))):
+                         ("epsilon", (0.0, -1e-8, 1e-40, 1e38, float("nan"))), ("weightDecay", (-0.1, float("inf")))):
         for v in values:
             m = adamw(fake, bits)
             setattr(m, name, v)
@@ -211,15 +211,15 @@ def test_adamw(fake, bits):  # noqa: F811
         m = adamw(fake, bits)
         n = getattr(m, name)[1].nElement()
         for bad in (fake(n + 1), fake(n, strides=(2,))):
-            getattr(m, name)[1] = bad
+            setattr(m, name, changed(getattr(m, name), 1, bad))
             with pytest.raises(gt.THCError, match="for tensor 2"):
                 m.update()
         m = adamw(fake, bits)
-        getattr(m, name).pop()
+        setattr(m, name, getattr(m, name)[:-1])
         with pytest.raises(ValueError):
             m.update()
     m = adamw(fake, bits)
-    m.weights[0] = fake(7, 3, strides=(1, 7))
+    m.weights = changed(m.weights, 0, fake(7, 3, strides=(1, 7)))
     with pytest.raises(gt.THCError, match="contiguous weights"):
         m.update()
     # the same tensor twice, the end of one in another, a gradient in what is written
@@ -227,11 +227,12 @@ def test_adamw(fake, bits):  # noqa: F811
                            ("gradWeights", 2, lambda m: getattr(m, kept[-1])[2] if bits == 32 else m.weights[2])):
         m = adamw(fake, bits)
         if name == "weights":
-            m.weights.append(m.weights[2]); m.gradWeights.append(fake(300))
+            m.weights += (m.weights[2],)
+            m.gradWeights += (fake(300),)
             for k in kept:
-                getattr(m, k).append(fake(getattr(m, k)[2].nElement()))
+                setattr(m, k, getattr(m, k) + (fake(getattr(m, k)[2].nElement()),))
         else:
-            getattr(m, name)[i] = other(m)
+            setattr(m, name, changed(getattr(m, name), i, other(m)))
         with pytest.raises(gt.THCError, match="shares memory"):
             m.update()
     m = adamw(fake, bits)
@@ -239,9 +240,15 @@ def test_adamw(fake, bits):  # noqa: F811
     with pytest.raises(gt.THCError, match="shares memory"):
         m.update()
     m = adamw(fake, bits)
-    m.gradWeights[0] = m.weights[1].narrow(1, 256 - 20, 21)
+    m.gradWeights = changed(m.gradWeights, 0, m.weights[1].narrow(1, 256 - 20, 21))
     with pytest.raises(gt.THCError, match="shares memory"):
         m.update()
+
+
+def changed(tensors, i, t):
+    tensors = list(tensors)
+    tensors[i] = t
+    return tensors
 
 
 def test_adamw_arguments(fake):  # noqa: F811
@@ -256,28 +263,30 @@ def test_adamw_arguments(fake):  # noqa: F811
     m = adamw(fake, 8)
     with pytest.raises(ValueError):
         m.moments(m.mean[:2], m.square)
-    shared = list(m.square)
-    shared[1] = m.mean[1]
     with pytest.raises(gt.THCError, match="shares memory"):
-        m.moments(m.mean, shared)
-    m.scales[2] = fake(5).narrow(1, 2, 4)
+        m.moments(m.mean, changed(m.square, 1, m.mean[1]))
+    m.scales = changed(m.scales, 2, fake(5).narrow(1, 2, 4))
     with pytest.raises(gt.THCError, match="boundary of 8 bytes"):
         m.update()
     with pytest.raises(gt.THCError, match="boundary of 8 bytes"):
         m.moments(m.mean, m.square)
-    m = adamw(fake)
-    m._array("weights", m.weights)
-    assert m.__getstate__()["_arrays"] == {}
 
 
-def test_adamw_notices_other_tensors(fake):  # noqa: F811
-    """The arrays that the library is given are those of the lists as they are now."""
+def test_adamw_keeps_the_tensors_it_is_given(fake):  # noqa: F811
+    """What the library gets are the tensors of the fields, also after others have been put there; a field is no list to be changed behind it."""
     m = adamw(fake)
-    first = m._array("mean", m.mean)
-    assert m._array("mean", m.mean) is first
-    m.mean[1] = fake(256)
-    again = m._array("mean", m.mean)
-    assert [C.addressof(again[i].contents) for i in range(3)] == [C.addressof(t._p.contents) for t in m.mean]
+    with pytest.raises(TypeError):
+        m.mean[1] = fake(256)
+    with pytest.raises(TypeError):
+        m.mean = [fake(256), np.zeros(3)]
+    m.mean = [fake(7, 3), fake(256), fake(300)]
+    array = m._arrays("mean")[0]
+    assert [C.addressof(array[i].contents) for i in range(3)] == [C.addressof(t._p.contents) for t in m.mean]
+    state = m.__getstate__()
+    assert state["_lists"]["mean"] is m.mean
+    twin = object.__new__(optim.AdamW)
+    twin.__setstate__(state)
+    assert twin.mean == m.mean and twin.beta1 == m.beta1
 
 
 def test_tensors_of_another_device(fake):  # noqa: F811
@@ -291,7 +300,7 @@ def test_tensors_of_another_device(fake):  # noqa: F811
     with pytest.raises(gt.THCError, match="Invalid argument 4: tensor of device 2"):
         m.forward([fake(8, 6), fake(5, 2), fake(5, 2), fake(5, 6, device=2)])
     m = adamw(fake)
-    m.square[2] = fake(300, device=2)
+    m.square = changed(m.square, 2, fake(300, device=2))
     with pytest.raises(gt.THCError, match="Invalid argument 5: tensor of device 2"):
         m.update()
 
