@@ -21,7 +21,8 @@
 namespace thc {
 
 constexpr int kAdamBlock = 256;                                // values under one scale
-constexpr int kAdamChunk = 2048;                               // values of a block's turn: a warp has 256
+constexpr int kAdamTurn = 2048;                                // values of a block's turn: a warp has 256
+constexpr int kAdamTurns = 4;                                  // turns of a chunk, for which a block looks its tensor up, where there are plenty
 constexpr unsigned kCodeBits = 0x37800000u;                    // of 2^-16
 constexpr int kMeanShift = 20, kRootShift = 19;
 constexpr float kCodeFloor = 0x1p-16f, kMeanTop = 0.9375f - 0x1p-16f, kRootTop = 0.96875f - 0x1p-16f;   // f(B), and what the largest codes stand for
@@ -37,7 +38,7 @@ struct AdamTensor {
 // As many as fit a launch's parameters; first[i]: the number of tensor i's first chunk.  The smaller table is for the usual few tensors: parameters are copied with
 // every launch.
 template <int N> struct AdamTable {
-  int count;
+  int count, turns;          // turns of a chunk
   unsigned first[N + 1];
   AdamTensor t[N];
 };
@@ -90,10 +91,16 @@ template <int N> static __device__ __forceinline__ int tensor_of(const AdamTable
   return lo;
 }
 
+static __device__ __forceinline__ void load_four(float *v, const float *p) {
+  const float4 q = *reinterpret_cast<const float4 *>(p);
+  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
+static __device__ __forceinline__ void store_four(float *p, const float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+
 // ---- moments in 32 bits
 static __device__ __forceinline__ float reciprocal(float v) {     // within a step
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 static __device__ __forceinline__ float square_root(float v) {
@@ -102,86 +109,101 @@ static __device__ __forceinline__ float square_root(float v) {
   return r;
 }
 static __device__ __forceinline__ float adam_weight(float w, float m, float root, const AdamStep &s, const AdamFactors &f) {
-  return fmaf(-f.rate, m * reciprocal(fmaf(root, f.root, s.eps)), w * s.keep);
+  return fmaf(-f.rate, m * reciprocal(fmaf(root, f.root, s.eps)), w * s.keep);      // (epsilon is no subnormal)
 }
 static __device__ __forceinline__ void adam_value(float &w, float g, float &m, float &v, const AdamStep &s, const AdamFactors &f) {
   m = fmaf(s.beta1, m, s.rest1 * g);
   v = fmaf(s.beta2, v, s.rest2 * (g * g));
   w = adam_weight(w, m, square_root(v), s, f);
 }
-// Eight values a thread: all of a turn's loads are on their way before the first is needed, in the first turn before the step's factors are made.
+// Eight values a thread, in pieces of four where addresses allow it.  The step's factors are made while the loads are on their way.  A block for each 2048 values: the
+// scheduler's blocks come and go at different times, so that loads and stores mix; blocks that stay and take turns took 282 us for 61 M values, these 257, 6.65 TB/s.
 template <int N>
-static __global__ void __launch_bounds__(256, 4) adam_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
+static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
-  __shared__ AdamFactors shared;
-  AdamFactors f;
-  const unsigned chunks = table.first[table.count];
-  bool started = false;
-  auto start = [&] {
-    if (started) return;
-    adam_factors(s, shared);
-    __syncthreads();
-    f = shared;
-    started = true;
-  };
-  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int i = tensor_of(table, chunk);
-    const AdamTensor &a = table.t[i];
-    const long from = (chunk - table.first[i]) * (long)kAdamChunk;
-    const int n = (int)min((long)kAdamChunk, a.n - from);
-    float *w = a.w + from, *m = (float *)a.m + from, *v = (float *)a.v + from;
-    const float *g = a.g + from;
-    if (n == kAdamChunk && (((uintptr_t)w | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) == 0) {
-      float4 ww[2], gg[2], mm[2], vv[2];
+  __shared__ AdamFactors f;
+  const int i = tensor_of(table, blockIdx.x), t = threadIdx.x;
+  const AdamTensor &a = table.t[i];
+  const long from = (blockIdx.x - table.first[i]) * (long)kAdamTurn;      // (t[0] of an empty table is not set, and then not used)
+  const int n = blockIdx.x < table.first[table.count] ? (int)min((long)kAdamTurn, a.n - from) : 0;      // none: a step of no values counts all the same
+  float *w = a.w + from, *m = (float *)a.m + from, *v = (float *)a.v + from;
+  const float *g = a.g + from;
+  const bool vec = n == kAdamTurn && (((uintptr_t)w | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) == 0;
+  float ww[8], gg[8], mm[8], vv[8];
+  if (vec) {
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int at = j * 256 + threadIdx.x;
-        gg[j] = __ldcs(reinterpret_cast<const float4 *>(g) + at);
-        ww[j] = reinterpret_cast<float4 *>(w)[at];
-        mm[j] = reinterpret_cast<float4 *>(m)[at];
-        vv[j] = reinterpret_cast<float4 *>(v)[at];
-      }
-      start();
+    for (int j = 0; j < 8; j += 4) {
+      const int at = j * 256 + t * 4;
+      load_four(gg + j, g + at); load_four(ww + j, w + at); load_four(mm + j, m + at); load_four(vv + j, v + at);
+    }
+  } else {
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int at = j * 256 + threadIdx.x;
-        adam_value(ww[j].x, gg[j].x, mm[j].x, vv[j].x, s, f);
-        adam_value(ww[j].y, gg[j].y, mm[j].y, vv[j].y, s, f);
-        adam_value(ww[j].z, gg[j].z, mm[j].z, vv[j].z, s, f);
-        adam_value(ww[j].w, gg[j].w, mm[j].w, vv[j].w, s, f);
-        reinterpret_cast<float4 *>(w)[at] = ww[j];
-        reinterpret_cast<float4 *>(m)[at] = mm[j];
-        reinterpret_cast<float4 *>(v)[at] = vv[j];
-      }
-    } else {
-      float ww[8], gg[8], mm[8], vv[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int at = j * 256 + threadIdx.x;
-        if (at < n) { ww[j] = w[at]; gg[j] = g[at]; mm[j] = m[at]; vv[j] = v[at]; }
-      }
-      start();
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int at = j * 256 + threadIdx.x;
-        if (at < n) {
-          adam_value(ww[j], gg[j], mm[j], vv[j], s, f);
-          w[at] = ww[j]; m[at] = mm[j]; v[at] = vv[j];
-        }
-      }
+    for (int j = 0; j < 8; j++) {
+      const int at = j * 256 + t;
+      ww[j] = gg[j] = mm[j] = vv[j] = 0.f;
+      if (at < n) { gg[j] = g[at]; ww[j] = w[at]; mm[j] = m[at]; vv[j] = v[at]; }
     }
   }
-  start();
+  adam_factors(s, f);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 8; j++) adam_value(ww[j], gg[j], mm[j], vv[j], s, f);
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      const int at = j * 256 + t * 4;
+      store_four(w + at, ww + j); store_four(m + at, mm + j); store_four(v + at, vv + j);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int at = j * 256 + t;
+      if (at < n) { w[at] = ww[j]; m[at] = mm[j]; v[at] = vv[j]; }
+    }
+  }
   adam_count(s, f.step);
 }
 
 // ---- moments in 8 bits
-static __device__ __forceinline__ float code_value(unsigned code, int shift, float scale) {
-  return __fmul_rn(__fadd_rn(__uint_as_float(kCodeBits + (code << shift)), -kCodeFloor), scale);
+// Two values side by side: sm_100a multiplies, or adds, both in one instruction, which this kernel is short of.  A sum of two products of pairs is made a fused one
+// by the assembler, whatever its rounding says (12.9), and so would not be the sum that codes are defined by: those are added one by one.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float &x, float &y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+static __device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
-// The code of x >= 0 with `noise` below 2^shift on its bits.
-static __device__ __forceinline__ unsigned value_code(float x, float inverse, int shift, unsigned noise, unsigned most) {
-  return min((__float_as_uint(__fadd_rn(__fmul_rn(x, inverse), kCodeFloor)) + noise - (kCodeBits - (1u << (shift - 17)))) >> shift, most);
+static __device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+static __device__ __forceinline__ Pair fused(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+static __device__ __forceinline__ void add_singly(Pair a, Pair b, float &x, float &y) {
+  float ax, ay, bx, by;
+  a.get(ax, ay);
+  b.get(bx, by);
+  x = __fadd_rn(ax, bx);
+  y = __fadd_rn(ay, by);
+}
+static __device__ __forceinline__ float code_float(unsigned code, int shift) { return __uint_as_float(kCodeBits + (code << shift)); }      // f(B) more than it stands for
+static __device__ __forceinline__ Pair code_pair(unsigned codes, int j, int shift, Pair scale) {      // of bytes j and j + 1
+  return (Pair(code_float(__byte_perm(codes, 0, 0x4440 + j), shift), code_float(__byte_perm(codes, 0, 0x4441 + j), shift)) + Pair(-kCodeFloor, -kCodeFloor)) * scale;
+}
+// The code of x >= 0, times 1 / scale, with `noise` below 2^shift on its bits.  The largest value of a block needs no bound: on the way to its code, whose fraction
+// is zero, are at most three roundings of 2^-24 after that of the constant 1 / top, which is -0.32 of that for m and 0.68 for r, and the sum's half: 3.6 and 2.8 of the last bit
+// in all, where the noise leaves 8 (m) and 4 (r) to the next code.  In a block that is not finite codes do not matter.
+static __device__ __forceinline__ unsigned value_code(float x, int shift, unsigned noise) {
+  return (__float_as_uint(__fadd_rn(x, kCodeFloor)) + noise - (kCodeBits - (1u << (shift - 17)))) >> shift;
 }
 // 32 random bits of a place, but for the last step of the hash, h ^ h >> 16, which is taken along with the halves: products with odd numbers (the fractions of
 // the golden ratio, of e and of 2 e as words) between shifts
@@ -193,10 +215,10 @@ constexpr unsigned kPlaceStep = 0x9e3779b9u;
 static __device__ __forceinline__ unsigned mean_noise(unsigned h) { return ((h << 4) ^ (h >> 12)) & 0xffff0u; }     // 16 bits below 2^kMeanShift
 static __device__ __forceinline__ unsigned root_noise(unsigned h) { return (h >> 13) & 0x7fff8u; }                  // and below 2^kRootShift
 static __device__ __forceinline__ unsigned step_key(unsigned seed, unsigned step, unsigned number) { return (seed ^ step * kPlaceStep) + number * 0x6a09e667u; }
-// The larger of two, a NaN being the largest.
-static __device__ __forceinline__ float larger(float a, float b) {
+// The larger size of two values, with a sign that says nothing; a NaN is the largest.
+static __device__ __forceinline__ float larger_size(float a, float b) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 static __device__ __forceinline__ float warp_largest(float v) {
@@ -206,16 +228,14 @@ static __device__ __forceinline__ float warp_largest(float v) {
 }
 // Four values of a warp's 256: those from 4 lane on, in either half.
 static __device__ __forceinline__ void load_four(float (&v)[4], const float *p, int n, bool vec) {
-  if (vec) {
-    const float4 q = *reinterpret_cast<const float4 *>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
+  if (vec) load_four(v, p);
+  else {
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = j < n ? p[j] : 0.f;
   }
 }
 static __device__ __forceinline__ void store_four(float *p, const float (&v)[4], int n, bool vec) {
-  if (vec) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  if (vec) store_four(p, v);
   else {
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -230,7 +250,17 @@ static __device__ __forceinline__ unsigned codes_of(const unsigned *codes, int h
   if (left < 4) q = left > 0 ? q & ((1u << (8 * left)) - 1) : 0;
   return q;
 }
-// A warp for a block of 256 values, eight a lane.
+// Brings what a warp reads of a block to L2, 20 lines.
+static __device__ __forceinline__ void bring(const AdamTensor &a, long block, int lane) {
+  if (lane >= 20 || (block + 1) * kAdamBlock > a.n) return;
+  const char *line = lane < 8 ? (const char *)(a.w + block * kAdamBlock) + lane * 128 : lane < 16 ? (const char *)(a.g + block * kAdamBlock) + (lane - 8) * 128 :
+                     lane < 18 ? (const char *)((const unsigned *)a.m + block * 64) + (lane - 16) * 128 : (const char *)((const unsigned *)a.v + block * 64) + (lane - 18) * 128;
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+}
+// A warp for a block of 256 values, eight a lane; a block looks a tensor up for four turns of 2048.  46 M values: 143 us, 5.2 TB/s; what holds it back is the work on
+// codes, 73 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the codes and branch.
+// Blocks stay, four an SM with 64 registers: a block for each chunk takes 156 us, five blocks an SM in 48 registers 150 (170 with what is brought ahead), a turn's loads in
+// registers ahead of it 178, and nothing brought ahead 158.
 template <int N>
 static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
@@ -240,115 +270,138 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
   const AdamFactors f = shared;
   const unsigned chunks = table.first[table.count];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long jump = 8l * table.turns * gridDim.x - 8l * (table.turns - 1);      // from the last block of a turn to the first of the next chunk
   for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int i = tensor_of(table, chunk);
     const AdamTensor &a = table.t[i];
-    const long block = (chunk - table.first[i]) * (long)(kAdamChunk / kAdamBlock) + warp, from = block * kAdamBlock;
-    if (from >= a.n) continue;
-    const int n = (int)min((long)kAdamBlock, a.n - from);
-    float *w = a.w + from;
-    const float *g = a.g + from;
-    unsigned *mc = (unsigned *)a.m + block * 64, *rc = (unsigned *)a.v + block * 64;
-    const bool whole = n == kAdamBlock, vw = whole && ((uintptr_t)w & 15) == 0, vg = whole && ((uintptr_t)g & 15) == 0;
-    float m[2][4], r[2][4], ww[2][4];
-    unsigned mq[2], rq[2];
-    const float2 scale = *reinterpret_cast<const float2 *>(a.scales + 2 * block);
+    long block = (chunk - table.first[i]) * (long)(kAdamTurn / kAdamBlock * table.turns) + warp;
+    for (int turn = 0; turn < table.turns && block * kAdamBlock < a.n; turn++, block += kAdamTurn / kAdamBlock) {
+      const long from = block * kAdamBlock;
+      const int n = (int)min((long)kAdamBlock, a.n - from);
+      float *w = a.w + from;
+      const float *g = a.g + from;
+      unsigned *mc = (unsigned *)a.m + block * 64, *rc = (unsigned *)a.v + block * 64;
+      const bool whole = n == kAdamBlock, vw = whole && ((uintptr_t)w & 15) == 0, vg = whole && ((uintptr_t)g & 15) == 0;
+      float m[2][4], r[2][4], ww[2][4];
+      unsigned mq[2], rq[2];
+      const float2 scale = *reinterpret_cast<const float2 *>(a.scales + 2 * block);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int at = h * 128 + lane * 4;
-      load_four(m[h], g + at, n - at, vg);
-      load_four(ww[h], w + at, n - at, vw);
-      mq[h] = codes_of(mc, h, lane, n);
-      rq[h] = codes_of(rc, h, lane, n);
-    }
-    float top_m = 0.f, top_r = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float gj = m[h][j];
-        const float was = code_value(mq[h] >> (8 * j) & 127u, kMeanShift, scale.x), root = code_value(rq[h] >> (8 * j) & 255u, kRootShift, scale.y);
-        const float sign = __uint_as_float(__float_as_uint(was) ^ (mq[h] << (24 - 8 * j) & 0x80000000u));
-        m[h][j] = __fadd_rn(__fmul_rn(s.beta1, sign), __fmul_rn(s.rest1, gj));
-        r[h][j] = __fsqrt_rn(__fadd_rn(__fmul_rn(s.beta2, __fmul_rn(root, root)), __fmul_rn(s.rest2, __fmul_rn(gj, gj))));
-        top_m = larger(top_m, fabsf(m[h][j]));
-        top_r = larger(top_r, r[h][j]);
-        ww[h][j] = adam_weight(ww[h][j], m[h][j], r[h][j], s, f);
+      for (int h = 0; h < 2; h++) {
+        const int at = h * 128 + lane * 4;
+        load_four(m[h], g + at, n - at, vg);
+        load_four(ww[h], w + at, n - at, vw);
+        mq[h] = codes_of(mc, h, lane, n);
+        rq[h] = codes_of(rc, h, lane, n);
       }
-      store_four(w + h * 128 + lane * 4, ww[h], n - (h * 128 + lane * 4), vw);
-    }
-    top_m = warp_largest(top_m);
-    top_r = warp_largest(top_r);
-    // (a NaN stays one, and makes the block's values NaN)
-    float scale_m = __fmul_rn(top_m, 1.f / kMeanTop), scale_r = __fmul_rn(top_r, 1.f / kRootTop);
-    if (scale_m < 0x1p-126f) scale_m = 0.f;
-    if (scale_r < 0x1p-126f) scale_r = 0.f;
-    const float inverse_m = scale_m == 0.f ? 0.f : __fdiv_rn(1.f, scale_m), inverse_r = scale_r == 0.f ? 0.f : __fdiv_rn(1.f, scale_r);
-    const unsigned key = step_key(s.seed, f.step, (unsigned)(s.number + i)) + (unsigned)(from + lane * 4) * kPlaceStep;
+      bring(a, block + (turn + 1 < table.turns ? 8 : jump), lane);
+      float top_m = 0.f, top_r = 0.f;
+      const Pair scale_m2(scale.x, scale.x), scale_r2(scale.y, scale.y), beta1(s.beta1, s.beta1), beta2(s.beta2, s.beta2), rest1(s.rest1, s.rest1), rest2(s.rest2, s.rest2);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      mq[h] = rq[h] = 0;
+      for (int h = 0; h < 2; h++) {
+        const unsigned sizes = mq[h] & 0x7f7f7f7fu;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {                       // (zeros, those behind the values among them, have the code zero whatever the noise)
-        const unsigned bits = place_bits(key + (unsigned)(h * 128 + j) * kPlaceStep);
-        const unsigned cm = value_code(fabsf(m[h][j]), inverse_m, kMeanShift, mean_noise(bits), 127u) + (m[h][j] < 0.f ? 128u : 0u);
-        mq[h] += cm << (8 * j);
-        rq[h] += value_code(r[h][j], inverse_r, kRootShift, root_noise(bits), 255u) << (8 * j);
+        for (int j = 0; j < 4; j += 2) {
+          const Pair gj(m[h][j], m[h][j + 1]), root = code_pair(rq[h], j, kRootShift, scale_r2);
+          float x, y;
+          code_pair(sizes, j, kMeanShift, scale_m2).get(x, y);
+          x = __uint_as_float(__float_as_uint(x) ^ (mq[h] << (24 - 8 * j) & 0x80000000u));
+          y = __uint_as_float(__float_as_uint(y) ^ (mq[h] << (16 - 8 * j) & 0x80000000u));
+          add_singly(beta1 * Pair(x, y), rest1 * gj, m[h][j], m[h][j + 1]);
+          add_singly(beta2 * (root * root), rest2 * (gj * gj), x, y);
+          r[h][j] = __fsqrt_rn(x);
+          r[h][j + 1] = __fsqrt_rn(y);
+          top_m = larger_size(larger_size(top_m, m[h][j]), m[h][j + 1]);
+          top_r = larger_size(larger_size(top_r, r[h][j]), r[h][j + 1]);
+          // the weights' step, as adam_weight
+          fused(Pair(r[h][j], r[h][j + 1]), Pair(f.root, f.root), Pair(s.eps, s.eps)).get(x, y);
+          fused(Pair(-f.rate, -f.rate), Pair(m[h][j], m[h][j + 1]) * Pair(reciprocal(x), reciprocal(y)), Pair(ww[h][j], ww[h][j + 1]) * Pair(s.keep, s.keep))
+              .get(ww[h][j], ww[h][j + 1]);
+        }
+        store_four(w + h * 128 + lane * 4, ww[h], n - (h * 128 + lane * 4), vw);
       }
-      mc[h * 32 + lane] = mq[h];
-      rc[h * 32 + lane] = rq[h];
+      top_m = warp_largest(fabsf(top_m));
+      top_r = warp_largest(fabsf(top_r));
+      // (a NaN stays one, and makes the block's values NaN)
+      float scale_m = __fmul_rn(top_m, 1.f / kMeanTop), scale_r = __fmul_rn(top_r, 1.f / kRootTop);
+      if (scale_m < 0x1p-126f) scale_m = 0.f;
+      if (scale_r < 0x1p-126f) scale_r = 0.f;
+      const float by_m = scale_m == 0.f ? 0.f : __frcp_rn(scale_m), by_r = scale_r == 0.f ? 0.f : __frcp_rn(scale_r);
+      const unsigned key = step_key(s.seed, f.step, (unsigned)(s.number + i)) + (unsigned)(from + lane * 4) * kPlaceStep;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        mq[h] = rq[h] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {                       // (zeros, those behind the values among them, have the code zero whatever the noise)
+          float x[2], y[2];
+          (Pair(fabsf(m[h][j]), fabsf(m[h][j + 1])) * Pair(by_m, by_m)).get(x[0], x[1]);
+          (Pair(r[h][j], r[h][j + 1]) * Pair(by_r, by_r)).get(y[0], y[1]);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const unsigned bits = place_bits(key + (unsigned)(h * 128 + j + e) * kPlaceStep);
+            mq[h] += (value_code(x[e], kMeanShift, mean_noise(bits)) + (m[h][j + e] < 0.f ? 128u : 0u)) << (8 * (j + e));
+            rq[h] += value_code(y[e], kRootShift, root_noise(bits)) << (8 * (j + e));
+          }
+        }
+        mc[h * 32 + lane] = mq[h];
+        rc[h * 32 + lane] = rq[h];
+      }
+      if (lane == 0) *reinterpret_cast<float2 *>(a.scales + 2 * block) = make_float2(scale_m, scale_r);
     }
-    if (lane == 0) *reinterpret_cast<float2 *>(a.scales + 2 * block) = make_float2(scale_m, scale_r);
   }
   adam_count(s, f.step);
 }
 
-// What the codes stand for: m into w, v into g's place (named as the table's weights and gradients).
+// What the codes stand for: m into w, v into g's place (named as the table's weights and gradients).  46 M values: 73 us, 6.4 TB/s.
 template <int N>
 static __global__ void __launch_bounds__(256) adam8_moments_kernel(const __grid_constant__ AdamTable<N> table) {
   pdl_begin();
-  const unsigned chunks = table.first[table.count];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int i = tensor_of(table, chunk);
-    const AdamTensor &a = table.t[i];
-    const long block = (chunk - table.first[i]) * (long)(kAdamChunk / kAdamBlock) + warp, from = block * kAdamBlock;
-    if (from >= a.n) continue;
-    const int n = (int)min((long)kAdamBlock, a.n - from);
-    float *mean = a.w + from, *square = const_cast<float *>(a.g) + from;
-    const unsigned *mc = (const unsigned *)a.m + block * 64, *rc = (const unsigned *)a.v + block * 64;
-    const bool whole = n == kAdamBlock, vm = whole && ((uintptr_t)mean & 15) == 0, vs = whole && ((uintptr_t)square & 15) == 0;
-    const float2 scale = *reinterpret_cast<const float2 *>(a.scales + 2 * block);
+  const int i = tensor_of(table, blockIdx.x), lane = threadIdx.x & 31;
+  const AdamTensor &a = table.t[i];
+  const long block = (blockIdx.x - table.first[i]) * (long)(kAdamTurn / kAdamBlock) + (threadIdx.x >> 5), from = block * kAdamBlock;
+  if (from >= a.n) return;
+  const float2 scale = *reinterpret_cast<const float2 *>(a.scales + 2 * block);
+  unsigned mq[2], rq[2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const unsigned mq = mc[h * 32 + lane], rq = rc[h * 32 + lane];
-      const int at = h * 128 + lane * 4;
-      float m[4], v[4];
+  for (int h = 0; h < 2; h++) {
+    mq[h] = ((const unsigned *)a.m)[block * 64 + h * 32 + lane];
+    rq[h] = ((const unsigned *)a.v)[block * 64 + h * 32 + lane];
+  }
+  const int n = (int)min((long)kAdamBlock, a.n - from);
+  float *mean = a.w + from, *square = const_cast<float *>(a.g) + from;
+  const bool whole = n == kAdamBlock, vm = whole && ((uintptr_t)mean & 15) == 0, vs = whole && ((uintptr_t)square & 15) == 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const unsigned cm = mq >> (8 * j) & 255u;
-        const float value = code_value(cm & 127u, kMeanShift, scale.x), root = code_value(rq >> (8 * j) & 255u, kRootShift, scale.y);
-        m[j] = cm & 128u ? -value : value;
-        v[j] = __fmul_rn(root, root);
-      }
-      store_four(mean + at, m, n - at, vm);
-      store_four(square + at, v, n - at, vs);
+  for (int h = 0; h < 2; h++) {
+    const int at = h * 128 + lane * 4;
+    float m[4], v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const Pair root = code_pair(rq[h], j, kRootShift, Pair(scale.y, scale.y));
+      (root * root).get(v[j], v[j + 1]);
+      code_pair(mq[h] & 0x7f7f7f7fu, j, kMeanShift, Pair(scale.x, scale.x)).get(m[j], m[j + 1]);
     }
+#pragma unroll
+    for (int j = 0; j < 4; j++) m[j] = __uint_as_float(__float_as_uint(m[j]) ^ (mq[h] << (24 - 8 * j) & 0x80000000u));
+    store_four(mean + at, m, n - at, vm);
+    store_four(square + at, v, n - at, vs);
   }
 }
 
 // ---- launches
 enum AdamKind { kAdam32, kAdam8, kAdamMoments };
 template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTensor> &all, const AdamStep &step) {
+  long total = 0;
+  for (const AdamTensor &t : all) total += t.n;
   size_t i = 0;
   do {
     AdamTable<N> table;
+    table.turns = kind == kAdam8 && total >= (long)kAdamTurn * kAdamTurns * 16 * ctx().sm_count ? kAdamTurns : 1;
+    const long per = (long)kAdamTurn * table.turns;
     AdamStep s = step;
     s.number = (int)i;
     table.count = 0;
     table.first[0] = 0;
     for (; i < all.size() && table.count < N; i++) {
-      const long chunks = (all[i].n + kAdamChunk - 1) / kAdamChunk;
+      const long chunks = (all[i].n + per - 1) / per;
       THC_CHECK(chunks < (1l << 31), "tensors of more than 2^42 values");
       if (table.count && table.first[table.count] + (unsigned long)chunks >= (1ul << 31)) break;
       table.t[table.count] = all[i];
@@ -356,7 +409,7 @@ template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTe
       table.count++;
     }
     s.last = i == all.size();
-    const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, kind == kAdamMoments ? 1u << 30 : (unsigned)ctx().sm_count * 4));
+    const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, kind == kAdam8 ? (unsigned)ctx().sm_count * 4 : 1u << 31));
     if (kind == kAdam32) pdl_launch(adam_kernel<N>, blocks, 256, 0, table, s);
     else if (kind == kAdam8) pdl_launch(adam8_kernel<N>, blocks, 256, 0, table, s);
     else pdl_launch(adam8_moments_kernel<N>, blocks, 256, 0, table);
@@ -398,9 +451,24 @@ class Spans {
   };
   std::vector<Span> spans_;
 };
-static void check_flat(const THGPUTensor *t, long n, int argn, int i, const char *what) {
-  if (!t || nelem(t) != n || !is_contiguous(t)) fail("Invalid argument %d: contiguous %s of %ld values expected for tensor %d", argn, what, n, i + 1);
-}
+// A tensor of the call, contiguous, of n values (-1: of any number), of this device; called for every tensor, some hundreds a step.
+class Flat {
+ public:
+  float *operator()(const THGPUTensor *t, long n, int argn, int i, const char *what) const {
+    if (!t) fail("Invalid argument %d: tensors expected", argn);
+    const long k = t->nDimension == 1 ? t->size[0] : nelem(t);
+    if ((n >= 0 && k != n) || !((t->nDimension == 1 && t->stride[0] == 1) || is_contiguous(t)))
+      fail("Invalid argument %d: contiguous %s of %ld values expected for tensor %d", argn, what, n >= 0 ? n : k, i + 1);
+    if (!t->storage) return nullptr;
+    const long tag = (long)(intptr_t)t->storage->allocatorContext;
+    if (tag > 0 && tag != here_) fail("Invalid argument %d: tensor of device %ld while device %ld is current", argn, tag, here_);
+    return data_ptr(t);
+  }
+
+ private:
+  const long here_ = std::max(device_if_initialised(), 0) + 1;      // (as check_here)
+};
+static long values_of(const THGPUTensor *t) { return !t ? 0 : t->nDimension == 1 ? t->size[0] : nelem(t); }
 static void add_codes(Spans &spans, const std::vector<AdamTensor> &all, bool codes_written, bool g_written) {
   auto blocks = [](const AdamTensor &t) { return (t.n + kAdamBlock - 1) / kAdamBlock; };
   for (const AdamTensor &t : all) spans.add(t.w, t.n, true);
@@ -437,22 +505,20 @@ THC_API int THGPUNN_AdamW_update(int n, THGPUTensor **weights, THGPUTensor **gra
   THC_BEGIN
   THC_ARG(n >= 0, 1, "a number of tensors expected");
   THC_ARG(n == 0 || (weights && grads && means && squares), 2, "tensors expected");
-  check_flat(step, 2, 6, 0, "step");
+  const Flat flat;
+  flat(step, 2, 6, 0, "step");
   check_rates(lr, beta1, beta2, eps, decay, 7);
-  check_here({nullptr, nullptr, nullptr, nullptr, nullptr, step});
   Spans spans;
   spans.add(data_ptr(step), 2, true);
-  std::vector<AdamTensor> all;
-  all.reserve(n);
+  std::vector<AdamTensor> all(n);
   for (int i = 0; i < n; i++) {
-    THC_ARG(weights[i], 2, "tensors expected");
-    const long k = nelem(weights[i]);
-    check_flat(weights[i], k, 2, i, "weights");
-    check_flat(grads[i], k, 3, i, "gradients");
-    check_flat(means[i], k, 4, i, "means");
-    check_flat(squares[i], k, 5, i, "squares");
-    check_here({nullptr, weights[i], grads[i], means[i], squares[i]});
-    all.push_back(AdamTensor{data_ptr(weights[i]), data_ptr(grads[i]), data_ptr(means[i]), data_ptr(squares[i]), nullptr, k});
+    AdamTensor &t = all[i];
+    t.w = flat(weights[i], -1, 2, i, "weights");
+    t.n = values_of(weights[i]);
+    t.g = flat(grads[i], t.n, 3, i, "gradients");
+    t.m = flat(means[i], t.n, 4, i, "means");
+    t.v = flat(squares[i], t.n, 5, i, "squares");
+    t.scales = nullptr;
   }
   for (const AdamTensor &t : all) spans.add(t.w, t.n, true);
   for (const AdamTensor &t : all) spans.add(t.g, t.n, false);
@@ -469,24 +535,22 @@ THC_API int THGPUNN_AdamW8_update(int n, THGPUTensor **weights, THGPUTensor **gr
   THC_BEGIN
   THC_ARG(n >= 0, 1, "a number of tensors expected");
   THC_ARG(n == 0 || (weights && grads && meanCodes && rootCodes && scales), 2, "tensors expected");
-  check_flat(step, 2, 7, 0, "step");
+  const Flat flat;
+  flat(step, 2, 7, 0, "step");
   check_rates(lr, beta1, beta2, eps, decay, 8);
-  check_here({nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, step});
   Spans spans;
   spans.add(data_ptr(step), 2, true);
-  std::vector<AdamTensor> all;
-  all.reserve(n);
+  std::vector<AdamTensor> all(n);
   for (int i = 0; i < n; i++) {
-    THC_ARG(weights[i], 2, "tensors expected");
-    const long k = nelem(weights[i]), blocks = (k + kAdamBlock - 1) / kAdamBlock;
-    check_flat(weights[i], k, 2, i, "weights");
-    check_flat(grads[i], k, 3, i, "gradients");
-    check_flat(meanCodes[i], 64 * blocks, 4, i, "codes of means");
-    check_flat(rootCodes[i], 64 * blocks, 5, i, "codes of roots");
-    check_flat(scales[i], 2 * blocks, 6, i, "scales");
-    check_here({nullptr, weights[i], grads[i], meanCodes[i], rootCodes[i], scales[i]});
-    all.push_back(AdamTensor{data_ptr(weights[i]), data_ptr(grads[i]), data_ptr(meanCodes[i]), data_ptr(rootCodes[i]), data_ptr(scales[i]), k});
-    THC_ARG(((uintptr_t)all[i].scales & 7) == 0, 6, "scales on a boundary of 8 bytes expected");
+    AdamTensor &t = all[i];
+    t.w = flat(weights[i], -1, 2, i, "weights");
+    t.n = values_of(weights[i]);
+    const long blocks = (t.n + kAdamBlock - 1) / kAdamBlock;
+    t.g = flat(grads[i], t.n, 3, i, "gradients");
+    t.m = flat(meanCodes[i], 64 * blocks, 4, i, "codes of means");
+    t.v = flat(rootCodes[i], 64 * blocks, 5, i, "codes of roots");
+    t.scales = flat(scales[i], 2 * blocks, 6, i, "scales");
+    THC_ARG(((uintptr_t)t.scales & 7) == 0, 6, "scales on a boundary of 8 bytes expected");
   }
   add_codes(spans, all, true, false);
   spans.check();
@@ -499,20 +563,19 @@ THC_API int THGPUNN_AdamW8_moments(int n, THGPUTensor **meanCodes, THGPUTensor *
   THC_BEGIN
   THC_ARG(n >= 0, 1, "a number of tensors expected");
   THC_ARG(n == 0 || (meanCodes && rootCodes && scales && means && squares), 2, "tensors expected");
+  const Flat flat;
   Spans spans;
-  std::vector<AdamTensor> all;
-  all.reserve(n);
+  std::vector<AdamTensor> all(n);
   for (int i = 0; i < n; i++) {
-    THC_ARG(means[i], 5, "tensors expected");
-    const long k = nelem(means[i]), blocks = (k + kAdamBlock - 1) / kAdamBlock;
-    check_flat(means[i], k, 5, i, "means");
-    check_flat(squares[i], k, 6, i, "squares");
-    check_flat(meanCodes[i], 64 * blocks, 2, i, "codes of means");
-    check_flat(rootCodes[i], 64 * blocks, 3, i, "codes of roots");
-    check_flat(scales[i], 2 * blocks, 4, i, "scales");
-    check_here({nullptr, meanCodes[i], rootCodes[i], scales[i], means[i], squares[i]});
-    all.push_back(AdamTensor{data_ptr(means[i]), data_ptr(squares[i]), data_ptr(meanCodes[i]), data_ptr(rootCodes[i]), data_ptr(scales[i]), k});
-    THC_ARG(((uintptr_t)all[i].scales & 7) == 0, 4, "scales on a boundary of 8 bytes expected");
+    AdamTensor &t = all[i];
+    t.n = values_of(means[i]);
+    const long blocks = (t.n + kAdamBlock - 1) / kAdamBlock;
+    t.m = flat(meanCodes[i], 64 * blocks, 2, i, "codes of means");
+    t.v = flat(rootCodes[i], 64 * blocks, 3, i, "codes of roots");
+    t.scales = flat(scales[i], 2 * blocks, 4, i, "scales");
+    t.w = flat(means[i], -1, 5, i, "means");
+    t.g = flat(squares[i], t.n, 6, i, "squares");
+    THC_ARG(((uintptr_t)t.scales & 7) == 0, 4, "scales on a boundary of 8 bytes expected");
   }
   add_codes(spans, all, false, true);
   spans.check();

@@ -319,34 +319,49 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
   const long t = Cols::token();
   const int team = threadIdx.x / T, warp = threadIdx.x % T / 32, lane = threadIdx.x & 31, pieces = (D + T * U * Cols::W - 1) / (T * U * Cols::W);
   const bool live = t < tokens;
+  constexpr int B = U * Cols::W <= 4 ? 4 : 2;      // rows on their way at once
   Cols g(0);
   if (live && pieces == 1) g.load(dy.p + t * dy.ld, D);
   for (int i0 = 0; i0 < k; i0 += kDotSlots) {
     const int n = min(kDotSlots, k - i0);
-    for (int i = 0; live && i < n; i++) {
-      const long r = row_at(__ldg(positions + t * k + i0 + i), most);
-      float dot = 0.f;
-      if (r >= 0) {
-        const float f = w ? __ldg(w + t * k + i0 + i) : 1.f;
-        for (int p = 0; p < pieces; p++) {
-          Cols b(p), o(p);
-          if (dw) b.load(rows.p + r * rows.ld, D);
-          if (pieces > 1) {
-            g.c = b.c;
-            g.load(dy.p + t * dy.ld, D);
-          }
+    for (int i = 0; live && i < n; i += B) {
+      long r[B];
+      float f[B], dot[B];
+#pragma unroll
+      for (int b = 0; b < B; b++) {
+        const long slot = t * k + i0 + i + b;
+        r[b] = i + b < n ? row_at(__ldg(positions + slot), most) : -1;
+        f[b] = r[b] < 0 ? 0.f : w ? __ldg(w + slot) : 1.f;
+        dot[b] = 0.f;
+      }
+      for (int p = 0; p < pieces; p++) {
+        Cols row[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+          row[b] = Cols(p);
+          row[b].zero();
+          if (dw && r[b] >= 0) row[b].load(rows.p + r[b] * rows.ld, D);
+        }
+        if (pieces > 1) {
+          g = Cols(p);
+          g.load(dy.p + t * dy.ld, D);
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++) {
 #pragma unroll
           for (int j = 0; j < U * Cols::W; j++) {
-            if (dw) dot = fmaf(g.v[j], b.v[j], dot);
-            o.v[j] = f * g.v[j];
+            dot[b] = fmaf(row[b].v[j], g.v[j], dot[b]);
+            row[b].v[j] = f[b] * g.v[j];
           }
-          if (drows) o.store(drows + r * D, D);
+          if (drows && r[b] >= 0) row[b].store(drows + r[b] * D, D);
         }
       }
-      if (dw) {
+      if (!dw) continue;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (lane == 0) dots[team][warp][i] = dot;
+      for (int b = 0; b < B; b++) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], o);
+        if (lane == 0 && i + b < n) dots[team][warp][i + b] = r[b] < 0 ? 0.f : dot[b];     // (0 times a NaN of gradOutput)
       }
     }
     if (!dw) continue;
@@ -381,7 +396,7 @@ template <class F> static void with_columns(long tokens, int D, bool vec, bool w
     else if (team == 128) f(std::integral_constant<int, 128>(), U, VEC);
     else f(std::integral_constant<int, 256>(), U, VEC);
   };
-  const bool few = !whole && tokens * (long)D < ctx().sm_count * 4096l;
+  const bool few = !whole && tokens * (long)D <= ctx().sm_count * (vec ? 8192l : 2048l);
   auto with_u = [&](auto VEC) {
     if (few) go(VEC, std::integral_constant<int, 1>());
     else go(VEC, std::integral_constant<int, 4>());

@@ -97,39 +97,48 @@ template <int V> static __device__ __forceinline__ Chosen choose_in_turn(const f
 constexpr int kFewChosen = 16;      // 22 scores are left on average, at 20 they are 31
 struct Candidates {
   float score[32];
-  int expert[32];
+  unsigned short place[32];
 };
 template <int V> static __device__ __forceinline__ bool choose_at_once(const float (&v)[V], float most, float top, Candidates &left, int lane, int k, Chosen &c) {
   float bound = top;
-  for (int i = 1; i < k; i++) {
+  auto next = [&] {
     most = most == bound ? -INFINITY : most;
     bound = warp_max(most);
-  }
+  };
+  int rounds = k - 1;
+  for (; rounds >= 4; rounds -= 4) { next(); next(); next(); next(); }
+  for (; rounds > 0; rounds--) next();
   bound = fmaxf(bound, -3.402823466e+38f);      // (an open score)
+  unsigned in[V];
   int n = 0;
 #pragma unroll
   for (int j = 0; j < V; j++) {
-    const bool in = v[j] >= bound;
-    const unsigned all = __ballot_sync(0xffffffffu, in);
-    const int at = n + __popc(all & ((1u << lane) - 1));
-    if (in && at < 32) {
-      left.score[at] = v[j];
-      left.expert[at] = j * 32 + lane + 1;
-    }
-    n += __popc(all);
+    in[j] = __ballot_sync(0xffffffffu, v[j] >= bound);
+    n += __popc(in[j]);
   }
   if (n > 32) return false;
+  left.score[lane] = -INFINITY;                 // behind the last one
   __syncwarp();
-  c = Chosen{-INFINITY, 0, lane};
-  if (lane < n) {
-    c.score = left.score[lane];
-    c.slot = 0;
+  const unsigned lower = (1u << lane) - 1;
+  n = 0;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    const int at = n + __popc(in[j] & lower);
+    if (v[j] >= bound) {
+      left.score[at] = v[j];
+      left.place[at] = (unsigned short)(j * 32 + lane);
+    }
+    n += __popc(in[j]);
   }
-  for (int i = 0; i < n; i++) {
-    const float o = left.score[i];
-    if (lane < n) c.slot += o > c.score || (o == c.score && i < lane);
+  __syncwarp();
+  // the place of a score among all: how many are larger, or as large and before it
+  c = Chosen{left.score[lane] + 0.f, 0, 0};     // (both zeros alike)
+  for (int i = 0; i < n; i += 4) {
+    const float4 o = *reinterpret_cast<const float4 *>(&left.score[i]);
+    c.slot += (o.x > c.score) + (o.y > c.score) + (o.z > c.score) + (o.w > c.score);
   }
-  if (lane < n && c.slot < k) c.expert = left.expert[lane];
+  c.slot += __popc(__match_any_sync(0xffffffffu, __float_as_uint(c.score)) & lower);
+  if (lane < n && c.slot < k) c.expert = left.place[lane] + 1;
   return true;
 }
 
@@ -137,12 +146,19 @@ template <int V>
 static __global__ void __launch_bounds__(256) router_forward_kernel(const float *__restrict__ x, long ld, float *__restrict__ weights, float *__restrict__ experts,
                                                                     long rows, int E, int k, bool normalize) {
   pdl_begin();
-  __shared__ Candidates left[V >= 4 ? 8 : 1];
+  __shared__ __align__(16) Candidates left[V >= 4 ? 8 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long row = blockIdx.x * 8l + warp;
   if (row >= rows) return;
   float v[V];
-  WarpRow<V, false>::load(x + row * ld, lane, E, v);
+  const float *mine = x + row * ld + lane;
+  if (E == 32 * V) {
+#pragma unroll
+    for (int j = 0; j < V; j++) v[j] = __ldg(mine + j * 32);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j++) v[j] = j * 32 + lane < E ? __ldg(mine + j * 32) : -INFINITY;
+  }
   float most = v[0];
 #pragma unroll
   for (int j = 1; j < V; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(v[j]));
