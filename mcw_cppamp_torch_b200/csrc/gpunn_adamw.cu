@@ -47,11 +47,12 @@ struct AdamStep {
   float *step;               // steps taken, and the count of blocks that are done (zero between launches)
   bool last;                 // the launch that counts the step
   float lr, beta1, beta2, rest1, rest2, eps, keep;    // rest: 1 - beta, keep: 1 - lr decay
-  double b1, b2;
+  float log1, log2;          // of the betas
   unsigned seed;
   int number;                // of the table's first tensor
 };
-// What a step's number decides: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).  1 - b^t loses a float's digits for small t: in 64 bits.
+// What a step's number t decides: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).  1 - b^t = -expm1(t log b): t log b carries its rounding to the result at most as it is,
+// where a power of b near one would lose it.
 struct AdamFactors {
   float rate, root;
   unsigned step;
@@ -59,22 +60,19 @@ struct AdamFactors {
 // By threads 0 and 1 into shared memory; a barrier has to follow.
 static __device__ __forceinline__ void adam_factors(const AdamStep &s, AdamFactors &f) {
   if (threadIdx.x > 1) return;
-  const unsigned step = (unsigned)s.step[0] + 1;
-  double b = threadIdx.x ? s.b2 : s.b1, p = 1.0;
-  for (unsigned t = step; t; t >>= 1, b *= b)
-    if (t & 1) p *= b;
+  const float step = truncf(s.step[0]) + 1.f, rest = -expm1f(step * (threadIdx.x ? s.log2 : s.log1));
   if (threadIdx.x == 0) {
-    f.rate = (float)(s.lr / (1.0 - p));
-    f.step = step;
-  } else f.root = (float)(1.0 / sqrt(1.0 - p));
+    f.rate = s.lr / rest;
+    f.step = (unsigned)step;
+  } else f.root = 1.f / sqrtf(rest);
 }
-// The last block of the last launch counts the step: by then every block has read its number.
+// The last block of the last launch counts the step: by then every block has read, and used, its number.  Nothing else passes between blocks here, so that there is
+// no fence to wait for.
 static __device__ __forceinline__ void adam_count(const AdamStep &s, unsigned step) {
   if (!s.last) return;
   __syncthreads();
   if (threadIdx.x != 0) return;
   unsigned *done = reinterpret_cast<unsigned *>(s.step + 1);
-  __threadfence();
   if (atomicAdd(done, 1u) == gridDim.x - 1) {
     s.step[0] = (float)step;
     *done = 0;
@@ -490,7 +488,7 @@ static AdamStep adam_step(THGPUTensor *step, double lr, double beta1, double bet
   s.last = false;
   s.lr = (float)lr; s.beta1 = (float)beta1; s.beta2 = (float)beta2; s.rest1 = (float)(1.0 - beta1); s.rest2 = (float)(1.0 - beta2);
   s.eps = (float)eps; s.keep = (float)(1.0 - lr * decay);
-  s.b1 = beta1; s.b2 = beta2;
+  s.log1 = (float)std::log(beta1); s.log2 = (float)std::log(beta2);      // (of zero: minus infinity, and then 1 - b^t is one)
   s.seed = (unsigned)(unsigned long)seed;
   s.number = 0;
   return s;

@@ -144,21 +144,38 @@ static __global__ void __launch_bounds__(1024) slots_rank_kernel(const float *__
   const bool leads = lane == __ffs(same) - 1;
   if (leads && e > 0) ahead[warp * groups + e - 1] = __popc(same);
   if (leads && e < 0) atomicAdd(&wrong, __popc(same));
+  // the others' four at a time, of one block each
+  const bool whole = ((uintptr_t)experts & 15) == 0;
 #pragma unroll 4
-  for (int s0 = 0; s0 < slots; s0 += 1024) {
-    if (s0 == from) continue;
-    const int s = s0 + t, x = s < slots ? slot_expert(experts[s], groups) : 0;
-    if (x > 0) atomicAdd(&(s0 < from ? before : after)[x - 1], 1);
-    else if (x < 0) atomicAdd(&wrong, 1);
+  for (int s = 4 * t; s < slots; s += 4096) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (whole && s + 4 <= slots) {
+      const float4 q = __ldg(reinterpret_cast<const float4 *>(experts + s));
+      x[0] = q.x; x[1] = q.y; x[2] = q.z; x[3] = q.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (s + j < slots) x[j] = __ldg(experts + s + j);
+    }
+    if (s >= from && s < from + 1024) continue;
+    int *count = s < from ? before : after;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int o = slot_expert(x[j], groups);
+      if (o > 0) atomicAdd(&count[o - 1], 1);
+      else if (o < 0) atomicAdd(&wrong, 1);
+    }
   }
   __syncthreads();
   int total = 0;                                                  // thread g: group g, at most 1024 of them
   if (t < groups) {
-    int at = before[t];
+    int n[32], at = before[t];
+#pragma unroll
+    for (int w = 0; w < 32; w++) n[w] = ahead[w * groups + t];
+#pragma unroll
     for (int w = 0; w < 32; w++) {
-      const int n = ahead[w * groups + t];
       ahead[w * groups + t] = at;
-      at += n;
+      at += n[w];
     }
     total = at + after[t];
     if (blockIdx.x == 0) count_deliver(tell, t, total);
@@ -172,8 +189,7 @@ static __global__ void __launch_bounds__(1024) slots_rank_kernel(const float *__
   }
   if (lane == 31) sums[warp] = run;
   __syncthreads();
-  int base = run - total;
-  for (int w = 0; w < warp; w++) base += sums[w];
+  const int base = run - total + __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0);
   if (t < groups) before[t] = base;
   __syncthreads();
   if (mine < slots) positions[mine] = e > 0 ? (float)(before[e - 1] + ahead[warp * groups + e - 1] + __popc(same & ((1u << lane) - 1)) + 1) : 0.f;
@@ -204,6 +220,14 @@ template <int T, int U, bool VEC> struct Columns {
       } else v[u] = at < n ? __ldg(row + at) : 0.f;
     }
   }
+  // to L2, a lane for each line
+  __device__ __forceinline__ void bring(const float *row, int n) const {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = c + u * T * W;
+      if (at < n && (threadIdx.x * W) % 32 == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + at));
+    }
+  }
   __device__ __forceinline__ void store(float *__restrict__ row, int n) const {
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -223,11 +247,12 @@ struct Rows {            // a matrix of rows at a distance
 // rows[pos(t, i)] = x[t]
 template <int T, int U, bool VEC>
 static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const float *__restrict__ positions, float *__restrict__ rows, long tokens, int k, int D, long most) {
-  pdl_begin();
   typedef Columns<T, U, VEC> Cols;
   const long t = Cols::token();
-  if (t >= tokens) return;
   Cols a(blockIdx.y);
+  if (t < tokens) a.bring(x.p + t * x.ld, D);      // while the slots are still being ranked: 3 of 68 us for 8192 x 4096
+  pdl_begin();
+  if (t >= tokens) return;
   a.load(x.p + t * x.ld, D);
   for (int i = 0; i < k; i++) {
     const long r = row_at(__ldg(positions + t * k + i), most);
@@ -236,25 +261,31 @@ static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const floa
 }
 
 // The same for few slots, with the ranking: a block for a token and 256 U W of its columns.  A slot's place is the number of slots that name a lower expert,
-// or the same and come before it.
+// or the same and come before it.  One more block counts for the host, which so gets its counts before any row is copied.
 template <int U, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const float *__restrict__ experts, float *__restrict__ positions, float *__restrict__ rows, int k,
                                                                   int D, int slots, int groups, CountStage tell) {
   pdl_begin();
-  extern __shared__ int expert[];       // [slots], the token's rows [k], and in the first block the counts [groups + 1]
-  int *mine = expert + slots, *count = mine + k;
+  extern __shared__ int expert[];       // [slots] and the token's rows [k], or the counts [groups + 1]
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.y) return;
+    for (int g = t; g <= groups; g += 256) expert[g] = 0;
+    __syncthreads();
+    for (int s = t; s < slots; s += 256) {
+      const int e = slot_expert(experts[s], groups);
+      if (e != 0) atomicAdd(&expert[e > 0 ? e - 1 : groups], 1);
+    }
+    __syncthreads();
+    for (int g = t; g <= groups; g += 256) count_deliver(tell, g, expert[g]);
+    return;
+  }
+  int *mine = expert + slots;
   const long token = blockIdx.x;
-  const bool first = blockIdx.x == 0 && blockIdx.y == 0;
   Columns<256, U, VEC> a(blockIdx.y);
   a.load(x.p + token * x.ld, D);
-  if (first)
-    for (int g = t; g <= groups; g += 256) count[g] = 0;
   for (int s = t; s < slots; s += 256) expert[s] = slot_expert(experts[s], groups);
   __syncthreads();
-  if (first)
-    for (int s = t; s < slots; s += 256)
-      if (expert[s] != 0) atomicAdd(&count[expert[s] > 0 ? expert[s] - 1 : groups], 1);
   for (int i = warp; i < k; i += 8) {
     const int at = (int)token * k + i, e = expert[at];
     int before = 0;
@@ -266,8 +297,6 @@ static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const 
     }
   }
   __syncthreads();
-  if (first)
-    for (int g = t; g <= groups; g += 256) count_deliver(tell, g, count[g]);
   for (int i = 0; i < k; i++)
     if (mine[i] >= 0) a.store(rows + mine[i] * (long)D, D);
 }
@@ -419,9 +448,9 @@ static void dispatch(Rows x, const float *experts, long tokens, int k, int D, in
   const long slots = tokens * k;
   const bool vec = pieces_of_four({x, Rows{rows, D}}, D);
   if (are_few(slots, k)) {
-    const size_t smem = sizeof(int) * (slots + k + groups + 1);
-    if (vec) pdl_launch(few_rows_out_kernel<1, true>, dim3((unsigned)tokens, (unsigned)ceil_div(D, 1024)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
-    else pdl_launch(few_rows_out_kernel<1, false>, dim3((unsigned)tokens, (unsigned)ceil_div(D, 256)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
+    const size_t smem = sizeof(int) * std::max(slots + k, groups + 1l);
+    if (vec) pdl_launch(few_rows_out_kernel<1, true>, dim3((unsigned)tokens + 1, (unsigned)ceil_div(D, 1024)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
+    else pdl_launch(few_rows_out_kernel<1, false>, dim3((unsigned)tokens + 1, (unsigned)ceil_div(D, 256)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
     check_launch("Dispatch_updateOutput");
     return;
   }

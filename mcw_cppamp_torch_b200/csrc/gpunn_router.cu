@@ -199,6 +199,8 @@ static __global__ void __launch_bounds__(256) router_backward_kernel(const float
     expert = (int)experts[row * k + lane] - 1;
     if (expert >= 0) { w = weights[row * k + lane]; d = g[row * ldg + lane]; }
   }
+  float v[V];
+  if (x) Row::load(x + row * ldx, lane, E, v);
   const float spread = warp_total(w * d);
   float out[V];
 #pragma unroll
@@ -212,8 +214,7 @@ static __global__ void __launch_bounds__(256) router_backward_kernel(const float
       if (Row::at(j, lane) == to) out[j] += add;
   }
   if (x) {
-    float v[V], top = -INFINITY, total = 0.f;
-    Row::load(x + row * ldx, lane, E, v);
+    float top = -INFINITY, total = 0.f;
 #pragma unroll
     for (int j = 0; j < V; j++) top = fmaxf(top, v[j]);
 #pragma unroll

@@ -24,6 +24,7 @@ void (*g_clear_error)(void) = nullptr;
 PyObject *g_error_type = nullptr;
 // ctypes types whose instances are one pointer: POINTER(THGPUTensor), POINTER(THGPUStorage)
 PyTypeObject *g_tensor_type = nullptr, *g_storage_type = nullptr;
+PyObject *g_type_name = nullptr;   // "_type_", what ctypes calls the type of an array's items
 
 // None, or an instance of exactly this type: a pointer to something else is for ctypes to convert or reject.
 bool pointer_of(PyObject *o, PyTypeObject *type, void **out) {
@@ -43,6 +44,17 @@ template <class T> bool take(PyObject *o, T &out) {
     if (!pointer_of(o, std::is_same<Pointee, THGPUTensor>::value ? g_tensor_type : g_storage_type, &p)) return false;
     out = (T)p;
     return true;
+  } else if constexpr (std::is_same<T, THGPUTensor **>::value) {   // a ctypes array of tensor pointers, whose length is another argument
+    PyObject *item = PyObject_GetAttr((PyObject *)Py_TYPE(o), g_type_name);
+    if (!item) { PyErr_Clear(); return false; }
+    const bool same = item == (PyObject *)g_tensor_type;
+    Py_DECREF(item);
+    Py_buffer b;
+    if (!same || PyObject_GetBuffer(o, &b, PyBUF_C_CONTIGUOUS) != 0) { PyErr_Clear(); return false; }
+    const bool array = b.ndim == 1;   // (and no pointer to one, whose own bytes a buffer would be)
+    out = (THGPUTensor **)b.buf;      // (the caller's argument keeps it alive)
+    PyBuffer_Release(&b);
+    return array;
   } else if constexpr (std::is_floating_point<T>::value) {
     if (PyFloat_CheckExact(o)) { out = (T)PyFloat_AS_DOUBLE(o); return true; }
     if (!PyLong_Check(o)) return false;
@@ -140,7 +152,8 @@ const Entry kEntries[] = {
   E(THGPUNN_ClassNLLCriterion_updateGradInput) E(THGPUNN_SGD_update) E(THGPUNN_LayerNorm_updateOutput) E(THGPUNN_LayerNorm_backward)
   E(THGPUNN_FusedLinear_updateOutput) E(THGPUNN_FusedLinear_backward) E(THGPUNN_GroupedLinear_updateOutput)
   E(THGPUNN_GroupedLinear_backward) E(THGPUNN_Router_updateOutput) E(THGPUNN_Router_updateGradInput) E(THGPUNN_Dispatch_updateOutput)
-  E(THGPUNN_Dispatch_updateGradInput) E(THGPUNN_Combine_updateOutput) E(THGPUNN_Combine_backward)
+  E(THGPUNN_Dispatch_updateGradInput) E(THGPUNN_Combine_updateOutput) E(THGPUNN_Combine_backward) E(THGPUNN_AdamW_update) E(THGPUNN_AdamW8_update)
+  E(THGPUNN_AdamW8_moments)
   UNARY(EU) COMPARE(EC)
 };
 
@@ -187,6 +200,7 @@ PyObject *setup(PyObject *, PyObject *args) {
   g_tensor_type = (PyTypeObject *)tensor;
   Py_INCREF(storage);
   g_storage_type = (PyTypeObject *)storage;
+  if (!g_type_name && !(g_type_name = PyUnicode_InternFromString("_type_"))) return nullptr;
   Py_RETURN_NONE;
 }
 // wrap(name, address, slow) -> callable, or None for a function without an invoker

@@ -210,6 +210,27 @@ def test_codes_are_those_of_the_definition(gt, b1, b2, seed, size, off):
     assert opt.step.float().tolist() == [6, 0]
 
 
+def test_codes_of_many_values(gt):
+    """So many that a block takes several turns at one tensor: the definition's codes all the same, in tensors whose ends lie anywhere in a turn."""
+    sizes = [16 << 20, 2999999, 300, 2048 * 5, 8192 * 3 + 256]
+    g = [normal(60 + i, n) * F(0.01) for i, n in enumerate(sizes)]
+    W = [gt.GPUTensor(n).fill(0.0) for n in sizes]
+    G = [gt.gpu(x) for x in g]
+    opt = gt.optim.AdamW(W, G, bits=8, seed=5)
+    like, w = [Eight(n) for n in sizes], [np.zeros(n) for n in sizes]
+    for t in (1, 2):
+        opt.update()
+        for i, n in enumerate(sizes):
+            m, root = like[i].step(g[i], 0.9, 0.999, i, t, 5)
+            for a, b in zip(state(opt, i, n), (like[i].m, like[i].r, like[i].scale_m, like[i].scale_r)):
+                assert np.array_equal(a, b)
+            # as in test_codes_are_those_of_the_definition
+            move = 1e-3 / (1 - 0.9 ** t) * m.astype(np.float64) / (root.astype(np.float64) / np.sqrt(1 - 0.999 ** t) + 1e-8)
+            new = W[i].float().astype(np.float64)
+            assert np.all(np.abs(new - (w[i] * (1 - 1e-5) - move)) <= 3 * U * np.abs(w[i]) + 12 * U * np.abs(move) + 1e-44)
+            w[i] = new
+
+
 def test_padding_codes_are_zero(gt):
     opt = gt.optim.AdamW(gt.gpu(normal(1, 300)), gt.gpu(normal(2, 300)), bits=8)
     opt.update()

@@ -40,7 +40,7 @@ def f32(a):
 
 # few slots, which each block ranks for itself, on both sides of the line, and many; rows that 16-byte accesses divide and others
 CASES = [(1, 1, 1, 1), (1, 8, 64, 4096), (3, 2, 4, 5), (24, 8, 64, 1028), (511, 4, 37, 333), (512, 4, 37, 64), (513, 4, 37, 64), (700, 3, 1, 20), (30, 70, 9, 40), (1, 3000, 7, 16),
-         (5000, 1, 4096, 36), (40, 5, 4096, 36), (3000, 8, 256, 129), (20000, 6, 130, 32), (97, 2, 5, 5000), (2500, 2, 300, 1024)]
+         (5000, 1, 4096, 36), (40, 5, 4096, 36), (8192, 4, 9, 5), (32769, 1, 9, 5), (1100, 3, 1024, 7), (1100, 3, 1025, 7), (3000, 8, 256, 129), (20000, 6, 130, 32), (97, 2, 5, 5000), (2500, 2, 300, 1024)]
 
 
 @pytest.mark.parametrize("tokens,k,groups,size", CASES)
@@ -113,6 +113,21 @@ def test_memory_behind_the_rows_stays(gt, tokens):
     rows = m.forward([gt.gpu(x), gt.gpu(f32(e))])[0]
     assert np.array_equal(rows.float(), x[order // 2]) and rows.data_ptr() == room.data_ptr()
     assert np.all(room.float()[order.size:] == 7.0)
+
+
+@pytest.mark.parametrize("tokens,k", [(90, 3), (1100, 3), (1366, 3), (13000, 3)])
+def test_numbers_at_any_address(gt, tokens, k):
+    """Expert numbers that start one value behind a 16-byte boundary, as part of a larger storage; none in the last rows."""
+    x, e = normal(1, tokens, 6), experts_of(2, tokens, k, 50)
+    e[tokens - 7:] = 0
+    order, places, counts = plan(e, 50)
+    for off in (1, 2, 3):
+        room = gt.GPUTensor(tokens * k + 8).fill(-1.0)
+        E = room.narrow(1, 1 + off, tokens * k).view(tokens, k)
+        E.copy(f32(e))
+        m = gt.nn.Dispatch(50)
+        rows, told = m.forward([gt.gpu(x), E])
+        assert np.array_equal(rows.float(), x[order // k]) and np.array_equal(told, counts) and np.array_equal(m.positions.float(), places)
 
 
 def test_rows_apart_and_transposed(gt):

@@ -99,16 +99,17 @@ def test_closed_experts(gt, experts, k, normalize):
     assert np.array_equal(a, m.backward(gt.gpu(x), gt.gpu(g)).float()) and not a[np.isneginf(x)].any()
 
 
-def test_equal_scores(gt):
-    """By their place, zeros of both signs alike."""
-    r = np.random.RandomState(0)
-    for experts, k in ((64, 8), (130, 32), (9, 9)):
-        x = r.randint(-2, 3, (200, experts)).astype(np.float32)
-        x[::2][x[::2] == 0] = -0.0
-        x[5], x[6], x[7, ::2] = 1.0, 0.0, -0.0
-        x[7, 1::2] = 0.0
-        check(gt, x, k, True)
-        check(gt, x, k, False)
+@pytest.mark.parametrize("experts,k", [(64, 8), (130, 32), (9, 9), (130, 8), (96, 16), (97, 17), (256, 8), (300, 16), (512, 1), (1000, 6), (1024, 16)])
+@pytest.mark.parametrize("levels", [3, 40, 1000])
+def test_equal_scores(gt, experts, k, levels):
+    """By their place, zeros of both signs alike: many of each score, so that more than 32 may be as large as the last chosen one, and few."""
+    x = np.random.RandomState(0).randint(-levels, levels, (200, experts)).astype(np.float32)
+    x[::2][x[::2] == 0] = -0.0
+    x[5], x[6], x[7, ::2] = 1.0, 0.0, -0.0
+    x[7, 1::2] = 0.0
+    x[8], x[8, experts // 2] = -np.inf, 0.0
+    check(gt, x, k, True)
+    check(gt, x, k, False)
 
 
 def test_scores_that_are_not_finite(gt):

@@ -315,5 +315,9 @@ def test_missing_tensors():
             call()
     with pytest.raises(gt.THCError, match="Invalid argument 6: tensors expected"):
         L.THGPUNN_AdamW_update(1, none, none, none, none, None, 1e-3, 0.9, 0.999, 1e-8, 0.0)
-    with pytest.raises(gt.THCError, match="tensors expected"):
-        L.THGPUNN_AdamW8_moments(1, none, none, none, none, none)
+    for array in (none, C.cast(none, C.POINTER(TP))):      # an array, or a pointer to its first
+        with pytest.raises(gt.THCError, match="tensors expected"):
+            L.THGPUNN_AdamW8_moments(1, array, array, array, array, array)
+    for bad in (5, (C.c_long * 2)(), [None]):
+        with pytest.raises((C.ArgumentError, TypeError)):
+            L.THGPUNN_AdamW8_moments(1, bad, none, none, none, none)
