@@ -112,6 +112,32 @@ def test_equal_scores(gt, experts, k, levels):
     check(gt, x, k, False)
 
 
+@pytest.mark.parametrize("experts", [16, 33, 64, 77, 128, 200, 256])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_many_rows(gt, experts, normalize):
+    """So many rows that several share a warp: the same choices as of a few, weights but for the order of their sums."""
+    r = np.random.RandomState(experts)
+    parts = [scores(experts, 200, experts), scores(1, 61, experts, 0.6, 3), r.randint(-2, 3, (50, experts)).astype(np.float32),
+             r.randint(-60, 60, (80, experts)).astype(np.float32), scores(2, 20, experts)]
+    parts[4][3, 5], parts[4][7, [3, 9]], parts[4][11, 2], parts[4][15, 2:] = np.nan, (np.nan, np.inf), np.inf, -np.inf
+    parts[2][::2][parts[2][::2] == 0] = -0.0
+    x = np.concatenate(parts)
+    times = 24000 // len(x) + 1
+    X = np.concatenate([np.tile(x, (times, 1)), x[:3]])
+    for k in (1, 2, 6, 8):
+        w, e = (t.float() for t in gt.nn.Router(k, normalize).forward(gt.gpu(x)))
+        assert np.array_equal(e, choose(x, k))
+        W, E = (t.float() for t in gt.nn.Router(k, normalize).forward(gt.gpu(X)))
+        assert np.array_equal(E, np.concatenate([np.tile(e, (times, 1)), e[:3]]))
+        want = np.concatenate([np.tile(w, (times, 1)), w[:3]])
+        # the sums of up to 256 exponentials in two orders, 8 + 5 and 32 + 3 additions deep, and the quotients' own half step each
+        assert np.array_equal(np.isnan(W), np.isnan(want)) and np.all(np.abs(W - want)[~np.isnan(W)] <= (50 * U * np.abs(want))[~np.isnan(W)])
+    flat = gt.GPUTensor(X.size + 1)
+    off = flat.narrow(1, 2, X.size).view(*X.shape)             # no 16-byte addresses
+    off.copy(X)
+    assert np.array_equal(gt.nn.Router(8, normalize).forward(off)[1].float(), E)
+
+
 def test_scores_that_are_not_finite(gt):
     x = scores(1, 6, 40)
     x[0, 7] = np.nan
