@@ -84,6 +84,25 @@ def test_experts_named_twice_and_extremes(gt):
     assert m.backward([gt.GPUTensor(), gt.GPUTensor()], gt.GPUTensor())[0].nElement() == 0
 
 
+@pytest.mark.parametrize("size", [2100007, 1 << 21])
+def test_long_rows(gt, size):
+    """Rows of more pieces than a grid's second dimension has blocks, were they as short as those of short rows."""
+    x, e = normal(1, 2, size), np.array([[2, 1], [0, 2]])
+    order, places, counts = plan(e, 2)
+    m = gt.nn.Dispatch(2)
+    rows, told = m.forward([gt.gpu(x), gt.gpu(f32(e))])
+    assert np.array_equal(rows.float(), x[order // 2]) and np.array_equal(told, counts)
+    assert np.array_equal(m.backward([gt.gpu(x), gt.gpu(f32(e))], rows)[0].float(), x * np.array([[2], [1]], np.float32))
+    w = np.array([[0.5, 2], [3, -1]], np.float32)
+    c = gt.nn.Combine()
+    input = [rows, gt.gpu(w), m.positions]
+    assert np.array_equal(c.forward(input).float(), x * np.array([[2.5], [-1]], np.float32))
+    back = c.backward(input, gt.gpu(x))
+    assert np.array_equal(back[0].float(), (w.reshape(-1, 1) * np.repeat(x, 2, 0))[order])
+    dot = (x.astype(np.float64) ** 2).sum(1)
+    assert np.all(np.abs(back[1].float() - (e > 0) * dot[:, None]) <= (size / 32 + 10) * U * dot[:, None])
+
+
 @pytest.mark.parametrize("tokens", [50, 3000])
 @pytest.mark.parametrize("bad", [0.5, -1.0, 10.0, np.nan, np.inf, -np.inf, 1e30, -0.5])
 def test_numbers_that_are_no_experts(gt, tokens, bad):
@@ -217,6 +236,9 @@ def test_places_of_no_row(gt):
     m.gradRows = room.narrow(1, 1, 6)
     input = [gt.gpu(z), gt.gpu(w), gt.gpu(places)]
     assert np.all(np.abs(m.forward(input).float() - y) <= 4 * U * mass)
+    big = 2.0 ** 24 + 4                                        # beyond what a float counts: of more rows than that, too
+    many = gt.GPUTensor(2 ** 24 + 3, 1).fill(1.0)
+    assert not gt.nn.Combine().forward([many, None, gt.gpu(np.full((3, 2), big, np.float32))]).float().any()
     m.backward(input, gt.gpu(g))
     assert np.all(np.abs(room.float()[:6] - gz) <= U * np.abs(gz)) and np.all(room.float()[6:] == 7.0)
     assert np.all(np.abs(m.gradWeights.float() - gw) <= 12 * U * wmass)
