@@ -19,9 +19,11 @@ namespace thc {
 constexpr long kMostSlots = 1l << 24;     // positions are floats
 constexpr int kMostGroups = 4096;
 constexpr long kMostValues = 1l << 23;    // of a row: its pieces are a dimension of the grid
-constexpr long kFewSlots = 2048;          // up to here every block ranks its token's slots by itself,
-constexpr long kRankedSlots = 32768;      // and up to here a launch of its own ranks them, where the groups are
-constexpr int kRankedGroups = 1024;       // no more than these
+// Three ways to rank the slots, us a call with 64 groups and rows of 16 values: by every block of the copy for its own token (2048 slots: 9.3, 4096: 14.3), in a launch of
+// its own (10.1, 10.3; 16384: 11.7, 32768: 13.7, 65536: 17.2), in two (11.7, 11.8, 11.9, 12.2, 12.8).  Between the last two, with rows of 1024 values, the line lies
+// at 32768 as well (34.3 and 34.7; 65536: 62.4 and 60.0); with 1024 groups further on (36.5 and 42.1; 64.5 and 72.5).
+constexpr long kFewSlots = 2048, kRankedSlots = 32768;
+constexpr int kRankedGroups = 1024;       // of the second way: a thread each
 
 // The expert of a slot, from 1; 0: none; -1: the number stands for no expert.
 static __device__ __forceinline__ int slot_expert(float e, int groups) {
@@ -51,63 +53,59 @@ static __global__ void __launch_bounds__(256) slots_count_kernel(const float *__
   for (int g = threadIdx.x; g <= groups; g += 256) hist[(long)g * gridDim.x + blockIdx.x] = count[g];
 }
 
-static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__restrict__ experts, long slots, int per, int groups, const int *__restrict__ hist,
-                                                                 float *__restrict__ positions, CountStage tell) {
+static __global__ void __launch_bounds__(1024) slots_place_kernel(const float *__restrict__ experts, long slots, int per, int groups, const int *__restrict__ hist,
+                                                                  float *__restrict__ positions, CountStage tell) {
   pdl_begin();
   extern __shared__ int place[];                   // [8 warps][groups]: rows before the warp's next one of a group
-  int *total = place + 8 * groups, *before = total + groups;   // [groups]: a group's rows, and those of the pieces before this one
-  __shared__ int sums[256];
+  int *before = place + 8 * groups, *total = before + groups;   // [groups]: a group's rows in the pieces before this one, and in all; [groups + 1] with the bad numbers
+  __shared__ int sums[32];
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, chunks = gridDim.x;
   const long from = blockIdx.x * (long)per, to = min(slots, from + per);
-  const int share = (per / 8 + 31) & ~31;
-  const long mine = from + (long)warp * share, end = min(to, mine + share);
-  for (int g = t; g < 8 * groups; g += 256) place[g] = 0;
+  const int share = (per / 8 + 31) & ~31;          // of the first eight warps; the others help with the sums
+  const long mine = warp < 8 ? from + (long)warp * share : to, end = min(to, mine + share);
+  for (int g = t; g < 8 * groups; g += 1024) place[g] = 0;
   __syncthreads();
   for (long s = mine + lane; s < end; s += 32) {
     const int e = slot_expert(experts[s], groups);
     if (e > 0) atomicAdd(&place[warp * groups + e - 1], 1);
   }
-  for (int g = warp; g <= groups; g += 8) {
-    int all = 0, ahead = 0;
+  for (int g = 4 * warp; g <= groups; g += 128) {     // (four groups at a time: what comes from L2 is on its way together)
+    int all[4] = {}, ahead[4] = {};
+#pragma unroll 5
     for (int c = lane; c < chunks; c += 32) {
-      const int n = hist[(long)g * chunks + c];
-      all += n;
-      if (c < (int)blockIdx.x) ahead += n;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int n = g + i <= groups ? hist[(long)(g + i) * chunks + c] : 0;
+        all[i] += n;
+        if (c < (int)blockIdx.x) ahead[i] += n;
+      }
     }
-    all = __reduce_add_sync(0xffffffffu, all);
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    if (lane == 0) {
-      if (g < groups) { total[g] = all; before[g] = ahead; }
-      if (blockIdx.x == 0) count_deliver(tell, g, all);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      all[i] = __reduce_add_sync(0xffffffffu, all[i]);
+      ahead[i] = __reduce_add_sync(0xffffffffu, ahead[i]);
+      if (lane == i && g + i <= groups) {
+        total[g + i] = all[i];
+        if (g + i < groups) before[g + i] = ahead[i];
+      }
     }
   }
   __syncthreads();
+  if (blockIdx.x == 0)                             // (neighbours together: each store is a message to the host)
+    for (int g = t; g <= groups; g += 1024) count_deliver(tell, g, total[g]);
   // the groups' first rows: each thread has some neighbouring groups
-  const int some = (groups + 255) / 256, g0 = min(groups, t * some), g1 = min(groups, g0 + some);
+  const int some = (groups + 1023) / 1024, g0 = min(groups, t * some), g1 = min(groups, g0 + some);
   int own = 0;
   for (int g = g0; g < g1; g++) own += total[g];
-  sums[t] = own;
-  __syncthreads();
-  if (warp == 0) {
-    int s = 0;
+  int run = own;
 #pragma unroll
-    for (int i = 0; i < 8; i++) s += sums[lane * 8 + i];
-    int run = s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-    }
-    run -= s;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int n = sums[lane * 8 + i];
-      sums[lane * 8 + i] = run;
-      run += n;
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
   }
+  if (lane == 31) sums[warp] = run;
   __syncthreads();
-  int first = sums[t];
+  int first = run - own + __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0);
   for (int g = g0; g < g1; g++) {
     int at = first + before[g];
     for (int w = 0; w < 8; w++) {
@@ -130,8 +128,7 @@ static __global__ void __launch_bounds__(256) slots_place_kernel(const float *__
   }
 }
 
-// In one launch, where every block can as well count all slots by itself: 1024 threads with a slot each.  16384 slots, 16 groups: some 4 us before the host has the counts,
-// where the two launches above take 6.
+// In one launch, where every block can as well count all slots by itself: 1024 threads with a slot each.
 static __global__ void __launch_bounds__(1024) slots_rank_kernel(const float *__restrict__ experts, int slots, int groups, float *__restrict__ positions,
                                                                  CountStage tell) {
   pdl_begin();
@@ -471,13 +468,13 @@ static void dispatch(Rows x, const float *experts, long tokens, int k, int D, in
     int *hist = (int *)ws_alloc(sizeof(int) * (groups + 1) * chunks);
     pdl_launch(slots_count_kernel, (unsigned)chunks, 256, sizeof(int) * (groups + 1), experts, slots, per, groups, hist);
     check_launch("Dispatch_updateOutput");
-    constexpr size_t most = sizeof(int) * 10 * kMostGroups;
+    constexpr size_t most = sizeof(int) * (10 * kMostGroups + 1);
     static PerDevice allowed;
     allowed.get(ctx().device, [&] {
       THC_CUDA(cudaFuncSetAttribute(slots_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
       return 1;
     });
-    pdl_launch(slots_place_kernel, (unsigned)chunks, 256, sizeof(int) * 10 * groups, experts, slots, per, groups, hist, positions, tell);
+    pdl_launch(slots_place_kernel, (unsigned)chunks, 1024, sizeof(int) * (10 * groups + 1), experts, slots, per, groups, hist, positions, tell);
     check_launch("Dispatch_updateOutput");
   }
   with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
