@@ -409,7 +409,7 @@ template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTe
     s.last = i == all.size();
     const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, kind == kAdam8 ? (unsigned)ctx().sm_count * 4 : 1u << 31));
     if (kind == kAdam32) pdl_launch(adam_kernel<N>, blocks, 256, 0, table, s);
-    else if (kind == kAdam8) pdl_launch(adam8_kernel<N>, blocks, 256, 0, table, s);
+    else if (kind == kAdam8) launch_on_stream(table.turns == 1, adam8_kernel<N>, blocks, 256, 0, table, s);      // (blocks that stay would take room from the end of the kernel before)
     else pdl_launch(adam8_moments_kernel<N>, blocks, 256, 0, table);
     check_launch(kind == kAdamMoments ? "AdamW_moments" : "AdamW_update");
   } while (i < all.size());

@@ -355,14 +355,15 @@ static __global__ void __launch_bounds__(256) router_backward_kernel(const float
   const int lane = threadIdx.x & 31;
   const long row = blockIdx.x * 8l + (threadIdx.x >> 5);
   if (row >= rows) return;
-  float w = 0.f, d = 0.f;
+  float w = 0.f, d = 0.f, v[V];
   int expert = -1;
   if (lane < k) {
     expert = (int)experts[row * k + lane] - 1;
-    if (expert >= 0) { w = weights[row * k + lane]; d = g[row * ldg + lane]; }
+    w = weights[row * k + lane];
+    d = g[row * ldg + lane];
   }
-  float v[V];
   if (x) Row::load(x + row * ldx, lane, E, v);
+  if (expert < 0) w = d = 0.f;                  // (whatever lay there)
   const float spread = warp_total(w * d);
   float out[V];
 #pragma unroll
