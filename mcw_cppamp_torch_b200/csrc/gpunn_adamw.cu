@@ -22,7 +22,6 @@ namespace thc {
 
 constexpr int kAdamBlock = 256;                                // values under one scale
 constexpr int kAdamTurn = 2048;                                // values of a block's turn: a warp has 256
-constexpr int kAdamTurns = 4;                                  // turns of a chunk, for which a block looks its tensor up, where there are plenty
 constexpr unsigned kCodeBits = 0x37800000u;                    // of 2^-16
 constexpr int kMeanShift = 20, kRootShift = 19;
 constexpr float kCodeFloor = 0x1p-16f, kMeanTop = 0.9375f - 0x1p-16f, kRootTop = 0.96875f - 0x1p-16f;   // f(B), and what the largest codes stand for
@@ -38,7 +37,7 @@ struct AdamTensor {
 // As many as fit a launch's parameters; first[i]: the number of tensor i's first chunk.  The smaller table is for the usual few tensors: parameters are copied with
 // every launch.
 template <int N> struct AdamTable {
-  int count, turns;          // turns of a chunk
+  int count;
   unsigned first[N + 1];
   AdamTensor t[N];
 };
@@ -255,10 +254,10 @@ static __device__ __forceinline__ void bring(const AdamTensor &a, long block, in
                      lane < 18 ? (const char *)((const unsigned *)a.m + block * 64) + (lane - 16) * 128 : (const char *)((const unsigned *)a.v + block * 64) + (lane - 18) * 128;
   asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
 }
-// A warp for a block of 256 values, eight a lane; a block looks a tensor up for four turns of 2048.  46 M values: 143 us, 5.2 TB/s; what holds it back is the work on
-// codes, 73 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the codes and branch.
-// Blocks stay, four an SM with 64 registers: a block for each chunk takes 156 us, five blocks an SM in 48 registers 150 (170 with what is brought ahead), a turn's loads in
-// registers ahead of it 178, and nothing brought ahead 158.
+// A warp for a block of 256 values, eight a lane, and for others at the same distance, the next of which is brought to L2 meanwhile.  46 M values: 151 us, 4.9 TB/s; what
+// holds it back is the work on codes, 73 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the
+// codes and branch.  Tried, with a tensor looked up for four turns at a time (143): a block for each chunk, which does not stay, 156; five blocks an SM in 48 registers 150
+// (170 with what is brought ahead); a turn's loads in registers ahead of it 178; nothing brought ahead 158.
 template <int N>
 static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
@@ -268,13 +267,12 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
   const AdamFactors f = shared;
   const unsigned chunks = table.first[table.count];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long jump = 8l * table.turns * gridDim.x - 8l * (table.turns - 1);      // from the last block of a turn to the first of the next chunk
+  const long jump = (long)(kAdamTurn / kAdamBlock) * gridDim.x;      // to the warp's next block, if it is of the same tensor
   for (unsigned chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int i = tensor_of(table, chunk);
     const AdamTensor &a = table.t[i];
-    long block = (chunk - table.first[i]) * (long)(kAdamTurn / kAdamBlock * table.turns) + warp;
-    for (int turn = 0; turn < table.turns && block * kAdamBlock < a.n; turn++, block += kAdamTurn / kAdamBlock) {
-      const long from = block * kAdamBlock;
+    const long block = (chunk - table.first[i]) * (long)(kAdamTurn / kAdamBlock) + warp, from = block * kAdamBlock;
+    if (from < a.n) {
       const int n = (int)min((long)kAdamBlock, a.n - from);
       float *w = a.w + from;
       const float *g = a.g + from;
@@ -291,7 +289,7 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
         mq[h] = codes_of(mc, h, lane, n);
         rq[h] = codes_of(rc, h, lane, n);
       }
-      bring(a, block + (turn + 1 < table.turns ? 8 : jump), lane);
+      bring(a, block + jump, lane);
       float top_m = 0.f, top_r = 0.f;
       const Pair scale_m2(scale.x, scale.x), scale_r2(scale.y, scale.y), beta1(s.beta1, s.beta1), beta2(s.beta2, s.beta2), rest1(s.rest1, s.rest1), rest2(s.rest2, s.rest2);
 #pragma unroll
@@ -387,19 +385,15 @@ static __global__ void __launch_bounds__(256) adam8_moments_kernel(const __grid_
 // ---- launches
 enum AdamKind { kAdam32, kAdam8, kAdamMoments };
 template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTensor> &all, const AdamStep &step) {
-  long total = 0;
-  for (const AdamTensor &t : all) total += t.n;
   size_t i = 0;
   do {
     AdamTable<N> table;
-    table.turns = kind == kAdam8 && total >= (long)kAdamTurn * kAdamTurns * 16 * ctx().sm_count ? kAdamTurns : 1;
-    const long per = (long)kAdamTurn * table.turns;
     AdamStep s = step;
     s.number = (int)i;
     table.count = 0;
     table.first[0] = 0;
     for (; i < all.size() && table.count < N; i++) {
-      const long chunks = (all[i].n + per - 1) / per;
+      const long chunks = (all[i].n + kAdamTurn - 1) / kAdamTurn;
       THC_CHECK(chunks < (1l << 31), "tensors of more than 2^42 values");
       if (table.count && table.first[table.count] + (unsigned long)chunks >= (1ul << 31)) break;
       table.t[table.count] = all[i];
@@ -409,7 +403,7 @@ template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTe
     s.last = i == all.size();
     const unsigned chunks = table.first[table.count], blocks = std::max(1u, std::min(chunks, kind == kAdam8 ? (unsigned)ctx().sm_count * 4 : 1u << 31));
     if (kind == kAdam32) pdl_launch(adam_kernel<N>, blocks, 256, 0, table, s);
-    else if (kind == kAdam8) launch_on_stream(table.turns == 1, adam8_kernel<N>, blocks, 256, 0, table, s);      // (blocks that stay would take room from the end of the kernel before)
+    else if (kind == kAdam8) pdl_launch(adam8_kernel<N>, blocks, 256, 0, table, s);
     else pdl_launch(adam8_moments_kernel<N>, blocks, 256, 0, table);
     check_launch(kind == kAdamMoments ? "AdamW_moments" : "AdamW_update");
   } while (i < all.size());

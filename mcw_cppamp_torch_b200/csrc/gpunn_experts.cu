@@ -407,9 +407,12 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
   }
 }
 
-// f(integral constants T, U, VEC) for rows of D values: the widest team that leaves the fewest columns over, or (whole) one as wide as a row, at most a block; one
-// piece a thread where the rows are few, so that they are spread over all SMs.
-template <class F> static void with_columns(long tokens, int D, bool vec, bool whole, F f) {
+// f(integral constants T, U, VEC) for rows of D values, k of which come to a token: the widest team that leaves the fewest columns over, or (whole) one as wide as a row, at
+// most a block.  U: four pieces a thread, and two rows at a time, or one piece and up to eight rows.  One piece is for few rows, which are spread over more
+// SMs by it, and for rows that four pieces a thread would leave half a warp without work, both where k is more than the two rows at a time.
+// Combine, 8 rows a token, us with one and with four: 24 x 4096 3.1 and 4.5, 128 x 4096 3.6 and 4.6, 256 x 4096 5.3 and 4.4, 4096 x 64 3.7 and 5.5; backward 128 x 1024 3.6 and 5.7,
+// 512 x 1024 6.9 and 6.0, 4096 x 64 6.5 and 9.2.  2 rows a token: 8192 x 64 4.5 and 3.5.
+template <class F> static void with_columns(long tokens, int D, int k, bool vec, bool whole, F f) {
   auto go = [&](auto VEC, auto U) {
     constexpr int per = (decltype(VEC)::value ? 4 : 1) * decltype(U)::value;
     int team = 256;
@@ -425,9 +428,11 @@ template <class F> static void with_columns(long tokens, int D, bool vec, bool w
     else if (team == 128) f(std::integral_constant<int, 128>(), U, VEC);
     else f(std::integral_constant<int, 256>(), U, VEC);
   };
-  const bool few = !whole && tokens * (long)D <= ctx().sm_count * (vec ? 8192l : 2048l);
+  const int w = vec ? 4 : 1;
+  const bool few = tokens * (long)D <= ctx().sm_count * (whole ? 512l : 1024l) * w, narrow = D <= 32 * w;
+  const bool one = k > 2 && (few || narrow) && (!whole || D <= 256 * w);
   auto with_u = [&](auto VEC) {
-    if (few) go(VEC, std::integral_constant<int, 1>());
+    if (one) go(VEC, std::integral_constant<int, 1>());
     else go(VEC, std::integral_constant<int, 4>());
   };
   if (vec) with_u(std::true_type());
@@ -477,7 +482,7 @@ static void dispatch(Rows x, const float *experts, long tokens, int k, int D, in
     pdl_launch(slots_place_kernel, (unsigned)chunks, 1024, sizeof(int) * (10 * groups + 1), experts, slots, per, groups, hist, positions, tell);
     check_launch("Dispatch_updateOutput");
   }
-  with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
+  with_columns(tokens, D, 1, vec, false, [&](auto T, auto U, auto VEC) {      // (reads a row a token)
     constexpr int t = decltype(T)::value, u = decltype(U)::value, width = t * u * (decltype(VEC)::value ? 4 : 1);
     pdl_launch(rows_out_kernel<t, u, decltype(VEC)::value>, dim3((unsigned)ceil_div(tokens, 256 / t), (unsigned)ceil_div(D, width)), 256, 0, x, positions, rows, tokens, k,
                D, slots);
@@ -487,7 +492,7 @@ static void dispatch(Rows x, const float *experts, long tokens, int k, int D, in
 
 static void sum_rows(Rows rows, long most, const float *w, const float *positions, Rows residual, float *y, long tokens, int k, int D, const char *what) {
   const bool vec = pieces_of_four({rows, residual, Rows{y, D}}, D);
-  with_columns(tokens, D, vec, false, [&](auto T, auto U, auto VEC) {
+  with_columns(tokens, D, k, vec, false, [&](auto T, auto U, auto VEC) {
     constexpr int t = decltype(T)::value, u = decltype(U)::value, width = t * u * (decltype(VEC)::value ? 4 : 1);
     pdl_launch(rows_sum_kernel<t, u, decltype(VEC)::value>, dim3((unsigned)ceil_div(tokens, 256 / t), (unsigned)ceil_div(D, width)), 256, 0, rows, w, positions, residual,
                y, tokens, k, D, most);
@@ -629,7 +634,7 @@ THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, T
   auto run = [&](Rows x) {
     float *gx = gradInput && rows ? data_ptr(gradInput) : nullptr, *gw = gradWeights ? data_ptr(gradWeights) : nullptr;
     const bool vec = pieces_of_four({x, Rows{g.p, g.ld}, Rows{gx, D}}, (int)D);
-    with_columns(tokens, (int)D, vec, true, [&](auto T, auto U, auto VEC) {
+    with_columns(tokens, (int)D, (int)k, vec, true, [&](auto T, auto U, auto VEC) {
       constexpr int t = decltype(T)::value, u = decltype(U)::value;
       pdl_launch(rows_sum_backward_kernel<t, u, decltype(VEC)::value>, (unsigned)ceil_div(tokens, 256 / t), 256, 0, x, weights ? data_ptr(w) : nullptr, data_ptr(p),
                  Rows{g.p, g.ld}, gx, gw, tokens, (int)k, (int)D, rows);

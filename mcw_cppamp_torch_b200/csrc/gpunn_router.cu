@@ -100,7 +100,10 @@ template <int V> static __device__ __forceinline__ Chosen choose_in_turn(const f
 }
 // The k largest at once.  The k-th largest of the lanes' largest is no more than the k-th of all, so that those from it on, some 32 log(32 / (32 - k)) of scores in
 // random order, are all that is left to rank: each is compared with each.  False where they are more than the lanes, with nothing done.
-constexpr int kFewChosen = 16;      // 22 scores are left on average, at 20 they are 31
+// With k above 16 too many are left (22 on average, 31 at 20); with few chosen of few scores, the rounds are shorter.  16384 rows, us in turn and at once: 64 scores, 4 chosen 4.7 and 4.8,
+// 8 chosen 6.5 and 5.7; 128 scores, 2 chosen 4.7 and 5.2, 3 chosen 5.4 and 5.3; 256 scores, 1 chosen 5.3 and 5.8, 2 chosen 6.6 and 6.0; 1024 scores, 1 chosen 16.0 and 18.2, 2 chosen 20.2 and 18.4.
+constexpr int kFewChosen = 16;
+static __host__ __device__ __forceinline__ constexpr bool at_once(int V, int k) { return k <= kFewChosen && k > 1 && k * (V + 2) >= 16; }
 struct Candidates {
   float score[32];
   unsigned short place[32];
@@ -167,9 +170,7 @@ static __device__ __forceinline__ void route_row(const float *__restrict__ x, fl
   const float top = warp_max(most);
   Chosen c;
   bool done = false;
-  if constexpr (V >= 4) {
-    if (k <= kFewChosen && top == top) done = choose_at_once<V>(v, most, top, left, lane, k, c);
-  }
+  if (at_once(V, k) && top == top) done = choose_at_once<V>(v, most, top, left, lane, k, c);
   if (!done) c = choose_in_turn<V>(v, lane, k);
   const float e = c.expert ? expf(c.score - top) : 0.f;
   float total = 0.f;
