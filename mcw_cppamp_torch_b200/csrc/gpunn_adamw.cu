@@ -41,7 +41,7 @@ template <int N> struct AdamTable {
   unsigned first[N + 1];
   AdamTensor t[N];
 };
-constexpr int kFewTensors = 24, kManyTensors = 512;
+constexpr int kFewTensors = 24, kSomeTensors = 64, kMoreTensors = 160, kManyTensors = 512;
 struct AdamStep {
   float *step;               // steps taken, and the count of blocks that are done (zero between launches)
   bool last;                 // the launch that counts the step
@@ -410,6 +410,8 @@ template <int N> static void adam_launch(AdamKind kind, const std::vector<AdamTe
 }
 static void adam_launch(AdamKind kind, const std::vector<AdamTensor> &all, const AdamStep &step) {
   if (all.size() <= kFewTensors) adam_launch<kFewTensors>(kind, all, step);
+  else if (all.size() <= kSomeTensors) adam_launch<kSomeTensors>(kind, all, step);
+  else if (all.size() <= kMoreTensors) adam_launch<kMoreTensors>(kind, all, step);
   else adam_launch<kManyTensors>(kind, all, step);
 }
 
@@ -426,7 +428,23 @@ class Spans {
     else spans_.push_back(s);
   }
   void check() {
-    if (!std::is_sorted(spans_.begin(), spans_.end())) std::sort(spans_.begin(), spans_.end());
+    // Spans of one kind mostly come in order: those runs are merged, unless there are many.
+    std::vector<size_t> runs{0};
+    for (size_t i = 1; i < spans_.size() && runs.size() <= 16; i++)
+      if (spans_[i] < spans_[i - 1]) runs.push_back(i);
+    if (runs.size() > 16) std::sort(spans_.begin(), spans_.end());
+    else {
+      runs.push_back(spans_.size());
+      for (; runs.size() > 2; ) {
+        std::vector<size_t> next{0};
+        for (size_t i = 2; i < runs.size(); i += 2) {
+          std::inplace_merge(spans_.begin() + runs[i - 2], spans_.begin() + runs[i - 1], spans_.begin() + runs[i]);
+          next.push_back(runs[i]);
+        }
+        if (next.back() != spans_.size()) next.push_back(spans_.size());
+        runs.swap(next);
+      }
+    }
     uintptr_t end = 0, end_written = 0;
     for (const Span &s : spans_) {
       THC_CHECK(s.from >= (s.written ? end : end_written), "a result shares memory with another tensor of the call");

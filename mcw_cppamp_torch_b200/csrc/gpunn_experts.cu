@@ -30,9 +30,9 @@ static __device__ __forceinline__ int slot_expert(float e, int groups) {
   return e >= 0.f && e <= (float)groups && e == truncf(e) ? (int)e : -1;
 }
 // The row at a place, or -1: a place that stands for none of the `rows` is passed over.
-static __device__ __forceinline__ long row_at(float place, long rows) {
-  const long r = (long)place;             // (of a NaN the lowest number there is, of an infinity the last one)
-  return r >= 1 && r <= rows ? r - 1 : -1;
+static __device__ __forceinline__ int row_at(float place, long rows) {
+  const int r = (int)place;               // (of an infinity the last number there is, of a NaN none above zero; places beyond 2^24 are none of Dispatch's)
+  return r >= 1 && r <= kMostSlots && r <= rows ? r - 1 : -1;
 }
 
 // ---- where the rows go -------------------------------------------------------------------------------------------------
@@ -239,6 +239,10 @@ template <int T, int U, bool VEC> struct Columns {
   }
 };
 
+// Rows on their way at once: eight with one piece of each a thread, else two, with four pieces of 16 bytes or eight of 4.  (Eight rows by four pieces of 4 bytes took more
+// registers and twice the time: 19056 x 333, 2 rows a token, 22.6 us against 11.4, backward 69 against 25; two rows by four pieces 11.4 and 33.)
+template <int U> static __host__ __device__ constexpr int rows_at_once() { return U == 1 ? 8 : 2; }
+
 struct Rows {            // a matrix of rows at a distance
   const float *p;
   long ld;
@@ -255,8 +259,8 @@ static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const floa
   if (t >= tokens) return;
   a.load(x.p + t * x.ld, D);
   for (int i = 0; i < k; i++) {
-    const long r = row_at(__ldg(positions + t * k + i), most);
-    if (r >= 0) a.store(rows + r * D, D);
+    const int r = row_at(__ldg(positions + t * k + i), most);
+    if (r >= 0) a.store(rows + (long)r * D, D);
   }
 }
 
@@ -312,9 +316,9 @@ static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const f
   Cols a(blockIdx.y);
   if (residual.p) a.load(residual.p + t * residual.ld, D);
   else a.zero();
-  constexpr int B = U * Cols::W <= 4 ? 8 : 2;      // rows on their way at once
+  constexpr int B = rows_at_once<U>();
   for (int i0 = 0; i0 < k; i0 += B) {
-    long r[B];
+    int r[B];
     float f[B];
     Cols b[B];
 #pragma unroll
@@ -344,22 +348,23 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
                                                                        float *__restrict__ drows, float *__restrict__ dw, long tokens, int k, int D, long most) {
   pdl_begin();
   typedef Columns<T, U, VEC> Cols;
-  __shared__ float dots[256 / T][T / 32][kDotSlots];
+  constexpr int WARPS = T > 32 ? T / 32 : 1;       // of a team
+  __shared__ float dots[256 / T][WARPS][kDotSlots];
   const long t = Cols::token();
-  const int team = threadIdx.x / T, warp = threadIdx.x % T / 32, lane = threadIdx.x & 31, pieces = (D + T * U * Cols::W - 1) / (T * U * Cols::W);
-  const bool live = t < tokens;
-  constexpr int B = U * Cols::W <= 4 ? 4 : 2;      // rows on their way at once
+  const int team = threadIdx.x / T, member = threadIdx.x % T, pieces = (D + T * U * Cols::W - 1) / (T * U * Cols::W);
+  const bool live = t < tokens;                    // (teams of a warp stay together: the others take part in its exchanges)
+  constexpr int B = U == 1 ? 4 : 2;                // as rows_at_once, with gradOutput's row in registers as well
   Cols g(0);
   if (live && pieces == 1) g.load(dy.p + t * dy.ld, D);
   for (int i0 = 0; i0 < k; i0 += kDotSlots) {
     const int n = min(kDotSlots, k - i0);
-    for (int i = 0; live && i < n; i += B) {
-      long r[B];
+    for (int i = 0; i < n; i += B) {
+      int r[B];
       float f[B], dot[B];
 #pragma unroll
       for (int b = 0; b < B; b++) {
         const long slot = t * k + i0 + i + b;
-        r[b] = i + b < n ? row_at(__ldg(positions + slot), most) : -1;
+        r[b] = live && i + b < n ? row_at(__ldg(positions + slot), most) : -1;
         f[b] = r[b] < 0 ? 0.f : w ? __ldg(w + slot) : 1.f;
         dot[b] = 0.f;
       }
@@ -371,7 +376,7 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
           row[b].zero();
           if (dw && r[b] >= 0) row[b].load(rows.p + r[b] * rows.ld, D);
         }
-        if (pieces > 1) {
+        if (live && pieces > 1) {
           g = Cols(p);
           g.load(dy.p + t * dy.ld, D);
         }
@@ -382,58 +387,60 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
             dot[b] = fmaf(row[b].v[j], g.v[j], dot[b]);
             row[b].v[j] = f[b] * g.v[j];
           }
-          if (drows && r[b] >= 0) row[b].store(drows + r[b] * D, D);
+          if (drows && r[b] >= 0) row[b].store(drows + (long)r[b] * D, D);
         }
       }
       if (!dw) continue;
 #pragma unroll
       for (int b = 0; b < B; b++) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], o);
-        if (lane == 0 && i + b < n) dots[team][warp][i + b] = r[b] < 0 ? 0.f : dot[b];     // (0 times a NaN of gradOutput)
+        for (int o = (T < 32 ? T : 32) / 2; o > 0; o >>= 1) dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], o);
+        if (member % 32 == 0 && i + b < n) dots[team][member / 32][i + b] = r[b] < 0 ? 0.f : dot[b];     // (0 times a NaN of gradOutput)
       }
     }
     if (!dw) continue;
     if constexpr (T > 32) __syncthreads();
     else __syncwarp();
-    if (live && threadIdx.x % T < n) {
-      float s = dots[team][0][threadIdx.x % T];
+    for (int i = member; live && i < n; i += T) {
+      float s = dots[team][0][i];
 #pragma unroll
-      for (int o = 1; o < T / 32; o++) s += dots[team][o][threadIdx.x % T];
-      dw[t * k + i0 + threadIdx.x % T] = s;
+      for (int o = 1; o < WARPS; o++) s += dots[team][o][i];
+      dw[t * k + i0 + i] = s;
     }
     if constexpr (T > 32) __syncthreads();
     else __syncwarp();
   }
 }
 
-// f(integral constants T, U, VEC) for rows of D values, k of which come to a token: the widest team that leaves the fewest columns over, or (whole) one as wide as a row, at
-// most a block.  U: four pieces a thread, and two rows at a time, or one piece and up to eight rows.  One piece is for few rows, which are spread over more
-// SMs by it, and for rows that four pieces a thread would leave half a warp without work, both where k is more than the two rows at a time.
-// Combine, 8 rows a token, us with one and with four: 24 x 4096 3.1 and 4.5, 128 x 4096 3.6 and 4.6, 256 x 4096 5.3 and 4.4, 4096 x 64 3.7 and 5.5; backward 128 x 1024 3.6 and 5.7,
-// 512 x 1024 6.9 and 6.0, 4096 x 64 6.5 and 9.2.  2 rows a token: 8192 x 64 4.5 and 3.5.
+// f(integral constants T, U, VEC) for rows of D values, k of which come to a token.  T: for rows that half a warp or less covers, and where a team has to have all of its row
+// (whole), the narrowest team that does, at most a block; else the widest that leaves the fewest columns over.  U: one piece a thread, and up to eight rows at a time, for few
+// rows, which that spreads over more SMs, and for narrow ones, both where k is more than two; else more pieces of two rows at a time.
+// Combine, 8 rows a token, us with one piece and with four: 24 x 4096 3.1 and 4.5, 128 x 4096 3.6 and 4.6, 256 x 4096 5.3 and 4.4, 4096 x 64 3.7 and 5.5; backward 128 x 1024
+// 3.6 and 5.7, 512 x 1024 6.9 and 6.0, 4096 x 64 6.5 and 9.2.  2 rows a token: 8192 x 64 4.5 and 3.5.  Teams of a warp and of eight lanes, 22024 x 20, 6 rows a token: 14 and 4.
 template <class F> static void with_columns(long tokens, int D, int k, bool vec, bool whole, F f) {
   auto go = [&](auto VEC, auto U) {
     constexpr int per = (decltype(VEC)::value ? 4 : 1) * decltype(U)::value;
     int team = 256;
-    if (whole) {
-      while (team > 32 && D <= team / 2 * per) team /= 2;
+    if (whole || D <= 32 * per) {
+      while (team > 8 && D <= team / 2 * per) team /= 2;
     } else if (D <= 16 * 256 * per) {
       auto width = [&](int t) { return (long)ceil_div(D, t * per) * t; };
       for (int t = 128; t >= 32; t /= 2)
         if (width(t) < width(team)) team = t;
     }
-    if (team == 32) f(std::integral_constant<int, 32>(), U, VEC);
+    if (team == 8) f(std::integral_constant<int, 8>(), U, VEC);
+    else if (team == 16) f(std::integral_constant<int, 16>(), U, VEC);
+    else if (team == 32) f(std::integral_constant<int, 32>(), U, VEC);
     else if (team == 64) f(std::integral_constant<int, 64>(), U, VEC);
     else if (team == 128) f(std::integral_constant<int, 128>(), U, VEC);
     else f(std::integral_constant<int, 256>(), U, VEC);
   };
   const int w = vec ? 4 : 1;
-  const bool few = tokens * (long)D <= ctx().sm_count * (whole ? 512l : 1024l) * w, narrow = D <= 32 * w;
+  const bool few = tokens * (long)D <= ctx().sm_count * (whole ? 512l : 1024l) * w, narrow = vec && D <= 128;
   const bool one = k > 2 && (few || narrow) && (!whole || D <= 256 * w);
   auto with_u = [&](auto VEC) {
     if (one) go(VEC, std::integral_constant<int, 1>());
-    else go(VEC, std::integral_constant<int, 4>());
+    else go(VEC, std::integral_constant<int, decltype(VEC)::value ? 4 : 8>());
   };
   if (vec) with_u(std::true_type());
   else with_u(std::false_type());

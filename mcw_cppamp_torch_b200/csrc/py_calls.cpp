@@ -24,7 +24,8 @@ void (*g_clear_error)(void) = nullptr;
 PyObject *g_error_type = nullptr;
 // ctypes types whose instances are one pointer: POINTER(THGPUTensor), POINTER(THGPUStorage)
 PyTypeObject *g_tensor_type = nullptr, *g_storage_type = nullptr;
-PyObject *g_type_name = nullptr;   // "_type_", what ctypes calls the type of an array's items
+PyObject *g_type_name = nullptr;      // "_type_", what ctypes calls the type of an array's items
+PyObject *g_pointer_name = nullptr;   // "_p", the pointer of a GPUTensor
 
 // None, or an instance of exactly this type: a pointer to something else is for ctypes to convert or reject.
 bool pointer_of(PyObject *o, PyTypeObject *type, void **out) {
@@ -201,6 +202,7 @@ PyObject *setup(PyObject *, PyObject *args) {
   Py_INCREF(storage);
   g_storage_type = (PyTypeObject *)storage;
   if (!g_type_name && !(g_type_name = PyUnicode_InternFromString("_type_"))) return nullptr;
+  if (!g_pointer_name && !(g_pointer_name = PyUnicode_InternFromString("_p"))) return nullptr;
   Py_RETURN_NONE;
 }
 // wrap(name, address, slow) -> callable, or None for a function without an invoker
@@ -281,6 +283,31 @@ PyObject *set_view(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!ok) return nullptr;
   Py_RETURN_NONE;
 }
+// pointers(tuple of GPUTensor) -> bytearray of the THGPUTensor pointers they hold (one null for none), to lie behind a ctypes array; the caller keeps the tensors
+PyObject *pointers(PyObject *, PyObject *tensors) {
+  if (!PyTuple_Check(tensors)) {
+    PyErr_SetString(PyExc_TypeError, "tuple of tensors expected");
+    return nullptr;
+  }
+  const Py_ssize_t n = PyTuple_GET_SIZE(tensors);
+  PyObject *out = PyByteArray_FromStringAndSize(nullptr, (Py_ssize_t)sizeof(void *) * (n ? n : 1));
+  if (!out) return nullptr;
+  char *to = PyByteArray_AS_STRING(out);
+  std::memset(to, 0, sizeof(void *));
+  for (Py_ssize_t i = 0; i < n; i++) {
+    PyObject *p = PyObject_GetAttr(PyTuple_GET_ITEM(tensors, i), g_pointer_name);
+    void *v = nullptr;
+    const bool ok = p && pointer_of(p, g_tensor_type, &v) && v;
+    Py_XDECREF(p);
+    if (!ok) {
+      Py_DECREF(out);
+      PyErr_SetString(PyExc_TypeError, "torch.GPUTensor expected");
+      return nullptr;
+    }
+    std::memcpy(to + i * sizeof(void *), &v, sizeof(void *));
+  }
+  return out;
+}
 // A dense float32 array as a TH tensor; false: not one (the caller takes the general route).
 struct HostFloat {
   Py_buffer b;
@@ -329,6 +356,7 @@ PyObject *download(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 PyMethodDef kMethods[] = {{"setup", setup, METH_VARARGS, nullptr}, {"wrap", wrap, METH_VARARGS, nullptr},
                           {"functions", functions, METH_VARARGS, nullptr}, {"sizes", sizes, METH_O, nullptr},
+                          {"pointers", pointers, METH_O, nullptr},
                           {"set_view", (PyCFunction)(void *)set_view, METH_FASTCALL, nullptr},
                           {"upload", (PyCFunction)(void *)upload, METH_FASTCALL, nullptr},
                           {"download", (PyCFunction)(void *)download, METH_FASTCALL, nullptr}, {}};

@@ -1,20 +1,20 @@
 """Parameter updates that keep a state of their own, over the tensors of `Module.parameters()` or `getParameters()`."""
+from . import _lib
 from ._lib import TP, lib
 from .tensor import GPUTensor
 
 BLOCK = 256     # values under one scale of the 8-bit moments
 
 
-def _tensors(t, what):
-    t = (t,) if isinstance(t, GPUTensor) else tuple(t)
-    for v in t:
-        if not isinstance(v, GPUTensor):
-            raise TypeError("%s: torch.GPUTensor expected (call :gpu() on the module first)" % what)
-    return t
-
-
-def _array(tensors):
-    return (TP * max(1, len(tensors)))(*[t._p for t in tensors])
+def _array(tensors, what):
+    """One tensor or several as a tuple, and the array of their pointers that the library takes, which the tuple has to outlive."""
+    tensors = (tensors,) if isinstance(tensors, GPUTensor) else tuple(tensors)
+    lib()
+    try:
+        pointers = _lib.calls.pointers(tensors)
+    except TypeError as e:
+        raise TypeError("AdamW %s: %s (call :gpu() on the module first)" % (what, e)) from None
+    return tensors, (TP * max(1, len(tensors))).from_buffer(pointers)
 
 
 class _Tensors:
@@ -27,8 +27,7 @@ class _Tensors:
         return self if obj is None else obj._lists[self.name][0]
 
     def __set__(self, obj, tensors):
-        tensors = _tensors(tensors, "AdamW " + self.name)
-        obj._lists[self.name] = tensors, _array(tensors)
+        obj._lists[self.name] = _array(tensors, self.name)
 
 
 class AdamW:
@@ -87,10 +86,10 @@ class AdamW:
             if mean is not None or square is not None:
                 raise ValueError("AdamW: moments of 32 bits are not copied")
             return self.mean, self.square
-        mean, square = ([GPUTensor(*w.size()) for w in self.weights] if t is None else _tensors(t, "AdamW moments") for t in (mean, square))
+        (mean, means), (square, squares) = (_array([GPUTensor(*w.size()) for w in self.weights] if t is None else t, "moments") for t in (mean, square))
         if not len(mean) == len(square) == len(self.weights):
             raise ValueError("AdamW: a tensor for each of the weights expected")
-        lib().THGPUNN_AdamW8_moments(len(mean), *self._arrays("meanCodes", "rootCodes", "scales"), _array(mean), _array(square))
+        lib().THGPUNN_AdamW8_moments(len(mean), *self._arrays("meanCodes", "rootCodes", "scales"), means, squares)
         return mean, square
 
 
