@@ -416,7 +416,7 @@ static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows
 // (whole), the narrowest team that does, at most a block; else the widest that leaves the fewest columns over.  U: one piece a thread, and up to eight rows at a time, for few
 // rows, which that spreads over more SMs, and for narrow ones, both where k is more than two; else more pieces of two rows at a time.
 // Combine, 8 rows a token, us with one piece and with four: 24 x 4096 3.1 and 4.5, 128 x 4096 3.6 and 4.6, 256 x 4096 5.3 and 4.4, 4096 x 64 3.7 and 5.5; backward 128 x 1024
-// 3.6 and 5.7, 512 x 1024 6.9 and 6.0, 4096 x 64 6.5 and 9.2.  2 rows a token: 8192 x 64 4.5 and 3.5.  Teams of a warp and of eight lanes, 22024 x 20, 6 rows a token: 14 and 4.
+// 3.6 and 5.7, 512 x 1024 6.9 and 6.0, 4096 x 64 6.5 and 9.2.  2 rows a token: 8192 x 64 4.5 and 3.5.  Teams of a warp and of eight lanes, 22024 x 20, 6 rows a token: 10.8 and 4.0.
 template <class F> static void with_columns(long tokens, int D, int k, bool vec, bool whole, F f) {
   auto go = [&](auto VEC, auto U) {
     constexpr int per = (decltype(VEC)::value ? 4 : 1) * decltype(U)::value;

@@ -353,8 +353,9 @@ static __global__ void __launch_bounds__(256) router_backward_kernel(const float
                                                                      long rows, int E, int k) {
   pdl_begin();
   typedef WarpRow<V, VEC> Row;
-  const int lane = threadIdx.x & 31;
-  const long row = blockIdx.x * 8l + (threadIdx.x >> 5);
+  __shared__ __align__(16) float share[8][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long row = blockIdx.x * 8l + warp;
   if (row >= rows) return;
   float w = 0.f, d = 0.f, v[V];
   int expert = -1;
@@ -365,17 +366,23 @@ static __global__ void __launch_bounds__(256) router_backward_kernel(const float
   }
   if (x) Row::load(x + row * ldx, lane, E, v);
   if (expert < 0) w = d = 0.f;                  // (whatever lay there)
+  // each expert's share to its place, through shared memory
+  float out[V], *mine = share[warp];
+#pragma unroll
+  for (int j = 0; j < V; j++) mine[j * 32 + lane] = 0.f;
   const float spread = warp_total(w * d);
-  float out[V];
+  __syncwarp();
+  if (expert >= 0 && expert < E) mine[expert] = x ? d : w * (d - spread);
+  __syncwarp();
+  if constexpr (VEC) {
 #pragma unroll
-  for (int j = 0; j < V; j++) out[j] = 0.f;
-  const float mine = x ? d : w * (d - spread);
-  for (int i = 0; i < k; i++) {
-    const int to = __shfl_sync(0xffffffffu, expert, i);
-    const float add = __shfl_sync(0xffffffffu, mine, i);
+    for (int j = 0; j < V; j += 4) {
+      const float4 q = *reinterpret_cast<const float4 *>(mine + Row::at(j, lane));
+      out[j] = q.x; out[j + 1] = q.y; out[j + 2] = q.z; out[j + 3] = q.w;
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < V; j++)
-      if (Row::at(j, lane) == to) out[j] += add;
+    for (int j = 0; j < V; j++) out[j] = mine[j * 32 + lane];
   }
   if (x) {
     float top = -INFINITY, total = 0.f;
