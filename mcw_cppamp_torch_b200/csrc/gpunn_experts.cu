@@ -248,7 +248,7 @@ struct Rows {            // a matrix of rows at a distance
   long ld;
 };
 
-// rows[pos(t, i)] = x[t]
+// rows[pos(t, i)] = x[t].  8192 x 4096, two rows a token: 60 us, 6.7 TB/s.
 template <int T, int U, bool VEC>
 static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const float *__restrict__ positions, float *__restrict__ rows, long tokens, int k, int D, long most) {
   typedef Columns<T, U, VEC> Cols;
@@ -265,7 +265,8 @@ static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const floa
 }
 
 // The same for few slots, with the ranking: a block for a token and 256 U W of its columns.  A slot's place is the number of slots that name a lower expert,
-// or the same and come before it.  One more block counts for the host, which so gets its counts before any row is copied.
+// or the same and come before it.  One more block counts for the host, which so gets its counts before any row is copied.  24 x 4096, 8 of 64 experts: 8.6 us from the call
+// to the counts, most of them on the way to the GPU and back.
 template <int U, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const float *__restrict__ experts, float *__restrict__ positions, float *__restrict__ rows, int k,
                                                                   int D, int slots, int groups, CountStage tell) {
@@ -305,7 +306,8 @@ static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const 
     if (mine[i] >= 0) a.store(rows + mine[i] * (long)D, D);
 }
 
-// y[t] = residual[t] + sum_i w(t, i) rows[pos(t, i)]; w and the residual may be null
+// y[t] = residual[t] + sum_i w(t, i) rows[pos(t, i)]; w and the residual may be null.  8192 x 4096, two rows a token: 58.7 us, 6.9 TB/s; 24 x 4096, eight rows and a
+// residual: 3.3 us a call; 19056 x 333, two rows: 11.4 us, 6.7 TB/s, from L2 in part.
 template <int T, int U, bool VEC>
 static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const float *__restrict__ w, const float *__restrict__ positions, Rows residual,
                                                               float *__restrict__ y, long tokens, int k, int D, long most) {
@@ -342,6 +344,7 @@ static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const f
 }
 
 // drows[pos(t, i)] = w(t, i) dy[t] and dw(t, i) = <dy[t], rows[pos(t, i)]>, either of them unless null; w may be null.  A team has all columns of its token.
+// 8192 x 2048, eight rows a token: 173 us, 6.6 TB/s; 19056 x 333, two rows: 25 us, 5.0 TB/s.
 constexpr int kDotSlots = 32;
 template <int T, int U, bool VEC>
 static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows, const float *__restrict__ w, const float *__restrict__ positions, Rows dy,

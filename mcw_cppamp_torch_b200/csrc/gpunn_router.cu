@@ -346,7 +346,8 @@ static __global__ void __launch_bounds__(64) router_forward_rows_kernel(const fl
   }
 }
 
-// The gradient of a row's scores.  x is read where the weights are of the whole softmax, and may else be null.
+// The gradient of a row's scores.  x is read where the weights are of the whole softmax, and may else be null.  32768 x 256, 8 chosen: 6.2 us without x (5.5 TB/s of what it
+// writes) and 15.3 with it; 7001 x 77: 3.9 with it.
 template <int V, bool VEC>
 static __global__ void __launch_bounds__(256) router_backward_kernel(const float *__restrict__ x, long ldx, const float *__restrict__ g, long ldg,
                                                                      const float *__restrict__ weights, const float *__restrict__ experts, float *__restrict__ gx,
