@@ -450,7 +450,7 @@ THC_API int THGPUNN_GroupedLinear_backward(THGPUTensor *input, const long *count
  * score and makes its row's weights NaN.  normalize: the weights of a row's chosen experts sum to one; else they are those of the softmax over all
  * its scores.  E <= 1024, k <= 32 and k <= E.
  * updateGradInput: gradInput [R, E] from gradWeights [R, k] and what updateOutput left; gradWeights of slots without an expert are not looked at.  With
- * normalize only input's size is. */
+ * normalize only input's size is.  Results of these and the next functions may not share memory with operands. */
 THC_API int THGPUNN_Router_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *experts, int k, int normalize);
 THC_API int THGPUNN_Router_updateGradInput(THGPUTensor *input, THGPUTensor *gradWeights, THGPUTensor *gradInput, THGPUTensor *weights,
     THGPUTensor *experts, int normalize);
@@ -466,8 +466,8 @@ THC_API int THGPUNN_Dispatch_updateGradInput(THGPUTensor *input, THGPUTensor *gr
 /* Combine (no counterpart in the reference): output [T, size] receives residual + the sum of each token's rows of input [R, size] times their
  * weights [T, k] (NULL: all one); positions as Dispatch leaves them: every row has one slot.  residual [T, size] or NULL.  Slots without a row, whose
  * position is 0 or none of the rows', add nothing whatever their weight.
- * backward: gradInput [R, size] receives each row's weight times its token's gradOutput, gradWeights [T, k] the products <gradOutput, row>, zero for slots
- * without a row; each is skipped when NULL.  The residual's gradient is gradOutput itself. */
+ * backward: gradInput [R, size] receives each row's weight times its token's gradOutput (rows that no slot has are left as they were), gradWeights [T, k] the
+ * products <gradOutput, row>, zero for slots without a row; each is skipped when NULL.  The residual's gradient is gradOutput itself.  size <= 2^23. */
 THC_API int THGPUNN_Combine_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *residual,
     THGPUTensor *output, long size);
 THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *gradOutput,
