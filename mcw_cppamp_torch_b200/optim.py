@@ -1,9 +1,20 @@
-"""Parameter updates that keep a state of their own, over the tensors of `Module.parameters()` or `getParameters()`."""
+"""Parameter updates that keep a state of their own, over the parameters of modules."""
 from . import _lib
 from ._lib import TP, lib
 from .tensor import GPUTensor
 
 BLOCK = 256     # values under one scale of the 8-bit moments
+
+
+def parameters(*modules):
+    """The weights and the gradients of modules, and of those that containers hold, as two lists."""
+    weights, gradients = [], []
+    for module in modules:
+        for m in module.modules_list():
+            w, g = m.parameters() or ([], [])
+            weights += w
+            gradients += g
+    return weights, gradients
 
 
 def _array(tensors, what):
@@ -31,15 +42,16 @@ class _Tensors:
 
 
 class AdamW:
-    """Adam with decoupled weight decay: update() takes a step of all `weights` by their `gradWeights`, tensors or lists of them as
-    `net.parameters()` and `net.getParameters()` give, in one launch.
+    """Adam with decoupled weight decay: update() takes a step of all `weights` by their `gradWeights`, tensors or lists of them as `parameters(net)` and
+    `net.getParameters()` give, in one launch.
 
-        opt = gt.optim.AdamW(*net.getParameters(), learningRate=1e-3)
+        opt = gt.optim.AdamW(*gt.optim.parameters(net), learningRate=1e-3)
         net.zeroGradParameters(); net.backward(...); opt.update()
 
     bits=32: the moments lie in `mean` and `square`, a tensor for each of the weights.  bits=8: in `meanCodes`, `rootCodes` and `scales`, 2.03 bytes a value
     instead of 8, rounded at random by `seed`; moments() gives what they stand for.  `step` holds the number of steps taken, on the device (up to 2^24), so that a
-    recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Gradients may share memory, what a step writes may not."""
+    recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Gradients may share memory, what a step writes may not.
+    Saved along with its module, gt.save([net, opt], path), it has the module's tensors again after loading."""
 
     weights, gradWeights, mean, square, meanCodes, rootCodes, scales = (_Tensors() for _ in range(7))      # tuples: a list put there becomes one
 

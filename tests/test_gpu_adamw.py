@@ -310,6 +310,27 @@ def test_saved_and_continued(gt, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("flat", [False, True])
+def test_saved_with_its_module(gt, tmp_path, bits, flat):
+    """After loading, and after the parameters have been brought into one storage, a step is one of the module's own tensors."""
+    net = gt.nn.Sequential().add(gt.nn.Linear(33, 20)).add(gt.nn.LayerNorm(20)).gpu()
+    params = gt.optim.parameters
+    opt = gt.optim.AdamW(*params(net), bits=bits, seed=3)
+    if flat:
+        net.getParameters()
+    for i, g in enumerate(params(net)[1]):
+        g.copy(normal(i, *g.size()))
+    opt.update()
+    gt.save([net, opt], str(tmp_path / "both"))
+    other, twin = gt.load(str(tmp_path / "both"))
+    before = [t.float() for t in params(net)[0]]
+    opt.update()
+    twin.update()
+    for a, b, c in zip(params(net)[0], params(other)[0], before):
+        assert np.array_equal(a.float(), b.float()) and not np.array_equal(a.float(), c)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_more_values_than_32_bits_count(gt, bits):
     """Both ends and the middle of one tensor of more than 2^31 values, as by themselves; the noise of a place counts on over 2^31."""
     n = 2 ** 31 + 2049 + 7

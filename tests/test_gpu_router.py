@@ -216,3 +216,29 @@ def test_no_rows_and_results_that_change_size(gt):
         w, e = m.forward(gt.gpu(x))
         assert w.size() == (rows, 3) and np.array_equal(e.float(), choose(x, 3))
         assert m.backward(gt.gpu(x), gt.gpu(np.ones((rows, 3), np.float32))).size() == (rows, 20)
+
+
+@pytest.mark.parametrize("experts", [256, 300])
+def test_more_values_than_32_bits_count(gt, experts):
+    """Rows at both ends of more than 2^31 scores, as by themselves, with equal scores between them."""
+    rows, k = 2 ** 31 // experts + 1009, 2
+    few = scores(4, 40, experts)
+    x = gt.GPUTensor(rows, experts).fill(0.5)
+    x.narrow(1, 1, 20).copy(few[:20])
+    x.narrow(1, rows - 19, 20).copy(few[20:])
+    gw = gt.GPUTensor(rows, k).fill(0.0)
+    g = np.random.RandomState(1).standard_normal((40, k)).astype(np.float32)
+    gw.narrow(1, 1, 20).copy(g[:20])
+    gw.narrow(1, rows - 19, 20).copy(g[20:])
+    m, small = gt.nn.Router(k, False), gt.nn.Router(k, False)
+    got, want = m.forward(x), [t.float() for t in small.forward(gt.gpu(few))]
+
+    def ends(t):
+        return np.concatenate([t.narrow(1, 1, 20).float(), t.narrow(1, rows - 19, 20).float()])
+    assert np.array_equal(ends(got[1]), want[1]) and np.all(np.abs(ends(got[0]) - want[0]) <= 50 * U * want[0])
+    between = got[1].narrow(1, rows // 2, 3).float()
+    assert np.array_equal(between, np.tile([1, 2], (3, 1)))
+    gi, wg = ends(m.backward(x, gw)), small.backward(gt.gpu(few), gt.gpu(g)).float()
+    # two evaluations of p (g - sum g w), whose p and w are those above
+    p = soft(few, choose(few, k), False)
+    assert np.all(np.abs(gi - wg) <= 2 * 60 * U * p * (np.abs(g).max(1) * 2)[:, None] + 1e-37)

@@ -272,6 +272,17 @@ def test_adamw_arguments(fake):  # noqa: F811
         m.moments(m.mean, m.square)
 
 
+def test_parameters_of_modules():
+    """Those of containers' modules too; modules without any add nothing."""
+    a, b = nn.Linear(3, 2), nn.LayerNorm(2)
+    net = nn.Sequential().add(a).add(nn.Sequential().add(nn.Router(1)).add(b)).add(nn.LayerNorm(2, affine=False))
+    weights, gradients = optim.parameters(net, a)
+    assert [id(t) for t in weights] == [id(t) for t in (a.weight, a.bias, b.weight, b.bias, a.weight, a.bias)]
+    assert [id(t) for t in gradients] == [id(t) for t in (a.gradWeight, a.gradBias, b.gradWeight, b.gradBias, a.gradWeight, a.gradBias)]
+    with pytest.raises(TypeError, match="call :gpu"):
+        optim.AdamW(*optim.parameters(net))
+
+
 def test_adamw_keeps_the_tensors_it_is_given(fake):  # noqa: F811
     """What the library gets are the tensors of the fields, also after others have been put there; a field is no list to be changed behind it."""
     m = adamw(fake)
