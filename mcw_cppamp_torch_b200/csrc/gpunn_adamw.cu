@@ -11,6 +11,14 @@
 // 1 - b2, a thousandth of itself or less, where codes are 6 to 13 % apart, and rounded to the nearest it would stay where it is for good.  Random bits are a
 // hash of the value's place, the tensor's number, the step's and a seed, and every operation on the way to a code is a rounded one of its own, in the order
 // written here: the same state, gradients and seed give the same codes.
+//
+// A value below the least codes, 2^-19 of its block's largest m and 2^-20 of the largest r, is mostly rounded to zero and now and then up, and an m that was rounded up
+// over an r that was rounded down would move its weight by hundreds of learning rates.  So what the step divides by has two bounds.  It is no less than 2^-19 of the
+// scale that r was decoded with, from where a gradient's share of v, (1 - b2) / (1 - b2^t), is a sixteenth at most; before that one gradient over its own root moves a
+// weight by less than half a rate.  And it is no less than |m| over the most that any gradients could make it: by Cauchy's inequality |m| <= C sqrt(v) with
+// C = (1 - b1) / sqrt((1 - b2) (1 - b1^2 / b2)), 7.3 at 0.9 and 0.999, which the bias corrections make less; C at least 2, for the codes' noise about a steady
+// gradient's 1.  Of a block with one value whose gradients are of size 1 the others, with 1e-6 (1e-7): steps of up to 183 (213) rates, 1.8 (7.4) in the mean, without
+// bounds, and with them 7.3 in the first sixteen steps, 1.8 behind them, 0.22 (0.09) in the mean.  Exact moments give 1.1 and 0.23.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -47,13 +55,15 @@ struct AdamStep {
   bool last;                 // the launch that counts the step
   float lr, beta1, beta2, rest1, rest2, eps, keep;    // rest: 1 - beta, keep: 1 - lr decay
   float log1, log2;          // of the betas
+  float most;                // learning rates a step in 8 bits is at most
   unsigned seed;
   int number;                // of the table's first tensor
 };
 // What a step's number t decides: lr / (1 - b1^t) and 1 / sqrt(1 - b2^t).  1 - b^t = -expm1(t log b): t log b carries its rounding to the result at most as it is,
 // where a power of b near one would lose it.
+// In 8 bits also what of m, and of a scale, the step's divisor is at least.
 struct AdamFactors {
-  float rate, root;
+  float rate, root, share, least;
   unsigned step;
 };
 // By threads 0 and 1 into shared memory; a barrier has to follow.
@@ -62,8 +72,12 @@ static __device__ __forceinline__ void adam_factors(const AdamStep &s, AdamFacto
   const float step = truncf(s.step[0]) + 1.f, rest = -expm1f(step * (threadIdx.x ? s.log2 : s.log1));
   if (threadIdx.x == 0) {
     f.rate = s.lr / rest;
+    f.share = 1.f / (s.most * rest);
     f.step = (unsigned)step;
-  } else f.root = 1.f / sqrtf(rest);
+  } else {
+    f.root = 1.f / sqrtf(rest);
+    f.least = rest >= 16.f * s.rest2 ? 0x1p-19f : 0.f;
+  }
 }
 // The last block of the last launch counts the step: by then every block has read, and used, its number.  Nothing else passes between blocks here, so that there is
 // no fence to wait for.
@@ -218,6 +232,12 @@ static __device__ __forceinline__ float larger_size(float a, float b) {
   asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// The largest size of three; a NaN if there is one.
+static __device__ __forceinline__ float largest_size(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 static __device__ __forceinline__ float warp_largest(float v) {
   float r;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -254,8 +274,8 @@ static __device__ __forceinline__ void bring(const AdamTensor &a, long block, in
                      lane < 18 ? (const char *)((const unsigned *)a.m + block * 64) + (lane - 16) * 128 : (const char *)((const unsigned *)a.v + block * 64) + (lane - 18) * 128;
   asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
 }
-// A warp for a block of 256 values, eight a lane, and for others at the same distance, the next of which is brought to L2 meanwhile.  46 M values: 151 us, 4.9 TB/s; what
-// holds it back is the work on codes, 73 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the
+// A warp for a block of 256 values, eight a lane, and for others at the same distance, the next of which is brought to L2 meanwhile.  46 M values: 154 us, 4.8 TB/s; what
+// holds it back is the work on codes, 88 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the
 // codes and branch.  Tried, with a tensor looked up for four turns at a time (143): a block for each chunk, which does not stay, 156; five blocks an SM in 48 registers 150
 // (170 with what is brought ahead); a turn's loads in registers ahead of it 178; nothing brought ahead 158.
 template <int N>
@@ -264,7 +284,8 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
   __shared__ AdamFactors shared;
   adam_factors(s, shared);
   __syncthreads();
-  const AdamFactors f = shared;
+  AdamFactors f = shared;
+  f.share /= f.root;
   const unsigned chunks = table.first[table.count];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long jump = (long)(kAdamTurn / kAdamBlock) * gridDim.x;      // to the warp's next block, if it is of the same tensor
@@ -291,6 +312,8 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
       }
       bring(a, block + jump, lane);
       float top_m = 0.f, top_r = 0.f;
+      const float least = f.least * scale.y;
+      const Pair share(f.share, f.share);
       const Pair scale_m2(scale.x, scale.x), scale_r2(scale.y, scale.y), beta1(s.beta1, s.beta1), beta2(s.beta2, s.beta2), rest1(s.rest1, s.rest1), rest2(s.rest2, s.rest2);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -308,10 +331,13 @@ static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_const
           r[h][j + 1] = __fsqrt_rn(y);
           top_m = larger_size(larger_size(top_m, m[h][j]), m[h][j + 1]);
           top_r = larger_size(larger_size(top_r, r[h][j]), r[h][j + 1]);
-          // the weights' step, as adam_weight
-          fused(Pair(r[h][j], r[h][j + 1]), Pair(f.root, f.root), Pair(s.eps, s.eps)).get(x, y);
-          fused(Pair(-f.rate, -f.rate), Pair(m[h][j], m[h][j + 1]) * Pair(reciprocal(x), reciprocal(y)), Pair(ww[h][j], ww[h][j + 1]) * Pair(s.keep, s.keep))
-              .get(ww[h][j], ww[h][j + 1]);
+          // the weights' step, as adam_weight but for its bounds
+          const Pair mj(m[h][j], m[h][j + 1]);
+          (mj * share).get(x, y);
+          x = largest_size(r[h][j], least, x);
+          y = largest_size(r[h][j + 1], least, y);
+          fused(Pair(x, y), Pair(f.root, f.root), Pair(s.eps, s.eps)).get(x, y);
+          fused(Pair(-f.rate, -f.rate), mj * Pair(reciprocal(x), reciprocal(y)), Pair(ww[h][j], ww[h][j + 1]) * Pair(s.keep, s.keep)).get(ww[h][j], ww[h][j + 1]);
         }
         store_four(w + h * 128 + lane * 4, ww[h], n - (h * 128 + lane * 4), vw);
       }
@@ -501,6 +527,8 @@ static AdamStep adam_step(THGPUTensor *step, double lr, double beta1, double bet
   s.lr = (float)lr; s.beta1 = (float)beta1; s.beta2 = (float)beta2; s.rest1 = (float)(1.0 - beta1); s.rest2 = (float)(1.0 - beta2);
   s.eps = (float)eps; s.keep = (float)(1.0 - lr * decay);
   s.log1 = (float)std::log(beta1); s.log2 = (float)std::log(beta2);      // (of zero: minus infinity, and then 1 - b^t is one)
+  const double left = 1.0 - beta1 * beta1 / beta2;      // (beta2 zero: minus infinity, or with beta1 zero too a NaN: no bound)
+  s.most = left > 0 ? (float)std::max(2.0, (1.0 - beta1) / std::sqrt((1.0 - beta2) * left)) : INFINITY;
   s.seed = (unsigned)(unsigned long)seed;
   s.number = 0;
   return s;
