@@ -466,7 +466,7 @@ THC_API int THGPUNN_Dispatch_updateGradInput(THGPUTensor *input, THGPUTensor *gr
 /* Combine (no counterpart in the reference): output [T, size] receives residual + the sum of each token's rows of input [R, size] times their
  * weights [T, k] (NULL: all one); positions as Dispatch leaves them: every row has one slot.  residual [T, size] or NULL.  Slots without a row, whose
  * position is 0 or none of the rows', add nothing whatever their weight.
- * backward: gradInput [R, size] receives each row's weight times its token's gradOutput (rows that no slot has are left as they were), gradWeights [T, k] the
+ * backward: gradInput [R, size] receives each row's weight times its token's gradOutput (zero for rows that no slot has), gradWeights [T, k] the
  * products <gradOutput, row>, zero for slots without a row; each is skipped when NULL.  The residual's gradient is gradOutput itself.  size <= 2^23. */
 THC_API int THGPUNN_Combine_updateOutput(THGPUTensor *input, THGPUTensor *weights, THGPUTensor *positions, THGPUTensor *residual,
     THGPUTensor *output, long size);

@@ -204,7 +204,7 @@ template <int T, int U, bool VEC> struct Columns {
   int c;                                              // the thread's first column; its u-th piece is u T W further on
   Columns() = default;
   __device__ __forceinline__ explicit Columns(long piece) : c((int)(piece * (T * U * W)) + (int)(threadIdx.x % T) * W) {}
-  static __device__ __forceinline__ long token() { return blockIdx.x * (long)(256 / T) + threadIdx.x / T; }
+  static __device__ __forceinline__ long token(int before = 0) { return (blockIdx.x - before) * (long)(256 / T) + threadIdx.x / T; }     // (blocks before its own)
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int j = 0; j < U * W; j++) v[j] = 0.f;
@@ -343,17 +343,86 @@ static __global__ void __launch_bounds__(256) rows_sum_kernel(Rows rows, const f
   a.store(y + t * D, D);
 }
 
+// Rows that no slot names, which Combine's gradient makes zero: blocks of their own look for them, each among some rows, in all slots, whose places they read in 16-byte
+// pieces ahead.  A place stands for the row that row_at gives: its distance from the block's first row's place is exact, and in the sum with 2^23, rounded down, the low bits are
+// its whole part; distances below zero, beyond the rows and no numbers become words that are too large.
+constexpr int kClearRows = 32768;         // of a block at most: a bit each
+constexpr int kClearBlocks = 64;
+static __device__ __noinline__ void clear_rows(unsigned *named, const float *__restrict__ positions, long slots, float *__restrict__ rows, long first, int n, int D) {
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  for (int w = t; w * 32 < n; w += 256) named[w] = 0;
+  __syncthreads();
+  const unsigned words = (unsigned)__cvta_generic_to_shared(named), valid = first < kMostSlots ? (unsigned)min((long)n, kMostSlots - first) : 0;
+  const float from = (float)(first + 1);               // (exact where rows are valid)
+  auto name = [&](float place) {
+    const unsigned r = __float_as_uint(__fadd_rd(place - from, 8388608.f)) - 0x4b000000u;
+    asm volatile("{ .reg .pred p; setp.lt.u32 p, %0, %1; @p red.shared.or.b32 [%2], %3; }" ::"r"(r), "r"(valid), "r"(words + (r >> 5) * 4), "r"(1u << (r & 31)) : "memory");
+  };
+  const long head = min(slots, (long)((16 - ((uintptr_t)positions & 15)) & 15) / 4), quads = (slots - head) / 4;
+  if (t < head) name(__ldg(positions + t));
+  if (t < slots - head - 4 * quads) name(__ldg(positions + head + 4 * quads + t));
+  const float4 *p = reinterpret_cast<const float4 *>(positions + head);
+  float4 q[4], next[4];
+  auto load = [&](float4 (&v)[4], long s) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = s + 256 * i < quads ? __ldg(p + s + 256 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(q, t);
+  for (long s = t; s < quads; s += 1024) {
+    load(next, s + 1024);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      name(q[i].x); name(q[i].y); name(q[i].z); name(q[i].w);
+      q[i] = next[i];
+    }
+  }
+  __syncthreads();
+  const bool vec = D % 4 == 0 && ((uintptr_t)rows & 15) == 0;
+  for (int w = warp; w * 32 < n; w += 8) {
+    unsigned none = ~named[w];
+    if (n - w * 32 < 32) none &= (1u << (n - w * 32)) - 1;
+    for (; none; none &= none - 1) {
+      float *row = rows + (first + w * 32 + __ffs(none) - 1) * D;
+      if (vec)
+        for (int c = 4 * lane; c < D; c += 128) *reinterpret_cast<float4 *>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+      else
+        for (int c = lane; c < D; c += 32) row[c] = 0.f;
+    }
+  }
+}
+
+// All rows zero.  (A memory operation between kernels takes 2 us more than one that starts as a programmatic dependent.)
+static __global__ void __launch_bounds__(256) clear_all_kernel(float *__restrict__ p, long n) {
+  pdl_begin();
+  const long head = min(n, (long)((16 - ((uintptr_t)p & 15)) & 15) / 4), quads = (n - head) / 4, step = gridDim.x * 256l;
+  const long t = blockIdx.x * 256l + threadIdx.x;
+  if (t < head) p[t] = 0.f;
+  if (t < n - head - 4 * quads) p[head + 4 * quads + t] = 0.f;
+  float4 *q = reinterpret_cast<float4 *>(p + head);
+  for (long i = t; i < quads; i += step) q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
 // drows[pos(t, i)] = w(t, i) dy[t] and dw(t, i) = <dy[t], rows[pos(t, i)]>, either of them unless null; w may be null.  A team has all columns of its token.
 // 8192 x 2048, eight rows a token: 173 us, 6.6 TB/s; 19056 x 333, two rows: 25 us, 5.0 TB/s.
 constexpr int kDotSlots = 32;
 template <int T, int U, bool VEC>
 static __global__ void __launch_bounds__(256) rows_sum_backward_kernel(Rows rows, const float *__restrict__ w, const float *__restrict__ positions, Rows dy,
-                                                                       float *__restrict__ drows, float *__restrict__ dw, long tokens, int k, int D, long most) {
+                                                                       float *__restrict__ drows, float *__restrict__ dw, long tokens, int k, int D, long most,
+                                                                       int clears, int each) {
   pdl_begin();
   typedef Columns<T, U, VEC> Cols;
   constexpr int WARPS = T > 32 ? T / 32 : 1;       // of a team
-  __shared__ float dots[256 / T][WARPS][kDotSlots];
-  const long t = Cols::token();
+  __shared__ union {
+    float dots[256 / T][WARPS][kDotSlots];
+    unsigned named[kClearRows / 32];
+  } shared;
+  if ((int)blockIdx.x < clears) {
+    const long first = blockIdx.x * (long)each;
+    clear_rows(shared.named, positions, tokens * k, drows, first, (int)min((long)each, most - first), D);
+    return;
+  }
+  auto &dots = shared.dots;
+  const long t = Cols::token(clears);
   const int team = threadIdx.x / T, member = threadIdx.x % T, pieces = (D + T * U * Cols::W - 1) / (T * U * Cols::W);
   const bool live = t < tokens;                    // (teams of a warp stay together: the others take part in its exchanges)
   constexpr int B = U == 1 ? 4 : 2;                // as rows_at_once, with gradOutput's row in registers as well
@@ -638,6 +707,21 @@ THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, T
   const long xs[2] = {rows, D}, ws[2] = {tokens, k};
   if (gradInput) size_result(gradInput, 2, xs, {input, weights, positions, gradOutput, gradWeights}, 5);
   if (gradWeights) size_result(gradWeights, 2, ws, {input, weights, positions, gradOutput, gradInput}, 6);
+  // Rows that no slot names: looked for by blocks in front of the tokens', unless these would read more than a twelfth of what the others move, or take longer, as with many narrow
+  // rows.  Then all rows are zero first.  us a call without either, searched, and cleared: 8192 x 2048, 8 rows a token 172.1, 172.1; 1537 x 333, 4 rows 5.8, 5.9; 19056 x 333, 2 rows
+  // 25.1, 25.2; 512 x 1024, 8 rows 5.9, 7.2; 4096 x 64, 8 rows 4.8, 7.6, 8.1; 32768 x 64, 2 rows 6.7, 12.8, 10.4; 32768 x 128, 8 rows 55.0, 56.9.
+  int clears = 0, each = 0;
+  if (gradInput && rows) {
+    clears = (int)std::min((rows + 255) / 256, std::min((long)kClearBlocks, std::max(1l, D / 4)));
+    clears = std::max(clears, ceil_div(rows, kClearRows));
+    const bool search = tokens * k <= kClearRows || (D >= 128 && clears <= D / 4);
+    if (!tokens || !search) {
+      const long blocks = std::min((rows * D + 4095) / 4096, ctx().sm_count * 8l);
+      pdl_launch(clear_all_kernel, (unsigned)blocks, 256, 0, data_ptr(gradInput), rows * D);
+      check_launch("Combine_backward");
+      clears = 0;
+    } else each = ceil_div(rows, clears);
+  }
   if (tokens == 0 || (!gradInput && !gradWeights)) return 0;
   TensorRef p(tensor_new_contiguous(positions)), w(weights ? tensor_new_contiguous(weights) : nullptr);
   DenseRows g(gradOutput);
@@ -646,8 +730,8 @@ THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, T
     const bool vec = pieces_of_four({x, Rows{g.p, g.ld}, Rows{gx, D}}, (int)D);
     with_columns(tokens, (int)D, (int)k, vec, true, [&](auto T, auto U, auto VEC) {
       constexpr int t = decltype(T)::value, u = decltype(U)::value;
-      pdl_launch(rows_sum_backward_kernel<t, u, decltype(VEC)::value>, (unsigned)ceil_div(tokens, 256 / t), 256, 0, x, weights ? data_ptr(w) : nullptr, data_ptr(p),
-                 Rows{g.p, g.ld}, gx, gw, tokens, (int)k, (int)D, rows);
+      pdl_launch(rows_sum_backward_kernel<t, u, decltype(VEC)::value>, (unsigned)(ceil_div(tokens, 256 / t) + clears), 256, 0, x, weights ? data_ptr(w) : nullptr, data_ptr(p),
+                 Rows{g.p, g.ld}, gx, gw, tokens, (int)k, (int)D, rows, clears, each);
     });
     check_launch("Combine_backward");
   };
