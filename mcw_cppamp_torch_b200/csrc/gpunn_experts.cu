@@ -19,10 +19,12 @@ namespace thc {
 constexpr long kMostSlots = 1l << 24;     // positions are floats
 constexpr int kMostGroups = 4096;
 constexpr long kMostValues = 1l << 23;    // of a row: its pieces are a dimension of the grid
-// Three ways to rank the slots, us a call with 64 groups and rows of 16 values: by every block of the copy for its own token (2048 slots: 9.3, 4096: 14.3), in a launch of
-// its own (10.1, 10.3; 16384: 11.7, 32768: 13.7, 65536: 17.2), in two (11.7, 11.8, 11.9, 12.2, 12.8).  Between the last two, with rows of 1024 values, the line lies
+// Three ways to rank the slots, us a call with 64 groups: by every block of the copy for its own token, in a launch of its own, in two.  The first reads all slots in each of its
+// blocks, one for a token and 1024 of its columns, or 256 without 16-byte pieces: where blocks times slots are 2^20 or fewer.  Blocks x slots, first and second way: 96 x 192 9.1 and
+// 9.7; 512 x 1024 9.5 and 10.6; 256 x 2048 9.9 and 10.9; 2048 x 512 9.5 and 9.8; 1024 x 1024 9.8 and 10.6; 1024 x 2048 11 to 14 and 11; 2048 x 2048 15 and 11; 32768 x 2048 108 and 14.
+// The second and the third, rows of 16 values: 16384 slots 11.7 and 11.9, 32768 13.7 and 12.2, 65536 17.2 and 12.8.  With rows of 1024 values the line lies
 // at 32768 as well (34.3 and 34.7; 65536: 62.4 and 60.0); with 1024 groups further on (36.5 and 42.1; 64.5 and 72.5).
-constexpr long kFewSlots = 2048, kRankedSlots = 32768;
+constexpr long kFewSlots = 2048, kFewReads = 1l << 20, kRankedSlots = 32768;
 constexpr int kRankedGroups = 1024;       // of the second way: a thread each
 
 // The expert of a slot, from 1; 0: none; -1: the number stands for no expert.
@@ -526,12 +528,12 @@ static bool pieces_of_four(std::initializer_list<Rows> all, int D) {
 
 // ---- launches
 // Whether slots may be ranked block by block.
-static bool are_few(long slots, int k) { return slots <= kFewSlots && k <= 64; }
+static bool are_few(long slots, int k, long blocks) { return slots <= kFewSlots && k <= 64 && slots * blocks <= kFewReads; }
 
 static void dispatch(Rows x, const float *experts, long tokens, int k, int D, int groups, float *positions, float *rows, const CountStage &tell) {
   const long slots = tokens * k;
   const bool vec = pieces_of_four({x, Rows{rows, D}}, D);
-  if (are_few(slots, k)) {
+  if (are_few(slots, k, tokens * ceil_div(D, vec ? 1024 : 256))) {
     const size_t smem = sizeof(int) * std::max(slots + k, groups + 1l);
     if (vec) pdl_launch(few_rows_out_kernel<1, true>, dim3((unsigned)tokens + 1, (unsigned)ceil_div(D, 1024)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
     else pdl_launch(few_rows_out_kernel<1, false>, dim3((unsigned)tokens + 1, (unsigned)ceil_div(D, 256)), 256, smem, x, experts, positions, rows, k, D, (int)slots, groups, tell);
