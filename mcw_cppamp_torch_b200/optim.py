@@ -28,6 +28,19 @@ def _array(tensors, what):
     return tensors, (TP * max(1, len(tensors))).from_buffer(pointers)
 
 
+def _once(weights, gradients):
+    """Each of the weights once, by its memory, with its gradient: a module that occurs several times lists its tensors as often."""
+    seen, kept = {}, []
+    for i, (w, g) in enumerate(zip(weights, gradients)):
+        at, n = w.data_ptr(), w.nElement()
+        first, gradient = seen.setdefault((at, n), (i, g.data_ptr())) if n else (i, None)
+        if first == i:
+            kept.append(i)
+        elif gradient != g.data_ptr():
+            raise ValueError("AdamW: tensors %d and %d are the same weights, with two gradients" % (first + 1, i + 1))
+    return tuple(weights[i] for i in kept), tuple(gradients[i] for i in kept)
+
+
 class _Tensors:
     """A sequence of tensors as a field: kept as a tuple, so that the array of them that the library takes is made once for each that is put there."""
 
@@ -50,7 +63,8 @@ class AdamW:
 
     bits=32: the moments lie in `mean` and `square`, a tensor for each of the weights.  bits=8: in `meanCodes`, `rootCodes` and `scales`, 2.03 bytes a value
     instead of 8, rounded at random by `seed`; moments() gives what they stand for.  `step` holds the number of steps taken, on the device (up to 2^24), so that a
-    recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Gradients may share memory, what a step writes may not.
+    recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Weights that are listed again, as those of a module that occurs twice,
+    are updated once.  Gradients may share memory, what a step writes may not.
     Saved along with its module, gt.save([net, opt], path), it has the module's tensors again after loading."""
 
     weights, gradWeights, mean, square, meanCodes, rootCodes, scales = (_Tensors() for _ in range(7))      # tuples: a list put there becomes one
@@ -60,6 +74,9 @@ class AdamW:
         self.weights, self.gradWeights = weights, gradWeights
         if len(self.weights) != len(self.gradWeights):
             raise ValueError("AdamW: a gradient for each tensor expected")
+        once = _once(self.weights, self.gradWeights)
+        if len(once[0]) < len(self.weights):
+            self.weights, self.gradWeights = once
         if bits not in (8, 32):
             raise ValueError("AdamW: moments are held in 8 or in 32 bits")
         self.learningRate, self.beta1, self.beta2, self.epsilon, self.weightDecay = learningRate, beta1, beta2, epsilon, weightDecay
