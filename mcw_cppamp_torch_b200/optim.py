@@ -48,7 +48,11 @@ class _Tensors:
         self.name = name
 
     def __get__(self, obj, owner=None):
-        return self if obj is None else obj._lists[self.name][0]
+        if obj is None:
+            return self
+        if self.name not in obj._lists:      # the other width's moments
+            raise AttributeError("AdamW: no %s among the tensors of this one" % self.name)
+        return obj._lists[self.name][0]
 
     def __set__(self, obj, tensors):
         obj._lists[self.name] = _array(tensors, self.name)

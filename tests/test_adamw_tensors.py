@@ -1,10 +1,11 @@
-"""Which tensors optim.AdamW updates: each once, also where a module occurs twice."""
+"""Which tensors optim.AdamW updates: each once, also where a module occurs twice; and the fields of the other width's moments."""
 import numpy as np
 import pytest
 
 import mcw_cppamp_torch_b200 as gt
 from mcw_cppamp_torch_b200 import nn, optim
 from test_feedforward_refusals import fake  # noqa: F401
+from test_routing_refusals import adamw
 
 
 def test_weights_listed_again(fake):  # noqa: F811
@@ -18,6 +19,14 @@ def test_weights_listed_again(fake):  # noqa: F811
         optim.AdamW([b, a, again], [gb, ga, fake(7, 3)])
     # the start of a tensor is another one; whether they share memory the call says
     assert len(optim._once((b, b.narrow(1, 1, 9)), (gb, gb.narrow(1, 1, 9)))[0]) == 2
+
+
+def test_moments_of_the_other_width(fake):  # noqa: F811
+    m = adamw(fake, 32)
+    del m._lists["scales"], m._lists["meanCodes"]
+    assert not hasattr(m, "scales") and getattr(m, "meanCodes", None) is None and hasattr(m, "mean")
+    with pytest.raises(AttributeError, match="no scales"):
+        m.scales
 
 
 @pytest.mark.gpu
