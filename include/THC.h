@@ -481,7 +481,7 @@ THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, T
  * of sqrt(v)): 64, 64 and 2 floats for each 256 values of a tensor or part of them, zero at the start.  A code c stands for
  * (f(b + c * 2^s) - f(b)) * scale, f(i) the float of the bits i, b those of 2^-16; codes of m have a sign bit above 7 others and s = 20, those of
  * sqrt(v) 8 bits and s = 19.  Values are rounded up or down at random by their distance from the codes beside them, by a hash of the place, the tensor's index, the
- * step and `seed`: the same call on the same state gives the same bits.  A gradient that is not finite makes its block's moments so.
+ * step and `seed`: the same call on the same state gives the same bits.  With a seed of few bits set neighbours have the same noise some steps apart.  A gradient that is not finite makes its block's moments so.
  * For the sake of values far below their block's largest, w's step divides by no less than 2^-19 scale in sqrt(v)'s place where 1 - beta2^t >= 16 (1 - beta2), scale that of the
  * block's sqrt(v) before the call, nor by less than makes the step lr * max(2, (1 - beta1) / sqrt((1 - beta2) (1 - beta1^2 / beta2))), before eps (no such bound where
  * beta1^2 >= beta2): no gradients make a step of Adam's with exact moments longer.

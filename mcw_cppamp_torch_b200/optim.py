@@ -4,6 +4,9 @@ from ._lib import TP, lib
 from .tensor import GPUTensor
 
 BLOCK = 256     # values under one scale of the 8-bit moments
+# The rounding noise of 8-bit moments is a hash of (seed ^ step * odd number) + place * the same number: with the seed 0 a place's noise is that of its neighbour a step later, with
+# other seeds of few bits some steps later.  Of this one (digits of e), in a million steps, no two that are up to eight apart have the same noise less than a million places apart.
+SEED = 0xb7e15163
 
 
 def parameters(*modules):
@@ -66,14 +69,14 @@ class AdamW:
         net.zeroGradParameters(); net.backward(...); opt.update()
 
     bits=32: the moments lie in `mean` and `square`, a tensor for each of the weights.  bits=8: in `meanCodes`, `rootCodes` and `scales`, 2.03 bytes a value
-    instead of 8, rounded at random by `seed`; moments() gives what they stand for.  `step` holds the number of steps taken, on the device (up to 2^24), so that a
+    instead of 8, rounded at random by `seed` (a word with many bits set: see SEED); moments() gives what they stand for.  `step` holds the number of steps taken, on the device (up to 2^24), so that a
     recorded update counts on when it is replayed; learningRate and the others are those of the recording.  Weights that are listed again, as those of a module that occurs twice,
     are updated once.  Gradients may share memory, what a step writes may not.
     Saved along with its module, gt.save([net, opt], path), it has the module's tensors again after loading."""
 
     weights, gradWeights, mean, square, meanCodes, rootCodes, scales = (_Tensors() for _ in range(7))      # tuples: a list put there becomes one
 
-    def __init__(self, weights, gradWeights, learningRate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, bits=32, seed=0):
+    def __init__(self, weights, gradWeights, learningRate=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, bits=32, seed=SEED):
         self._lists = {}
         self.weights, self.gradWeights = weights, gradWeights
         if len(self.weights) != len(self.gradWeights):

@@ -1,10 +1,13 @@
-"""Which tensors optim.AdamW updates: each once, also where a module occurs twice; and the fields of the other width's moments."""
+"""Which tensors optim.AdamW updates: each once, also where a module occurs twice; the fields of the other width's moments; the default seed."""
+import inspect
+
 import numpy as np
 import pytest
 
 import mcw_cppamp_torch_b200 as gt
 from mcw_cppamp_torch_b200 import nn, optim
 from test_feedforward_refusals import fake  # noqa: F401
+from test_gpu_adamw import hashed
 from test_routing_refusals import adamw
 
 
@@ -27,6 +30,17 @@ def test_moments_of_the_other_width(fake):  # noqa: F811
     assert not hasattr(m, "scales") and getattr(m, "meanCodes", None) is None and hasattr(m, "mean")
     with pytest.raises(AttributeError, match="no scales"):
         m.scales
+
+
+def test_noise_of_the_default_seed():
+    """No place has the noise that a place near it had some steps before.  (Two times 2^12 hashes of 32 bits have 2^24 / 2^32 equal pairs by chance.)"""
+    seed = inspect.signature(optim.AdamW).parameters["seed"].default
+    noise = [hashed(4096, 0, step, seed) for step in range(1, 40)]
+    for i, a in enumerate(noise):
+        for b in noise[i + 1:i + 9]:
+            assert len(np.intersect1d(a, b)) <= 2
+    # a hash that does repeat is seen
+    assert len(np.intersect1d(hashed(4096, 0, 1, 0), hashed(4096, 0, 2, 0))) == 4095
 
 
 @pytest.mark.gpu
