@@ -267,15 +267,15 @@ static __global__ void __launch_bounds__(256) rows_out_kernel(Rows x, const floa
 }
 
 // The same for few slots, with the ranking: a block for a token and 256 U W of its columns.  A slot's place is the number of slots that name a lower expert,
-// or the same and come before it.  The first block counts for the host: behind the others it would start, if these are more than find room at once, when some of them have copied their
-// rows.  24 x 4096, 8 of 64 experts: 8.6 us from the call to the counts, most of them on the way to the GPU and back.
+// or the same and come before it.  One more block counts for the host, which so gets its counts before any row is copied.  24 x 4096, 8 of 64 experts: 8.6 us from the call
+// to the counts, most of them on the way to the GPU and back.
 template <int U, bool VEC>
 static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const float *__restrict__ experts, float *__restrict__ positions, float *__restrict__ rows, int k,
                                                                   int D, int slots, int groups, CountStage tell) {
   pdl_begin();
   extern __shared__ int expert[];       // [slots] and the token's rows [k], or the counts [groups + 1]
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == gridDim.x - 1) {
     if (blockIdx.y) return;
     for (int g = t; g <= groups; g += 256) expert[g] = 0;
     __syncthreads();
@@ -288,7 +288,7 @@ static __global__ void __launch_bounds__(256) few_rows_out_kernel(Rows x, const 
     return;
   }
   int *mine = expert + slots;
-  const long token = blockIdx.x - 1;
+  const long token = blockIdx.x;
   Columns<256, U, VEC> a(blockIdx.y);
   a.load(x.p + token * x.ld, D);
   for (int s = t; s < slots; s += 256) expert[s] = slot_expert(experts[s], groups);
