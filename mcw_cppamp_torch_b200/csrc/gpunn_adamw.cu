@@ -276,7 +276,7 @@ static __device__ __forceinline__ void bring(const AdamTensor &a, long block, in
 }
 // A warp for a block of 256 values, eight a lane, and for others at the same distance, the next of which is brought to L2 meanwhile.  46 M values: 154 us, 4.8 TB/s; what
 // holds it back is the work on codes, 88 instructions a value and lane, half of them on whole numbers, which issue at half rate, and the roots, which have to be exact for the
-// codes and branch.  Tried, with a tensor looked up for four turns at a time (143): a block for each chunk, which does not stay, 156; five blocks an SM in 48 registers 150
+// codes and branch.  Tried before the step's bounds, with a tensor looked up for four turns at a time (143): a block for each chunk, which does not stay, 156; five blocks an SM in 48 registers 150
 // (170 with what is brought ahead); a turn's loads in registers ahead of it 178; nothing brought ahead 158.
 template <int N>
 static __global__ void __launch_bounds__(256, 4) adam8_kernel(const __grid_constant__ AdamTable<N> table, const AdamStep s) {

@@ -6,7 +6,8 @@
 //   Combine   y[t] = residual[t] + sum_i w(t, i) rows[pos(t, i)];  drows[pos(t, i)] = w(t, i) dy[t],  dw(t, i) = <dy[t], rows[pos(t, i)]>
 //
 // A row is D values of 4 bytes and is read or written once: all of it is bound by HBM, in small calls by launches.  Each thread of a token's team takes the
-// same columns of all its rows, so that nothing but the dot products crosses threads, and every result has one writer and one order.
+// same columns of all its rows, so that nothing but the dot products crosses threads, and every result has one writer and one order
+// (in Combine's gradient of rows of which each has one slot; rows without one are zero).
 #include <cstring>
 #include <type_traits>
 #include <vector>

@@ -4,7 +4,7 @@
 //   w_i = exp(s_i - max) / sum exp(s_j - max), j over the chosen (normalize) or over all
 //   ds_j = w_j (g_j - sum_i g_i w_i) on the chosen and zero elsewhere (normalize), else p_j ([j chosen] g_j - sum_i g_i w_i) with p the whole softmax
 //
-// A row is read once, by a warp or eight lanes of one, and stays in registers: 4 E bytes a row and 8 k out.  Work on the scores binds it, not bytes: 35 MB in 10.4 us
+// A row is read once, by a warp or eight lanes of one, and stays in registers: 4 E bytes a row and 8 k out.  Work on the scores and its latency bind it, not bytes: 36 MB in 11.4 us
 // are half of what HBM gives.
 #include <type_traits>
 
@@ -198,8 +198,8 @@ static __global__ void __launch_bounds__(256) router_forward_kernel(const float 
 // Many rows: four by a warp, eight lanes each, so that what a row costs apart from its scores is shared.  A lane has 4 V scores, which with V a place make 32 sets a
 // row whose largest give the bound as above.  The candidates' places in the lane's registers are bits of a word; they are read again, from L1, on their way to
 // shared memory.  A warp that meets a NaN or more candidates than there is room for takes its rows one after the other.
-// 32768 x 256, 8 chosen: 10.4 us against 12.7 by warps for a row, 4 chosen 8.0 against 10.9; 24000 rows 8.7 against 9.8.  With fewer rows the longer way of a warp shows (16384:
-// 7.7 against 7.1), with 16 chosen the rounds of the bound, which take three exchanges where a whole warp takes one instruction (17.9 against 15.8).
+// 32768 x 256, 8 chosen: 11.6 us against 13.3 by warps for a row, 4 chosen 9.3 against 11.9; 24000 rows 9.3 against 10.1.  With fewer rows the longer way of a warp shows (16384:
+// 7.7 against 7.1), with 16 chosen the rounds of the bound, which take three exchanges where a whole warp takes one instruction (18.1 against 16.2).
 constexpr long kManyRows = 24000;
 constexpr int kManyChosen = 8;
 struct FourRows {

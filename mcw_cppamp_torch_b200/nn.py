@@ -698,7 +698,7 @@ class Dispatch(Module):
 class Combine(Module):
     """The sum of each token's rows times their weights: of the input [rows, weights, positions] or [rows, weights, positions, residual], rows sorted as by
     Dispatch and weights and positions [tokens, k] (weights None: all one), plus the residual [tokens, size].  Slots whose position is 0 add nothing.
-    `size` is needed where there may be no rows at all and no residual.
+    A row is one slot's: the backward pass writes its gradient once.  `size` is needed where there may be no rows at all and no residual.
     gradInput is [the rows' gradient, the weights', None] or with a residual [the rows' gradient, the weights', None, gradOutput], the last the
     given tensor itself, which is not saved or cloned with the module.  Rows that no position names, as when some are set to 0 behind Dispatch, have zeros for their gradient."""
 
