@@ -712,7 +712,7 @@ THC_API int THGPUNN_Combine_backward(THGPUTensor *input, THGPUTensor *weights, T
   if (gradWeights) size_result(gradWeights, 2, ws, {input, weights, positions, gradOutput, gradInput}, 6);
   // Rows that no slot names: looked for by blocks in front of the tokens', unless these would read more than a twelfth of what the others move, or take longer, as with many narrow
   // rows.  Then all rows are zero first.  us a call without either, searched, and cleared: 8192 x 2048, 8 rows a token 172.1, 172.1; 1537 x 333, 4 rows 5.8, 5.9; 19056 x 333, 2 rows
-  // 25.1, 25.2; 512 x 1024, 8 rows 5.9, 7.2; 4096 x 64, 8 rows 4.8, 7.6, 8.1; 32768 x 64, 2 rows 6.7, 12.8, 10.4; 32768 x 128, 8 rows 55.0, 56.9.
+  // 25.1, 25.2; 512 x 1024, 8 rows 5.9 to 7.1, 6.0 to 7.2; 4096 x 64, 8 rows 4.8, 7.6, 8.1; 32768 x 64, 2 rows 6.7, 12.8, 10.4; 32768 x 128, 8 rows 55.0, 56.9.
   int clears = 0, each = 0;
   if (gradInput && rows) {
     clears = (int)std::min((rows + 255) / 256, std::min((long)kClearBlocks, std::max(1l, D / 4)));
